@@ -15,6 +15,8 @@ from typing import Optional
 
 import torch
 
+from ..csrc import ops
+
 
 @dataclass
 class LayerCache:
@@ -33,6 +35,7 @@ class GroupLayout:
     layout: tuple                       # of (name, heads, width): what a token keeps in this group
     window: int                         # 0: every token is kept
     slots: tuple                        # cache slots in this group
+    dtype: Optional[torch.dtype] = None  # None: the compute dtype
 
     @property
     def num_kv_heads(self) -> int:
@@ -45,20 +48,24 @@ class GroupLayout:
     def elements_per_token(self) -> int:
         return len(self.slots) * sum(h * w for _n, h, w in self.layout)
 
+    def bytes_per_token(self, itemsize: int) -> int:
+        """``itemsize``: of the compute dtype."""
+        return self.elements_per_token() * (itemsize if self.dtype is None else self.dtype.itemsize)
+
     def bytes_per_page(self, page_size: int, itemsize: int) -> int:
-        return self.elements_per_token() * page_size * itemsize
+        return self.bytes_per_token(itemsize) * page_size
 
 
 def plan_groups(cache_requests) -> list[GroupLayout]:
-    """Groups cache slots by (layout, window). A model without any paged mixer still gets one (empty) group so that
+    """Groups cache slots by (layout, window, element type). A model without any paged mixer still gets one (empty) group so that
     the block-table plumbing is uniform."""
     by_key: dict = {}
     for slot, (req, _state) in enumerate(cache_requests):
         if req is None:
             continue
-        key = (req.layout(), 0 if req.window is None else int(req.window))
+        key = (req.layout(), 0 if req.window is None else int(req.window), getattr(req, "dtype", None))
         by_key.setdefault(key, []).append(slot)
-    groups = [GroupLayout(k[0], k[1], tuple(v)) for k, v in by_key.items()]
+    groups = [GroupLayout(k[0], k[1], tuple(v), k[2]) for k, v in by_key.items()]
     return groups or [GroupLayout((), 0, ())]
 
 
@@ -73,7 +80,7 @@ class DeviceCache:
         for g in self.groups:
             named = {}
             for name, heads, width in (g.layout if g.slots else ()):
-                named[name] = torch.zeros((len(g.slots), num_pages, heads, page_size, width), dtype=dtype, device=self.device)
+                named[name] = torch.zeros((len(g.slots), num_pages, heads, page_size, width), dtype=g.dtype or dtype, device=self.device)
                 self.pages.append(named[name])
             self.group_tensors.append(named)
         self.states = {}
@@ -100,6 +107,15 @@ class DeviceCache:
     def bytes_per_page(self) -> int:
         item = torch.empty((), dtype=self.dtype).element_size()
         return sum(g.bytes_per_page(self.page_size, item) for g in self.groups)
+
+    def copy_pages(self, group: int, src, dst) -> None:
+        """Page ``dst[i]`` of a group becomes page ``src[i]`` in every cache slot and tensor of the group (``ops.copy_pages``)."""
+        ops.copy_pages(list(self.group_tensors[group].values()), src, dst)
+
+    def copy_state(self, src: int, dst: int) -> None:
+        """State slot ``dst`` becomes slot ``src``, in every mixer that keeps state."""
+        for s in self.states.values():
+            s[dst].copy_(s[src])
 
     def total_bytes(self) -> int:
         total = sum(p.numel() * p.element_size() for p in self.pages)

@@ -27,6 +27,7 @@ def _add_engine_options(p: argparse.ArgumentParser) -> None:
     p.add_argument("--config", help="a config.json instead of --model (needs --random-weights)")
     p.add_argument("--random-weights", type=int, metavar="SEED", help="seeded random weights for --preset/--config")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    p.add_argument("--cache-dtype", default=None, choices=["int4"], help="hold keys and values in 4 bits instead of --dtype")
     p.add_argument("--block-size", type=int, default=16, help="tokens per KV page")
     p.add_argument("--num-blocks", type=int, default=None, help="override the page count; by default sized from free device memory")
     p.add_argument("--activation-reserve", type=float, default=0.15, help="share of free memory held back for activations")
@@ -60,7 +61,7 @@ def _engine(args):
     from .config import preset
     from .engine import Engine
 
-    options = dict(dtype=args.dtype, block_size=args.block_size, num_blocks=args.num_blocks,
+    options = dict(dtype=args.dtype, cache_dtype=args.cache_dtype, block_size=args.block_size, num_blocks=args.num_blocks,
                    activation_reserve=args.activation_reserve, max_batch_tokens=args.max_batch_tokens,
                    max_batch_seqs=args.max_batch_seqs, max_model_len=args.max_model_len, max_queued=args.max_queued,
                    watermark=args.watermark,
@@ -165,7 +166,7 @@ def cmd_plan(args) -> int:
     else:
         config = config_from_dict(preset(args.preset) if args.preset else json.load(open(args.config)))
     try:
-        plan = plan_memory(config, args.dtype, int(args.memory_gib * (1 << 30)), args.block_size, args.activation_reserve,
+        plan = plan_memory(config, args.dtype, int(args.memory_gib * (1 << 30)), args.block_size, args.activation_reserve, cache_dtype=args.cache_dtype,
                            name=args.preset or args.model or args.config)
     except PlanError as e:
         print(f"does not fit: {e}", file=sys.stderr)
@@ -229,6 +230,7 @@ def main(argv=None) -> int:
     pl.add_argument("--preset")
     pl.add_argument("--config")
     pl.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    pl.add_argument("--cache-dtype", default=None, choices=["int4"], help="keys and values held in 4 bits")
     pl.add_argument("--memory-gib", type=float, default=183359 / 1024, help="device memory (default: a B200)")
     pl.add_argument("--block-size", type=int, default=16)
     pl.add_argument("--activation-reserve", type=float, default=0.15)

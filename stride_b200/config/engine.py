@@ -12,12 +12,14 @@ from typing import Optional
 
 import torch
 
+CACHE_DTYPES = (None, "int4")
 DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
 
 @dataclass
 class EngineConfig:
     dtype: str = "bfloat16"
+    cache_dtype: Optional[str] = None        # None: pages in ``dtype``; "int4": keys and values held in 4 bits (and a scale and centre per 32)
     block_size: int = 16                     # tokens per cache page
     num_blocks: Optional[int] = None         # pages per group; None: sized from free device memory
     activation_reserve: float = 0.15         # share of free memory kept back when sizing the pool
@@ -37,6 +39,8 @@ class EngineConfig:
     def __post_init__(self):
         if self.dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}, got {self.dtype!r}")
+        if self.cache_dtype not in CACHE_DTYPES:
+            raise ValueError(f"cache_dtype must be one of {CACHE_DTYPES}, got {self.cache_dtype!r}")
         if self.block_size <= 0:
             raise ValueError("block_size must be positive")
         if self.num_blocks is not None and self.num_blocks <= 0:

@@ -55,6 +55,7 @@ class LlamaConfig:
     max_position_embeddings: int = 8192
     tie_word_embeddings: bool = False
     attention_bias: bool = False
+    qk_norm: bool = False                    # an RMS norm with a weight on every query and key head, before the rotation
     hidden_act: str = "silu"
     bos_token_id: Optional[int] = None
     eos_token_id: tuple = ()
@@ -105,6 +106,7 @@ class LlamaConfig:
             max_position_embeddings=_positive_int(d, "max_position_embeddings", 8192),
             tie_word_embeddings=bool(d.get("tie_word_embeddings", False)),
             attention_bias=bool(d.get("attention_bias", False)),
+            qk_norm=bool(d.get("qk_norm", False)),
             hidden_act=act,
             bos_token_id=d.get("bos_token_id"),
             eos_token_id=eos_ids,
@@ -118,15 +120,18 @@ class LlamaConfig:
 
     @staticmethod
     def complete_from_checkpoint(d: dict, tensor_names: set) -> dict:
-        """Two options that the reference settles by what the checkpoint holds, never by config.json
+        """Options that the reference settles by what the checkpoint holds, never by config.json
         (python/stride_worker/model.py:127-128,159-169): the head is tied when ``lm_head.weight`` is absent,
-        and the q/k/v projections have biases when the bias tensors are there. A config.json that gives the
+        and the q/k/v projections have biases when the bias tensors are there; likewise (beyond the reference) the norms of
+        query and key heads. A config.json that gives the
         key is taken at its word (and checked against the checkpoint at load); one that leaves it out gets it
         from the checkpoint here."""
         if "tie_word_embeddings" not in d:
             d["tie_word_embeddings"] = "lm_head.weight" not in tensor_names
         if "attention_bias" not in d:
             d["attention_bias"] = any(n.endswith(".self_attn.q_proj.bias") for n in tensor_names)
+        if "qk_norm" not in d:
+            d["qk_norm"] = any(n.endswith(".self_attn.q_norm.weight") for n in tensor_names)
         return d
 
     def with_max_positions(self, count: int) -> "LlamaConfig":
@@ -166,6 +171,7 @@ class LlamaConfig:
             "max_position_embeddings": self.max_position_embeddings,
             "tie_word_embeddings": self.tie_word_embeddings,
             "attention_bias": self.attention_bias,
+            **({"qk_norm": True} if self.qk_norm else {}),
             "mlp_bias": False,
             "hidden_act": self.hidden_act,
         }
@@ -221,7 +227,8 @@ class LlamaConfig:
                 mixer=MixerSpec(kind="attention", hidden=self.hidden_size, num_heads=self.num_attention_heads,
                                 num_kv_heads=self.num_key_value_heads, head_dim=self.head_dim,
                                 scale=self.head_dim ** -0.5, window=None, bias=self.attention_bias, position=position,
-                                prefix=p + "self_attn."),
+                                prefix=p + "self_attn.",
+                                params=(("qk_norm", "weighted"), ("norm_eps", self.rms_norm_eps)) if self.qk_norm else ()),
                 feed_forward=FeedForwardSpec(kind="swiglu", hidden=self.hidden_size, intermediate=self.intermediate_size,
                                              activation=self.hidden_act, prefix=p + "mlp."),
                 mixer_norm=NormSpec(kind="rmsnorm", width=self.hidden_size, eps=self.rms_norm_eps,

@@ -59,12 +59,12 @@ class MemoryPlan:
 
 
 def plan_memory(config, dtype: str = "bfloat16", memory_bytes: int = B200_MEMORY_BYTES, block_size: int = 16,
-                activation_fraction: float = 0.15, name: str | None = None, max_requests: int = 256) -> MemoryPlan:
+                activation_fraction: float = 0.15, name: str | None = None, max_requests: int = 256, cache_dtype: str | None = None) -> MemoryPlan:
     """``config``: the typed configuration of any registered architecture. Its sizes are taken from the model's
     own parts (the tensors they declare, what their mixers keep per token and per request), not from arithmetic
     on the configuration class. ``activation_fraction`` of what the weights leave is held back for activations,
     workspace and fragmentation (the worker's ``--activation-reserve``, python/stride_worker/worker.py:182-225);
-    state of fixed size is set aside for ``max_requests`` requests. Raises ``PlanError`` when the weights do not
+    state of fixed size is set aside for ``max_requests`` requests; ``cache_dtype`` ``int4`` counts pages held in 4 bits. Raises ``PlanError`` when the weights do not
     fit or not even one page is left."""
     if dtype not in ITEMSIZE:
         raise PlanError(f"dtype must be one of {sorted(ITEMSIZE)}, got {dtype!r}")
@@ -73,7 +73,12 @@ def plan_memory(config, dtype: str = "bfloat16", memory_bytes: int = B200_MEMORY
     if not 0.0 <= activation_fraction < 1.0:
         raise PlanError("activation_fraction must be in [0, 1)")
     from ..engine.loading import footprint      # the parts live above this package; asked for only when a plan is made
-    sizes = footprint(config, dtype)
+    try:
+        sizes = footprint(config, dtype, cache_dtype)
+    except ValueError as e:
+        if cache_dtype is None:
+            raise
+        raise PlanError(str(e)) from None       # a layer whose pages are not held so
     name = name or getattr(config, "name", "model")
     weight_bytes = sizes["weight_bytes"] + sizes["state_bytes_per_request"] * max_requests
     if weight_bytes >= memory_bytes:

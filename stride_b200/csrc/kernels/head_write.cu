@@ -1,0 +1,357 @@
+// What stands between the q/k/v projection and attention, in one pass: bias, an RMS norm with a weight on every query and key head, the
+// rotation, and the write of keys and values into their pages, as they are or held in 4 bits (int4_cache.cuh).
+//   x = row + bias;  y = x rsqrt(mean(x^2) + eps) w (queries and keys, where weights are given);  entry i turns with entry i + hd/2
+// Everything is 32-bit between the load and the store: a query, key or value is rounded once, to the element type or to 4 bits.
+#include "int4_cache.cuh"
+
+namespace stride {
+
+constexpr int kWriteWarps = 4;
+
+struct HeadWrite {
+    const void* rows;               // [tokens, (nq + 2 nkv) hd]
+    void* q_out;                    // head h of token t at q_out[t * q_out_stride + h * hd]
+    const float* bias;              // [(nq + 2 nkv) hd] or null
+    const float* q_norm;            // [hd], both or none
+    const float* k_norm;
+    const int32_t* positions;
+    const int32_t* slots;           // null: nothing is stored
+    const float* cos;               // [num_positions, hd / 2]
+    const float* sin;
+    void* k_pages;
+    void* v_pages;
+    int* status;
+    long long q_out_stride;
+    float eps;
+    int tokens, nq, nkv, hd, page_size, num_pages, num_positions, rotate;
+};
+
+// A warp a unit: a query head, or a key head with its value head. Lane l holds entry 32 j + l of the head in x[j], so a group of 32 is
+// one register of the warp.
+template <typename T, bool FOUR>
+__global__ void __launch_bounds__(kWriteWarps * 32) head_write_kernel(const HeadWrite a) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ float staged[kWriteWarps][four::kMaxHeadDim];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t = blockIdx.x, unit = blockIdx.y * kWriteWarps + warp;
+    if (unit >= a.nq + a.nkv) return;
+    const int hd = a.hd, half = hd >> 1, G = four::groups_of(hd), heads = a.nq + 2 * a.nkv;
+    const T* row = static_cast<const T*>(a.rows) + static_cast<size_t>(t) * heads * hd;
+    const int pos = a.rotate ? a.positions[t] : 0;
+    if (a.rotate && (pos < 0 || pos >= a.num_positions)) {
+        if (lane == 0) four::complain(a.status, four::kCodeNoPosition);
+        return;
+    }
+    const bool is_q = unit < a.nq;
+    const int slot = a.slots != nullptr && !is_q ? a.slots[t] : -1;
+    if (!is_q && slot < 0) return;
+    const int page = is_q ? 0 : slot / a.page_size, offset = is_q ? 0 : slot % a.page_size;
+    if (page >= a.num_pages) {
+        if (lane == 0) four::complain(a.status, four::kCodeNoSlot);
+        return;
+    }
+    const int kvh = unit - a.nq;
+    float x[four::kMaxGroups], v[four::kMaxGroups];
+    auto load = [&](int head, float* out) {
+#pragma unroll
+        for (int j = 0; j < four::kMaxGroups; ++j) {
+            const int d = 32 * j + lane;
+            out[j] = 0.f;
+            if (j < G && d < hd) {
+                out[j] = to_f32(row[static_cast<size_t>(head) * hd + d]);
+                if (a.bias != nullptr) out[j] = __fadd_rn(out[j], a.bias[static_cast<size_t>(head) * hd + d]);
+            }
+        }
+    };
+    load(unit, x);                                             // key head kvh is head nq + kvh of the row
+    if (!is_q) load(unit + a.nkv, v);
+    const float* weight = is_q ? a.q_norm : a.k_norm;
+    if (weight != nullptr) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < four::kMaxGroups; ++j) sum = fmaf(x[j], x[j], sum);
+        const float inv = rsqrtf(__fadd_rn(__fdiv_rn(warp_sum(sum), static_cast<float>(hd)), a.eps));
+#pragma unroll
+        for (int j = 0; j < four::kMaxGroups; ++j)
+            if (32 * j + lane < hd) x[j] = __fmul_rn(__fmul_rn(x[j], inv), weight[32 * j + lane]);
+    }
+    if (a.rotate) {
+        const float* cs = a.cos + static_cast<size_t>(pos) * half;
+        const float* sn = a.sin + static_cast<size_t>(pos) * half;
+#pragma unroll
+        for (int j = 0; j < four::kMaxGroups; ++j)
+            if (32 * j + lane < hd) staged[warp][32 * j + lane] = x[j];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < four::kMaxGroups; ++j) {
+            const int d = 32 * j + lane;
+            if (d < half)
+                x[j] = __fadd_rn(__fmul_rn(x[j], cs[d]), __fmul_rn(-staged[warp][d + half], sn[d]));
+            else if (d < hd)
+                x[j] = __fadd_rn(__fmul_rn(x[j], cs[d - half]), __fmul_rn(staged[warp][d - half], sn[d - half]));
+        }
+    }
+    if (is_q) {
+        T* out = static_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.q_out_stride + static_cast<size_t>(unit) * hd;
+#pragma unroll
+        for (int j = 0; j < four::kMaxGroups; ++j)
+            if (32 * j + lane < hd) out[32 * j + lane] = from_f32<T>(x[j]);
+        return;
+    }
+    const size_t at = (static_cast<size_t>(page) * a.nkv + kvh) * a.page_size + offset;
+    if constexpr (!FOUR) {
+        T* k = static_cast<T*>(a.k_pages) + at * hd;
+        T* w = static_cast<T*>(a.v_pages) + at * hd;
+#pragma unroll
+        for (int j = 0; j < four::kMaxGroups; ++j)
+            if (32 * j + lane < hd) {
+                k[32 * j + lane] = from_f32<T>(x[j]);
+                w[32 * j + lane] = from_f32<T>(v[j]);
+            }
+    } else {
+        const int bytes = four::row_bytes(hd);
+        uint8_t* rows[2] = {static_cast<uint8_t*>(a.k_pages) + at * bytes, static_cast<uint8_t*>(a.v_pages) + at * bytes};
+        float s[2][four::kMaxGroups], c[2][four::kMaxGroups];
+        bool fine = true;
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int j = 0; j < four::kMaxGroups; ++j) {
+                if (j >= G) continue;
+                const bool there = 32 * j + lane < hd;
+                const float e = which ? v[j] : x[j];
+                fine = fine && (!there || isfinite(e));
+                float lo = there ? e : INFINITY, hi = there ? e : -INFINITY;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                }
+                four::group_params(lo, hi, s[which][j], c[which][j]);
+                fine = fine && isfinite(s[which][j]) && isfinite(c[which][j]);
+            }
+        fine = __all_sync(0xffffffffu, fine);
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int j = 0; j < four::kMaxGroups; ++j) {
+                if (j >= G) continue;
+                const float e = which ? v[j] : x[j];
+                float sj = s[which][j], cj = c[which][j];
+                uint32_t n = 8;
+                if (!fine)
+                    sj = cj = which ? 0.f : __int_as_float(0x7fc00000);
+                else if (32 * j + lane < hd && sj > 0.f)
+                    n = four::number_of(e, cj, __frcp_rn(sj));
+                if (which == 0) {
+                    uint32_t word = n << (4 * (lane & 7));
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+                    if ((lane & 7) == 0) reinterpret_cast<uint32_t*>(rows[0])[(lane >> 3) * G + j] = word;
+                } else {
+                    uint32_t word = n << (4 * (lane & 3));
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+                    if ((lane & 3) == 0) reinterpret_cast<uint16_t*>(rows[1])[(lane >> 2) * G + j] = static_cast<uint16_t>(word);
+                }
+                if (lane == 0) reinterpret_cast<uint32_t*>(rows[which] + 16 * G)[j] = four::pack_params(sj, cj);
+            }
+    }
+}
+
+// What the slots of a 4-bit cache stand for: k_out, v_out [n, nkv, hd]. A slot below zero reads as zeros. A warp a row.
+template <typename T>
+__global__ void __launch_bounds__(kWriteWarps * 32)
+int4_read_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const int32_t* __restrict__ slots, T* __restrict__ k_out,
+                 T* __restrict__ v_out, int n, int nkv, int hd, int page_size, int num_pages, int* status) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, G = four::groups_of(hd), bytes = four::row_bytes(hd);
+    const long long unit = static_cast<long long>(blockIdx.x) * kWriteWarps + (threadIdx.x >> 5);
+    if (unit >= static_cast<long long>(n) * nkv) return;
+    const int i = static_cast<int>(unit / nkv), kvh = static_cast<int>(unit % nkv);
+    const int slot = slots[i];
+    int page = slot < 0 ? -1 : slot / page_size;
+    if (page >= num_pages) {
+        if (lane == 0) four::complain(status, four::kCodeNoSlot);
+        page = -1;
+    }
+    T* out[2] = {k_out + unit * hd, v_out + unit * hd};
+    if (page < 0) {
+        for (int d = lane; d < hd; d += 32) out[0][d] = out[1][d] = from_f32<T>(0.f);
+        return;
+    }
+    const size_t at = ((static_cast<size_t>(page) * nkv + kvh) * page_size + slot % page_size) * bytes;
+    const uint8_t* rows[2] = {k_pages + at, v_pages + at};
+    for (int j = 0; j < G; ++j) {
+        const int d = 32 * j + lane;
+        if (d >= hd) break;
+        const uint32_t kn = reinterpret_cast<const uint32_t*>(rows[0])[(lane >> 3) * G + j] >> (4 * (lane & 7)) & 15u;
+        const uint32_t vn = static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(rows[1])[(lane >> 2) * G + j]) >> (4 * (lane & 3)) & 15u;
+        const uint32_t kp = reinterpret_cast<const uint32_t*>(rows[0] + 16 * G)[j], vp = reinterpret_cast<const uint32_t*>(rows[1] + 16 * G)[j];
+        out[0][d] = from_f32<T>(four::value_of(kn, four::bf16_low(kp), four::bf16_high(kp)));
+        out[1][d] = from_f32<T>(four::value_of(vn, four::bf16_low(vp), four::bf16_high(vp)));
+    }
+}
+
+// The keys of the first num_seqs requests as pages of 64 in bfloat16, for the attention of portions: a request's pages one after the other,
+// the requests' too, and the table that says so. A key is expanded once for all query tiles that read it. CTA (page, key head).
+constexpr int kExpandKeys = 64, kExpandThreads = 256;
+
+template <int G>
+__global__ void __launch_bounds__(kExpandThreads)
+int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table,
+                   int table_width, const int32_t* __restrict__ q_len, const int32_t* __restrict__ ctx_len, int num_seqs, int nkv, int page_size,
+                   int window, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int32_t* __restrict__ table_out, int out_pages,
+                   int* status) {
+    pdl_trigger();
+    constexpr int HD = 32 * G, BYTES = 20 * G;
+    __shared__ size_t row_at[kExpandKeys];
+    pdl_wait();
+    int seq = -1, index = 0, at = 0;                        // this page is number `index` of request `seq`
+    for (int s = 0; s < num_seqs; ++s) {
+        const int pages = (ctx_len[s] + kExpandKeys - 1) / kExpandKeys;
+        if (static_cast<int>(blockIdx.x) < at + pages) {
+            seq = s;
+            index = blockIdx.x - at;
+            break;
+        }
+        at += pages;
+    }
+    if (seq < 0) return;
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && threadIdx.x == 0) {      // the last page there is room for
+        bool more = (index + 1) * kExpandKeys < ctx_len[seq];
+        for (int s = seq + 1; s < num_seqs; ++s) more = more || ctx_len[s] > 0;
+        if (more) four::complain(status, four::kCodeTooManyKeys);
+    }
+    const int ctx = ctx_len[seq], kvh = blockIdx.y, key0 = index * kExpandKeys;
+    const int first = window > 0 ? max(0, ctx - q_len[seq] - window + 1) : 0;
+    if (kvh == 0 && threadIdx.x == 0) table_out[static_cast<size_t>(seq) * out_pages + index] = blockIdx.x;
+    if (key0 + kExpandKeys <= first) return;                // behind every window
+    if (threadIdx.x < kExpandKeys) {
+        const int key = key0 + threadIdx.x;
+        size_t row = ~size_t(0);
+        if (key >= first && key < ctx) {
+            const int page = key / page_size < table_width ? block_table[static_cast<size_t>(seq) * table_width + key / page_size] : -1;
+            if (page < 0 || page >= num_pages)
+                four::complain(status, four::kCodeNoPage);
+            else
+                row = ((static_cast<size_t>(page) * nkv + kvh) * page_size + key % page_size) * BYTES;
+        }
+        row_at[threadIdx.x] = row;
+    }
+    __syncthreads();
+    const size_t out_row = (static_cast<size_t>(blockIdx.x) * nkv + kvh) * kExpandKeys;
+    // a key without a page (before the windows, behind the end) becomes zeros: attention masks it
+    for (int i = threadIdx.x; i < kExpandKeys * 4; i += kExpandThreads) {           // keys: part a of a row, 8 entries of every group
+        const int r = i >> 2, a = i & 3;
+        const bool there = row_at[r] != ~size_t(0);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pages + (there ? row_at[r] : 0));
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint4 out = make_uint4(0, 0, 0, 0);
+            if (there) {
+                const uint32_t w = words[a * G + g], p = words[4 * G + g];
+                const float s = four::bf16_low(p), c = four::bf16_high(p);
+                uint32_t pair[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __nv_bfloat162 v = __floats2bfloat162_rn(four::value_of(w >> (8 * e) & 15u, s, c), four::value_of(w >> (8 * e + 4) & 15u, s, c));
+                    pair[e] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+                out = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+            }
+            *reinterpret_cast<uint4*>(k_out + (out_row + r) * HD + 32 * g + 8 * a) = out;
+        }
+    }
+    for (int i = threadIdx.x; i < kExpandKeys * 8; i += kExpandThreads) {           // values: part a of a row, 4 entries of every group
+        const int r = i >> 3, a = i & 7;
+        const bool there = row_at[r] != ~size_t(0);
+        const uint8_t* row = v_pages + (there ? row_at[r] : 0);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint2 out = make_uint2(0, 0);
+            if (there) {
+                const uint32_t w = reinterpret_cast<const uint16_t*>(row)[a * G + g], p = reinterpret_cast<const uint32_t*>(row + 16 * G)[g];
+                const float s = four::bf16_low(p), c = four::bf16_high(p);
+                const __nv_bfloat162 x = __floats2bfloat162_rn(four::value_of(w & 15u, s, c), four::value_of(w >> 4 & 15u, s, c));
+                const __nv_bfloat162 y = __floats2bfloat162_rn(four::value_of(w >> 8 & 15u, s, c), four::value_of(w >> 12, s, c));
+                out = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+            }
+            *reinterpret_cast<uint2*>(v_out + (out_row + r) * HD + 32 * g + 4 * a) = out;
+        }
+    }
+}
+
+}  // namespace stride
+
+using namespace stride;
+
+// rows: [tokens, (nq + 2 nkv) hd]; q_out: rows of q_out_stride elements (`rows` itself, with its row length, for queries in place).
+// bits4: pages hold 4 bits (uint8 [num_pages, nkv, page_size, 20 ceil(hd / 32)]), else elements [num_pages, nkv, page_size, hd]. slots null, or
+// a slot below zero: keys and values are not stored. Slots of one launch are distinct. Returns -2 for odd head sizes and those above 256.
+extern "C" int stride_head_write(const void* rows, void* q_out, long long q_out_stride, const float* bias, const float* q_norm, const float* k_norm,
+                                 float eps, const int32_t* positions, const int32_t* slots, const float* cos, const float* sin, int num_positions,
+                                 void* k_pages, void* v_pages, int num_pages, int bits4, int tokens, int nq, int nkv, int hd, int page_size, int rotate,
+                                 int dtype, int* status, cudaStream_t stream) {
+    if (tokens < 0 || nq <= 0 || nkv <= 0 || hd <= 0 || page_size <= 0 || num_pages <= 0 || q_out_stride < static_cast<long long>(nq) * hd ||
+        (q_norm == nullptr) != (k_norm == nullptr) || (rotate && num_positions <= 0) || static_cast<long long>(num_pages) * page_size > 2147483647LL)
+        return STRIDE_BAD_ARGUMENT;
+    if (hd > four::kMaxHeadDim || (rotate && hd % 2)) return STRIDE_UNSUPPORTED;
+    if (bits4 && (reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 4) return STRIDE_UNSUPPORTED;
+    const int units = nq + nkv, ctas_y = (units + kWriteWarps - 1) / kWriteWarps;
+    if (ctas_y > 65535) return STRIDE_UNSUPPORTED;
+    if (tokens == 0) return 0;
+    const HeadWrite a{rows, q_out, bias, q_norm, k_norm, positions, slots, cos, sin, k_pages, v_pages, status, q_out_stride, eps,
+                      tokens, nq, nkv, hd, page_size, num_pages, num_positions, rotate};
+    const dim3 grid(tokens, ctas_y), block(kWriteWarps * 32);
+    if (dtype == STRIDE_DTYPE_F32)
+        bits4 ? stride::launch(head_write_kernel<float, true>, grid, block, 0, stream, a)
+              : stride::launch(head_write_kernel<float, false>, grid, block, 0, stream, a);
+    else if (dtype == STRIDE_DTYPE_BF16)
+        bits4 ? stride::launch(head_write_kernel<__nv_bfloat16, true>, grid, block, 0, stream, a)
+              : stride::launch(head_write_kernel<__nv_bfloat16, false>, grid, block, 0, stream, a);
+    else
+        return STRIDE_BAD_ARGUMENT;
+    return STRIDE_LAUNCH_STATUS();
+}
+
+extern "C" int stride_int4_read(const void* k_pages, const void* v_pages, const int32_t* slots, void* k_out, void* v_out, int n, int nkv, int hd,
+                                int page_size, int num_pages, int dtype, int* status, cudaStream_t stream) {
+    if (n < 0 || nkv <= 0 || hd <= 0 || page_size <= 0 || num_pages <= 0) return STRIDE_BAD_ARGUMENT;
+    if (hd > four::kMaxHeadDim || (reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 4) return STRIDE_UNSUPPORTED;
+    if (n == 0) return 0;
+    const long long ctas = (static_cast<long long>(n) * nkv + kWriteWarps - 1) / kWriteWarps;
+    if (ctas > 2147483647LL) return STRIDE_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>(ctas)), block(kWriteWarps * 32);
+    const auto k = static_cast<const uint8_t*>(k_pages);
+    const auto v = static_cast<const uint8_t*>(v_pages);
+    if (dtype == STRIDE_DTYPE_F32)
+        stride::launch(int4_read_kernel<float>, grid, block, 0, stream, k, v, slots, static_cast<float*>(k_out), static_cast<float*>(v_out), n, nkv, hd,
+                       page_size, num_pages, status);
+    else if (dtype == STRIDE_DTYPE_BF16)
+        stride::launch(int4_read_kernel<__nv_bfloat16>, grid, block, 0, stream, k, v, slots, static_cast<__nv_bfloat16*>(k_out),
+                       static_cast<__nv_bfloat16*>(v_out), n, nkv, hd, page_size, num_pages, status);
+    else
+        return STRIDE_BAD_ARGUMENT;
+    return STRIDE_LAUNCH_STATUS();
+}
+
+// k_out, v_out: [out_pages, nkv, 64, hd] bfloat16; table_out: [num_seqs, out_pages]. out_pages: at least the sum over the requests of
+// ceil(ctx_len / 64). Pages that no query of its request's portion can see are left as they were. Head sizes 64 and 128.
+extern "C" int stride_int4_expand(const void* k_pages, const void* v_pages, int num_pages, const int32_t* block_table, int table_width,
+                                  const int32_t* q_len, const int32_t* ctx_len, int num_seqs, int nkv, int hd, int page_size, int window, void* k_out,
+                                  void* v_out, int32_t* table_out, int out_pages, int* status, cudaStream_t stream) {
+    if (num_seqs < 0 || nkv <= 0 || page_size <= 0 || num_pages <= 0 || table_width <= 0 || window < 0 || out_pages <= 0) return STRIDE_BAD_ARGUMENT;
+    if ((hd != 64 && hd != 128) || nkv > 65535) return STRIDE_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 4 ||
+        (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16)
+        return STRIDE_UNSUPPORTED;
+    if (num_seqs == 0) return 0;
+    const auto kernel = hd == 64 ? int4_expand_kernel<2> : int4_expand_kernel<4>;
+    stride::launch(kernel, dim3(out_pages, nkv), dim3(kExpandThreads), 0, stream, static_cast<const uint8_t*>(k_pages), static_cast<const uint8_t*>(v_pages),
+                   num_pages, block_table, table_width, q_len, ctx_len, num_seqs, nkv, page_size, window, static_cast<__nv_bfloat16*>(k_out),
+                   static_cast<__nv_bfloat16*>(v_out), table_out, out_pages, status);
+    return STRIDE_LAUNCH_STATUS();
+}

@@ -1,0 +1,96 @@
+// Copies of pages inside the pools of a cache: for each pair (from, to) page `to` of every pool and layer becomes page `from`.
+//
+// A pool is [layers, num_pages, page_bytes]. The pairs travel as the kernel's parameters, so a call needs neither a copy to the device nor
+// memory of its own, and a captured graph holds the pairs it was captured with. No page is both read and written, so the order of the
+// copies does not matter (the caller checks). Attention may ask for keys of earlier steps before the kernel in front of it has ended: this one
+// lets nothing start early. Bound by the bytes: every page is read once and written once.
+#include "common.cuh"
+
+namespace stride {
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyPools = 8;
+constexpr int kCopyPairs = 448;         // what fits into 4 KB of parameters beside the pools
+constexpr int kCopyPacks = 4;           // packs a thread has under way at once
+
+struct PageCopies {
+    unsigned char* base[kCopyPools];
+    long long page_bytes[kCopyPools], layer_bytes[kCopyPools];
+    int layers[kCopyPools];
+    int pools;
+    int2 pairs[kCopyPairs];
+};
+
+// CTA (x, y, z): part x of the page, pair y, layer z counted over all pools. P: the pack that bases and page sizes are multiples of.
+template <typename P>
+__global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_constant__ PageCopies a) {
+    int layer = blockIdx.z, pool = 0;
+    while (layer >= a.layers[pool]) layer -= a.layers[pool++];
+    const long long packs = a.page_bytes[pool] / static_cast<long long>(sizeof(P));
+    const long long first = static_cast<long long>(blockIdx.x) * kCopyThreads * kCopyPacks + threadIdx.x;
+    const int2 pair = a.pairs[blockIdx.y];
+    unsigned char* base = a.base[pool] + layer * a.layer_bytes[pool];
+    const P* from = reinterpret_cast<const P*>(base + pair.x * a.page_bytes[pool]);
+    P* to = reinterpret_cast<P*>(base + pair.y * a.page_bytes[pool]);
+    P v[kCopyPacks];
+#pragma unroll
+    for (int i = 0; i < kCopyPacks; ++i)
+        if (first + i * kCopyThreads < packs) v[i] = from[first + i * kCopyThreads];
+#pragma unroll
+    for (int i = 0; i < kCopyPacks; ++i)
+        if (first + i * kCopyThreads < packs) to[first + i * kCopyThreads] = v[i];
+}
+
+template <typename P>
+void launch_copies(const PageCopies& a, long long most_bytes, int pairs, int layers, cudaStream_t stream) {
+    const long long packs = most_bytes / static_cast<long long>(sizeof(P)), per_cta = kCopyThreads * kCopyPacks;
+    stride::launch_alone(page_copy_kernel<P>, dim3(static_cast<unsigned>((packs + per_cta - 1) / per_cta), pairs, layers), dim3(kCopyThreads), 0, stream, a);
+}
+
+}  // namespace stride
+
+using namespace stride;
+
+// pools: n_pools device addresses; layers, num_pages, page_bytes: of each pool. from, to: `pairs` page numbers of every pool (host memory). The
+// caller has checked that no page of `to` comes twice or also in `from`.
+extern "C" int stride_copy_pages(const long long* pools, const int* layers, const int* num_pages, const long long* page_bytes, int n_pools, const int* from,
+                                 const int* to, int pairs, cudaStream_t stream) {
+    if (n_pools < 0 || pairs < 0) return STRIDE_BAD_ARGUMENT;
+    for (int p = 0; p < n_pools; ++p) {
+        if (pools[p] == 0 || layers[p] <= 0 || num_pages[p] <= 0 || page_bytes[p] <= 0) return STRIDE_BAD_ARGUMENT;
+        for (int i = 0; i < pairs; ++i)
+            if (from[i] < 0 || to[i] < 0 || from[i] >= num_pages[p] || to[i] >= num_pages[p]) return STRIDE_BAD_ARGUMENT;
+    }
+    for (int p0 = 0; p0 < n_pools; p0 += kCopyPools) {
+        PageCopies a;
+        a.pools = n_pools - p0 < kCopyPools ? n_pools - p0 : kCopyPools;
+        long long all = 0, most = 0;
+        int total = 0;
+        for (int p = 0; p < kCopyPools; ++p) {
+            const bool used = p < a.pools;
+            a.base[p] = used ? reinterpret_cast<unsigned char*>(pools[p0 + p]) : nullptr;
+            a.page_bytes[p] = used ? page_bytes[p0 + p] : 0;
+            a.layer_bytes[p] = used ? page_bytes[p0 + p] * num_pages[p0 + p] : 0;
+            a.layers[p] = used ? layers[p0 + p] : 0;
+            if (!used) continue;
+            if (total + static_cast<long long>(layers[p0 + p]) > 65535) return STRIDE_UNSUPPORTED;
+            total += layers[p0 + p];
+            all |= pools[p0 + p] | page_bytes[p0 + p];
+            most = most > page_bytes[p0 + p] ? most : page_bytes[p0 + p];
+        }
+        if (most > (1LL << 40)) return STRIDE_UNSUPPORTED;
+        for (int i0 = 0; i0 < pairs; i0 += kCopyPairs) {
+            const int n = pairs - i0 < kCopyPairs ? pairs - i0 : kCopyPairs;
+            for (int i = 0; i < kCopyPairs; ++i) a.pairs[i] = i < n ? make_int2(from[i0 + i], to[i0 + i]) : make_int2(0, 0);
+            if (all % 16 == 0)
+                launch_copies<uint4>(a, most, n, total, stream);
+            else if (all % 4 == 0)
+                launch_copies<uint32_t>(a, most, n, total, stream);
+            else
+                launch_copies<uint8_t>(a, most, n, total, stream);
+            const int code = STRIDE_LAUNCH_STATUS();
+            if (code) return code;
+        }
+    }
+    return 0;
+}

@@ -66,6 +66,14 @@ _SIGNATURES = {
                                                          c_void_p, c_int, c_float, c_void_p, c_void_p]),
     "stride_gemm_stream_add_norm": ("gemm_bf16_stream", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong,
                                                          c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "stride_head_write": ("head_write", [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "stride_int4_read": ("head_write", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "stride_attention_int4_exact": ("attention_int4", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                                       c_int, c_int, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "stride_int4_expand": ("head_write", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                                          c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "stride_copy_pages": ("page_copy", [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "stride_scale_rows": ("elementwise", [c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_int, c_void_p]),
     "stride_paged_decode_attention": ("attention_decode", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                                            c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int,
@@ -255,6 +263,8 @@ _CLASS_OF = {
     "stride_ssm_step": "state space: recurrence", "stride_ssm_chunks": "state space: recurrence",
     "stride_gated_group_norm": "gate + norm of parts",
     "stride_paged_decode_attention_biased": "attention (decode)",
+    "stride_head_write": "rotation + head norms + cache write", "stride_int4_read": "4-bit cache: values", "stride_int4_expand": "4-bit cache: values",
+    "stride_attention_int4_exact": "attention (exact kernel)", "stride_copy_pages": "copies of pages",
 }
 
 
@@ -359,6 +369,23 @@ def _code(dtype: torch.dtype) -> int:
         return DTYPE_CODE[dtype]
     except KeyError:
         raise KernelError(f"element type {dtype} is not supported (float32 and bfloat16 are)") from None
+
+
+def _here(t: torch.Tensor, name: str, dtype=None) -> int:
+    """``_dev`` for a tensor that must also live on the current device: the launch goes to that device's stream."""
+    at = _dev(t, name, dtype)
+    if t.get_device() != torch.cuda.current_device():
+        raise KernelError(f"{name} lives on cuda:{t.get_device()}, but the current device is cuda:{torch.cuda.current_device()}")
+    return at
+
+
+def _here_opt(t, name: str, count: int, dtype) -> int | None:
+    """``_here`` for an optional vector of ``count`` elements."""
+    if t is None:
+        return None
+    if t.numel() != count:
+        raise KernelError(f"{name} must hold {count} elements, got {t.numel()}")
+    return _here(t, name, dtype)
 
 
 def require_device() -> None:
@@ -1479,7 +1506,11 @@ _WAIT_CODES = {1: "matrix product: producer", 2: "matrix product: tensor-core is
                61: "float32 product: copies", 62: "float32 product: tensor-core issuer", 63: "float32 product: cutting warps",
                71: "latent attention: copies of keys", 72: "latent attention: tensor-core issuer", 73: "latent attention: softmax"}
 _WAIT_CODES.update({c: "prefill attention (attention_prefill_tc.cu)" for c in range(11, 22)})
-_OTHER_CODES = {32: "decode attention was given a token whose position is not below the context bound of its launch"}
+_OTHER_CODES = {32: "decode attention was given a token whose position is not below the context bound of its launch",
+                33: "attention over a 4-bit cache met a key whose block-table entry names no page of the cache",
+                34: "a cache write or read was given a slot behind the cache's last page",
+                35: "a rotation was given a position behind its tables",
+                36: "attention of portions over a 4-bit cache: the requests hold more keys than the call said"}
 
 
 def reset_kernel_status(device=None) -> None:
@@ -2008,6 +2039,209 @@ def paged_attention_prefill(q, q_stride: int, out, k_pages, v_pages, block_table
         _dev(q_start, "q_start", torch.int32), _dev(q_len, "q_len", torch.int32), _dev(ctx_len, "ctx_len", torch.int32),
         num_seqs, tokens, nq, nkv, hd, page_size, float(scale), int(window), -float(softcap) if precise_cap else float(softcap), _opt(sinks, "sinks", torch.float32),
         _opt(slopes, "slopes", torch.float32), *_rel_args(rel, nq), _stream()), "paged_attention_prefill")
+
+
+# ------------------------------------------------------------- a cache held in 4 bits
+INT4_GROUP = 32             # entries that share a scale and a centre
+
+
+def int4_row_bytes(hd: int) -> int:
+    """Bytes of one head of one token in a cache held in 4 bits (csrc/kernels/int4_cache.cuh says what they are)."""
+    return 20 * -(-hd // INT4_GROUP)
+
+
+def _pages_args(k_pages, v_pages, nkv: int, page_size: int, row: int, dtype) -> tuple:
+    """(keys, values, number of pages) of pages [num_pages, nkv, page_size, row], checked."""
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if t.dim() != 4 or tuple(t.shape[1:]) != (nkv, page_size, row) or t.shape[0] == 0:
+            raise KernelError(f"{name} must be [num_pages, {nkv}, {page_size}, {row}], got {tuple(t.shape)}")
+    if k_pages.shape[0] != v_pages.shape[0]:
+        raise KernelError("keys and values must have the same number of pages")
+    return _here(k_pages, "k_pages", dtype), _here(v_pages, "v_pages", dtype), k_pages.shape[0]
+
+
+def _head_write(what: str, bits4: bool, qkv, bias, q_norm, k_norm, eps, positions, slot_mapping, cos, sin, k_pages, v_pages, nq, nkv, hd, page_size,
+                rotate, q_out) -> None:
+    if min(nq, nkv, hd, page_size) <= 0:
+        raise KernelError(f"{what}: heads, head size and page size must be positive")
+    tokens, width = qkv.shape
+    if width != (nq + 2 * nkv) * hd:
+        raise KernelError("qkv has the wrong width")
+    if (q_norm is None) != (k_norm is None):
+        raise KernelError("the norms of queries and keys come together")
+    code = _code(qkv.dtype)
+    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd) if bits4 else hd, torch.uint8 if bits4 else qkv.dtype)
+    if q_out is None:
+        out, stride = _here(qkv, "qkv"), width
+    else:
+        if q_out.dim() != 2 or q_out.shape[0] < tokens or q_out.shape[1] != nq * hd or q_out.dtype != qkv.dtype or q_out.stride(1) != 1 or \
+                q_out.stride(0) < nq * hd:
+            raise KernelError("q_out must be rows [tokens, nq * hd] of qkv's element type")
+        if not q_out.is_cuda or q_out.get_device() != qkv.get_device():
+            raise KernelError("q_out must live on qkv's device")
+        out, stride = q_out.data_ptr(), q_out.stride(0)
+    if positions.numel() < tokens or (slot_mapping is not None and slot_mapping.numel() < tokens):
+        raise KernelError("positions and slots must cover the tokens")
+    if rotate and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] * 2 != hd):
+        raise KernelError("cos and sin must be [positions, hd / 2]")
+    _check(_fn("stride_head_write")(
+        _here(qkv, "qkv"), out, stride, _here_opt(bias, "bias", width, torch.float32), _here_opt(q_norm, "q_norm", hd, torch.float32),
+        _here_opt(k_norm, "k_norm", hd, torch.float32), float(eps), _here(positions, "positions", torch.int32),
+        None if slot_mapping is None else _here(slot_mapping, "slot_mapping", torch.int32), _here(cos, "cos", torch.float32),
+        _here(sin, "sin", torch.float32), cos.shape[0] if rotate else 0, k, v, pages, int(bits4), tokens, nq, nkv, hd, page_size, int(rotate), code,
+        _status_ptr(qkv.device), _stream()), what)
+
+
+def qk_norm_rope_write(qkv, bias, q_norm, k_norm, eps: float, positions, slot_mapping, cos, sin, k_pages, v_pages, nq: int, nkv: int, hd: int,
+                       page_size: int, rotate: bool = True, q_out=None) -> None:
+    """Bias, the RMS norm of every query and key head with a weight of the head's size (float32 [hd]; None: no norms), the rotation of
+    ``rope_kv_write`` and the write of keys and values into their pages, in one pass and rounded once. Queries stay in ``qkv``, or go to
+    ``q_out`` [tokens, nq * hd]. ``slot_mapping`` None, or a slot of -1: nothing is stored. The slots of a call are distinct."""
+    _head_write("qk_norm_rope_write", False, qkv, bias, q_norm, k_norm, eps, positions, slot_mapping, cos, sin, k_pages, v_pages, nq, nkv, hd,
+                page_size, rotate, q_out)
+
+
+def rope_kv_write_int4(qkv, bias, q_norm, k_norm, eps: float, positions, slot_mapping, cos, sin, k_pages, v_pages, nq: int, nkv: int, hd: int,
+                       page_size: int, rotate: bool = True, q_out=None) -> None:
+    """``qk_norm_rope_write`` into pages held in 4 bits, uint8 [num_pages, nkv, page_size, int4_row_bytes(hd)]: an entry is rounded once, to a
+    sixteenth of the range of its group of 32. A token with a key or value that is not finite reads as no number in that key head."""
+    _head_write("rope_kv_write_int4", True, qkv, bias, q_norm, k_norm, eps, positions, slot_mapping, cos, sin, k_pages, v_pages, nq, nkv, hd, page_size,
+                rotate, q_out)
+
+
+def read_int4(k_pages, v_pages, slots, k_out, v_out, nkv: int, hd: int, page_size: int) -> None:
+    """What slots of a cache held in 4 bits stand for: ``k_out`` and ``v_out`` [n, nkv, hd] (float32 or bfloat16) for ``slots`` int32 [n]; a slot
+    of -1 reads as zeros."""
+    if min(nkv, hd, page_size) <= 0:
+        raise KernelError("read_int4: heads, head size and page size must be positive")
+    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd), torch.uint8)
+    for t in (k_out, v_out):
+        if tuple(t.shape) != (slots.numel(), nkv, hd) or t.dtype != k_out.dtype:
+            raise KernelError("k_out and v_out must be [slots, nkv, hd] of one element type")
+    _check(_fn("stride_int4_read")(k, v, _here(slots, "slots", torch.int32), _here(k_out, "k_out"), _here(v_out, "v_out"), slots.numel(), nkv, hd,
+                                   page_size, pages, _code(k_out.dtype), _status_ptr(k_out.device), _stream()), "read_int4")
+
+
+def _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap, dtype=None) -> tuple:
+    """(q, out, keys, values, number of pages) of the attention kernels over a cache held in 4 bits, checked."""
+    if min(nq, nkv, hd, page_size) <= 0 or nq % nkv:
+        raise KernelError(f"{nq} query heads of {hd} do not group into {nkv} key heads")
+    if window < 0 or softcap < 0:
+        raise KernelError("a window or a cap on scores is not below zero")
+    tokens = out.shape[0]
+    if out.dim() != 2 or out.shape[1] != nq * hd or out.dtype != q.dtype:
+        raise KernelError("attention output has the wrong width or element type")
+    if q_stride < nq * hd or (tokens and q.numel() < (tokens - 1) * q_stride + nq * hd):
+        raise KernelError("q is too small for its rows")
+    if block_table.dim() != 2:
+        raise KernelError("block_table must be [requests, pages]")
+    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd), torch.uint8)
+    return _here(q, "q", dtype), _here(out, "out", dtype), k, v, pages
+
+
+def _covers(t, name: str, count: int) -> int:
+    if t.numel() < count:
+        raise KernelError(f"{name} must cover {count} entries, got {t.numel()}")
+    return _here(t, name, torch.int32)
+
+
+def paged_attention_int4(q, q_stride: int, out, k_pages, v_pages, block_table, seq_of_token, positions, nq: int, nkv: int, hd: int, page_size: int,
+                         scale: float, window: int = 0, softcap: float = 0.0, sinks=None, slopes=None) -> None:
+    """``paged_attention`` over pages held in 4 bits: any mix of rows, any head size up to 256, float32 or bfloat16. The exact kernel: the
+    result of a row has the same bits however the work is cut."""
+    qp, op, k, v, pages = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap)
+    tokens = out.shape[0]
+    _check(_fn("stride_attention_int4_exact")(
+        qp, q_stride, op, k, v, pages, _here(block_table, "block_table", torch.int32), block_table.shape[1],
+        _covers(seq_of_token, "seq_of_token", tokens), _covers(positions, "positions", tokens), tokens, nq, nkv, hd, page_size, float(scale), int(window),
+        float(softcap), _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32), _code(q.dtype),
+        _status_ptr(q.device), _stream()), "paged_attention_int4")
+
+
+def decode_int4_scratch_floats(tokens: int, nq: int, nkv: int, hd: int, max_context: int) -> int:
+    """float32 elements of scratch that ``paged_attention_decode_int4`` needs for these sizes."""
+    return 1
+
+
+def paged_attention_decode_int4(q, q_stride: int, out, k_pages, v_pages, block_table, seq_of_token, positions, scratch, nq: int, nkv: int, hd: int,
+                                page_size: int, scale: float, window: int, max_context: int, softcap: float = 0.0, sinks=None, slopes=None) -> None:
+    """``paged_attention_decode`` over pages held in 4 bits: one query per row, bfloat16, head sizes 64 and 128."""
+    paged_attention_int4(q, q_stride, out, k_pages, v_pages, block_table, seq_of_token, positions, nq, nkv, hd, page_size, scale, window, softcap, sinks,
+                         slopes)
+
+
+INT4_EXPANDED_PAGE = 64     # keys of a page of the expanded keys and values
+
+
+def _int4_expanded_pages(num_seqs: int, keys: int) -> int:
+    """Pages for ``keys`` keys of ``num_seqs`` requests, up to the next quarter of a power of two: few sizes, for the copies' descriptors."""
+    need = max(32, -(-keys // INT4_EXPANDED_PAGE) + num_seqs)
+    step = 1 << max(0, need.bit_length() - 3)
+    return -(-need // step) * step
+
+
+def prefill_int4_scratch_ints(num_seqs: int, keys: int, nkv: int, hd: int) -> int:
+    """int32 elements of scratch that ``paged_attention_prefill_int4`` needs for ``num_seqs`` requests that hold at most ``keys`` keys together."""
+    pages = _int4_expanded_pages(num_seqs, keys)
+    return pages * nkv * INT4_EXPANDED_PAGE * hd + num_seqs * pages
+
+
+def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_table, q_start, q_len, ctx_len, scratch, num_seqs: int, keys: int,
+                                 nq: int, nkv: int, hd: int, page_size: int, scale: float, window: int, softcap: float = 0.0, sinks=None, slopes=None,
+                                 precise_cap: bool = False) -> None:
+    """``paged_attention_prefill_tc`` over pages held in 4 bits, for the first ``num_seqs`` requests of the step (portions of any length), which own
+    the rows of ``out``: bfloat16, head sizes 64 and 128. ``keys``: at least what those requests hold together; ``scratch``: int32, at least
+    ``prefill_int4_scratch_ints`` elements, for one stream at a time. The keys and values that the portions see are expanded once, to pages
+    of 64 in bfloat16 (a rounding of 2^-9 of an entry, as a bfloat16 cache has it), and attended to from there."""
+    qp, op, k, v, pages = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap, torch.bfloat16)
+    if not fast_attention_supported(q.dtype, nq, nkv, hd):
+        raise KernelError(f"paged_attention_prefill_int4: {nq} heads of {hd} on {nkv} are not supported (paged_attention_int4 takes them)")
+    if num_seqs < 0 or keys < 0 or scratch.numel() < prefill_int4_scratch_ints(num_seqs, keys, nkv, hd):
+        raise KernelError("paged_attention_prefill_int4: the scratch is too small for the requests and keys")
+    tokens = out.shape[0]
+    if tokens == 0 or num_seqs == 0:
+        return
+    out_pages = _int4_expanded_pages(num_seqs, keys)
+    if block_table.shape[0] < num_seqs:
+        raise KernelError("block_table must have a row a request")
+    half = out_pages * nkv * INT4_EXPANDED_PAGE * hd * 2
+    wide_k = _here(scratch, "scratch", torch.int32)
+    wide_v, table = wide_k + half, wide_k + 2 * half
+    starts, lens, held = (_covers(t, name, num_seqs) for t, name in ((q_start, "q_start"), (q_len, "q_len"), (ctx_len, "ctx_len")))
+    sink, slope = _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32)
+    status, stream = _status_ptr(q.device), _stream()
+    _check(_fn("stride_int4_expand")(k, v, pages, _here(block_table, "block_table", torch.int32), block_table.shape[1], lens, held, num_seqs, nkv, hd,
+                                     page_size, int(window), wide_k, wide_v, table, out_pages, status, stream), "paged_attention_prefill_int4")
+    _check(_fn("stride_paged_prefill_attention_tc")(
+        qp, q_stride, op, wide_k, wide_v, out_pages, table, out_pages, starts, lens, held, num_seqs, tokens, nq, nkv, hd, INT4_EXPANDED_PAGE, float(scale),
+        int(window), -float(softcap) if precise_cap else float(softcap), sink, slope, None, 0, status, stream), "paged_attention_prefill_int4")
+
+
+# ------------------------------------------------------------------- copies of pages
+def copy_pages(pools, src, dst) -> None:
+    """Page ``dst[i]`` of every pool becomes page ``src[i]``, in all its layers. ``pools``: tensors [layers, num_pages, ...]; ``src`` and ``dst``:
+    page numbers (sequences of ints). A page is copied from or to, not both, and to at most once. A captured graph keeps the pairs it was
+    captured with."""
+    src, dst = [int(p) for p in src], [int(p) for p in dst]
+    if len(src) != len(dst):
+        raise KernelError("copy_pages: every page copied from goes with one copied to")
+    targets = set(dst)
+    if len(targets) != len(dst):
+        raise KernelError("copy_pages: a page is copied to twice")
+    if not targets.isdisjoint(src):
+        raise KernelError("copy_pages: a page is copied from and to")
+    for t in pools:
+        if t.dim() < 3:
+            raise KernelError(f"copy_pages: a pool is [layers, num_pages, ...], got {tuple(t.shape)}")
+        if src and not (0 <= min(min(src), min(dst)) and max(max(src), max(dst)) < t.shape[1]):
+            raise KernelError(f"copy_pages: a page lies outside a pool of {t.shape[1]}")
+    at = [_here(t, "pool") for t in pools]
+    if not src or not at:
+        return
+    n = len(at)
+    sizes = [t.stride(1) * t.element_size() if t.shape[1] > 1 else t[0].numel() * t.element_size() for t in pools]
+    _check(_fn("stride_copy_pages")((c_longlong * n)(*at), (c_int * n)(*[t.shape[0] for t in pools]), (c_int * n)(*[t.shape[1] for t in pools]),
+                                    (c_longlong * n)(*sizes), n, (c_int * len(src))(*src), (c_int * len(dst))(*dst), len(src), _stream()), "copy_pages")
 
 
 # --------------------------------------------------------------------- sampling

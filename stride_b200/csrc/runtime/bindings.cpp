@@ -90,6 +90,15 @@ PYBIND11_MODULE(_runtime, m) {
         .def("pages_for", &CacheManager::pages_for)
         .def("has", &CacheManager::has)
         .def("open", &CacheManager::open, py::arg("request"), py::arg("tenant") = "default")
+        .def("fork",
+             [](CacheManager& c, RequestKey parent, RequestKey child, size_t num_tokens) {
+                 auto copies = c.fork(parent, child, num_tokens);
+                 py::list out;
+                 for (auto& x : copies) out.append(py::make_tuple(x.group, x.from, x.to));
+                 return py::make_tuple(out, py::make_tuple(c.state_slot(parent), c.state_slot(child)));
+             },
+             py::arg("parent"), py::arg("child"), py::arg("num_tokens"),
+             "Opens `child` with the parent's first tokens. Returns ([(group, page to copy, page to copy to)], (the parent's state slot, the child's)).")
         .def("adopt_prefix", &CacheManager::adopt_prefix)
         .def("ensure", &CacheManager::ensure, py::arg("request"), py::arg("num_tokens"), py::arg("reserve") = 0)
         .def("pages_missing", &CacheManager::pages_missing)

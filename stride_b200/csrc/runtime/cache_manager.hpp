@@ -89,6 +89,49 @@ public:
         return requests_.at(r).state_slot;
     }
 
+    // A page to be copied on the device.
+    struct PageCopy {
+        size_t group;
+        PageId from, to;
+    };
+
+    // Registers request `child` with the first `num_tokens` tokens of request `parent`: pages that these fill are shared, a page that they
+    // fill in part gets a copy of its own (the caller copies it on the device, and the state slots). All or nothing.
+    std::vector<PageCopy> fork(RequestKey parent, RequestKey child, size_t num_tokens) {
+        if (requests_.count(child)) throw std::invalid_argument("request " + std::to_string(child) + " already holds cache");
+        const RequestPages from = entry(parent);        // a copy: the map may move when the child is added
+        const size_t whole = num_tokens / page_size_, need = pages_for(num_tokens);
+        for (size_t g = 0; g < groups_.size(); ++g) {
+            if (from.tables[g].size() < need)
+                throw std::invalid_argument("request " + std::to_string(parent) + " holds fewer than " + std::to_string(num_tokens) + " tokens");
+            // the child's next query reads the last `window` keys: a page that the parent's window has passed since is gone
+            const size_t w = groups_[g].window, first = w == 0 || num_tokens + 1 <= w ? 0 : (num_tokens + 1 - w) / page_size_;
+            for (size_t i = first; i < need; ++i)
+                if (from.tables[g][i] < 0)
+                    throw std::invalid_argument("request " + std::to_string(parent) + " has given back pages that " + std::to_string(num_tokens) +
+                                                " tokens read");
+        }
+        for (auto& pool : pools_)
+            if (need > whole && pool.num_allocatable() < 1) throw OutOfPages(1, 0);
+        open(child, from.tenant);
+        RequestPages& e = entry(child);
+        std::vector<PageCopy> copies;
+        for (size_t g = 0; g < groups_.size(); ++g) {
+            for (size_t i = 0; i < whole; ++i) {
+                const PageId p = from.tables[g][i];
+                if (p >= 0) pools_[g].retain(p);
+                e.tables[g].push_back(p);
+            }
+            if (need > whole) {
+                e.tables[g].push_back(pools_[g].allocate(1)[0]);
+                copies.push_back({g, from.tables[g][whole], e.tables[g].back()});
+            }
+            e.trimmed[g] = std::min(from.trimmed[g], need);
+        }
+        e.shared_prefix_tokens = std::min(from.shared_prefix_tokens, whole * page_size_);
+        return copies;
+    }
+
     // Looks the tokens up in the prefix index and puts the pages found at the
     // head of the (still empty) table. Returns the number of tokens covered.
     size_t adopt_prefix(RequestKey r, const std::vector<TokenId>& tokens) {

@@ -175,6 +175,12 @@ public:
         }
     }
 
+    // One more reference to a page that somebody holds.
+    void retain(PageId p) {
+        if (refcount_.at(p) == 0) throw InvariantError("page " + std::to_string(p) + " shared while nobody holds it");
+        ++refcount_[p];
+    }
+
     // Drop one reference per page, last page first. A page that reaches zero
     // becomes cached if it is indexed, free otherwise.
     void release(const std::vector<PageId>& pages) {

@@ -99,12 +99,14 @@ class Engine:
         token_cap = self.cfg.max_batch_tokens
         row_cap = min(self.cfg.max_batch_seqs, token_cap)
         if model is not None:
-            self.model_config, self.model = load_model(model, self.cfg.dtype, device, token_cap, row_cap)
+            self.model_config, self.model = load_model(model, self.cfg.dtype, device, token_cap, row_cap,
+                                                          cache_dtype=self.cfg.cache_dtype)
         elif config is not None:
             self.model_config = config_from_dict(config) if isinstance(config, dict) else config
             if random_weights is None:
                 raise ValueError("a configuration without a model folder needs random_weights=<seed>")
-            self.model = random_model(self.model_config, random_weights, self.cfg.dtype, device, token_cap, row_cap)
+            self.model = random_model(self.model_config, random_weights, self.cfg.dtype, device, token_cap, row_cap,
+                                      cache_dtype=self.cfg.cache_dtype)
         else:
             raise ValueError("give a model folder or a configuration")
         spec = self.model.spec
@@ -315,6 +317,17 @@ class Engine:
         for key, tokens, position, want in work:
             batch.add(int(key), [int(t) for t in tokens], int(position), [int(w) for w in want])
         return self.runner.step(batch)
+
+    def fork(self, parent: int, child: int, num_tokens: int) -> None:
+        """Opens request ``child`` (a key like those of ``forward``) with the first ``num_tokens`` tokens of request ``parent``: whole
+        pages are shared, a page in part is copied, the state of mixers that keep some is copied as it stands, so with such mixers
+        ``num_tokens`` is what the parent has run. The caller manages both requests' pages from there on."""
+        if self._ahead is not None:
+            raise RuntimeError("a step of the engine's own requests is in flight; call step() until they are done")
+        copies, state = self.cache.fork(int(parent), int(child), int(num_tokens))
+        for group, src, dst in copies:
+            self.device_cache.copy_pages(group, [src], [dst])
+        self.device_cache.copy_state(*state)
 
     def get_weight(self, name: str) -> torch.Tensor:
         return self.model.get_weight(name)

@@ -16,10 +16,10 @@ from ..parts import DecoderModel, Runtime
 from ..weights import RandomSource, SafetensorsSource, save_file
 
 
-def build_model(config, source, dtype: str, device="cuda", token_capacity: int = 2048, row_capacity: int = 256):
-    """``config``: a typed configuration (anything with ``to_model_spec``)."""
+def build_model(config, source, dtype: str, device="cuda", token_capacity: int = 2048, row_capacity: int = 256, cache_dtype: str | None = None):
+    """``config``: a typed configuration (anything with ``to_model_spec``). ``cache_dtype``: ``int4`` for pages held in 4 bits."""
     ops.require_device()
-    runtime = Runtime(device, DTYPES[dtype], token_capacity, row_capacity)
+    runtime = Runtime(device, DTYPES[dtype], token_capacity, row_capacity, cache_dtype)
     model = DecoderModel(config.to_model_spec(), runtime)
     if source is None:
         raise ValueError("a weight source is needed")
@@ -36,7 +36,7 @@ def read_config(model_dir: str, source=None):
 
 
 def load_model(model_dir: str, dtype: str = "bfloat16", device="cuda", token_capacity: int = 2048, row_capacity: int = 256,
-               min_positions: int = 0):
+               min_positions: int = 0, cache_dtype: str | None = None):
     """``min_positions``: position tables for at least this many positions, where the configuration can give them
     (``with_max_positions``), even if the checkpoint names a shorter length."""
     source = SafetensorsSource(model_dir)
@@ -44,15 +44,15 @@ def load_model(model_dir: str, dtype: str = "bfloat16", device="cuda", token_cap
     spec_positions = getattr(config, "max_position_embeddings", None)
     if min_positions and spec_positions is not None and spec_positions < min_positions and hasattr(config, "with_max_positions"):
         config = config.with_max_positions(min_positions)
-    return config, build_model(config, source, dtype, device, token_capacity, row_capacity)
+    return config, build_model(config, source, dtype, device, token_capacity, row_capacity, cache_dtype)
 
 
 def random_model(config, seed: int, dtype: str = "bfloat16", device="cuda", token_capacity: int = 2048,
-                 row_capacity: int = 256, std: float = 0.02, vector_jitter: float = 0.0):
+                 row_capacity: int = 256, std: float = 0.02, vector_jitter: float = 0.0, cache_dtype: str | None = None):
     """Random weights drawn on the device, through the same declarations and
     checks as a checkpoint."""
     ops.require_device()
-    runtime = Runtime(device, DTYPES[dtype], token_capacity, row_capacity)
+    runtime = Runtime(device, DTYPES[dtype], token_capacity, row_capacity, cache_dtype)
     model = DecoderModel(config.to_model_spec(), runtime)
     source = RandomSource(model.declare(), seed, std=std, vector_jitter=vector_jitter, stored_dtype=DTYPES[dtype],
                           device=str(runtime.device))
@@ -82,7 +82,7 @@ def _declarations(config) -> dict:
     return DecoderModel(config.to_model_spec(), runtime).declare()
 
 
-def footprint(config, dtype: str = "bfloat16") -> dict:
+def footprint(config, dtype: str = "bfloat16", cache_dtype: str | None = None) -> dict:
     """What a model of this configuration needs in bytes, read from its own parts without touching a device: the
     declared tensors (matrices in the compute dtype, vectors and tables in 32 bits, as the loader keeps them),
     what its mixers keep per token in pages, and the state of fixed size per request. Works for any registered
@@ -91,10 +91,10 @@ def footprint(config, dtype: str = "bfloat16") -> dict:
 
     from ..cache import plan_groups
     item = torch.empty((), dtype=DTYPES[dtype]).element_size()
-    model = DecoderModel(config.to_model_spec(), Runtime("meta", DTYPES[dtype], 1, 1))
+    model = DecoderModel(config.to_model_spec(), Runtime("meta", DTYPES[dtype], 1, 1, cache_dtype))
     weights = sum(math.prod(d.shape) * (item if d.role == "matrix" else 4) for d in model.declare().values() if not d.optional)
     requests = model.cache_requests()
-    per_token = sum(g.elements_per_token() for g in plan_groups(requests)) * item
+    per_token = sum(g.bytes_per_token(item) for g in plan_groups(requests))
     state = sum(math.prod(s.shape) * torch.empty((), dtype=s.dtype).element_size() for _r, s in requests if s is not None)
     return {"weight_bytes": int(weights), "kv_bytes_per_token": int(per_token), "state_bytes_per_request": int(state)}
 

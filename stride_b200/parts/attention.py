@@ -37,7 +37,9 @@ Spec params, all optional:
   before a request's start. The last n - 1 projected rows of a request are its state (one float32 row in a state slot).
 * ``qk_norm`` ``weighted``: every query and key head goes through an RMS norm with a weight of the head's size shared by the
   heads (tensors ``q.norm``, ``k.norm``; ``norm_eps`` inside the root), after the convolution. One kernel does the
-  convolution, the norms and the write into the pages; a second one moves the tails on.
+  convolution, the norms and the write into the pages; a second one moves the tails on. Without a convolution the norms go with any
+  rotation, which comes behind them, with biases, and with the long names (``q_norm.weight``, ``k_norm.weight``): one kernel adds
+  the biases, norms, turns and writes the pages.
 * ``qk_norm`` ``rows``: an RMS norm over a token's whole query projection and one over its whole key projection (tensors ``q.norm``
   [heads * head_dim], ``k.norm`` [kv_heads * head_dim]), after the convolution, before the heads are told apart.
 * ``query_factor`` (coef, every), with ``qk_norm`` ``rows``: the query at position p is multiplied by
@@ -49,6 +51,10 @@ Spec params, all optional:
 * ``sinks`` ``zero``: no tensor; every head's denominator gains exp(0) = 1.
 * ``borrowed_kv``: the mixer has no key and value projections and reads the pages of the cache slot it is given, which
   another layer's mixer of the same shape writes.
+
+A runtime whose ``cache_dtype`` is ``int4`` holds the pages in 4 bits: the kernel that turns (and norms) queries and keys writes them so, and
+the attention kernels read them so. It goes with a rotation or none (with weighted head norms or none), windows, caps, sinks, slopes, gates
+and values taken from keys.
 
 When the position part asks for another order of a head's entries (``head_permutation``), the rows of the query and
 key projections (and of whatever else must follow them: values taken from keys, the gate, the columns of the output
@@ -136,7 +142,9 @@ class PagedAttention(Mixer):
         # what the plain path (projection, then the position part's rotation and cache write) cannot do goes through
         # the head-norm kernel, which adds the bias, norms and writes the pages itself when there is no rotation
         self.plain_position = s.position is None or s.position.kind == "none"
-        self.conv_path = self.taps > 0 or self.weighted_qk or self.row_norm
+        self.int4 = runtime.cache_dtype == "int4"
+        self.normed = self.weighted_qk and not self.taps and (self.int4 or not self.plain_position or not self.short_names)
+        self.conv_path = self.taps > 0 or (self.weighted_qk and not self.normed) or self.row_norm
         if self.conv_path and (self.unit_qk or self.unit_v or self.borrows or s.bias or self.head_gate or not self.plain_position
                                or not self.short_names or self.taps > 16):
             raise ValueError("a convolution, weighted head norms or norms over whole projections go with no rotation, no biases, no unit norms, no borrowed pages, "
@@ -153,6 +161,12 @@ class PagedAttention(Mixer):
             if size and 2 * size <= 2 * (self.hd + self.vd) and ops.fast_attention_supported(runtime.dtype, self.nq, self.nkv, size):
                 self.hd = self.vd = size
                 self.q_dim, self.kv_dim = self.nq * size, self.nkv * size
+        if self.normed and (self.own_prepare or self.values_are_keys):
+            raise ValueError("weighted head norms behind no convolution go with no other norms, no value width of their own, no borrowed pages and no "
+                             "values taken from keys")
+        if self.int4 and (self.own_prepare or self.buckets):
+            raise ValueError("keys and values in 4 bits go with no convolution, no unit norms and norms over whole projections, no value width of their "
+                             "own, no borrowed pages and no distance table")
         if self.own_prepare and not self.unit_rotated and not self.plain_position and (self.vd != self.hd or self.borrows):
             raise ValueError("a rotation with borrowed pages or a value width of its own is not supported")
         self.fused_gate = self.head_gate and self.own_prepare and self.plain_position
@@ -170,6 +184,7 @@ class PagedAttention(Mixer):
         if self.zero_sinks:
             self.sinks = torch.zeros(self.nq, dtype=torch.float32, device=runtime.device)
         self._fast = ops.fast_attention_supported(runtime.dtype, self.nq, self.nkv, self.hd) and self.vd == self.hd
+        self.sizes_by_context = self.int4 and self._fast        # a portion's keys are expanded
         self.accepts_folded = not self.gated          # the gate reads the normed input as a tensor
 
     # ----------------------------------------------------------------- weights
@@ -182,6 +197,9 @@ class PagedAttention(Mixer):
         w["g"], w["sink"] = p + "g", p + "sink"
         b["o"] = f"{p}o.b" if self.short_names else f"{p}o_proj.bias"
         return w, b
+
+    def _norm_name(self, n):
+        return f"{self.spec.prefix}{n}.norm" if self.short_names else f"{self.spec.prefix}{n}_norm.weight"
 
     def declare(self):
         w, b = self._names()
@@ -209,7 +227,7 @@ class PagedAttention(Mixer):
         if self.taps:
             d.update({f"{p}{n}.conv": TensorDecl((rows, self.taps), "vector") for n, rows in (("q", self.q_dim), ("k", self.kv_dim), ("v", self.v_dim))})
         if self.weighted_qk:
-            d.update({f"{p}{n}.norm": TensorDecl((self.hd,), "vector") for n in "qk"})
+            d.update({self._norm_name(n): TensorDecl((self.hd,), "vector") for n in "qk"})
         if self.row_norm:
             d.update({p + "q.norm": TensorDecl((self.q_dim,), "vector"), p + "k.norm": TensorDecl((self.kv_dim,), "vector")})
         if self.buckets:
@@ -266,8 +284,13 @@ class PagedAttention(Mixer):
             self.w_gate = self._reorder(weights[w["g"]]) if self.values_are_keys else weights[w["g"]]
         if self.has_sinks:
             self.sinks = weights[w["sink"]]
+        if self.normed:     # entries in the order of the heads'
+            self.wq_norm, self.wk_norm = (t if self.perm is None else t[self.perm.to(t.device)].contiguous()
+                                          for t in (weights[self._norm_name(n)] for n in "qk"))
         self._bind_rel(weights)
         self.position.bind(weights)
+        if (self.normed or self.int4) and self.position.rotation_tables() is None:
+            raise ValueError(f"head norms and a cache in 4 bits go with a position part that turns by tables, not with {self.spec.position.kind!r}")
 
     def _bind_own(self, weights, w, b):
         """The fused projection of the head-norm path: query rows, then key and value rows unless they are borrowed,
@@ -356,6 +379,9 @@ class PagedAttention(Mixer):
             out[w["sink"]] = self.sinks
         if self.has_output_bias:
             out[b["o"]] = self.output_bias
+        if self.normed:
+            for n, t in (("q", self.wq_norm), ("k", self.wk_norm)):
+                out[self._norm_name(n)] = t if self.perm is None else t[torch.argsort(self.perm).to(t.device)]
         if self.buckets:
             out[self.spec.prefix + "rel"] = self.stored_rel
         out.update(self.position.named_tensors())
@@ -363,6 +389,9 @@ class PagedAttention(Mixer):
 
     # ------------------------------------------------------------------- cache
     def cache_request(self):
+        if self.int4:
+            row = ops.int4_row_bytes(self.hd)
+            return CacheRequest(window=self.spec.window, tensors=(("k", self.nkv, row), ("v", self.nkv, row)), dtype=torch.uint8)
         if self.vd != self.hd:
             return CacheRequest(window=self.spec.window, tensors=(("k", self.nkv, self.hd), ("v", self.nkv, self.vd)))
         return CacheRequest(self.nkv, self.hd, self.spec.window)
@@ -392,6 +421,15 @@ class PagedAttention(Mixer):
                 x = folded.tensor()
             ops.linear(x, self.w_qkv, qkv)
             self._norm_and_store(qkv, ctx, cache, tokens)
+        elif self.normed or self.int4:
+            if folded:
+                x = folded.tensor()
+            ops.linear(x, self.w_qkv, qkv)
+            cos, sin, rotate = self.position.rotation_tables()
+            write = ops.rope_kv_write_int4 if self.int4 else ops.qk_norm_rope_write
+            write(qkv, self.bias, self.wq_norm, self.wk_norm, self.norm_eps, ctx.positions[:tokens],
+                  ctx.slot_mapping[cache.group][:tokens] if cache.writes else None, cos, sin, cache.k_pages, cache.v_pages, self.nq, self.nkv, self.hd,
+                  cache.page_size, rotate)
         elif not self._project_and_rotate(folded.xt if folded else x, qkv, ctx, cache, tokens, folded):
             if folded:
                 x = folded.tensor()
@@ -478,6 +516,9 @@ class PagedAttention(Mixer):
         gates' logits stand in the rows of ``qkv`` and the decode kernel took the rows after the portions)."""
         table = ctx.block_table[cache.group]
         geometry = (self.nq, self.nkv, self.hd, cache.page_size, self.scale, self.window)
+        if self.int4:
+            self._attend_int4(qkv, attn, table, ctx, cache, tokens, geometry)
+            return tokens
         if not self._fast:
             # the exact kernel: the whole 32-bit path, and bfloat16 sizes the tensor-core kernels refuse
             split = min(ctx.decode_tail_start, tokens) if qkv.dtype == torch.float32 else 0     # portions before, single tokens after
@@ -505,6 +546,24 @@ class PagedAttention(Mixer):
                                        self.q_dim + self.kv_cols if self.fused_gate else -1, self.rel, self.precise_cap)
             return split if self.fused_gate else tokens
         return tokens
+
+
+    def _attend_int4(self, qkv, attn, table, ctx, cache, tokens, geometry):
+        pages, rules = (cache.k_pages, cache.v_pages, table), (self.softcap, self.sinks, self.slopes)
+        split = min(ctx.decode_tail_start, tokens) if self._fast else tokens        # portions before, single decoded tokens after
+        if not self._fast or (split > 0 and not ctx.portion_keys):
+            # the exact kernel: the whole 32-bit path, sizes the tensor-core kernels refuse, and a step that does not say what its portions hold
+            ops.paged_attention_int4(qkv[:split], self.qkv_dim, attn[:split], *pages, ctx.seq_of_token[:split], ctx.positions[:split], *geometry, *rules)
+        elif split > 0:
+            seqs, keys = ctx.decode_tail_seq, ctx.portion_keys
+            scratch = self.rt.scratch("int4_expanded", ops.prefill_int4_scratch_ints(seqs, keys, self.nkv, self.hd), torch.int32)
+            ops.paged_attention_prefill_int4(qkv[:split], self.qkv_dim, attn[:split], *pages, ctx.q_start, ctx.q_len, ctx.ctx_len, scratch, seqs, keys,
+                                             *geometry, *rules, self.precise_cap)
+        if tokens > split:
+            n = tokens - split
+            scratch = self.rt.scratch("attention_splits_int4", ops.decode_int4_scratch_floats(n, self.nq, self.nkv, self.hd, ctx.context_bound))
+            ops.paged_attention_decode_int4(qkv[split:tokens], self.qkv_dim, attn[split:tokens], *pages, ctx.seq_of_token[split:tokens],
+                                            ctx.positions[split:tokens], scratch, *geometry, ctx.context_bound, *rules)
 
 
 register_part("mixer", "attention", PagedAttention)

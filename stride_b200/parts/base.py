@@ -67,13 +67,14 @@ class CacheRequest:
     The plain form is keys and values of one shape: ``CacheRequest(num_kv_heads, head_dim, window)``. A mixer
     that keeps something else names its tensors: ``CacheRequest(tensors=(("latent", 1, 24),))`` keeps one vector
     of 24 numbers per token; ``(("k", 4, 64), ("v", 4, 32))`` keys and values of different widths. Every tensor
-    of a request is laid out [num_pages, heads, page_size, width] in the compute dtype and shares the request's
-    page ids, so one block table and one slot mapping serve them all.
+    of a request is laid out [num_pages, heads, page_size, width] and shares the request's page ids, so one block table
+    and one slot mapping serve them all. ``dtype``: the tensors' element type (None: the compute dtype).
     """
     num_kv_heads: int = 0
     head_dim: int = 0
     window: Optional[int] = None     # None: every token is kept
     tensors: tuple = ()              # of (name, heads, width); empty: ("k", ...) and ("v", ...) of the plain form
+    dtype: Optional[torch.dtype] = None
 
     def layout(self) -> tuple:
         if self.tensors:

@@ -51,6 +51,10 @@ class DecoderModel:
             if getattr(e, "enters_pass", None) is not None and self.pass_input is None:
                 raise ValueError("a schedule entry starts a pass, but the model has no pass input")
         self.caches = None          # list of LayerCache, one per schedule entry; set by DeviceCache.attach
+        if runtime.cache_dtype is not None:
+            for request, _state in self.cache_requests():
+                if request is not None and request.dtype is None:
+                    raise ValueError(f"a layer keeps {', '.join(n for n, _h, _w in request.layout())} in pages that cannot be held in {runtime.cache_dtype}")
         self.capture = None         # when a list, every run appends the float32 hidden state (diagnostics)
 
     # ----------------------------------------------------------------- weights

@@ -25,9 +25,12 @@ class Runtime:
     # Kinds of the model's mixers (those inside a parallel mixer too), for a part whose form depends on what else the model holds.
     mixer_kinds: frozenset = frozenset()
 
-    def __init__(self, device, dtype: torch.dtype, token_capacity: int, row_capacity: int):
+    def __init__(self, device, dtype: torch.dtype, token_capacity: int, row_capacity: int, cache_dtype: str | None = None):
+        if cache_dtype not in (None, "int4"):
+            raise ValueError(f"the cache is held in the compute dtype (None) or in \"int4\", not in {cache_dtype!r}")
         self.device = torch.device(device)
         self.dtype = dtype
+        self.cache_dtype = cache_dtype      # what mixers keep their pages in: None for ``dtype``
         self.token_capacity = int(token_capacity)
         self.row_capacity = int(row_capacity)
         self._buffers: dict[tuple, torch.Tensor] = {}
