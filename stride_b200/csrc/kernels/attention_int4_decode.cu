@@ -1,0 +1,618 @@
+// Decode attention over a paged cache held in 4 bits (int4_cache.cuh), split over the keys, on the tensor cores.
+//
+// A single query reads every key of its request: the bytes of the cache bound it, 5 bits an entry. So that the work on an entry stays below
+// the time its bytes take, an entry is never turned into a value: numbers go to the matrix instructions as they are, scales and centres are
+// applied to scores and weights, of which there are 32 times fewer.
+//
+//   score(t) = sum_g s_tg (q_g . n_t - 8 sum q_g) + c_tg sum q_g          out = sum_t (P_t s_tg) n_t - 8 sum_t P_t s_tg + sum_t P_t c_tg
+//
+// * A number of 4 bits under the mask 0x000f000f (or 0x00f000f0) is a pair of 16-bit floating point numbers below the smallest normal one: n 2^-24
+//   (or n 2^-20). Matrix instructions take those exactly, so one instruction unpacks two entries. The factors are powers of two: the query's
+//   entries that meet the second kind are divided by 16 beforehand, the outputs of the second kind afterwards.
+// * Keys are the A operand (16 tokens by 16 entries), the 8 columns of B are the group's query heads; the products of a group of 32 entries end in
+//   an accumulator of their own, which starts at -8 sum q_g. Values are the A operand of the second product (16 entries by 16 tokens), the
+//   weights P_t s_tg, rounded once to 16 bits, its B operand: a transpose of 8 x 8 in the warp. What the offset of 8 adds is summed from the same
+//   rounded weights by a product with ones, so it cancels. Centres go through a product of their own in bfloat16, whose three-part sums of the
+//   query are exact.
+// * The query is scaled by a power of two to below 2^15. The reference R of a weight 2^(score - R) is the running maximum of score + log2 of the
+//   token's largest scale or centre, so that what is rounded to 16 bits lies below 2^8 and its largest above 2^-1 whatever the values' size;
+//   R moves only when a product passes 2^8 (a vote per tile), and then everything is rescaled.
+//
+// A warp owns tiles of 16 keys and a ring of copies: one bulk copy for the tile's keys and one for its values where pages hold whole tiles
+// (a page's rows of one head lie side by side), 16- or 8-byte copies by all lanes otherwise. Splits are merged as in attention_decode.cu, by the
+// CTA that draws the last ticket.
+#include "int4_cache.cuh"
+#include "mma.cuh"
+#include "tcgen05.cuh"      // mbarrier helpers
+
+namespace stride {
+namespace four {
+
+constexpr int kTile = 16;               // keys of a warp's tile
+constexpr int kWarps = 4;
+constexpr int kUnit = kTile * kWarps;   // keys that a CTA's warps cover with a tile each
+constexpr int kStages = 4;
+constexpr int kMaxTiles = 32;           // of a warp: a lane looks each one's page up
+constexpr int kTicketInts = 65536;      // ticket counters at the start of the scratch, one per (token, key head)
+constexpr int kCodeBeyondBound = 32;    // as in attention_decode.cu
+constexpr int kCodeCopyWait = 81;       // a wait for a tile's copies ran out
+constexpr float kLimit = 256.f;         // what a weight's product with a scale or centre may reach before R moves
+constexpr float kLeastLog = -90.f;      // log2 of the least scale or centre that R counts: a weight stays below 2^98
+
+struct Decode {
+    const __nv_bfloat16* q;
+    __nv_bfloat16* out;
+    const uint8_t* k_pages;
+    const uint8_t* v_pages;
+    const int32_t* table;
+    const int32_t* seq_of_token;
+    const int32_t* positions;
+    const float* sinks;
+    const float* slopes;
+    float* part_o;          // [token][head][split][hd]
+    float* part_ml;         // [token][head][split][2]: R, sum of weights
+    int* tickets;
+    int* status;
+    int q_stride, table_width, num_pages, nq, nkv, page_size, window, split_keys, num_splits;
+    float scale_log2e, cap_log2e, scale_over_cap;        // cap_log2e 0: no cap
+};
+
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void small_copy(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+// D = A B + C, 16-bit floating point (or bfloat16) inputs, 32-bit accumulators.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The transpose of an 8 x 8 matrix of 16-bit entries: lane l holds entries 2 (l % 4) and the next of row l / 4.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t y;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+__device__ __forceinline__ float exp2_quick(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int G>
+__device__ __forceinline__ void load_words(uint32_t (&w)[G], const void* p) {       // G words from shared memory, 4 G bytes aligned
+    if constexpr (G == 4) {
+        const uint4 v = *static_cast<const uint4*>(p);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+        const uint2 v = *static_cast<const uint2*>(p);
+        w[0] = v.x; w[1] = v.y;
+    }
+}
+// The token of a tile that stands in row r of the score tile: an order in which the lanes that read together find their rows in different banks
+// (rows are 20 G bytes apart).
+template <int G>
+__device__ __forceinline__ int token_of(int r) {
+    return G == 4 ? (r & 8) + (r & 1) * 4 + ((r & 7) >> 1) : (r & 3) * 4 + (r >> 2);
+}
+// The largest of the scales and of the centres' sizes in a row's parameters.
+template <int G>
+__device__ __forceinline__ float amplitude(const uint32_t (&p)[G]) {
+    __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&p[0]));
+#pragma unroll
+    for (int g = 1; g < G; ++g) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&p[g])));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+
+// G: groups of a head (head size 32 G). NT: tiles of 8 query heads.
+template <int G, int NT, bool BULK>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(const Decode a) {
+    constexpr int HD = 32 * G, ROW = 20 * G, TILE = kTile * ROW;
+    pdl_trigger();
+    pdl_wait();
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) uint64_t bars[kWarps][kStages];
+    const int split = blockIdx.x, kvh = blockIdx.y, t = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int group = a.nq / a.nkv, seq = a.seq_of_token[t], pos = seq < 0 ? 0 : a.positions[t];
+    __nv_bfloat16* out = a.out + (static_cast<size_t>(t) * a.nq + kvh * group) * HD;
+    if (seq < 0 || pos >= a.num_splits * a.split_keys) {       // a padded row, or one beyond the bound that the launch was sized for: zeros, no ticket
+        if (split == 0) {
+            for (int i = threadIdx.x; i < group * HD; i += blockDim.x) out[i] = __float2bfloat16_rn(0.f);
+            if (seq >= 0 && threadIdx.x == 0) complain(a.status, kCodeBeyondBound);
+        }
+        return;
+    }
+    const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0, lo = split * a.split_keys;
+    if (lo > pos || lo + a.split_keys <= first) return;        // uniform for the CTA
+    const int32_t* table = a.table + static_cast<size_t>(seq) * a.table_width;
+    const int n_tiles = a.split_keys / kUnit;
+    auto tile_base = [&](int j) { return lo + j * kUnit + warp * kTile; };
+    // the bytes at which a key's row of this head lies, or all ones where there is no such page
+    auto row_at = [&](int key) {
+        const int index = key / a.page_size, page = index < a.table_width ? table[index] : -1;
+        if (page < 0 || page >= a.num_pages) {
+            complain(a.status, kCodeNoPage);
+            return ~size_t(0);
+        }
+        return ((static_cast<size_t>(page) * a.nkv + kvh) * a.page_size + key % a.page_size) * ROW;
+    };
+    size_t my_row = ~size_t(0);         // BULK: of the tile with this lane's number
+    bool mine = lane < n_tiles && tile_base(lane) <= pos && tile_base(lane) + kTile > first;
+    if (BULK && mine) {
+        my_row = row_at(tile_base(lane));
+        mine = my_row != ~size_t(0);
+    }
+    const uint32_t live = __ballot_sync(0xffffffffu, mine);
+    unsigned char* ring = smem + warp * kStages * 2 * TILE;
+    if (BULK) {
+        if (lane == 0)
+            for (int s = 0; s < kStages; ++s) tc::mbar_init(tc::smem_u32(&bars[warp][s]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        __syncwarp();
+    }
+    auto issue = [&](int j) {
+        if (BULK) {
+            if (j < n_tiles && lane == j && mine) {
+                const uint32_t dst = tc::smem_u32(ring + (j % kStages) * 2 * TILE), bar = tc::smem_u32(&bars[warp][j % kStages]);
+                tc::mbar_expect_tx(bar, 2 * TILE);
+                bulk_copy(dst, a.k_pages + my_row, TILE, bar);
+                bulk_copy(dst + TILE, a.v_pages + my_row, TILE, bar);
+            }
+            return;
+        }
+        if (j < n_tiles && (live >> j & 1u)) {
+            size_t row = ~size_t(0);
+            const int key = tile_base(j) + lane;
+            if (lane < kTile && key >= first && key <= pos) row = row_at(key);
+            const uint32_t dst = tc::smem_u32(ring + (j % kStages) * 2 * TILE);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {               // 16 rows of 5 pieces
+                const int piece = i * 32 + lane, r = piece / 5, at = piece * 4 * G;
+                const size_t from = __shfl_sync(0xffffffffu, row, r & 15);
+                if (piece < kTile * 5) {
+                    if (from != ~size_t(0)) {
+                        small_copy<4 * G>(dst + at, a.k_pages + from + (piece - r * 5) * 4 * G);
+                        small_copy<4 * G>(dst + TILE + at, a.v_pages + from + (piece - r * 5) * 4 * G);
+                    } else {
+                        for (int b = 0; b < 4 * G; b += 4)
+                            *reinterpret_cast<uint32_t*>(ring + (j % kStages) * 2 * TILE + at + b) =
+                                *reinterpret_cast<uint32_t*>(ring + (j % kStages) * 2 * TILE + TILE + at + b) = 0u;
+                    }
+                }
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) issue(s);
+
+    // ---- the query: lane (g, c) holds, of head 8 nt + g, entries 32 grp + 8 c .. + 7
+    uint32_t qb[NT][G][2][2], cb[NT][2];            // B operands: of the numbers, of the centres
+    float start[NT][G][2], factor[NT][2], slope[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int head = 8 * nt + g;
+        float x[G][8], most = 0.f;
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+            const __nv_bfloat16* src = a.q + static_cast<size_t>(t) * a.q_stride + static_cast<size_t>(kvh * group + head) * HD + 32 * grp + 8 * c;
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (head < group) {
+                if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+                    raw = *reinterpret_cast<const uint4*>(src);
+                } else {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+                    raw = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                }
+            }
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[grp][i] = i & 1 ? bf16_high(w[i >> 1]) : bf16_low(w[i >> 1]);
+                most = fmaxf(most, fabsf(x[grp][i]));
+            }
+        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // times 2^(up - 127), so that the largest entry lies in [2^14, 2^15); a query below 2^-113 keeps what 2^127 makes of it
+        const int up = min(254, 268 - static_cast<int>(__float_as_uint(most) >> 23));
+        const float by = __uint_as_float(static_cast<uint32_t>(up) << 23);
+        float sums[G], own = 0.f;
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[grp][i] *= by;
+                sum += x[grp][i];
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sums[grp] = sum * 5.9604644775390625e-08f;              // in the units of the numbers, 2^-24
+            if ((c % G) == grp && c < G) own = sums[grp];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                qb[nt][grp][m][0] = pack_f16(x[grp][2 * m], x[grp][2 * m + 4]);
+                qb[nt][grp][m][1] = pack_f16(x[grp][2 * m + 1] * 0.0625f, x[grp][2 * m + 5] * 0.0625f);
+            }
+            start[nt][grp][0] = -8.f * __shfl_sync(0xffffffffu, sums[grp], 8 * c);
+            start[nt][grp][1] = -8.f * __shfl_sync(0xffffffffu, sums[grp], 8 * c + 4);
+        }
+        {       // the sum in three parts of 8 bits
+            const float hi = __bfloat162float(__float2bfloat16_rn(own)), mid = __bfloat162float(__float2bfloat16_rn(own - hi));
+            cb[nt][0] = pack_bf16(hi, mid);
+            cb[nt][1] = pack_bf16(own - hi - mid, 0.f);
+        }
+        const float down = __uint_as_float(static_cast<uint32_t>(254 - up) << 23) * ((a.cap_log2e > 0.f ? a.scale_over_cap : a.scale_log2e) * 16777216.f);
+        factor[nt][0] = __shfl_sync(0xffffffffu, down, 8 * c);
+        factor[nt][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            slope[nt][e] = a.slopes != nullptr && 8 * nt + 2 * c + e < group ? a.slopes[kvh * group + 8 * nt + 2 * c + e] * 1.4426950408889634f : 0.f;
+    }
+
+    float R[NT][2], l[NT][2], o[NT][G][2][4], ones[NT][G][4], cen[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        R[nt][0] = R[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            cen[nt][e] = 0.f;
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) ones[nt][grp][e] = o[nt][grp][0][e] = o[nt][grp][1][e] = 0.f;
+        }
+    }
+    const int row_a = token_of<G>(g), row_b = token_of<G>(g + 8);                                   // tokens of this lane's score rows
+    const int col[4] = {token_of<G>(2 * c), token_of<G>(2 * c + 1), token_of<G>(2 * c + 8), token_of<G>(2 * c + 9)};        // of its weights
+    bool alive = true;
+    uint32_t uses = 0;
+    for (int j = 0; j < n_tiles; ++j) {
+        if (BULK) {
+            if ((live >> j & 1u) && alive) {
+                alive = __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&bars[warp][j % kStages]), uses >> (j % kStages) & 1u, a.status, kCodeCopyWait));
+                uses ^= 1u << (j % kStages);
+            }
+        } else {
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+        }
+        if ((live >> j & 1u) && alive) {
+            const unsigned char* ks = ring + (j % kStages) * 2 * TILE;
+            const unsigned char* vs = ks + TILE;
+            const int base = tile_base(j);
+            uint32_t kw[2][G], kp[2][G], vp[2][G], vw[4][G / 2], vc[4];
+            load_words<G>(kw[0], ks + row_a * ROW + c * 4 * G);
+            load_words<G>(kw[1], ks + row_b * ROW + c * 4 * G);
+            load_words<G>(kp[0], ks + row_a * ROW + 16 * G);
+            load_words<G>(kp[1], ks + row_b * ROW + 16 * G);
+            const uint32_t ca = *reinterpret_cast<const uint32_t*>(ks + row_a * ROW + 16 * G + 4 * (c % G)),
+                           cc = *reinterpret_cast<const uint32_t*>(ks + row_b * ROW + 16 * G + 4 * (c % G));
+            load_words<G>(vp[0], vs + row_a * ROW + 16 * G);
+            load_words<G>(vp[1], vs + row_b * ROW + 16 * G);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (G == 4) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(vs + col[i] * ROW + g * 2 * G);
+                    vw[i][0] = v.x;
+                    vw[i][1] = v.y;
+                } else {
+                    vw[i][0] = *reinterpret_cast<const uint32_t*>(vs + col[i] * ROW + g * 2 * G);
+                }
+                vc[i] = *reinterpret_cast<const uint32_t*>(vs + col[i] * ROW + 16 * G + 4 * (g % G));
+            }
+            const bool edge = base + kTile - 1 > pos || base < first;
+            const bool ok_a = base + row_a <= pos && base + row_a >= first, ok_b = base + row_b <= pos && base + row_b >= first;
+            if (edge) {         // rows of the page behind the token, or before its window, may hold anything: their scales and centres count for nothing
+#pragma unroll
+                for (int grp = 0; grp < G; ++grp) {
+                    if (!ok_a) vp[0][grp] = 0u;
+                    if (!ok_b) vp[1][grp] = 0u;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (base + col[i] > pos || base + col[i] < first) vc[i] = 0u;
+            }
+            const float amp[2] = {amplitude<G>(vp[0]), amplitude<G>(vp[1])};
+            float P[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_bf16(x, __byte_perm(ca, ca, 0x3232), __byte_perm(cc, cc, 0x3232), __byte_perm(ca, ca, 0x3232), __byte_perm(cc, cc, 0x3232), cb[nt][0],
+                         cb[nt][1]);
+#pragma unroll
+                for (int grp = 0; grp < G; ++grp) {
+                    float acc[4] = {start[nt][grp][0], start[nt][grp][1], start[nt][grp][0], start[nt][grp][1]};
+                    const uint32_t w0 = kw[0][grp], w1 = kw[1][grp], u0 = w0 >> 8, u1 = w1 >> 8;
+                    mma_f16(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[nt][grp][0][0], qb[nt][grp][0][1]);
+                    mma_f16(acc, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qb[nt][grp][1][0], qb[nt][grp][1][1]);
+                    const float s0 = bf16_low(kp[0][grp]), s1 = bf16_low(kp[1][grp]);
+                    x[0] = fmaf(s0, acc[0], x[0]);
+                    x[1] = fmaf(s0, acc[1], x[1]);
+                    x[2] = fmaf(s1, acc[2], x[2]);
+                    x[3] = fmaf(s1, acc[3], x[3]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] *= factor[nt][e & 1];
+                    if (a.cap_log2e > 0.f) x[e] = a.cap_log2e * tanh_quick(x[e]);
+                    if (a.slopes != nullptr) x[e] = fmaf(slope[nt][e & 1], static_cast<float>(base + (e < 2 ? row_a : row_b) - pos), x[e]);
+                    if (edge && !(e < 2 ? ok_a : ok_b)) x[e] = -INFINITY;
+                    P[nt][e] = exp2_quick(x[e] - R[nt][e & 1]);
+                }
+                const float high = fmaxf(fmaxf(P[nt][0], P[nt][1]) * amp[0], fmaxf(P[nt][2], P[nt][3]) * amp[1]);
+                if (__any_sync(0xffffffffu, !(high <= kLimit))) {          // (at first R is -inf, and weights are infinite or no numbers)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float most = fmaxf(x[e] + fmaxf(__log2f(amp[0]), kLeastLog), x[e + 2] + fmaxf(__log2f(amp[1]), kLeastLog));
+#pragma unroll
+                        for (int s = 4; s < 32; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+                        const float next = fmaxf(R[nt][e], most);
+                        const float by = R[nt][e] == -INFINITY ? 0.f : exp2_quick(R[nt][e] - next);
+                        R[nt][e] = next;
+                        l[nt][e] *= by;
+                        cen[nt][e] *= by;
+#pragma unroll
+                        for (int grp = 0; grp < G; ++grp) {
+                            ones[nt][grp][e] *= by;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                o[nt][grp][h][e] *= by;
+                                o[nt][grp][h][e + 2] *= by;
+                            }
+                        }
+                        // (-inf: the column has seen no key, or only such as are no numbers, which the weights then are, too)
+                        P[nt][e] = exp2_quick(x[e] - (next == -INFINITY ? 0.f : next));
+                        P[nt][e + 2] = exp2_quick(x[e + 2] - (next == -INFINITY ? 0.f : next));
+                    }
+                }
+                l[nt][0] += P[nt][0] + P[nt][2];
+                l[nt][1] += P[nt][1] + P[nt][3];
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                mma_bf16(cen[nt], __byte_perm(vc[0], vc[1], 0x7632), 0u, __byte_perm(vc[2], vc[3], 0x7632), 0u, transposed(pack_bf16(P[nt][0], P[nt][1])),
+                         transposed(pack_bf16(P[nt][2], P[nt][3])));
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+                const uint32_t x0 = __byte_perm(vw[0][grp >> 1], vw[1][grp >> 1], grp & 1 ? 0x7632 : 0x5410),
+                               x1 = __byte_perm(vw[2][grp >> 1], vw[3][grp >> 1], grp & 1 ? 0x7632 : 0x5410), y0 = x0 >> 8, y1 = x1 >> 8;
+                const float s0 = bf16_low(vp[0][grp]), s1 = bf16_low(vp[1][grp]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint32_t b0 = transposed(pack_f16(P[nt][0] * s0, P[nt][1] * s0)), b1 = transposed(pack_f16(P[nt][2] * s1, P[nt][3] * s1));
+                    mma_f16(o[nt][grp][0], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, b0, b1);
+                    mma_f16(o[nt][grp][1], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, b0, b1);
+                    mma_f16(ones[nt][grp], 0x3c003c00u, 0u, 0x3c003c00u, 0u, b0, b1);
+                }
+            }
+        }
+        __syncwarp();           // every lane is done with the stage before it is refilled
+        issue(j + kStages);
+    }
+
+    // ---- the warps' results side by side in shared memory (the rings are no longer needed)
+    const int s_lo = first / a.split_keys, n = pos / a.split_keys - s_lo + 1;      // live splits
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(smem);
+    constexpr int RS = HD + 2;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int head = 8 * nt + 2 * c + e;
+            float sum = l[nt][e];
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+            float* dst = red + (warp * group + head) * RS;
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+                const float centre = __shfl_sync(0xffffffffu, cen[nt][e], 4 * grp + c) - 8.f * ones[nt][grp][e];
+                if (head < group) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        dst[32 * grp + 4 * g + 2 * h] = fmaf(o[nt][grp][h][e], 16777216.f, centre);
+                        dst[32 * grp + 4 * g + 2 * h + 1] = fmaf(o[nt][grp][h][e + 2], 1048576.f, centre);
+                    }
+                }
+            }
+            if (head < group && g == 0) {
+                dst[HD] = R[nt][e];
+                dst[HD + 1] = sum;
+            }
+        }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < group * HD; idx += blockDim.x) {
+        const int row = idx / HD, d = idx - row * HD;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, red[(w * group + row) * RS + HD]);
+        float acc = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float* src = red + (w * group + row) * RS;
+            const float f = mm == -INFINITY ? 0.f : exp2f(src[HD] - mm);       // a warp without keys has weight 0
+            acc += f * src[d];
+            sum += f * src[HD + 1];
+        }
+        if (n == 1) {           // no other split
+            if (a.sinks != nullptr && mm != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -mm));
+            out[idx] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);      // 0: no key had a page
+            continue;
+        }
+        const size_t slot = (static_cast<size_t>(t) * a.nq + kvh * group + row) * a.num_splits + split;
+        a.part_o[slot * HD + d] = acc;
+        if (d == 0) {
+            a.part_ml[slot * 2] = mm;
+            a.part_ml[slot * 2 + 1] = sum;
+        }
+    }
+    if (n == 1) return;
+    // ---- the CTA that finishes last for this (token, key head) merges the splits
+    __shared__ int is_last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* ticket = a.tickets + static_cast<size_t>(t) * a.nkv + kvh;
+        is_last = atomicAdd(ticket, 1) == n - 1;
+        if (is_last) *ticket = 0;       // ready for the next launch; nobody else touches it before then
+    }
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+    float* weights = red;                       // [group][n]
+    float* total = red + group * n;             // [group]
+    for (int row = warp; row < group; row += kWarps) {
+        const size_t base = (static_cast<size_t>(t) * a.nq + kvh * group + row) * a.num_splits + s_lo;
+        float most = -INFINITY;
+        for (int sp = lane; sp < n; sp += 32) {
+            const float v = __ldcg(a.part_ml + (base + sp) * 2);
+            weights[row * n + sp] = v;
+            most = fmaxf(most, v);
+        }
+        most = warp_max(most);
+        float sum = 0.f;
+        for (int sp = lane; sp < n; sp += 32) {
+            const float w = most == -INFINITY ? 0.f : exp2f(weights[row * n + sp] - most);
+            weights[row * n + sp] = w;
+            sum += w * __ldcg(a.part_ml + (base + sp) * 2 + 1);
+        }
+        sum = warp_sum(sum);
+        if (a.sinks != nullptr && most != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -most));
+        if (lane == 0) total[row] = sum;
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < group * (HD / 4); idx += blockDim.x) {
+        const int row = idx / (HD / 4), d = (idx - row * (HD / 4)) * 4;
+        const size_t base = (static_cast<size_t>(t) * a.nq + kvh * group + row) * a.num_splits + s_lo;
+        const float4* column = reinterpret_cast<const float4*>(a.part_o + base * HD + d);
+        const float* w = weights + row * n;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int sp = 0; sp < n; ++sp) {
+            const float4 v = __ldcg(column + static_cast<size_t>(sp) * (HD / 4));
+            acc.x = fmaf(w[sp], v.x, acc.x);
+            acc.y = fmaf(w[sp], v.y, acc.y);
+            acc.z = fmaf(w[sp], v.z, acc.z);
+            acc.w = fmaf(w[sp], v.w, acc.w);
+        }
+        const float inv = total[row] == 0.f ? 0.f : 1.f / total[row];
+        uint2 packed;
+        packed.x = pack_bf16(acc.x * inv, acc.y * inv);
+        packed.y = pack_bf16(acc.z * inv, acc.w * inv);
+        if (reinterpret_cast<uintptr_t>(a.out) % 8 == 0)
+            *reinterpret_cast<uint2*>(out + row * HD + d) = packed;
+        else
+            for (int i = 0; i < 4; ++i) out[row * HD + d + i] = __float2bfloat16_rn((&acc.x)[i] * inv);
+    }
+}
+
+// Keys per CTA, a multiple of 64 up to 2048: by the launch's sizes alone, so that a captured graph stays valid.
+inline int choose_split_keys(int tokens, int nkv, int max_context) {
+    const long long units = static_cast<long long>(tokens) * nkv * ((max_context + kUnit - 1) / kUnit);
+    long long u = (units + 820) / 821;
+    if (u < 4) u = (units + 206) / 207;
+    u = u < 2 ? 2 : (u > kMaxTiles ? kMaxTiles : u);
+    return static_cast<int>(u) * kUnit;
+}
+
+template <int G, int NT>
+int launch_decode(const Decode& a, int tokens, cudaStream_t stream) {
+    constexpr int smem = kWarps * kStages * 2 * kTile * 20 * G;
+    const int group = a.nq / a.nkv;
+    static_assert(kWarps * 8 * NT * (32 * G + 2) * 4 <= smem || NT > 1, "the merge fits into the rings");
+    const long long merge = static_cast<long long>(group) * (a.num_splits + 1) * 4, warps = static_cast<long long>(kWarps) * group * (32 * G + 2) * 4;
+    if (merge > smem || warps > smem) return STRIDE_UNSUPPORTED;
+    const bool bulk = a.page_size % kTile == 0;
+    cudaError_t e = allow_shared<decode_kernel<G, NT, true>>(smem);
+    if (e == cudaSuccess) e = allow_shared<decode_kernel<G, NT, false>>(smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const dim3 grid(a.num_splits, a.nkv, tokens);
+    if (bulk)
+        stride::launch(decode_kernel<G, NT, true>, grid, dim3(kWarps * 32), smem, stream, a);
+    else
+        stride::launch(decode_kernel<G, NT, false>, grid, dim3(kWarps * 32), smem, stream, a);
+    return STRIDE_LAUNCH_STATUS();
+}
+
+}  // namespace four
+}  // namespace stride
+
+using namespace stride;
+
+extern "C" {
+
+// Number of float32 scratch elements the launcher needs for these sizes.
+long long stride_decode_int4_scratch_floats(int tokens, int nq, int nkv, int hd, int max_context) {
+    if (tokens <= 0 || nq <= 0 || nkv <= 0 || max_context <= 0) return 0;
+    const int split_keys = four::choose_split_keys(tokens, nkv, max_context);
+    const long long splits = (static_cast<long long>(max_context) + split_keys - 1) / split_keys;
+    return four::kTicketInts + static_cast<long long>(tokens) * nq * splits * (hd + 2);
+}
+
+// One query token per row. `scratch` must be zero when it is first used (every launch leaves its tickets zero) and belongs to one stream at a
+// time. A row whose position does not lie below `max_context` gets zeros, and code 32 in the status word; a key whose page is none of the
+// cache's is left out, with code 33. Returns -2 for sizes it does not run: head sizes other than 64 and 128, groups above 16, more than
+// 65536 (token, key head) pairs, contexts of more than 8192 splits.
+int stride_decode_int4(const void* q, int q_stride, void* out, const void* k_pages, const void* v_pages, int num_pages, const int32_t* block_table,
+                       int table_width, const int32_t* seq_of_token, const int32_t* positions, float* scratch, long long scratch_floats, int tokens,
+                       int nq, int nkv, int hd, int page_size, float scale, int window, float softcap, const float* sinks, const float* slopes,
+                       int max_context, int* status, cudaStream_t stream) {
+    if (tokens < 0 || nq <= 0 || nkv <= 0 || page_size <= 0 || table_width <= 0 || num_pages <= 0 || window < 0 || softcap < 0.f || max_context <= 0 ||
+        nq % nkv || status == nullptr)
+        return STRIDE_BAD_ARGUMENT;
+    if ((hd != 64 && hd != 128) || nq / nkv > 16 || tokens > 65535 || nkv > 65535 || max_context > (1 << 30)) return STRIDE_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 16 || reinterpret_cast<uintptr_t>(scratch) % 16)
+        return STRIDE_UNSUPPORTED;
+    if (tokens == 0) return 0;
+    const int split_keys = four::choose_split_keys(tokens, nkv, max_context);
+    const int num_splits = (max_context + split_keys - 1) / split_keys;
+    if (num_splits > 8192 || static_cast<long long>(tokens) * nkv > four::kTicketInts) return STRIDE_UNSUPPORTED;
+    if (scratch == nullptr || scratch_floats < stride_decode_int4_scratch_floats(tokens, nq, nkv, hd, max_context)) return STRIDE_BAD_ARGUMENT;
+    static_assert(sizeof(int) == sizeof(float), "the tickets live in the float scratch");
+    four::Decode a;
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.out = static_cast<__nv_bfloat16*>(out);
+    a.k_pages = static_cast<const uint8_t*>(k_pages);
+    a.v_pages = static_cast<const uint8_t*>(v_pages);
+    a.table = block_table;
+    a.seq_of_token = seq_of_token;
+    a.positions = positions;
+    a.sinks = sinks;
+    a.slopes = slopes;
+    a.tickets = reinterpret_cast<int*>(scratch);
+    a.part_o = scratch + four::kTicketInts;
+    a.part_ml = a.part_o + static_cast<long long>(tokens) * nq * num_splits * hd;
+    a.status = status;
+    a.q_stride = q_stride;
+    a.table_width = table_width;
+    a.num_pages = num_pages;
+    a.nq = nq;
+    a.nkv = nkv;
+    a.page_size = page_size;
+    a.window = window;
+    a.split_keys = split_keys;
+    a.num_splits = num_splits;
+    a.scale_log2e = scale * 1.4426950408889634f;
+    a.cap_log2e = softcap * 1.4426950408889634f;
+    a.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;
+    const bool wide = nq / nkv > 8;
+    if (hd == 64) return wide ? four::launch_decode<2, 2>(a, tokens, stream) : four::launch_decode<2, 1>(a, tokens, stream);
+    return wide ? four::launch_decode<4, 2>(a, tokens, stream) : four::launch_decode<4, 1>(a, tokens, stream);
+}
+
+}  // extern "C"

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kWriteWarps * 32) head_write_kernel(const Head
                 if (j >= G) continue;
                 const bool there = 32 * j + lane < hd;
                 const float e = which ? v[j] : x[j];
-                fine = fine && (!there || isfinite(e));
+                fine = fine && (!there || fabsf(e) < four::kMaxEntry);
                 float lo = there ? e : INFINITY, hi = there ? e : -INFINITY;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) {
@@ -129,7 +129,6 @@ __global__ void __launch_bounds__(kWriteWarps * 32) head_write_kernel(const Head
                     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
                 }
                 four::group_params(lo, hi, s[which][j], c[which][j]);
-                fine = fine && isfinite(s[which][j]) && isfinite(c[which][j]);
             }
         fine = __all_sync(0xffffffffu, fine);
 #pragma unroll

@@ -73,6 +73,9 @@ _SIGNATURES = {
                                                        c_int, c_int, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "stride_int4_expand": ("head_write", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
                                           c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "stride_decode_int4": ("attention_int4_decode", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                                     c_longlong, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p, c_int,
+                                                     c_void_p, c_void_p]),
     "stride_copy_pages": ("page_copy", [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "stride_scale_rows": ("elementwise", [c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_int, c_void_p]),
     "stride_paged_decode_attention": ("attention_decode", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
@@ -264,7 +267,7 @@ _CLASS_OF = {
     "stride_gated_group_norm": "gate + norm of parts",
     "stride_paged_decode_attention_biased": "attention (decode)",
     "stride_head_write": "rotation + head norms + cache write", "stride_int4_read": "4-bit cache: values", "stride_int4_expand": "4-bit cache: values",
-    "stride_attention_int4_exact": "attention (exact kernel)", "stride_copy_pages": "copies of pages",
+    "stride_attention_int4_exact": "attention (exact kernel)", "stride_decode_int4": "attention (decode)", "stride_copy_pages": "copies of pages",
 }
 
 
@@ -1504,7 +1507,7 @@ _WAIT_CODES = {1: "matrix product: producer", 2: "matrix product: tensor-core is
                51: "tokens-as-rows product: activation copies", 52: "tokens-as-rows product: weight copies",
                53: "tokens-as-rows product: tensor-core issuer", 54: "tokens-as-rows product: epilogue",
                61: "float32 product: copies", 62: "float32 product: tensor-core issuer", 63: "float32 product: cutting warps",
-               71: "latent attention: copies of keys", 72: "latent attention: tensor-core issuer", 73: "latent attention: softmax"}
+               71: "latent attention: copies of keys", 72: "latent attention: tensor-core issuer", 73: "latent attention: softmax", 81: "decode attention over a 4-bit cache: a tile copy"}
 _WAIT_CODES.update({c: "prefill attention (attention_prefill_tc.cu)" for c in range(11, 22)})
 _OTHER_CODES = {32: "decode attention was given a token whose position is not below the context bound of its launch",
                 33: "attention over a 4-bit cache met a key whose block-table entry names no page of the cache",
@@ -2160,14 +2163,26 @@ def paged_attention_int4(q, q_stride: int, out, k_pages, v_pages, block_table, s
 
 def decode_int4_scratch_floats(tokens: int, nq: int, nkv: int, hd: int, max_context: int) -> int:
     """float32 elements of scratch that ``paged_attention_decode_int4`` needs for these sizes."""
-    return 1
+    f = _bound.get("stride_decode_int4_scratch_floats")
+    if f is None:
+        f = build.load_kernel_library("attention_int4_decode").stride_decode_int4_scratch_floats
+        f.argtypes = [c_int, c_int, c_int, c_int, c_int]
+        f.restype = c_longlong
+        _bound["stride_decode_int4_scratch_floats"] = f
+    return int(f(tokens, nq, nkv, hd, max_context))
 
 
 def paged_attention_decode_int4(q, q_stride: int, out, k_pages, v_pages, block_table, seq_of_token, positions, scratch, nq: int, nkv: int, hd: int,
                                 page_size: int, scale: float, window: int, max_context: int, softcap: float = 0.0, sinks=None, slopes=None) -> None:
-    """``paged_attention_decode`` over pages held in 4 bits: one query per row, bfloat16, head sizes 64 and 128."""
-    paged_attention_int4(q, q_stride, out, k_pages, v_pages, block_table, seq_of_token, positions, nq, nkv, hd, page_size, scale, window, softcap, sinks,
-                         slopes)
+    """``paged_attention_decode`` over pages held in 4 bits: one query per row, bfloat16, head sizes 64 and 128. ``max_context`` exceeds every
+    position; ``scratch``: float32, zero when it is first used, at least ``decode_int4_scratch_floats`` elements, for one stream at a time."""
+    qp, op, k, v, pages = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap, torch.bfloat16)
+    tokens = out.shape[0]
+    _check(_fn("stride_decode_int4")(
+        qp, q_stride, op, k, v, pages, _here(block_table, "block_table", torch.int32), block_table.shape[1],
+        _covers(seq_of_token, "seq_of_token", tokens), _covers(positions, "positions", tokens), _here(scratch, "scratch", torch.float32),
+        scratch.numel(), tokens, nq, nkv, hd, page_size, float(scale), int(window), float(softcap), _here_opt(sinks, "sinks", nq, torch.float32),
+        _here_opt(slopes, "slopes", nq, torch.float32), int(max_context), _status_ptr(q.device), _stream()), "paged_attention_decode_int4")
 
 
 INT4_EXPANDED_PAGE = 64     # keys of a page of the expanded keys and values
