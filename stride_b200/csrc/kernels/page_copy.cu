@@ -17,7 +17,6 @@ struct PageCopies {
     unsigned char* base[kCopyPools];
     long long page_bytes[kCopyPools], layer_bytes[kCopyPools];
     int layers[kCopyPools];
-    int pools;
     int2 pairs[kCopyPairs];
 };
 
@@ -51,43 +50,41 @@ void launch_copies(const PageCopies& a, long long most_bytes, int pairs, int lay
 
 using namespace stride;
 
-// pools: n_pools device addresses; layers, num_pages, page_bytes: of each pool. from, to: `pairs` page numbers of every pool (host memory). The
-// caller has checked that no page of `to` comes twice or also in `from`.
-extern "C" int stride_copy_pages(const long long* pools, const int* layers, const int* num_pages, const long long* page_bytes, int n_pools, const int* from,
-                                 const int* to, int pairs, cudaStream_t stream) {
+// pools: of each of the n_pools pools its device address, layers, pages and bytes of a page. from, to: `pairs` page numbers of every pool. All of
+// them host memory. The caller has checked that no page of `to` comes twice or also in `from`.
+extern "C" int stride_copy_pages(const long long* pools, int n_pools, const int* from, const int* to, int pairs, cudaStream_t stream) {
     if (n_pools < 0 || pairs < 0) return STRIDE_BAD_ARGUMENT;
     for (int p = 0; p < n_pools; ++p) {
-        if (pools[p] == 0 || layers[p] <= 0 || num_pages[p] <= 0 || page_bytes[p] <= 0) return STRIDE_BAD_ARGUMENT;
+        const long long* q = pools + 4 * p;
+        if (q[0] == 0 || q[1] <= 0 || q[2] <= 0 || q[3] <= 0) return STRIDE_BAD_ARGUMENT;
+        if (q[1] > 65535 || q[3] > (1LL << 40)) return STRIDE_UNSUPPORTED;
         for (int i = 0; i < pairs; ++i)
-            if (from[i] < 0 || to[i] < 0 || from[i] >= num_pages[p] || to[i] >= num_pages[p]) return STRIDE_BAD_ARGUMENT;
+            if (from[i] < 0 || to[i] < 0 || from[i] >= q[2] || to[i] >= q[2]) return STRIDE_BAD_ARGUMENT;
     }
-    for (int p0 = 0; p0 < n_pools; p0 += kCopyPools) {
+    for (int p0 = 0; p0 < n_pools;) {
         PageCopies a;
-        a.pools = n_pools - p0 < kCopyPools ? n_pools - p0 : kCopyPools;
         long long all = 0, most = 0;
-        int total = 0;
-        for (int p = 0; p < kCopyPools; ++p) {
-            const bool used = p < a.pools;
-            a.base[p] = used ? reinterpret_cast<unsigned char*>(pools[p0 + p]) : nullptr;
-            a.page_bytes[p] = used ? page_bytes[p0 + p] : 0;
-            a.layer_bytes[p] = used ? page_bytes[p0 + p] * num_pages[p0 + p] : 0;
-            a.layers[p] = used ? layers[p0 + p] : 0;
-            if (!used) continue;
-            if (total + static_cast<long long>(layers[p0 + p]) > 65535) return STRIDE_UNSUPPORTED;
-            total += layers[p0 + p];
-            all |= pools[p0 + p] | page_bytes[p0 + p];
-            most = most > page_bytes[p0 + p] ? most : page_bytes[p0 + p];
+        int layers = 0, n = 0;                  // a launch takes up to eight pools and 65535 layers
+        for (; n < kCopyPools && p0 + n < n_pools && layers + pools[4 * (p0 + n) + 1] <= 65535; ++n) {
+            const long long* q = pools + 4 * (p0 + n);
+            a.base[n] = reinterpret_cast<unsigned char*>(q[0]);
+            a.layers[n] = static_cast<int>(q[1]);
+            a.page_bytes[n] = q[3];
+            a.layer_bytes[n] = q[3] * q[2];
+            layers += a.layers[n];
+            all |= q[0] | q[3];
+            most = most > q[3] ? most : q[3];
         }
-        if (most > (1LL << 40)) return STRIDE_UNSUPPORTED;
+        p0 += n;
         for (int i0 = 0; i0 < pairs; i0 += kCopyPairs) {
-            const int n = pairs - i0 < kCopyPairs ? pairs - i0 : kCopyPairs;
-            for (int i = 0; i < kCopyPairs; ++i) a.pairs[i] = i < n ? make_int2(from[i0 + i], to[i0 + i]) : make_int2(0, 0);
+            const int count = pairs - i0 < kCopyPairs ? pairs - i0 : kCopyPairs;
+            for (int i = 0; i < count; ++i) a.pairs[i] = make_int2(from[i0 + i], to[i0 + i]);
             if (all % 16 == 0)
-                launch_copies<uint4>(a, most, n, total, stream);
+                launch_copies<uint4>(a, most, count, layers, stream);
             else if (all % 4 == 0)
-                launch_copies<uint32_t>(a, most, n, total, stream);
+                launch_copies<uint32_t>(a, most, count, layers, stream);
             else
-                launch_copies<uint8_t>(a, most, n, total, stream);
+                launch_copies<uint8_t>(a, most, count, layers, stream);
             const int code = STRIDE_LAUNCH_STATUS();
             if (code) return code;
         }

@@ -76,7 +76,7 @@ _SIGNATURES = {
     "stride_decode_int4": ("attention_int4_decode", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                                      c_longlong, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p, c_int,
                                                      c_void_p, c_void_p]),
-    "stride_copy_pages": ("page_copy", [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    "stride_copy_pages": ("page_copy", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "stride_scale_rows": ("elementwise", [c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_int, c_void_p]),
     "stride_paged_decode_attention": ("attention_decode", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                                            c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int,
@@ -374,12 +374,22 @@ def _code(dtype: torch.dtype) -> int:
         raise KernelError(f"element type {dtype} is not supported (float32 and bfloat16 are)") from None
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or (lambda: torch.cuda.current_device())
+
+
 def _here(t: torch.Tensor, name: str, dtype=None) -> int:
-    """``_dev`` for a tensor that must also live on the current device: the launch goes to that device's stream."""
-    at = _dev(t, name, dtype)
-    if t.get_device() != torch.cuda.current_device():
-        raise KernelError(f"{name} lives on cuda:{t.get_device()}, but the current device is cuda:{torch.cuda.current_device()}")
-    return at
+    """``_dev`` for a tensor that must also live on the current device: the launch goes to that device's stream. (Small calls are bound by the
+    host, so it asks a tensor for each thing once.)"""
+    device = t.get_device()
+    if device < 0:
+        raise KernelError(f"{name} must live on a CUDA device; stride_b200 has no CPU path")
+    if device != _current_device():
+        raise KernelError(f"{name} lives on cuda:{device}, but the current device is cuda:{_current_device()}")
+    if not t.is_contiguous():
+        raise KernelError(f"{name} must be contiguous")
+    if dtype is not None and t.dtype is not dtype:
+        raise KernelError(f"{name} must be {dtype}, got {t.dtype}")
+    return t.data_ptr()
 
 
 def _here_opt(t, name: str, count: int, dtype) -> int | None:
@@ -389,6 +399,20 @@ def _here_opt(t, name: str, count: int, dtype) -> int | None:
     if t.numel() != count:
         raise KernelError(f"{name} must hold {count} elements, got {t.numel()}")
     return _here(t, name, dtype)
+
+
+_status_at: dict = {}       # device number -> address of its status word (the word lives as long as the process)
+
+
+def _status_here(device: int) -> int:
+    at = _status_at.get(device)
+    if at is None:
+        at = _status_at[device] = _status_ptr(torch.device("cuda", device))
+    return at
+
+
+def _stream_here(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def require_device() -> None:
@@ -2055,17 +2079,15 @@ def int4_row_bytes(hd: int) -> int:
 
 def _pages_args(k_pages, v_pages, nkv: int, page_size: int, row: int, dtype) -> tuple:
     """(keys, values, number of pages) of pages [num_pages, nkv, page_size, row], checked."""
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if t.dim() != 4 or tuple(t.shape[1:]) != (nkv, page_size, row) or t.shape[0] == 0:
-            raise KernelError(f"{name} must be [num_pages, {nkv}, {page_size}, {row}], got {tuple(t.shape)}")
-    if k_pages.shape[0] != v_pages.shape[0]:
-        raise KernelError("keys and values must have the same number of pages")
-    return _here(k_pages, "k_pages", dtype), _here(v_pages, "v_pages", dtype), k_pages.shape[0]
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[0] == 0 or shape[1] != nkv or shape[2] != page_size or shape[3] != row or v_pages.shape != shape:
+        raise KernelError(f"k_pages and v_pages must be [num_pages, {nkv}, {page_size}, {row}], got {tuple(shape)} and {tuple(v_pages.shape)}")
+    return _here(k_pages, "k_pages", dtype), _here(v_pages, "v_pages", dtype), shape[0]
 
 
 def _head_write(what: str, bits4: bool, qkv, bias, q_norm, k_norm, eps, positions, slot_mapping, cos, sin, k_pages, v_pages, nq, nkv, hd, page_size,
                 rotate, q_out) -> None:
-    if min(nq, nkv, hd, page_size) <= 0:
+    if nq <= 0 or nkv <= 0 or hd <= 0 or page_size <= 0:
         raise KernelError(f"{what}: heads, head size and page size must be positive")
     tokens, width = qkv.shape
     if width != (nq + 2 * nkv) * hd:
@@ -2074,25 +2096,26 @@ def _head_write(what: str, bits4: bool, qkv, bias, q_norm, k_norm, eps, position
         raise KernelError("the norms of queries and keys come together")
     code = _code(qkv.dtype)
     k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd) if bits4 else hd, torch.uint8 if bits4 else qkv.dtype)
+    rows, device = _here(qkv, "qkv"), qkv.get_device()
     if q_out is None:
-        out, stride = _here(qkv, "qkv"), width
+        out, stride = rows, width
     else:
         if q_out.dim() != 2 or q_out.shape[0] < tokens or q_out.shape[1] != nq * hd or q_out.dtype != qkv.dtype or q_out.stride(1) != 1 or \
                 q_out.stride(0) < nq * hd:
             raise KernelError("q_out must be rows [tokens, nq * hd] of qkv's element type")
-        if not q_out.is_cuda or q_out.get_device() != qkv.get_device():
+        if q_out.get_device() != device:
             raise KernelError("q_out must live on qkv's device")
         out, stride = q_out.data_ptr(), q_out.stride(0)
-    if positions.numel() < tokens or (slot_mapping is not None and slot_mapping.numel() < tokens):
-        raise KernelError("positions and slots must cover the tokens")
-    if rotate and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] * 2 != hd):
-        raise KernelError("cos and sin must be [positions, hd / 2]")
+    if rotate:
+        angles = cos.shape
+        if len(angles) != 2 or sin.shape != angles or angles[1] * 2 != hd:
+            raise KernelError("cos and sin must be [positions, hd / 2]")
     _check(_fn("stride_head_write")(
-        _here(qkv, "qkv"), out, stride, _here_opt(bias, "bias", width, torch.float32), _here_opt(q_norm, "q_norm", hd, torch.float32),
-        _here_opt(k_norm, "k_norm", hd, torch.float32), float(eps), _here(positions, "positions", torch.int32),
-        None if slot_mapping is None else _here(slot_mapping, "slot_mapping", torch.int32), _here(cos, "cos", torch.float32),
-        _here(sin, "sin", torch.float32), cos.shape[0] if rotate else 0, k, v, pages, int(bits4), tokens, nq, nkv, hd, page_size, int(rotate), code,
-        _status_ptr(qkv.device), _stream()), what)
+        rows, out, stride, _here_opt(bias, "bias", width, torch.float32), _here_opt(q_norm, "q_norm", hd, torch.float32),
+        _here_opt(k_norm, "k_norm", hd, torch.float32), eps, _covers(positions, "positions", tokens),
+        None if slot_mapping is None else _covers(slot_mapping, "slot_mapping", tokens), _here(cos, "cos", torch.float32),
+        _here(sin, "sin", torch.float32), angles[0] if rotate else 0, k, v, pages, 1 if bits4 else 0, tokens, nq, nkv, hd, page_size, 1 if rotate else 0,
+        code, _status_here(device), _stream_here(device)), what)
 
 
 def qk_norm_rope_write(qkv, bias, q_norm, k_norm, eps: float, positions, slot_mapping, cos, sin, k_pages, v_pages, nq: int, nkv: int, hd: int,
@@ -2118,28 +2141,31 @@ def read_int4(k_pages, v_pages, slots, k_out, v_out, nkv: int, hd: int, page_siz
     if min(nkv, hd, page_size) <= 0:
         raise KernelError("read_int4: heads, head size and page size must be positive")
     k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd), torch.uint8)
-    for t in (k_out, v_out):
-        if tuple(t.shape) != (slots.numel(), nkv, hd) or t.dtype != k_out.dtype:
-            raise KernelError("k_out and v_out must be [slots, nkv, hd] of one element type")
+    shape = k_out.shape
+    if len(shape) != 3 or shape[0] != slots.numel() or shape[1] != nkv or shape[2] != hd or v_out.shape != shape or v_out.dtype is not k_out.dtype:
+        raise KernelError("k_out and v_out must be [slots, nkv, hd] of one element type")
+    device = k_out.get_device()
     _check(_fn("stride_int4_read")(k, v, _here(slots, "slots", torch.int32), _here(k_out, "k_out"), _here(v_out, "v_out"), slots.numel(), nkv, hd,
-                                   page_size, pages, _code(k_out.dtype), _status_ptr(k_out.device), _stream()), "read_int4")
+                                   page_size, pages, _code(k_out.dtype), _status_here(device), _stream_here(device)), "read_int4")
 
 
 def _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap, dtype=None) -> tuple:
-    """(q, out, keys, values, number of pages) of the attention kernels over a cache held in 4 bits, checked."""
-    if min(nq, nkv, hd, page_size) <= 0 or nq % nkv:
+    """(q, out, keys, values, number of pages, block table, its width, number of the device) of the attention kernels over a cache held in 4
+    bits, checked."""
+    if nq <= 0 or nkv <= 0 or hd <= 0 or page_size <= 0 or nq % nkv:
         raise KernelError(f"{nq} query heads of {hd} do not group into {nkv} key heads")
     if window < 0 or softcap < 0:
         raise KernelError("a window or a cap on scores is not below zero")
-    tokens = out.shape[0]
-    if out.dim() != 2 or out.shape[1] != nq * hd or out.dtype != q.dtype:
+    shape = out.shape
+    if len(shape) != 2 or shape[1] != nq * hd or out.dtype is not q.dtype:
         raise KernelError("attention output has the wrong width or element type")
-    if q_stride < nq * hd or (tokens and q.numel() < (tokens - 1) * q_stride + nq * hd):
+    if q_stride < nq * hd or (shape[0] and q.numel() < (shape[0] - 1) * q_stride + nq * hd):
         raise KernelError("q is too small for its rows")
-    if block_table.dim() != 2:
+    table = block_table.shape
+    if len(table) != 2:
         raise KernelError("block_table must be [requests, pages]")
-    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd), torch.uint8)
-    return _here(q, "q", dtype), _here(out, "out", dtype), k, v, pages
+    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, 20 * -(-hd // INT4_GROUP), torch.uint8)
+    return _here(q, "q", dtype), _here(out, "out", dtype), k, v, pages, _here(block_table, "block_table", torch.int32), table[1], q.get_device()
 
 
 def _covers(t, name: str, count: int) -> int:
@@ -2152,13 +2178,13 @@ def paged_attention_int4(q, q_stride: int, out, k_pages, v_pages, block_table, s
                          scale: float, window: int = 0, softcap: float = 0.0, sinks=None, slopes=None) -> None:
     """``paged_attention`` over pages held in 4 bits: any mix of rows, any head size up to 256, float32 or bfloat16. The exact kernel: the
     result of a row has the same bits however the work is cut."""
-    qp, op, k, v, pages = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap)
+    qp, op, k, v, pages, table, width, device = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
+                                                                     softcap)
     tokens = out.shape[0]
     _check(_fn("stride_attention_int4_exact")(
-        qp, q_stride, op, k, v, pages, _here(block_table, "block_table", torch.int32), block_table.shape[1],
-        _covers(seq_of_token, "seq_of_token", tokens), _covers(positions, "positions", tokens), tokens, nq, nkv, hd, page_size, float(scale), int(window),
-        float(softcap), _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32), _code(q.dtype),
-        _status_ptr(q.device), _stream()), "paged_attention_int4")
+        qp, q_stride, op, k, v, pages, table, width, _covers(seq_of_token, "seq_of_token", tokens), _covers(positions, "positions", tokens), tokens, nq,
+        nkv, hd, page_size, scale, window, softcap, _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32),
+        _code(q.dtype), _status_here(device), _stream_here(device)), "paged_attention_int4")
 
 
 def decode_int4_scratch_floats(tokens: int, nq: int, nkv: int, hd: int, max_context: int) -> int:
@@ -2176,13 +2202,14 @@ def paged_attention_decode_int4(q, q_stride: int, out, k_pages, v_pages, block_t
                                 page_size: int, scale: float, window: int, max_context: int, softcap: float = 0.0, sinks=None, slopes=None) -> None:
     """``paged_attention_decode`` over pages held in 4 bits: one query per row, bfloat16, head sizes 64 and 128. ``max_context`` exceeds every
     position; ``scratch``: float32, zero when it is first used, at least ``decode_int4_scratch_floats`` elements, for one stream at a time."""
-    qp, op, k, v, pages = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap, torch.bfloat16)
+    qp, op, k, v, pages, table, width, device = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
+                                                                     softcap, torch.bfloat16)
     tokens = out.shape[0]
     _check(_fn("stride_decode_int4")(
-        qp, q_stride, op, k, v, pages, _here(block_table, "block_table", torch.int32), block_table.shape[1],
-        _covers(seq_of_token, "seq_of_token", tokens), _covers(positions, "positions", tokens), _here(scratch, "scratch", torch.float32),
-        scratch.numel(), tokens, nq, nkv, hd, page_size, float(scale), int(window), float(softcap), _here_opt(sinks, "sinks", nq, torch.float32),
-        _here_opt(slopes, "slopes", nq, torch.float32), int(max_context), _status_ptr(q.device), _stream()), "paged_attention_decode_int4")
+        qp, q_stride, op, k, v, pages, table, width, _covers(seq_of_token, "seq_of_token", tokens), _covers(positions, "positions", tokens),
+        _here(scratch, "scratch", torch.float32), scratch.numel(), tokens, nq, nkv, hd, page_size, scale, window, softcap,
+        _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32), max_context, _status_here(device),
+        _stream_here(device)), "paged_attention_decode_int4")
 
 
 INT4_EXPANDED_PAGE = 64     # keys of a page of the expanded keys and values
@@ -2208,7 +2235,8 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     the rows of ``out``: bfloat16, head sizes 64 and 128. ``keys``: at least what those requests hold together; ``scratch``: int32, at least
     ``prefill_int4_scratch_ints`` elements, for one stream at a time. The keys and values that the portions see are expanded once, to pages
     of 64 in bfloat16 (a rounding of 2^-9 of an entry, as a bfloat16 cache has it), and attended to from there."""
-    qp, op, k, v, pages = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap, torch.bfloat16)
+    qp, op, k, v, pages, rows, width, device = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
+                                                                    softcap, torch.bfloat16)
     if not fast_attention_supported(q.dtype, nq, nkv, hd):
         raise KernelError(f"paged_attention_prefill_int4: {nq} heads of {hd} on {nkv} are not supported (paged_attention_int4 takes them)")
     if num_seqs < 0 or keys < 0 or scratch.numel() < prefill_int4_scratch_ints(num_seqs, keys, nkv, hd):
@@ -2222,14 +2250,14 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     half = out_pages * nkv * INT4_EXPANDED_PAGE * hd * 2
     wide_k = _here(scratch, "scratch", torch.int32)
     wide_v, table = wide_k + half, wide_k + 2 * half
-    starts, lens, held = (_covers(t, name, num_seqs) for t, name in ((q_start, "q_start"), (q_len, "q_len"), (ctx_len, "ctx_len")))
+    starts, lens, held = _covers(q_start, "q_start", num_seqs), _covers(q_len, "q_len", num_seqs), _covers(ctx_len, "ctx_len", num_seqs)
     sink, slope = _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32)
-    status, stream = _status_ptr(q.device), _stream()
-    _check(_fn("stride_int4_expand")(k, v, pages, _here(block_table, "block_table", torch.int32), block_table.shape[1], lens, held, num_seqs, nkv, hd,
-                                     page_size, int(window), wide_k, wide_v, table, out_pages, status, stream), "paged_attention_prefill_int4")
+    status, stream = _status_here(device), _stream_here(device)
+    _check(_fn("stride_int4_expand")(k, v, pages, rows, width, lens, held, num_seqs, nkv, hd, page_size, window, wide_k, wide_v, table, out_pages, status,
+                                     stream), "paged_attention_prefill_int4")
     _check(_fn("stride_paged_prefill_attention_tc")(
-        qp, q_stride, op, wide_k, wide_v, out_pages, table, out_pages, starts, lens, held, num_seqs, tokens, nq, nkv, hd, INT4_EXPANDED_PAGE, float(scale),
-        int(window), -float(softcap) if precise_cap else float(softcap), sink, slope, None, 0, status, stream), "paged_attention_prefill_int4")
+        qp, q_stride, op, wide_k, wide_v, out_pages, table, out_pages, starts, lens, held, num_seqs, tokens, nq, nkv, hd, INT4_EXPANDED_PAGE, scale,
+        window, -softcap if precise_cap else softcap, sink, slope, None, 0, status, stream), "paged_attention_prefill_int4")
 
 
 # ------------------------------------------------------------------- copies of pages
@@ -2238,25 +2266,28 @@ def copy_pages(pools, src, dst) -> None:
     page numbers (sequences of ints). A page is copied from or to, not both, and to at most once. A captured graph keeps the pairs it was
     captured with."""
     src, dst = [int(p) for p in src], [int(p) for p in dst]
-    if len(src) != len(dst):
+    n = len(src)
+    if n != len(dst):
         raise KernelError("copy_pages: every page copied from goes with one copied to")
     targets = set(dst)
-    if len(targets) != len(dst):
+    if len(targets) != n:
         raise KernelError("copy_pages: a page is copied to twice")
     if not targets.isdisjoint(src):
         raise KernelError("copy_pages: a page is copied from and to")
+    least, most = (min(min(src), min(dst)), max(max(src), max(dst))) if n else (0, -1)
+    about = []                  # address, layers, pages and bytes of a page of every pool
     for t in pools:
-        if t.dim() < 3:
-            raise KernelError(f"copy_pages: a pool is [layers, num_pages, ...], got {tuple(t.shape)}")
-        if src and not (0 <= min(min(src), min(dst)) and max(max(src), max(dst)) < t.shape[1]):
-            raise KernelError(f"copy_pages: a page lies outside a pool of {t.shape[1]}")
-    at = [_here(t, "pool") for t in pools]
-    if not src or not at:
+        shape = t.shape
+        if len(shape) < 3:
+            raise KernelError(f"copy_pages: a pool is [layers, num_pages, ...], got {tuple(shape)}")
+        if least < 0 or most >= shape[1]:
+            raise KernelError(f"copy_pages: a page lies outside a pool of {shape[1]}")
+        about += (_here(t, "pool"), shape[0], shape[1], t.stride(1) * t.itemsize)
+    if not n or not about:
         return
-    n = len(at)
-    sizes = [t.stride(1) * t.element_size() if t.shape[1] > 1 else t[0].numel() * t.element_size() for t in pools]
-    _check(_fn("stride_copy_pages")((c_longlong * n)(*at), (c_int * n)(*[t.shape[0] for t in pools]), (c_int * n)(*[t.shape[1] for t in pools]),
-                                    (c_longlong * n)(*sizes), n, (c_int * len(src))(*src), (c_int * len(dst))(*dst), len(src), _stream()), "copy_pages")
+    device = pools[0].get_device()
+    _check(_fn("stride_copy_pages")((c_longlong * len(about))(*about), len(about) // 4, (c_int * n)(*src), (c_int * n)(*dst), n, _stream_here(device)),
+           "copy_pages")
 
 
 # --------------------------------------------------------------------- sampling
