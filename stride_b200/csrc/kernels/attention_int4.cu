@@ -108,28 +108,44 @@ attention_int4_exact_kernel(const T* __restrict__ q, int q_stride, T* __restrict
 
 using namespace stride;
 
-// q: [tokens, q_stride] with head h at columns [h hd, (h + 1) hd); out: [tokens, nq hd]; pages: uint8 [num_pages, nkv, page_size, 20 ceil(hd / 32)];
-// block_table: [seqs, table_width]. A key whose page is none of the cache's is left out, and the status word says so.
-extern "C" int stride_attention_int4_exact(const void* q, int q_stride, void* out, const void* k_pages, const void* v_pages, int num_pages,
-                                           const int32_t* block_table, int table_width, const int32_t* seq_of_token, const int32_t* positions, int tokens,
-                                           int nq, int nkv, int hd, int page_size, float scale, int window, float softcap, const float* sinks,
-                                           const float* slopes, int dtype, int* status, cudaStream_t stream) {
-    if (tokens < 0 || nq <= 0 || nkv <= 0 || hd <= 0 || page_size <= 0 || table_width <= 0 || num_pages <= 0 || window < 0 || softcap < 0.f || nq % nkv)
+struct Int4Attention {
+    const void* q;                  // [tokens, q_stride] with head h at columns [h hd, (h + 1) hd)
+    void* out;                      // [tokens, nq hd]
+    const uint8_t* k_pages;         // [num_pages, nkv, page_size, 20 ceil(hd / 32)]
+    const uint8_t* v_pages;
+    const int32_t* block_table;     // [requests, table_width]
+    const int32_t* seq_of_token;
+    const int32_t* positions;
+    const float* sinks;
+    const float* slopes;
+    int* status;
+    cudaStream_t stream;
+    int q_stride, num_pages, table_width, tokens, nq, nkv, hd, page_size, window;
+    float scale, softcap;
+    int dtype;
+};
+
+static_assert(sizeof(Int4Attention) == 136, "the record that the caller packs");
+
+// A key whose page is none of the cache's is left out, and the status word says so.
+extern "C" int stride_attention_int4_exact(const void* record) {
+    const Int4Attention a = read_record<Int4Attention>(record);
+    if (a.tokens < 0 || a.nq <= 0 || a.nkv <= 0 || a.hd <= 0 || a.page_size <= 0 || a.table_width <= 0 || a.num_pages <= 0 || a.window < 0 ||
+        a.softcap < 0.f || a.nq % a.nkv)
         return STRIDE_BAD_ARGUMENT;
-    const int ctas_y = (nq + kExactWarps - 1) / kExactWarps;
-    if (hd > four::kMaxHeadDim || ctas_y > 65535 || (reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 4)
+    const int ctas_y = (a.nq + kExactWarps - 1) / kExactWarps;
+    if (a.hd > four::kMaxHeadDim || ctas_y > 65535 || (reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4)
         return STRIDE_UNSUPPORTED;
-    if (tokens == 0) return 0;
-    const dim3 grid(tokens, ctas_y), block(kExactWarps * 32);
-    const auto k = static_cast<const uint8_t*>(k_pages);
-    const auto v = static_cast<const uint8_t*>(v_pages);
-    if (dtype == STRIDE_DTYPE_F32)
-        stride::launch(attention_int4_exact_kernel<float>, grid, block, 0, stream, static_cast<const float*>(q), q_stride, static_cast<float*>(out), k, v,
-                       num_pages, block_table, table_width, seq_of_token, positions, nq, nkv, hd, page_size, scale, window, softcap, sinks, slopes, status);
-    else if (dtype == STRIDE_DTYPE_BF16)
-        stride::launch(attention_int4_exact_kernel<__nv_bfloat16>, grid, block, 0, stream, static_cast<const __nv_bfloat16*>(q), q_stride,
-                       static_cast<__nv_bfloat16*>(out), k, v, num_pages, block_table, table_width, seq_of_token, positions, nq, nkv, hd, page_size,
-                       scale, window, softcap, sinks, slopes, status);
+    if (a.tokens == 0) return 0;
+    const dim3 grid(a.tokens, ctas_y), block(kExactWarps * 32);
+    if (a.dtype == STRIDE_DTYPE_F32)
+        stride::launch(attention_int4_exact_kernel<float>, grid, block, 0, a.stream, static_cast<const float*>(a.q), a.q_stride,
+                       static_cast<float*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions, a.nq,
+                       a.nkv, a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
+    else if (a.dtype == STRIDE_DTYPE_BF16)
+        stride::launch(attention_int4_exact_kernel<__nv_bfloat16>, grid, block, 0, a.stream, static_cast<const __nv_bfloat16*>(a.q), a.q_stride,
+                       static_cast<__nv_bfloat16*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions,
+                       a.nq, a.nkv, a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
     else
         return STRIDE_BAD_ARGUMENT;
     return STRIDE_LAUNCH_STATUS();

@@ -4,23 +4,24 @@
 // the time its bytes take, an entry is never turned into a value: numbers go to the matrix instructions as they are, scales and centres are
 // applied to scores and weights, of which there are 32 times fewer.
 //
-//   score(t) = sum_g s_tg (q_g . n_t - 8 sum q_g) + c_tg sum q_g          out = sum_t (P_t s_tg) n_t - 8 sum_t P_t s_tg + sum_t P_t c_tg
+//   score(t) = sum_g s_tg (q_g . n_t) + (c_tg - 8 s_tg) sum q_g          out = sum_t (P_t s_tg) n_t + sum_t P_t (c_tg - 8 s_tg)
 //
 // * A number of 4 bits under the mask 0x000f000f (or 0x00f000f0) is a pair of 16-bit floating point numbers below the smallest normal one: n 2^-24
 //   (or n 2^-20). Matrix instructions take those exactly, so one instruction unpacks two entries. The factors are powers of two: the query's
 //   entries that meet the second kind are divided by 16 beforehand, the outputs of the second kind afterwards.
 // * Keys are the A operand (16 tokens by 16 entries), the 8 columns of B are the group's query heads; the products of a group of 32 entries end in
-//   an accumulator of their own, which starts at -8 sum q_g. Values are the A operand of the second product (16 entries by 16 tokens), the
-//   weights P_t s_tg, rounded once to 16 bits, its B operand: a transpose of 8 x 8 in the warp. What the offset of 8 adds is summed from the same
-//   rounded weights by a product with ones, so it cancels. Centres go through a product of their own in bfloat16, whose three-part sums of the
-//   query are exact.
+//   an accumulator of their own, which the token's scale multiplies. Values are the A operand of the second product (16 entries by 16 tokens),
+//   the weights P_t s_tg its B operand: a transpose of 8 x 8 in the warp.
+// * Scales and centres themselves go through products in bfloat16, which they are exact in: with the sums of the query (in two parts, 16 bits) on
+//   the side of the keys, with P on the side of the values. P is rounded to bfloat16 once, P s to 16 bits from that, so what the offset of 8
+//   adds in one product the other takes off to 2^-12.
 // * The query is scaled by a power of two to below 2^15. The reference R of a weight 2^(score - R) is the running maximum of score + log2 of the
 //   token's largest scale or centre, so that what is rounded to 16 bits lies below 2^8 and its largest above 2^-1 whatever the values' size;
 //   R moves only when a product passes 2^8 (a vote per tile), and then everything is rescaled.
 //
-// A warp owns tiles of 16 keys and a ring of copies: one bulk copy for the tile's keys and one for its values where pages hold whole tiles
-// (a page's rows of one head lie side by side), 16- or 8-byte copies by all lanes otherwise. Splits are merged as in attention_decode.cu, by the
-// CTA that draws the last ticket.
+// A warp owns tiles of 32 keys and a ring of copies: a bulk copy for each 16 keys and one for their values where pages hold whole sixteens (a page's
+// rows of one head lie side by side), 16- or 8-byte copies by all lanes otherwise. Splits are merged as in attention_decode.cu, by the CTA
+// that draws the last ticket.
 #include "int4_cache.cuh"
 #include "mma.cuh"
 #include "tcgen05.cuh"      // mbarrier helpers
@@ -28,11 +29,12 @@
 namespace stride {
 namespace four {
 
-constexpr int kTile = 16;               // keys of a warp's tile
+constexpr int kSub = 16;                // keys of half a tile: rows of a matrix instruction, and of a copy
+constexpr int kTile = 2 * kSub;         // keys of a warp's tile
 constexpr int kWarps = 4;
 constexpr int kUnit = kTile * kWarps;   // keys that a CTA's warps cover with a tile each
-constexpr int kStages = 4;
-constexpr int kMaxTiles = 32;           // of a warp: a lane looks each one's page up
+constexpr int kStages = 3;
+constexpr int kMaxTiles = 16;           // of a warp: a lane looks each half's page up
 constexpr int kTicketInts = 65536;      // ticket counters at the start of the scratch, one per (token, key head)
 constexpr int kCodeBeyondBound = 32;    // as in attention_decode.cu
 constexpr int kCodeCopyWait = 81;       // a wait for a tile's copies ran out
@@ -69,13 +71,17 @@ __device__ __forceinline__ void small_copy(uint32_t dst, const void* src) {
         asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 // D = A B + C, 16-bit floating point (or bfloat16) inputs, 32-bit accumulators.
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2], float c0, float c1,
+                                        float c2, float c3) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2], float c0, float c1,
+                                         float c2, float c3) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 // The transpose of an 8 x 8 matrix of 16-bit entries: lane l holds entries 2 (l % 4) and the next of row l / 4.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
@@ -103,7 +109,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[G], const void* p) {   
         w[0] = v.x; w[1] = v.y;
     }
 }
-// The token of a tile that stands in row r of the score tile: an order in which the lanes that read together find their rows in different banks
+// The token of half a tile that stands in row r of the score tile: an order in which the lanes that read together find their rows in different banks
 // (rows are 20 G bytes apart).
 template <int G>
 __device__ __forceinline__ int token_of(int r) {
@@ -121,7 +127,7 @@ __device__ __forceinline__ float amplitude(const uint32_t (&p)[G]) {
 // G: groups of a head (head size 32 G). NT: tiles of 8 query heads.
 template <int G, int NT, bool BULK>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(const Decode a) {
-    constexpr int HD = 32 * G, ROW = 20 * G, TILE = kTile * ROW;
+    constexpr int HD = 32 * G, ROW = 20 * G, HALF = kSub * ROW, STAGE = 4 * HALF;      // a stage: keys and values of either half
     pdl_trigger();
     pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];
@@ -150,59 +156,60 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         }
         return ((static_cast<size_t>(page) * a.nkv + kvh) * a.page_size + key % a.page_size) * ROW;
     };
-    size_t my_row = ~size_t(0);         // BULK: of the tile with this lane's number
-    bool mine = lane < n_tiles && tile_base(lane) <= pos && tile_base(lane) + kTile > first;
+    // lane 2 j + h answers for half h of tile j
+    const int my_key = tile_base(lane >> 1) + (lane & 1) * kSub;
+    size_t my_row = ~size_t(0);
+    bool mine = lane < 2 * n_tiles && my_key <= pos && my_key + kSub > first;
     if (BULK && mine) {
-        my_row = row_at(tile_base(lane));
+        my_row = row_at(my_key);
         mine = my_row != ~size_t(0);
     }
     const uint32_t live = __ballot_sync(0xffffffffu, mine);
-    unsigned char* ring = smem + warp * kStages * 2 * TILE;
+    unsigned char* ring = smem + warp * kStages * STAGE;
     if (BULK) {
         if (lane == 0)
             for (int s = 0; s < kStages; ++s) tc::mbar_init(tc::smem_u32(&bars[warp][s]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         __syncwarp();
     }
-    auto issue = [&](int j) {
+    auto issue = [&](int j, int stage) {
         if (BULK) {
-            if (j < n_tiles && lane == j && mine) {
-                const uint32_t dst = tc::smem_u32(ring + (j % kStages) * 2 * TILE), bar = tc::smem_u32(&bars[warp][j % kStages]);
-                tc::mbar_expect_tx(bar, 2 * TILE);
-                bulk_copy(dst, a.k_pages + my_row, TILE, bar);
-                bulk_copy(dst + TILE, a.v_pages + my_row, TILE, bar);
+            // (the barrier's one arrival, with the count of bytes, keeps the phase open whichever copy lands first)
+            if (j < n_tiles && (lane >> 1) == j && mine) {
+                const uint32_t dst = tc::smem_u32(ring + stage * STAGE + (lane & 1) * 2 * HALF), bar = tc::smem_u32(&bars[warp][stage]);
+                const uint32_t halves = live >> (2 * j) & 3u;
+                if ((lane & 1) == (halves == 2u)) tc::mbar_expect_tx(bar, halves == 3u ? 4 * HALF : 2 * HALF);
+                bulk_copy(dst, a.k_pages + my_row, HALF, bar);
+                bulk_copy(dst + HALF, a.v_pages + my_row, HALF, bar);
             }
             return;
         }
-        if (j < n_tiles && (live >> j & 1u)) {
+        if (j < n_tiles && (live >> (2 * j) & 3u)) {
             size_t row = ~size_t(0);
             const int key = tile_base(j) + lane;
-            if (lane < kTile && key >= first && key <= pos) row = row_at(key);
-            const uint32_t dst = tc::smem_u32(ring + (j % kStages) * 2 * TILE);
+            if (key >= first && key <= pos) row = row_at(key);
+            unsigned char* to = ring + stage * STAGE;
 #pragma unroll
-            for (int i = 0; i < 3; ++i) {               // 16 rows of 5 pieces
-                const int piece = i * 32 + lane, r = piece / 5, at = piece * 4 * G;
-                const size_t from = __shfl_sync(0xffffffffu, row, r & 15);
-                if (piece < kTile * 5) {
-                    if (from != ~size_t(0)) {
-                        small_copy<4 * G>(dst + at, a.k_pages + from + (piece - r * 5) * 4 * G);
-                        small_copy<4 * G>(dst + TILE + at, a.v_pages + from + (piece - r * 5) * 4 * G);
-                    } else {
-                        for (int b = 0; b < 4 * G; b += 4)
-                            *reinterpret_cast<uint32_t*>(ring + (j % kStages) * 2 * TILE + at + b) =
-                                *reinterpret_cast<uint32_t*>(ring + (j % kStages) * 2 * TILE + TILE + at + b) = 0u;
-                    }
+            for (int i = 0; i < 5; ++i) {               // 32 rows of 5 pieces
+                const int piece = i * 32 + lane, r = piece / 5, at = (r >> 4) * 2 * HALF + (r & 15) * ROW + (piece - r * 5) * 4 * G;
+                const size_t from = __shfl_sync(0xffffffffu, row, r);
+                if (from != ~size_t(0)) {
+                    small_copy<4 * G>(tc::smem_u32(to + at), a.k_pages + from + (piece - r * 5) * 4 * G);
+                    small_copy<4 * G>(tc::smem_u32(to + HALF + at), a.v_pages + from + (piece - r * 5) * 4 * G);
+                } else {
+                    for (int b = 0; b < 4 * G; b += 4)
+                        *reinterpret_cast<uint32_t*>(to + at + b) = *reinterpret_cast<uint32_t*>(to + HALF + at + b) = 0u;
                 }
             }
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) issue(s);
+    for (int s = 0; s < kStages; ++s) issue(s, s);
 
     // ---- the query: lane (g, c) holds, of head 8 nt + g, entries 32 grp + 8 c .. + 7
-    uint32_t qb[NT][G][2][2], cb[NT][2];            // B operands: of the numbers, of the centres
-    float start[NT][G][2], factor[NT][2], slope[NT][2];
+    uint32_t qb[NT][G][2][2], cb[NT][2];            // B operands: of the numbers, of centres and scales
+    float factor[NT][2], slope[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int head = 8 * nt + g;
@@ -228,10 +235,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // times 2^(up - 127), so that the largest entry lies in [2^14, 2^15); a query below 2^-113 keeps what 2^127 makes of it
-        const int up = min(254, 268 - static_cast<int>(__float_as_uint(most) >> 23));
+        // times 2^(up - 127), so that the largest entry lies in [2^14, 2^15); a query below 2^-112 keeps what 2^126 makes of it
+        const int up = min(253, 268 - static_cast<int>(__float_as_uint(most) >> 23));
         const float by = __uint_as_float(static_cast<uint32_t>(up) << 23);
-        float sums[G], own = 0.f;
+        float own = 0.f;
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
             float sum = 0.f;
@@ -242,20 +249,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sums[grp] = sum * 5.9604644775390625e-08f;              // in the units of the numbers, 2^-24
-            if ((c % G) == grp && c < G) own = sums[grp];
+            if (c == grp) own = sum * 5.9604644775390625e-08f;      // in the units of the numbers, 2^-24; lanes c >= G: no group, 0
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 qb[nt][grp][m][0] = pack_f16(x[grp][2 * m], x[grp][2 * m + 4]);
                 qb[nt][grp][m][1] = pack_f16(x[grp][2 * m + 1] * 0.0625f, x[grp][2 * m + 5] * 0.0625f);
             }
-            start[nt][grp][0] = -8.f * __shfl_sync(0xffffffffu, sums[grp], 8 * c);
-            start[nt][grp][1] = -8.f * __shfl_sync(0xffffffffu, sums[grp], 8 * c + 4);
         }
-        {       // the sum in three parts of 8 bits
-            const float hi = __bfloat162float(__float2bfloat16_rn(own)), mid = __bfloat162float(__float2bfloat16_rn(own - hi));
-            cb[nt][0] = pack_bf16(hi, mid);
-            cb[nt][1] = pack_bf16(own - hi - mid, 0.f);
+        {       // the sum in two parts of 8 bits, for the centre and, times -8, for the scale
+            const float high = __bfloat162float(__float2bfloat16_rn(own));
+            cb[nt][0] = pack_bf16(high, own - high);
+            cb[nt][1] = pack_bf16(-8.f * high, -8.f * (own - high));
         }
         const float down = __uint_as_float(static_cast<uint32_t>(254 - up) << 23) * ((a.cap_log2e > 0.f ? a.scale_over_cap : a.scale_log2e) * 16777216.f);
         factor[nt][0] = __shfl_sync(0xffffffffu, down, 8 * c);
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             slope[nt][e] = a.slopes != nullptr && 8 * nt + 2 * c + e < group ? a.slopes[kvh * group + 8 * nt + 2 * c + e] * 1.4426950408889634f : 0.f;
     }
 
-    float R[NT][2], l[NT][2], o[NT][G][2][4], ones[NT][G][4], cen[NT][4];
+    float R[NT][2], l[NT][2], o[NT][G][2][4], cen[NT][4];       // cen: rows 0 .. G - 1 for the centres, from 4 on for the scales
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         R[nt][0] = R[nt][1] = -INFINITY;
@@ -274,135 +278,207 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         for (int e = 0; e < 4; ++e) {
             cen[nt][e] = 0.f;
 #pragma unroll
-            for (int grp = 0; grp < G; ++grp) ones[nt][grp][e] = o[nt][grp][0][e] = o[nt][grp][1][e] = 0.f;
+            for (int grp = 0; grp < G; ++grp) o[nt][grp][0][e] = o[nt][grp][1][e] = 0.f;
         }
     }
     const int row_a = token_of<G>(g), row_b = token_of<G>(g + 8);                                   // tokens of this lane's score rows
     const int col[4] = {token_of<G>(2 * c), token_of<G>(2 * c + 1), token_of<G>(2 * c + 8), token_of<G>(2 * c + 9)};        // of its weights
+    const uint32_t pick = g < 4 ? 0x7632u : 0x5410u;            // rows of `cen`: centres or scales
+    const bool bent = a.cap_log2e > 0.f || a.slopes != nullptr;
     bool alive = true;
     uint32_t uses = 0;
+    int stage = 0;
     for (int j = 0; j < n_tiles; ++j) {
+        const uint32_t halves = live >> (2 * j) & 3u;
         if (BULK) {
-            if ((live >> j & 1u) && alive) {
-                alive = __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&bars[warp][j % kStages]), uses >> (j % kStages) & 1u, a.status, kCodeCopyWait));
-                uses ^= 1u << (j % kStages);
+            if (halves && alive) {
+                alive = __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&bars[warp][stage]), uses >> stage & 1u, a.status, kCodeCopyWait));
+                uses ^= 1u << stage;
             }
         } else {
             cp_async_wait<kStages - 1>();
             __syncwarp();
         }
-        if ((live >> j & 1u) && alive) {
-            const unsigned char* ks = ring + (j % kStages) * 2 * TILE;
-            const unsigned char* vs = ks + TILE;
+        if (halves && alive) {
+            const unsigned char* at = ring + stage * STAGE;
             const int base = tile_base(j);
-            uint32_t kw[2][G], kp[2][G], vp[2][G], vw[4][G / 2], vc[4];
-            load_words<G>(kw[0], ks + row_a * ROW + c * 4 * G);
-            load_words<G>(kw[1], ks + row_b * ROW + c * 4 * G);
-            load_words<G>(kp[0], ks + row_a * ROW + 16 * G);
-            load_words<G>(kp[1], ks + row_b * ROW + 16 * G);
-            const uint32_t ca = *reinterpret_cast<const uint32_t*>(ks + row_a * ROW + 16 * G + 4 * (c % G)),
-                           cc = *reinterpret_cast<const uint32_t*>(ks + row_b * ROW + 16 * G + 4 * (c % G));
-            load_words<G>(vp[0], vs + row_a * ROW + 16 * G);
-            load_words<G>(vp[1], vs + row_b * ROW + 16 * G);
+            // some key of the tile is behind the token, before its window or without a page: what its row holds counts for nothing
+            const bool edge = halves != 3u || base + kTile - 1 > pos || base < first;
+            float x[NT][2][4], P[NT][2][4], amp[2][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (G == 4) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(vs + col[i] * ROW + g * 2 * G);
-                    vw[i][0] = v.x;
-                    vw[i][1] = v.y;
-                } else {
-                    vw[i][0] = *reinterpret_cast<const uint32_t*>(vs + col[i] * ROW + g * 2 * G);
-                }
-                vc[i] = *reinterpret_cast<const uint32_t*>(vs + col[i] * ROW + 16 * G + 4 * (g % G));
-            }
-            const bool edge = base + kTile - 1 > pos || base < first;
-            const bool ok_a = base + row_a <= pos && base + row_a >= first, ok_b = base + row_b <= pos && base + row_b >= first;
-            if (edge) {         // rows of the page behind the token, or before its window, may hold anything: their scales and centres count for nothing
+            for (int h = 0; h < 2; ++h) {
+                const unsigned char* ks = at + h * 2 * HALF;
+                uint32_t kw[2][G], kp[2][G];
+                load_words<G>(kw[0], ks + row_a * ROW + c * 4 * G);
+                load_words<G>(kw[1], ks + row_b * ROW + c * 4 * G);
+                load_words<G>(kp[0], ks + row_a * ROW + 16 * G);
+                load_words<G>(kp[1], ks + row_b * ROW + 16 * G);
+                const uint32_t ca = *reinterpret_cast<const uint32_t*>(ks + row_a * ROW + 16 * G + 4 * (c % G)),
+                               cc = *reinterpret_cast<const uint32_t*>(ks + row_b * ROW + 16 * G + 4 * (c % G));
+                const uint32_t c0 = __byte_perm(ca, ca, 0x3232), c1 = __byte_perm(cc, cc, 0x3232), c2 = __byte_perm(ca, ca, 0x1010),
+                               c3 = __byte_perm(cc, cc, 0x1010);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_bf16(x[nt][h], c0, c1, c2, c3, cb[nt], 0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int grp = 0; grp < G; ++grp) {
-                    if (!ok_a) vp[0][grp] = 0u;
-                    if (!ok_b) vp[1][grp] = 0u;
-                }
+                    const uint32_t w0 = kw[0][grp], w1 = kw[1][grp], u0 = w0 >> 8, u1 = w1 >> 8;
+                    const float s0 = bf16_low(kp[0][grp]), s1 = bf16_low(kp[1][grp]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (base + col[i] > pos || base + col[i] < first) vc[i] = 0u;
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float acc[4];
+                        mma_f16(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[nt][grp][0], 0.f, 0.f, 0.f, 0.f);
+                        mma_f16(acc, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qb[nt][grp][1], acc[0], acc[1], acc[2], acc[3]);
+                        x[nt][h][0] = fmaf(s0, acc[0], x[nt][h][0]);
+                        x[nt][h][1] = fmaf(s0, acc[1], x[nt][h][1]);
+                        x[nt][h][2] = fmaf(s1, acc[2], x[nt][h][2]);
+                        x[nt][h][3] = fmaf(s1, acc[3], x[nt][h][3]);
+                    }
+                }
+                uint32_t vp[2][G];
+                load_words<G>(vp[0], ks + HALF + row_a * ROW + 16 * G);
+                load_words<G>(vp[1], ks + HALF + row_b * ROW + 16 * G);
+                amp[h][0] = amplitude<G>(vp[0]);
+                amp[h][1] = amplitude<G>(vp[1]);
             }
-            const float amp[2] = {amplitude<G>(vp[0]), amplitude<G>(vp[1])};
-            float P[NT][4];
+            // x becomes the score in units of log2
+            if (bent) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float y = x[nt][h][e] * factor[nt][e & 1];
+                            if (a.cap_log2e > 0.f) y = a.cap_log2e * tanh_quick(y);
+                            x[nt][h][e] = fmaf(slope[nt][e & 1], static_cast<float>(base + h * kSub + (e < 2 ? row_a : row_b) - pos), y);
+                        }
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[nt][h][e] *= factor[nt][e & 1];
+            }
+            uint32_t seen = 0xfu;           // of the score rows: half 0 row_a, row_b, half 1 row_a, row_b
+            if (edge) {
+                seen = 0u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int key = base + h * kSub + (r ? row_b : row_a);
+                        const bool ok = (halves >> h & 1u) && key <= pos && key >= first;
+                        seen |= ok ? 1u << (2 * h + r) : 0u;
+                        if (!ok) {
+                            amp[h][r] = 0.f;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) x[nt][h][2 * r] = x[nt][h][2 * r + 1] = -INFINITY;
+                        }
+                    }
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_bf16(x, __byte_perm(ca, ca, 0x3232), __byte_perm(cc, cc, 0x3232), __byte_perm(ca, ca, 0x3232), __byte_perm(cc, cc, 0x3232), cb[nt][0],
-                         cb[nt][1]);
+                float high = 0.f;
 #pragma unroll
-                for (int grp = 0; grp < G; ++grp) {
-                    float acc[4] = {start[nt][grp][0], start[nt][grp][1], start[nt][grp][0], start[nt][grp][1]};
-                    const uint32_t w0 = kw[0][grp], w1 = kw[1][grp], u0 = w0 >> 8, u1 = w1 >> 8;
-                    mma_f16(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qb[nt][grp][0][0], qb[nt][grp][0][1]);
-                    mma_f16(acc, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qb[nt][grp][1][0], qb[nt][grp][1][1]);
-                    const float s0 = bf16_low(kp[0][grp]), s1 = bf16_low(kp[1][grp]);
-                    x[0] = fmaf(s0, acc[0], x[0]);
-                    x[1] = fmaf(s0, acc[1], x[1]);
-                    x[2] = fmaf(s1, acc[2], x[2]);
-                    x[3] = fmaf(s1, acc[3], x[3]);
-                }
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[e] *= factor[nt][e & 1];
-                    if (a.cap_log2e > 0.f) x[e] = a.cap_log2e * tanh_quick(x[e]);
-                    if (a.slopes != nullptr) x[e] = fmaf(slope[nt][e & 1], static_cast<float>(base + (e < 2 ? row_a : row_b) - pos), x[e]);
-                    if (edge && !(e < 2 ? ok_a : ok_b)) x[e] = -INFINITY;
-                    P[nt][e] = exp2_quick(x[e] - R[nt][e & 1]);
+                    for (int e = 0; e < 4; ++e) P[nt][h][e] = exp2_quick(x[nt][h][e] - R[nt][e & 1]);
                 }
-                const float high = fmaxf(fmaxf(P[nt][0], P[nt][1]) * amp[0], fmaxf(P[nt][2], P[nt][3]) * amp[1]);
-                if (__any_sync(0xffffffffu, !(high <= kLimit))) {          // (at first R is -inf, and weights are infinite or no numbers)
+                // (a maximum passes a NaN over: while R is -inf, in the first tile, every weight is infinite or none, and the sum shows it)
+                high = fmaxf(fmaxf(fmaxf(P[nt][0][0], P[nt][0][1]) * amp[0][0], fmaxf(P[nt][0][2], P[nt][0][3]) * amp[0][1]),
+                             fmaxf(fmaxf(P[nt][1][0], P[nt][1][1]) * amp[1][0], fmaxf(P[nt][1][2], P[nt][1][3]) * amp[1][1]));
+                if (__any_sync(0xffffffffu, !(high <= kLimit) || R[nt][0] == -INFINITY)) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float most = fmaxf(x[e] + fmaxf(__log2f(amp[0]), kLeastLog), x[e + 2] + fmaxf(__log2f(amp[1]), kLeastLog));
+                        float most = -INFINITY;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) most = fmaxf(most, x[nt][h][2 * r + e] + fmaxf(__log2f(amp[h][r]), kLeastLog));
 #pragma unroll
                         for (int s = 4; s < 32; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
-                        const float next = fmaxf(R[nt][e], most);
-                        const float by = R[nt][e] == -INFINITY ? 0.f : exp2_quick(R[nt][e] - next);
+                        const float next = fmaxf(R[nt][e], most), by = R[nt][e] == -INFINITY ? 0.f : exp2_quick(R[nt][e] - next);
                         R[nt][e] = next;
                         l[nt][e] *= by;
                         cen[nt][e] *= by;
 #pragma unroll
-                        for (int grp = 0; grp < G; ++grp) {
-                            ones[nt][grp][e] *= by;
+                        for (int grp = 0; grp < G; ++grp)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 o[nt][grp][h][e] *= by;
                                 o[nt][grp][h][e + 2] *= by;
                             }
-                        }
                         // (-inf: the column has seen no key, or only such as are no numbers, which the weights then are, too)
-                        P[nt][e] = exp2_quick(x[e] - (next == -INFINITY ? 0.f : next));
-                        P[nt][e + 2] = exp2_quick(x[e + 2] - (next == -INFINITY ? 0.f : next));
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) P[nt][h][2 * r + e] = exp2_quick(x[nt][h][2 * r + e] - (next == -INFINITY ? 0.f : next));
                     }
                 }
-                l[nt][0] += P[nt][0] + P[nt][2];
-                l[nt][1] += P[nt][1] + P[nt][3];
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                mma_bf16(cen[nt], __byte_perm(vc[0], vc[1], 0x7632), 0u, __byte_perm(vc[2], vc[3], 0x7632), 0u, transposed(pack_bf16(P[nt][0], P[nt][1])),
-                         transposed(pack_bf16(P[nt][2], P[nt][3])));
+            for (int h = 0; h < 2; ++h) {
+                const unsigned char* vs = at + h * 2 * HALF + HALF;
+                uint32_t vp[2][G], vw[4][G / 2], vc[4];
+                load_words<G>(vp[0], vs + row_a * ROW + 16 * G);
+                load_words<G>(vp[1], vs + row_b * ROW + 16 * G);
 #pragma unroll
-            for (int grp = 0; grp < G; ++grp) {
-                const uint32_t x0 = __byte_perm(vw[0][grp >> 1], vw[1][grp >> 1], grp & 1 ? 0x7632 : 0x5410),
-                               x1 = __byte_perm(vw[2][grp >> 1], vw[3][grp >> 1], grp & 1 ? 0x7632 : 0x5410), y0 = x0 >> 8, y1 = x1 >> 8;
-                const float s0 = bf16_low(vp[0][grp]), s1 = bf16_low(vp[1][grp]);
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (G == 4) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(vs + col[i] * ROW + g * 2 * G);
+                        vw[i][0] = v.x;
+                        vw[i][1] = v.y;
+                    } else {
+                        vw[i][0] = *reinterpret_cast<const uint32_t*>(vs + col[i] * ROW + g * 2 * G);
+                    }
+                    vc[i] = *reinterpret_cast<const uint32_t*>(vs + col[i] * ROW + 16 * G + 4 * (g % G));
+                }
+                if (edge) {
+#pragma unroll
+                    for (int grp = 0; grp < G; ++grp) {
+                        if (!(seen >> (2 * h) & 1u)) vp[0][grp] = 0u;
+                        if (!(seen >> (2 * h + 1) & 1u)) vp[1][grp] = 0u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = base + h * kSub + col[i];
+                        if (!(halves >> h & 1u) || key > pos || key < first) vc[i] = 0u;
+                    }
+                }
+                const uint32_t a0 = __byte_perm(vc[0], vc[1], pick), a2 = __byte_perm(vc[2], vc[3], pick);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const uint32_t b0 = transposed(pack_f16(P[nt][0] * s0, P[nt][1] * s0)), b1 = transposed(pack_f16(P[nt][2] * s1, P[nt][3] * s1));
-                    mma_f16(o[nt][grp][0], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, b0, b1);
-                    mma_f16(o[nt][grp][1], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, b0, b1);
-                    mma_f16(ones[nt][grp], 0x3c003c00u, 0u, 0x3c003c00u, 0u, b0, b1);
+                    const uint32_t pa = pack_bf16(P[nt][h][0], P[nt][h][1]), pb = pack_bf16(P[nt][h][2], P[nt][h][3]);
+                    P[nt][h][0] = bf16_low(pa);
+                    P[nt][h][1] = bf16_high(pa);
+                    P[nt][h][2] = bf16_low(pb);
+                    P[nt][h][3] = bf16_high(pb);
+                    l[nt][0] += P[nt][h][0] + P[nt][h][2];
+                    l[nt][1] += P[nt][h][1] + P[nt][h][3];
+                    const uint32_t b[2] = {transposed(pa), transposed(pb)};
+                    mma_bf16(cen[nt], a0, 0u, a2, 0u, b, cen[nt][0], cen[nt][1], cen[nt][2], cen[nt][3]);
+                }
+#pragma unroll
+                for (int grp = 0; grp < G; ++grp) {
+                    const uint32_t x0 = __byte_perm(vw[0][grp >> 1], vw[1][grp >> 1], grp & 1 ? 0x7632 : 0x5410),
+                                   x1 = __byte_perm(vw[2][grp >> 1], vw[3][grp >> 1], grp & 1 ? 0x7632 : 0x5410), y0 = x0 >> 8, y1 = x1 >> 8;
+                    const float s0 = bf16_low(vp[0][grp]), s1 = bf16_low(vp[1][grp]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t b[2] = {transposed(pack_f16(P[nt][h][0] * s0, P[nt][h][1] * s0)),
+                                               transposed(pack_f16(P[nt][h][2] * s1, P[nt][h][3] * s1))};
+                        float(&d)[4] = o[nt][grp][0];
+                        float(&f)[4] = o[nt][grp][1];
+                        mma_f16(d, x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, b, d[0], d[1], d[2], d[3]);
+                        mma_f16(f, y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, b, f[0], f[1], f[2], f[3]);
+                    }
                 }
             }
         }
         __syncwarp();           // every lane is done with the stage before it is refilled
-        issue(j + kStages);
+        issue(j + kStages, stage);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 
     // ---- the warps' results side by side in shared memory (the rings are no longer needed)
@@ -421,7 +497,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             float* dst = red + (warp * group + head) * RS;
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
-                const float centre = __shfl_sync(0xffffffffu, cen[nt][e], 4 * grp + c) - 8.f * ones[nt][grp][e];
+                const float centre = __shfl_sync(0xffffffffu, cen[nt][e], 4 * grp + c) - 8.f * __shfl_sync(0xffffffffu, cen[nt][e], 4 * (4 + grp) + c);
                 if (head < group) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -521,23 +597,29 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
     }
 }
 
-// Keys per CTA, a multiple of 64 up to 2048: by the launch's sizes alone, so that a captured graph stays valid.
+// Keys per CTA, a multiple of 128 up to 2048: by the launch's sizes alone, so that a captured graph stays valid.
 inline int choose_split_keys(int tokens, int nkv, int max_context) {
+    static const int forced = [] {      // tuning hook: STRIDE_DECODE_INT4_SPLIT_KEYS=<multiple of 128>
+        const char* e = getenv("STRIDE_DECODE_INT4_SPLIT_KEYS");
+        const int v = e ? atoi(e) : 0;
+        return v > 0 ? (v < kMaxTiles * kUnit ? (v + kUnit - 1) / kUnit * kUnit : kMaxTiles * kUnit) : 0;
+    }();
+    if (forced) return forced;
     const long long units = static_cast<long long>(tokens) * nkv * ((max_context + kUnit - 1) / kUnit);
     long long u = (units + 820) / 821;
     if (u < 4) u = (units + 206) / 207;
-    u = u < 2 ? 2 : (u > kMaxTiles ? kMaxTiles : u);
+    u = u < 1 ? 1 : (u > kMaxTiles ? kMaxTiles : u);
     return static_cast<int>(u) * kUnit;
 }
 
 template <int G, int NT>
 int launch_decode(const Decode& a, int tokens, cudaStream_t stream) {
-    constexpr int smem = kWarps * kStages * 2 * kTile * 20 * G;
+    constexpr int smem = kWarps * kStages * 2 * kTile * 20 * G;        // 61 KB at head size 128
     const int group = a.nq / a.nkv;
     static_assert(kWarps * 8 * NT * (32 * G + 2) * 4 <= smem || NT > 1, "the merge fits into the rings");
     const long long merge = static_cast<long long>(group) * (a.num_splits + 1) * 4, warps = static_cast<long long>(kWarps) * group * (32 * G + 2) * 4;
     if (merge > smem || warps > smem) return STRIDE_UNSUPPORTED;
-    const bool bulk = a.page_size % kTile == 0;
+    const bool bulk = a.page_size % kSub == 0;
     cudaError_t e = allow_shared<decode_kernel<G, NT, true>>(smem);
     if (e == cudaSuccess) e = allow_shared<decode_kernel<G, NT, false>>(smem);
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -564,55 +646,74 @@ long long stride_decode_int4_scratch_floats(int tokens, int nq, int nkv, int hd,
     return four::kTicketInts + static_cast<long long>(tokens) * nq * splits * (hd + 2);
 }
 
+struct DecodeCall {
+    const __nv_bfloat16* q;         // [tokens, q_stride] with head h at columns [h hd, (h + 1) hd)
+    __nv_bfloat16* out;             // [tokens, nq hd]
+    const uint8_t* k_pages;         // [num_pages, nkv, page_size, 20 hd / 32]
+    const uint8_t* v_pages;
+    const int32_t* block_table;     // [requests, table_width]
+    const int32_t* seq_of_token;
+    const int32_t* positions;
+    float* scratch;
+    const float* sinks;
+    const float* slopes;
+    int* status;
+    cudaStream_t stream;
+    long long scratch_floats;
+    int q_stride, num_pages, table_width, tokens, nq, nkv, hd, page_size, window, max_context;
+    float scale, softcap;
+};
+
+static_assert(sizeof(DecodeCall) == 152, "the record that the caller packs");
+
 // One query token per row. `scratch` must be zero when it is first used (every launch leaves its tickets zero) and belongs to one stream at a
 // time. A row whose position does not lie below `max_context` gets zeros, and code 32 in the status word; a key whose page is none of the
 // cache's is left out, with code 33. Returns -2 for sizes it does not run: head sizes other than 64 and 128, groups above 16, more than
 // 65536 (token, key head) pairs, contexts of more than 8192 splits.
-int stride_decode_int4(const void* q, int q_stride, void* out, const void* k_pages, const void* v_pages, int num_pages, const int32_t* block_table,
-                       int table_width, const int32_t* seq_of_token, const int32_t* positions, float* scratch, long long scratch_floats, int tokens,
-                       int nq, int nkv, int hd, int page_size, float scale, int window, float softcap, const float* sinks, const float* slopes,
-                       int max_context, int* status, cudaStream_t stream) {
-    if (tokens < 0 || nq <= 0 || nkv <= 0 || page_size <= 0 || table_width <= 0 || num_pages <= 0 || window < 0 || softcap < 0.f || max_context <= 0 ||
-        nq % nkv || status == nullptr)
+int stride_decode_int4(const void* record) {
+    const DecodeCall r = read_record<DecodeCall>(record);
+    if (r.tokens < 0 || r.nq <= 0 || r.nkv <= 0 || r.page_size <= 0 || r.table_width <= 0 || r.num_pages <= 0 || r.window < 0 || r.softcap < 0.f ||
+        r.max_context <= 0 || r.nq % r.nkv || r.status == nullptr)
         return STRIDE_BAD_ARGUMENT;
-    if ((hd != 64 && hd != 128) || nq / nkv > 16 || tokens > 65535 || nkv > 65535 || max_context > (1 << 30)) return STRIDE_UNSUPPORTED;
-    if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 16 || reinterpret_cast<uintptr_t>(scratch) % 16)
+    if ((r.hd != 64 && r.hd != 128) || r.nq / r.nkv > 16 || r.tokens > 65535 || r.nkv > 65535 || r.max_context > (1 << 30)) return STRIDE_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(r.k_pages) | reinterpret_cast<uintptr_t>(r.v_pages) | reinterpret_cast<uintptr_t>(r.scratch)) % 16)
         return STRIDE_UNSUPPORTED;
-    if (tokens == 0) return 0;
-    const int split_keys = four::choose_split_keys(tokens, nkv, max_context);
-    const int num_splits = (max_context + split_keys - 1) / split_keys;
-    if (num_splits > 8192 || static_cast<long long>(tokens) * nkv > four::kTicketInts) return STRIDE_UNSUPPORTED;
-    if (scratch == nullptr || scratch_floats < stride_decode_int4_scratch_floats(tokens, nq, nkv, hd, max_context)) return STRIDE_BAD_ARGUMENT;
+    if (r.tokens == 0) return 0;
+    const int split_keys = four::choose_split_keys(r.tokens, r.nkv, r.max_context);
+    const int num_splits = (r.max_context + split_keys - 1) / split_keys;
+    if (num_splits > 8192 || static_cast<long long>(r.tokens) * r.nkv > four::kTicketInts) return STRIDE_UNSUPPORTED;
+    if (r.scratch == nullptr || r.scratch_floats < stride_decode_int4_scratch_floats(r.tokens, r.nq, r.nkv, r.hd, r.max_context))
+        return STRIDE_BAD_ARGUMENT;
     static_assert(sizeof(int) == sizeof(float), "the tickets live in the float scratch");
     four::Decode a;
-    a.q = static_cast<const __nv_bfloat16*>(q);
-    a.out = static_cast<__nv_bfloat16*>(out);
-    a.k_pages = static_cast<const uint8_t*>(k_pages);
-    a.v_pages = static_cast<const uint8_t*>(v_pages);
-    a.table = block_table;
-    a.seq_of_token = seq_of_token;
-    a.positions = positions;
-    a.sinks = sinks;
-    a.slopes = slopes;
-    a.tickets = reinterpret_cast<int*>(scratch);
-    a.part_o = scratch + four::kTicketInts;
-    a.part_ml = a.part_o + static_cast<long long>(tokens) * nq * num_splits * hd;
-    a.status = status;
-    a.q_stride = q_stride;
-    a.table_width = table_width;
-    a.num_pages = num_pages;
-    a.nq = nq;
-    a.nkv = nkv;
-    a.page_size = page_size;
-    a.window = window;
+    a.q = r.q;
+    a.out = r.out;
+    a.k_pages = r.k_pages;
+    a.v_pages = r.v_pages;
+    a.table = r.block_table;
+    a.seq_of_token = r.seq_of_token;
+    a.positions = r.positions;
+    a.sinks = r.sinks;
+    a.slopes = r.slopes;
+    a.tickets = reinterpret_cast<int*>(r.scratch);
+    a.part_o = r.scratch + four::kTicketInts;
+    a.part_ml = a.part_o + static_cast<long long>(r.tokens) * r.nq * num_splits * r.hd;
+    a.status = r.status;
+    a.q_stride = r.q_stride;
+    a.table_width = r.table_width;
+    a.num_pages = r.num_pages;
+    a.nq = r.nq;
+    a.nkv = r.nkv;
+    a.page_size = r.page_size;
+    a.window = r.window;
     a.split_keys = split_keys;
     a.num_splits = num_splits;
-    a.scale_log2e = scale * 1.4426950408889634f;
-    a.cap_log2e = softcap * 1.4426950408889634f;
-    a.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;
-    const bool wide = nq / nkv > 8;
-    if (hd == 64) return wide ? four::launch_decode<2, 2>(a, tokens, stream) : four::launch_decode<2, 1>(a, tokens, stream);
-    return wide ? four::launch_decode<4, 2>(a, tokens, stream) : four::launch_decode<4, 1>(a, tokens, stream);
+    a.scale_log2e = r.scale * 1.4426950408889634f;
+    a.cap_log2e = r.softcap * 1.4426950408889634f;
+    a.scale_over_cap = r.softcap > 0.f ? r.scale / r.softcap : 0.f;
+    const bool wide = r.nq / r.nkv > 8;
+    if (r.hd == 64) return wide ? four::launch_decode<2, 2>(a, r.tokens, r.stream) : four::launch_decode<2, 1>(a, r.tokens, r.stream);
+    return wide ? four::launch_decode<4, 2>(a, r.tokens, r.stream) : four::launch_decode<4, 1>(a, r.tokens, r.stream);
 }
 
 }  // extern "C"

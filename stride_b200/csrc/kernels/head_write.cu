@@ -8,7 +8,7 @@ namespace stride {
 
 constexpr int kWriteWarps = 4;
 
-struct HeadWrite {
+struct HeadWrite {                  // a record that the caller packs: addresses, then 64-bit, then 32-bit numbers
     const void* rows;               // [tokens, (nq + 2 nkv) hd]
     void* q_out;                    // head h of token t at q_out[t * q_out_stride + h * hd]
     const float* bias;              // [(nq + 2 nkv) hd] or null
@@ -21,10 +21,13 @@ struct HeadWrite {
     void* k_pages;
     void* v_pages;
     int* status;
+    cudaStream_t stream;
     long long q_out_stride;
+    int num_positions, num_pages, bits4, tokens, nq, nkv, hd, page_size, rotate, dtype;
     float eps;
-    int tokens, nq, nkv, hd, page_size, num_pages, num_positions, rotate;
 };
+
+static_assert(sizeof(HeadWrite) == 160, "the record that the caller packs");
 
 // A warp a unit: a query head, or a key head with its value head. Lane l holds entry 32 j + l of the head in x[j], so a group of 32 is
 // one register of the warp.
@@ -290,67 +293,90 @@ using namespace stride;
 // rows: [tokens, (nq + 2 nkv) hd]; q_out: rows of q_out_stride elements (`rows` itself, with its row length, for queries in place).
 // bits4: pages hold 4 bits (uint8 [num_pages, nkv, page_size, 20 ceil(hd / 32)]), else elements [num_pages, nkv, page_size, hd]. slots null, or
 // a slot below zero: keys and values are not stored. Slots of one launch are distinct. Returns -2 for odd head sizes and those above 256.
-extern "C" int stride_head_write(const void* rows, void* q_out, long long q_out_stride, const float* bias, const float* q_norm, const float* k_norm,
-                                 float eps, const int32_t* positions, const int32_t* slots, const float* cos, const float* sin, int num_positions,
-                                 void* k_pages, void* v_pages, int num_pages, int bits4, int tokens, int nq, int nkv, int hd, int page_size, int rotate,
-                                 int dtype, int* status, cudaStream_t stream) {
-    if (tokens < 0 || nq <= 0 || nkv <= 0 || hd <= 0 || page_size <= 0 || num_pages <= 0 || q_out_stride < static_cast<long long>(nq) * hd ||
-        (q_norm == nullptr) != (k_norm == nullptr) || (rotate && num_positions <= 0) || static_cast<long long>(num_pages) * page_size > 2147483647LL)
+extern "C" int stride_head_write(const void* record) {
+    const HeadWrite a = read_record<HeadWrite>(record);
+    if (a.tokens < 0 || a.nq <= 0 || a.nkv <= 0 || a.hd <= 0 || a.page_size <= 0 || a.num_pages <= 0 ||
+        a.q_out_stride < static_cast<long long>(a.nq) * a.hd || (a.q_norm == nullptr) != (a.k_norm == nullptr) || (a.rotate && a.num_positions <= 0) ||
+        static_cast<long long>(a.num_pages) * a.page_size > 2147483647LL)
         return STRIDE_BAD_ARGUMENT;
-    if (hd > four::kMaxHeadDim || (rotate && hd % 2)) return STRIDE_UNSUPPORTED;
-    if (bits4 && (reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 4) return STRIDE_UNSUPPORTED;
-    const int units = nq + nkv, ctas_y = (units + kWriteWarps - 1) / kWriteWarps;
+    if (a.hd > four::kMaxHeadDim || (a.rotate && a.hd % 2)) return STRIDE_UNSUPPORTED;
+    if (a.bits4 && (reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4) return STRIDE_UNSUPPORTED;
+    const int units = a.nq + a.nkv, ctas_y = (units + kWriteWarps - 1) / kWriteWarps;
     if (ctas_y > 65535) return STRIDE_UNSUPPORTED;
-    if (tokens == 0) return 0;
-    const HeadWrite a{rows, q_out, bias, q_norm, k_norm, positions, slots, cos, sin, k_pages, v_pages, status, q_out_stride, eps,
-                      tokens, nq, nkv, hd, page_size, num_pages, num_positions, rotate};
-    const dim3 grid(tokens, ctas_y), block(kWriteWarps * 32);
-    if (dtype == STRIDE_DTYPE_F32)
-        bits4 ? stride::launch(head_write_kernel<float, true>, grid, block, 0, stream, a)
-              : stride::launch(head_write_kernel<float, false>, grid, block, 0, stream, a);
-    else if (dtype == STRIDE_DTYPE_BF16)
-        bits4 ? stride::launch(head_write_kernel<__nv_bfloat16, true>, grid, block, 0, stream, a)
-              : stride::launch(head_write_kernel<__nv_bfloat16, false>, grid, block, 0, stream, a);
+    if (a.tokens == 0) return 0;
+    const dim3 grid(a.tokens, ctas_y), block(kWriteWarps * 32);
+    if (a.dtype == STRIDE_DTYPE_F32)
+        a.bits4 ? stride::launch(head_write_kernel<float, true>, grid, block, 0, a.stream, a)
+                : stride::launch(head_write_kernel<float, false>, grid, block, 0, a.stream, a);
+    else if (a.dtype == STRIDE_DTYPE_BF16)
+        a.bits4 ? stride::launch(head_write_kernel<__nv_bfloat16, true>, grid, block, 0, a.stream, a)
+                : stride::launch(head_write_kernel<__nv_bfloat16, false>, grid, block, 0, a.stream, a);
     else
         return STRIDE_BAD_ARGUMENT;
     return STRIDE_LAUNCH_STATUS();
 }
 
-extern "C" int stride_int4_read(const void* k_pages, const void* v_pages, const int32_t* slots, void* k_out, void* v_out, int n, int nkv, int hd,
-                                int page_size, int num_pages, int dtype, int* status, cudaStream_t stream) {
-    if (n < 0 || nkv <= 0 || hd <= 0 || page_size <= 0 || num_pages <= 0) return STRIDE_BAD_ARGUMENT;
-    if (hd > four::kMaxHeadDim || (reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 4) return STRIDE_UNSUPPORTED;
-    if (n == 0) return 0;
-    const long long ctas = (static_cast<long long>(n) * nkv + kWriteWarps - 1) / kWriteWarps;
+struct Int4Read {
+    const uint8_t* k_pages;
+    const uint8_t* v_pages;
+    const int32_t* slots;
+    void* k_out;            // [n, nkv, hd]
+    void* v_out;
+    int* status;
+    cudaStream_t stream;
+    int n, nkv, hd, page_size, num_pages, dtype;
+};
+
+static_assert(sizeof(Int4Read) == 80, "the record that the caller packs");
+
+extern "C" int stride_int4_read(const void* record) {
+    const Int4Read a = read_record<Int4Read>(record);
+    if (a.n < 0 || a.nkv <= 0 || a.hd <= 0 || a.page_size <= 0 || a.num_pages <= 0) return STRIDE_BAD_ARGUMENT;
+    if (a.hd > four::kMaxHeadDim || (reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4) return STRIDE_UNSUPPORTED;
+    if (a.n == 0) return 0;
+    const long long ctas = (static_cast<long long>(a.n) * a.nkv + kWriteWarps - 1) / kWriteWarps;
     if (ctas > 2147483647LL) return STRIDE_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(ctas)), block(kWriteWarps * 32);
-    const auto k = static_cast<const uint8_t*>(k_pages);
-    const auto v = static_cast<const uint8_t*>(v_pages);
-    if (dtype == STRIDE_DTYPE_F32)
-        stride::launch(int4_read_kernel<float>, grid, block, 0, stream, k, v, slots, static_cast<float*>(k_out), static_cast<float*>(v_out), n, nkv, hd,
-                       page_size, num_pages, status);
-    else if (dtype == STRIDE_DTYPE_BF16)
-        stride::launch(int4_read_kernel<__nv_bfloat16>, grid, block, 0, stream, k, v, slots, static_cast<__nv_bfloat16*>(k_out),
-                       static_cast<__nv_bfloat16*>(v_out), n, nkv, hd, page_size, num_pages, status);
+    if (a.dtype == STRIDE_DTYPE_F32)
+        stride::launch(int4_read_kernel<float>, grid, block, 0, a.stream, a.k_pages, a.v_pages, a.slots, static_cast<float*>(a.k_out),
+                       static_cast<float*>(a.v_out), a.n, a.nkv, a.hd, a.page_size, a.num_pages, a.status);
+    else if (a.dtype == STRIDE_DTYPE_BF16)
+        stride::launch(int4_read_kernel<__nv_bfloat16>, grid, block, 0, a.stream, a.k_pages, a.v_pages, a.slots, static_cast<__nv_bfloat16*>(a.k_out),
+                       static_cast<__nv_bfloat16*>(a.v_out), a.n, a.nkv, a.hd, a.page_size, a.num_pages, a.status);
     else
         return STRIDE_BAD_ARGUMENT;
     return STRIDE_LAUNCH_STATUS();
 }
 
-// k_out, v_out: [out_pages, nkv, 64, hd] bfloat16; table_out: [num_seqs, out_pages]. out_pages: at least the sum over the requests of
-// ceil(ctx_len / 64). Pages that no query of its request's portion can see are left as they were. Head sizes 64 and 128.
-extern "C" int stride_int4_expand(const void* k_pages, const void* v_pages, int num_pages, const int32_t* block_table, int table_width,
-                                  const int32_t* q_len, const int32_t* ctx_len, int num_seqs, int nkv, int hd, int page_size, int window, void* k_out,
-                                  void* v_out, int32_t* table_out, int out_pages, int* status, cudaStream_t stream) {
-    if (num_seqs < 0 || nkv <= 0 || page_size <= 0 || num_pages <= 0 || table_width <= 0 || window < 0 || out_pages <= 0) return STRIDE_BAD_ARGUMENT;
-    if ((hd != 64 && hd != 128) || nkv > 65535) return STRIDE_UNSUPPORTED;
-    if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) % 4 ||
-        (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16)
+struct Int4Expand {
+    const uint8_t* k_pages;
+    const uint8_t* v_pages;
+    const int32_t* block_table;
+    const int32_t* q_len;
+    const int32_t* ctx_len;
+    __nv_bfloat16* k_out;           // [out_pages, nkv, 64, hd]
+    __nv_bfloat16* v_out;
+    int32_t* table_out;             // [num_seqs, out_pages]
+    int* status;
+    cudaStream_t stream;
+    int num_pages, table_width, num_seqs, nkv, hd, page_size, window, out_pages;
+};
+
+static_assert(sizeof(Int4Expand) == 112, "the record that the caller packs");
+
+// out_pages: at least the sum over the requests of ceil(ctx_len / 64) (else code 36 in the status word). Pages that no query of its request's
+// portion can see are left as they were. Head sizes 64 and 128.
+extern "C" int stride_int4_expand(const void* record) {
+    const Int4Expand a = read_record<Int4Expand>(record);
+    if (a.num_seqs < 0 || a.nkv <= 0 || a.page_size <= 0 || a.num_pages <= 0 || a.table_width <= 0 || a.window < 0 || a.out_pages <= 0)
+        return STRIDE_BAD_ARGUMENT;
+    if ((a.hd != 64 && a.hd != 128) || a.nkv > 65535) return STRIDE_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4 ||
+        (reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) % 16)
         return STRIDE_UNSUPPORTED;
-    if (num_seqs == 0) return 0;
-    const auto kernel = hd == 64 ? int4_expand_kernel<2> : int4_expand_kernel<4>;
-    stride::launch(kernel, dim3(out_pages, nkv), dim3(kExpandThreads), 0, stream, static_cast<const uint8_t*>(k_pages), static_cast<const uint8_t*>(v_pages),
-                   num_pages, block_table, table_width, q_len, ctx_len, num_seqs, nkv, page_size, window, static_cast<__nv_bfloat16*>(k_out),
-                   static_cast<__nv_bfloat16*>(v_out), table_out, out_pages, status);
+    if (a.num_seqs == 0) return 0;
+    const auto kernel = a.hd == 64 ? int4_expand_kernel<2> : int4_expand_kernel<4>;
+    stride::launch(kernel, dim3(a.out_pages, a.nkv), dim3(kExpandThreads), 0, a.stream, a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width,
+                   a.q_len, a.ctx_len, a.num_seqs, a.nkv, a.page_size, a.window, a.k_out, a.v_out, a.table_out, a.out_pages, a.status);
     return STRIDE_LAUNCH_STATUS();
 }

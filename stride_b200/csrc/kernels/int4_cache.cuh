@@ -14,9 +14,20 @@
 // can be scaled against a row's scales and centres without leaving the 32-bit range.)
 #pragma once
 
+#include <cstring>
+
 #include "common.cuh"
 
 namespace stride {
+
+// A launcher's arguments as one record that the caller packs.
+template <typename R>
+inline R read_record(const void* record) {
+    R r;
+    std::memcpy(&r, record, sizeof(R));
+    return r;
+}
+
 namespace four {
 
 constexpr int kGroup = 32;

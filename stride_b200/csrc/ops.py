@@ -10,7 +10,9 @@ from __future__ import annotations
 
 import ctypes
 import os as _os
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct as _struct
+from array import array as _array
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -66,16 +68,11 @@ _SIGNATURES = {
                                                          c_void_p, c_int, c_float, c_void_p, c_void_p]),
     "stride_gemm_stream_add_norm": ("gemm_bf16_stream", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong,
                                                          c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
-    "stride_head_write": ("head_write", [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
-                                         c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
-    "stride_int4_read": ("head_write", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
-    "stride_attention_int4_exact": ("attention_int4", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,
-                                                       c_int, c_int, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
-    "stride_int4_expand": ("head_write", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
-                                          c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
-    "stride_decode_int4": ("attention_int4_decode", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
-                                                     c_longlong, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p, c_int,
-                                                     c_void_p, c_void_p]),
+    "stride_head_write": ("head_write", [c_char_p]),
+    "stride_int4_read": ("head_write", [c_char_p]),
+    "stride_int4_expand": ("head_write", [c_char_p]),
+    "stride_attention_int4_exact": ("attention_int4", [c_char_p]),
+    "stride_decode_int4": ("attention_int4_decode", [c_char_p]),
     "stride_copy_pages": ("page_copy", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "stride_scale_rows": ("elementwise", [c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_int, c_void_p]),
     "stride_paged_decode_attention": ("attention_decode", [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
@@ -217,6 +214,22 @@ _SIGNATURES = {
     "stride_head_norm_gate": ("linear_recurrence", [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int,
                                                     c_float, c_int, c_void_p]),
 }
+
+
+# Launchers that take their arguments as one record (converting two dozen arguments one by one costs more than the launch): the record's layout,
+# the addresses first, then 64-bit, then 32-bit numbers, as the C side declares it.
+_RECORDS = {
+    "stride_head_write": _struct.Struct("@13Pq10if4x"),
+    "stride_int4_read": _struct.Struct("@7P6i"),
+    "stride_int4_expand": _struct.Struct("@10P8i"),
+    "stride_attention_int4_exact": _struct.Struct("@11P9i2fi"),
+    "stride_decode_int4": _struct.Struct("@12Pq10i2f"),
+}
+
+
+def _launch(name: str, what: str, *args) -> None:
+    """Calls a launcher of ``_RECORDS``; None stands for no address."""
+    _check(_fn(name)(_RECORDS[name].pack(*args)), what)
 
 
 def _fn(name: str, what: str | None = None):
@@ -377,28 +390,34 @@ def _code(dtype: torch.dtype) -> int:
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or (lambda: torch.cuda.current_device())
 
 
-def _here(t: torch.Tensor, name: str, dtype=None) -> int:
-    """``_dev`` for a tensor that must also live on the current device: the launch goes to that device's stream. (Small calls are bound by the
-    host, so it asks a tensor for each thing once.)"""
+def _device_of(t: torch.Tensor, name: str) -> int:
+    """The number of the device that a call's tensors live on: the current one, whose stream the launch goes to."""
     device = t.get_device()
     if device < 0:
         raise KernelError(f"{name} must live on a CUDA device; stride_b200 has no CPU path")
     if device != _current_device():
         raise KernelError(f"{name} lives on cuda:{device}, but the current device is cuda:{_current_device()}")
-    if not t.is_contiguous():
-        raise KernelError(f"{name} must be contiguous")
+    return device
+
+
+def _here(t: torch.Tensor, name: str, device: int, dtype=None) -> int:
+    """``_dev`` for a tensor that must live on the call's device. (Small calls are bound by the host: a tensor is asked for each thing once.)"""
+    if t.get_device() != device:
+        raise KernelError(f"{name} must live on cuda:{device}, the call's device")
     if dtype is not None and t.dtype is not dtype:
         raise KernelError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise KernelError(f"{name} must be contiguous")
     return t.data_ptr()
 
 
-def _here_opt(t, name: str, count: int, dtype) -> int | None:
-    """``_here`` for an optional vector of ``count`` elements."""
+def _here_opt(t, name: str, device: int, count: int) -> int:
+    """``_here`` for an optional float32 vector of ``count`` elements; 0 for none."""
     if t is None:
-        return None
+        return 0
     if t.numel() != count:
         raise KernelError(f"{name} must hold {count} elements, got {t.numel()}")
-    return _here(t, name, dtype)
+    return _here(t, name, device, torch.float32)
 
 
 _status_at: dict = {}       # device number -> address of its status word (the word lives as long as the process)
@@ -2077,12 +2096,18 @@ def int4_row_bytes(hd: int) -> int:
     return 20 * -(-hd // INT4_GROUP)
 
 
-def _pages_args(k_pages, v_pages, nkv: int, page_size: int, row: int, dtype) -> tuple:
+def _pages_args(k_pages, v_pages, nkv: int, page_size: int, row: int, device: int, dtype) -> tuple:
     """(keys, values, number of pages) of pages [num_pages, nkv, page_size, row], checked."""
     shape = k_pages.shape
-    if len(shape) != 4 or shape[0] == 0 or shape[1] != nkv or shape[2] != page_size or shape[3] != row or v_pages.shape != shape:
+    if len(shape) != 4 or v_pages.shape != shape or shape[1:] != (nkv, page_size, row) or shape[0] == 0:
         raise KernelError(f"k_pages and v_pages must be [num_pages, {nkv}, {page_size}, {row}], got {tuple(shape)} and {tuple(v_pages.shape)}")
-    return _here(k_pages, "k_pages", dtype), _here(v_pages, "v_pages", dtype), shape[0]
+    return _here(k_pages, "k_pages", device, dtype), _here(v_pages, "v_pages", device, dtype), shape[0]
+
+
+def _covers(t, name: str, device: int, count: int) -> int:
+    if t.numel() < count:
+        raise KernelError(f"{name} must cover {count} entries, got {t.numel()}")
+    return _here(t, name, device, torch.int32)
 
 
 def _head_write(what: str, bits4: bool, qkv, bias, q_norm, k_norm, eps, positions, slot_mapping, cos, sin, k_pages, v_pages, nq, nkv, hd, page_size,
@@ -2094,28 +2119,27 @@ def _head_write(what: str, bits4: bool, qkv, bias, q_norm, k_norm, eps, position
         raise KernelError("qkv has the wrong width")
     if (q_norm is None) != (k_norm is None):
         raise KernelError("the norms of queries and keys come together")
-    code = _code(qkv.dtype)
-    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd) if bits4 else hd, torch.uint8 if bits4 else qkv.dtype)
-    rows, device = _here(qkv, "qkv"), qkv.get_device()
+    dtype = qkv.dtype
+    code = _code(dtype)
+    if q_out is not None and (q_out.dim() != 2 or q_out.shape[0] < tokens or q_out.shape[1] != nq * hd or q_out.dtype is not dtype or
+                              q_out.stride(1) != 1 or q_out.stride(0) < nq * hd):
+        raise KernelError("q_out must be rows [tokens, nq * hd] of qkv's element type")
+    if rotate and (cos.dim() != 2 or sin.shape != cos.shape or cos.shape[1] * 2 != hd):
+        raise KernelError("cos and sin must be [positions, hd / 2]")
+    device = _device_of(qkv, "qkv")
+    rows = _here(qkv, "qkv", device)
     if q_out is None:
         out, stride = rows, width
+    elif q_out.get_device() != device:
+        raise KernelError("q_out must live on qkv's device")
     else:
-        if q_out.dim() != 2 or q_out.shape[0] < tokens or q_out.shape[1] != nq * hd or q_out.dtype != qkv.dtype or q_out.stride(1) != 1 or \
-                q_out.stride(0) < nq * hd:
-            raise KernelError("q_out must be rows [tokens, nq * hd] of qkv's element type")
-        if q_out.get_device() != device:
-            raise KernelError("q_out must live on qkv's device")
         out, stride = q_out.data_ptr(), q_out.stride(0)
-    if rotate:
-        angles = cos.shape
-        if len(angles) != 2 or sin.shape != angles or angles[1] * 2 != hd:
-            raise KernelError("cos and sin must be [positions, hd / 2]")
-    _check(_fn("stride_head_write")(
-        rows, out, stride, _here_opt(bias, "bias", width, torch.float32), _here_opt(q_norm, "q_norm", hd, torch.float32),
-        _here_opt(k_norm, "k_norm", hd, torch.float32), eps, _covers(positions, "positions", tokens),
-        None if slot_mapping is None else _covers(slot_mapping, "slot_mapping", tokens), _here(cos, "cos", torch.float32),
-        _here(sin, "sin", torch.float32), angles[0] if rotate else 0, k, v, pages, 1 if bits4 else 0, tokens, nq, nkv, hd, page_size, 1 if rotate else 0,
-        code, _status_here(device), _stream_here(device)), what)
+    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd) if bits4 else hd, device, torch.uint8 if bits4 else dtype)
+    _launch("stride_head_write", what, rows, out, _here_opt(bias, "bias", device, width), _here_opt(q_norm, "q_norm", device, hd),
+            _here_opt(k_norm, "k_norm", device, hd), _covers(positions, "positions", device, tokens),
+            0 if slot_mapping is None else _covers(slot_mapping, "slot_mapping", device, tokens), _here(cos, "cos", device, torch.float32),
+            _here(sin, "sin", device, torch.float32), k, v, _status_here(device), _stream_here(device), stride, cos.shape[0] if rotate else 0, pages, bits4,
+            tokens, nq, nkv, hd, page_size, rotate, code, eps)
 
 
 def qk_norm_rope_write(qkv, bias, q_norm, k_norm, eps: float, positions, slot_mapping, cos, sin, k_pages, v_pages, nq: int, nkv: int, hd: int,
@@ -2140,17 +2164,17 @@ def read_int4(k_pages, v_pages, slots, k_out, v_out, nkv: int, hd: int, page_siz
     of -1 reads as zeros."""
     if min(nkv, hd, page_size) <= 0:
         raise KernelError("read_int4: heads, head size and page size must be positive")
-    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd), torch.uint8)
     shape = k_out.shape
     if len(shape) != 3 or shape[0] != slots.numel() or shape[1] != nkv or shape[2] != hd or v_out.shape != shape or v_out.dtype is not k_out.dtype:
         raise KernelError("k_out and v_out must be [slots, nkv, hd] of one element type")
-    device = k_out.get_device()
-    _check(_fn("stride_int4_read")(k, v, _here(slots, "slots", torch.int32), _here(k_out, "k_out"), _here(v_out, "v_out"), slots.numel(), nkv, hd,
-                                   page_size, pages, _code(k_out.dtype), _status_here(device), _stream_here(device)), "read_int4")
+    code, device = _code(k_out.dtype), _device_of(k_out, "k_out")
+    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd), device, torch.uint8)
+    _launch("stride_int4_read", "read_int4", k, v, _here(slots, "slots", device, torch.int32), _here(k_out, "k_out", device), _here(v_out, "v_out", device),
+            _status_here(device), _stream_here(device), shape[0], nkv, hd, page_size, pages, code)
 
 
 def _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap, dtype=None) -> tuple:
-    """(q, out, keys, values, number of pages, block table, its width, number of the device) of the attention kernels over a cache held in 4
+    """(number of the device, q, out, keys, values, number of pages, block table, its width) of the attention kernels over a cache held in 4
     bits, checked."""
     if nq <= 0 or nkv <= 0 or hd <= 0 or page_size <= 0 or nq % nkv:
         raise KernelError(f"{nq} query heads of {hd} do not group into {nkv} key heads")
@@ -2164,27 +2188,21 @@ def _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nk
     table = block_table.shape
     if len(table) != 2:
         raise KernelError("block_table must be [requests, pages]")
-    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, 20 * -(-hd // INT4_GROUP), torch.uint8)
-    return _here(q, "q", dtype), _here(out, "out", dtype), k, v, pages, _here(block_table, "block_table", torch.int32), table[1], q.get_device()
-
-
-def _covers(t, name: str, count: int) -> int:
-    if t.numel() < count:
-        raise KernelError(f"{name} must cover {count} entries, got {t.numel()}")
-    return _here(t, name, torch.int32)
+    device = _device_of(q, "q")
+    k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd), device, torch.uint8)
+    return (device, _here(q, "q", device, dtype), _here(out, "out", device), k, v, pages, _here(block_table, "block_table", device, torch.int32), table[1])
 
 
 def paged_attention_int4(q, q_stride: int, out, k_pages, v_pages, block_table, seq_of_token, positions, nq: int, nkv: int, hd: int, page_size: int,
                          scale: float, window: int = 0, softcap: float = 0.0, sinks=None, slopes=None) -> None:
     """``paged_attention`` over pages held in 4 bits: any mix of rows, any head size up to 256, float32 or bfloat16. The exact kernel: the
     result of a row has the same bits however the work is cut."""
-    qp, op, k, v, pages, table, width, device = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
+    device, qp, op, k, v, pages, table, width = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
                                                                      softcap)
     tokens = out.shape[0]
-    _check(_fn("stride_attention_int4_exact")(
-        qp, q_stride, op, k, v, pages, table, width, _covers(seq_of_token, "seq_of_token", tokens), _covers(positions, "positions", tokens), tokens, nq,
-        nkv, hd, page_size, scale, window, softcap, _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32),
-        _code(q.dtype), _status_here(device), _stream_here(device)), "paged_attention_int4")
+    _launch("stride_attention_int4_exact", "paged_attention_int4", qp, op, k, v, table, _covers(seq_of_token, "seq_of_token", device, tokens),
+            _covers(positions, "positions", device, tokens), _here_opt(sinks, "sinks", device, nq), _here_opt(slopes, "slopes", device, nq),
+            _status_here(device), _stream_here(device), q_stride, pages, width, tokens, nq, nkv, hd, page_size, window, scale, softcap, _code(q.dtype))
 
 
 def decode_int4_scratch_floats(tokens: int, nq: int, nkv: int, hd: int, max_context: int) -> int:
@@ -2202,14 +2220,13 @@ def paged_attention_decode_int4(q, q_stride: int, out, k_pages, v_pages, block_t
                                 page_size: int, scale: float, window: int, max_context: int, softcap: float = 0.0, sinks=None, slopes=None) -> None:
     """``paged_attention_decode`` over pages held in 4 bits: one query per row, bfloat16, head sizes 64 and 128. ``max_context`` exceeds every
     position; ``scratch``: float32, zero when it is first used, at least ``decode_int4_scratch_floats`` elements, for one stream at a time."""
-    qp, op, k, v, pages, table, width, device = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
+    device, qp, op, k, v, pages, table, width = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
                                                                      softcap, torch.bfloat16)
     tokens = out.shape[0]
-    _check(_fn("stride_decode_int4")(
-        qp, q_stride, op, k, v, pages, table, width, _covers(seq_of_token, "seq_of_token", tokens), _covers(positions, "positions", tokens),
-        _here(scratch, "scratch", torch.float32), scratch.numel(), tokens, nq, nkv, hd, page_size, scale, window, softcap,
-        _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32), max_context, _status_here(device),
-        _stream_here(device)), "paged_attention_decode_int4")
+    _launch("stride_decode_int4", "paged_attention_decode_int4", qp, op, k, v, table, _covers(seq_of_token, "seq_of_token", device, tokens),
+            _covers(positions, "positions", device, tokens), _here(scratch, "scratch", device, torch.float32), _here_opt(sinks, "sinks", device, nq),
+            _here_opt(slopes, "slopes", device, nq), _status_here(device), _stream_here(device), scratch.numel(), q_stride, pages, width, tokens, nq, nkv, hd,
+            page_size, window, max_context, scale, softcap)
 
 
 INT4_EXPANDED_PAGE = 64     # keys of a page of the expanded keys and values
@@ -2235,7 +2252,7 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     the rows of ``out``: bfloat16, head sizes 64 and 128. ``keys``: at least what those requests hold together; ``scratch``: int32, at least
     ``prefill_int4_scratch_ints`` elements, for one stream at a time. The keys and values that the portions see are expanded once, to pages
     of 64 in bfloat16 (a rounding of 2^-9 of an entry, as a bfloat16 cache has it), and attended to from there."""
-    qp, op, k, v, pages, rows, width, device = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
+    device, qp, op, k, v, pages, rows, width = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
                                                                     softcap, torch.bfloat16)
     if not fast_attention_supported(q.dtype, nq, nkv, hd):
         raise KernelError(f"paged_attention_prefill_int4: {nq} heads of {hd} on {nkv} are not supported (paged_attention_int4 takes them)")
@@ -2248,16 +2265,16 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     if block_table.shape[0] < num_seqs:
         raise KernelError("block_table must have a row a request")
     half = out_pages * nkv * INT4_EXPANDED_PAGE * hd * 2
-    wide_k = _here(scratch, "scratch", torch.int32)
+    wide_k = _here(scratch, "scratch", device, torch.int32)
     wide_v, table = wide_k + half, wide_k + 2 * half
-    starts, lens, held = _covers(q_start, "q_start", num_seqs), _covers(q_len, "q_len", num_seqs), _covers(ctx_len, "ctx_len", num_seqs)
-    sink, slope = _here_opt(sinks, "sinks", nq, torch.float32), _here_opt(slopes, "slopes", nq, torch.float32)
+    starts, lens, held = (_covers(t, name, device, num_seqs) for t, name in ((q_start, "q_start"), (q_len, "q_len"), (ctx_len, "ctx_len")))
+    sink, slope = _here_opt(sinks, "sinks", device, nq), _here_opt(slopes, "slopes", device, nq)
     status, stream = _status_here(device), _stream_here(device)
-    _check(_fn("stride_int4_expand")(k, v, pages, rows, width, lens, held, num_seqs, nkv, hd, page_size, window, wide_k, wide_v, table, out_pages, status,
-                                     stream), "paged_attention_prefill_int4")
+    _launch("stride_int4_expand", "paged_attention_prefill_int4", k, v, rows, lens, held, wide_k, wide_v, table, status, stream, pages, width, num_seqs, nkv,
+            hd, page_size, window, out_pages)
     _check(_fn("stride_paged_prefill_attention_tc")(
         qp, q_stride, op, wide_k, wide_v, out_pages, table, out_pages, starts, lens, held, num_seqs, tokens, nq, nkv, hd, INT4_EXPANDED_PAGE, scale,
-        window, -softcap if precise_cap else softcap, sink, slope, None, 0, status, stream), "paged_attention_prefill_int4")
+        window, -softcap if precise_cap else softcap, sink or None, slope or None, None, 0, status, stream), "paged_attention_prefill_int4")
 
 
 # ------------------------------------------------------------------- copies of pages
@@ -2265,7 +2282,10 @@ def copy_pages(pools, src, dst) -> None:
     """Page ``dst[i]`` of every pool becomes page ``src[i]``, in all its layers. ``pools``: tensors [layers, num_pages, ...]; ``src`` and ``dst``:
     page numbers (sequences of ints). A page is copied from or to, not both, and to at most once. A captured graph keeps the pairs it was
     captured with."""
-    src, dst = [int(p) for p in src], [int(p) for p in dst]
+    try:
+        src, dst = (_array("i", p.tolist() if hasattr(p, "tolist") else p) for p in (src, dst))
+    except (TypeError, OverflowError) as e:
+        raise KernelError(f"copy_pages: page numbers are 32-bit integers ({e})") from None
     n = len(src)
     if n != len(dst):
         raise KernelError("copy_pages: every page copied from goes with one copied to")
@@ -2282,12 +2302,12 @@ def copy_pages(pools, src, dst) -> None:
             raise KernelError(f"copy_pages: a pool is [layers, num_pages, ...], got {tuple(shape)}")
         if least < 0 or most >= shape[1]:
             raise KernelError(f"copy_pages: a page lies outside a pool of {shape[1]}")
-        about += (_here(t, "pool"), shape[0], shape[1], t.stride(1) * t.itemsize)
+        device = _device_of(t, "pool")
+        about += (_here(t, "pool", device), shape[0], shape[1], t.stride(1) * t.itemsize)
     if not n or not about:
         return
-    device = pools[0].get_device()
-    _check(_fn("stride_copy_pages")((c_longlong * len(about))(*about), len(about) // 4, (c_int * n)(*src), (c_int * n)(*dst), n, _stream_here(device)),
-           "copy_pages")
+    _check(_fn("stride_copy_pages")((c_longlong * len(about))(*about), len(about) // 4, src.buffer_info()[0], dst.buffer_info()[0], n,
+                                    _stream_here(device)), "copy_pages")
 
 
 # --------------------------------------------------------------------- sampling
