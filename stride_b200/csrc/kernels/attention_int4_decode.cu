@@ -1,4 +1,4 @@
-// Decode attention over a paged cache held in 4 bits (int4_cache.cuh), split over the keys, on the tensor cores.
+// Decode attention over a paged cache held in 4 bits (int4_cache.cuh), on the tensor cores.
 //
 // A single query reads every key of its request: the bytes of the cache bound it, 5 bits an entry. So that the work on an entry stays below
 // the time its bytes take, an entry is never turned into a value: numbers go to the matrix instructions as they are, scales and centres are
@@ -16,12 +16,14 @@
 //   the side of the keys, with P on the side of the values. P is rounded to bfloat16 once, P s to 16 bits from that, so what the offset of 8
 //   adds in one product the other takes off to 2^-12.
 // * The query is scaled by a power of two to below 2^15. The reference R of a weight 2^(score - R) is the running maximum of score + log2 of the
-//   token's largest scale or centre, so that what is rounded to 16 bits lies below 2^8 and its largest above 2^-1 whatever the values' size;
-//   R moves only when a product passes 2^8 (a vote per tile), and then everything is rescaled.
+//   token's largest scale or centre, so that what is rounded to 16 bits lies below 2^8 and its largest near 1 whatever the values' size; R moves
+//   only when a product passes 2^8 (a vote per tile), and then everything is rescaled.
 //
+// The work of a launch is a row of units, 128 keys of one (token, key head) each, in the order of tokens and key heads; every CTA takes an equal
+// stretch of it (it works out from the positions where its own begins), so requests of any lengths keep all SMs busy to the end and a
+// (token, key head) is cut only where a stretch ends. Parts of one are merged by the CTA that draws its last ticket, in the order of the keys.
 // A warp owns tiles of 32 keys and a ring of copies: a bulk copy for each 16 keys and one for their values where pages hold whole sixteens (a page's
-// rows of one head lie side by side), 16- or 8-byte copies by all lanes otherwise. Splits are merged as in attention_decode.cu, by the CTA
-// that draws the last ticket.
+// rows of one head lie side by side), 16- or 8-byte copies by all lanes otherwise.
 #include "int4_cache.cuh"
 #include "mma.cuh"
 #include "tcgen05.cuh"      // mbarrier helpers
@@ -34,12 +36,13 @@ constexpr int kTile = 2 * kSub;         // keys of a warp's tile
 constexpr int kWarps = 4;
 constexpr int kUnit = kTile * kWarps;   // keys that a CTA's warps cover with a tile each
 constexpr int kStages = 3;
-constexpr int kMaxTiles = 16;           // of a warp: a lane looks each half's page up
+constexpr int kWindow = 16;             // tiles whose pages the lanes look up at once, a half each
 constexpr int kTicketInts = 65536;      // ticket counters at the start of the scratch, one per (token, key head)
 constexpr int kCodeBeyondBound = 32;    // as in attention_decode.cu
 constexpr int kCodeCopyWait = 81;       // a wait for a tile's copies ran out
-constexpr float kLimit = 256.f;         // what a weight's product with a scale or centre may reach before R moves
-constexpr float kLeastLog = -90.f;      // log2 of the least scale or centre that R counts: a weight stays below 2^98
+constexpr float kLimit = 256.f;         // what a weight's product with a scale may reach before R moves
+constexpr float kMostWeight = 1.1529215e18f;    // 2^60, what a weight may (its product with a centre, below 2^64, stays a number)
+constexpr float kLeastLog = -90.f;      // log2 of the least size that R counts: a weight stays below 2^98
 
 struct Decode {
     const __nv_bfloat16* q;
@@ -51,13 +54,24 @@ struct Decode {
     const int32_t* positions;
     const float* sinks;
     const float* slopes;
-    float* part_o;          // [token][head][split][hd]
-    float* part_ml;         // [token][head][split][2]: R, sum of weights
-    int* tickets;
+    float* part_o;          // [2 CTAs][group][hd]: what a stretch holds of a (token, key head) that it shares with others
+    float* part_ml;         // [2 CTAs][group][2]: R, sum of weights
+    int* tickets;           // [token][key head]
     int* status;
-    int q_stride, table_width, num_pages, nq, nkv, page_size, window, split_keys, num_splits;
+    int q_stride, table_width, num_pages, nq, nkv, page_size, window, tokens, max_context;
     float scale_log2e, cap_log2e, scale_over_cap;        // cap_log2e 0: no cap
 };
+
+// The keys of a token in units: first unit and how many; none for a padded row or one beyond the bound.
+struct Span {
+    int first, units;
+};
+__device__ __forceinline__ Span span_of(const Decode& a, int t) {
+    const int seq = a.seq_of_token[t], pos = a.positions[t];
+    if (seq < 0 || pos < 0 || pos >= a.max_context) return {0, 0};
+    const int first = a.window > 0 ? max(0, pos - a.window + 1) / kUnit : 0;
+    return {first, pos / kUnit - first + 1};
+}
 
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
@@ -115,13 +129,21 @@ template <int G>
 __device__ __forceinline__ int token_of(int r) {
     return G == 4 ? (r & 8) + (r & 1) * 4 + ((r & 7) >> 1) : (r & 3) * 4 + (r >> 2);
 }
-// The largest of the scales and of the centres' sizes in a row's parameters.
+// The largest of the scales in a row's parameters (positive, or zero): as 16-bit integers, two at once, whatever the other halves hold.
 template <int G>
-__device__ __forceinline__ float amplitude(const uint32_t (&p)[G]) {
-    __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&p[0]));
+__device__ __forceinline__ float largest_scale(const uint32_t (&p)[G]) {
+    uint32_t m = p[0];
 #pragma unroll
-    for (int g = 1; g < G; ++g) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&p[g])));
-    return fmaxf(__low2float(m), __high2float(m));
+    for (int g = 1; g < G; ++g) m = __vmaxu2(m, p[g]);
+    return bf16_low(m);
+}
+// log2 of the largest of a row's scales and its centres' sizes, 0 of them counted as 2^kLeastLog.
+template <int G>
+__device__ __forceinline__ float log2_size(const uint32_t (&p)[G]) {
+    float m = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) m = fmaxf(m, fmaxf(bf16_low(p[g]), fabsf(bf16_high(p[g]))));
+    return fmaxf(__log2f(m), kLeastLog);
 }
 
 // G: groups of a head (head size 32 G). NT: tiles of 8 query heads.
@@ -132,39 +154,66 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
     pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
-    const int split = blockIdx.x, kvh = blockIdx.y, t = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int group = a.nq / a.nkv, seq = a.seq_of_token[t], pos = seq < 0 ? 0 : a.positions[t];
-    __nv_bfloat16* out = a.out + (static_cast<size_t>(t) * a.nq + kvh * group) * HD;
-    if (seq < 0 || pos >= a.num_splits * a.split_keys) {       // a padded row, or one beyond the bound that the launch was sized for: zeros, no ticket
-        if (split == 0) {
-            for (int i = threadIdx.x; i < group * HD; i += blockDim.x) out[i] = __float2bfloat16_rn(0.f);
-            if (seq >= 0 && threadIdx.x == 0) complain(a.status, kCodeBeyondBound);
+    __shared__ int warp_sums[kWarps];
+    __shared__ int begin_token, begin_units;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, group = a.nq / a.nkv;
+
+    // ---- this CTA's stretch: `left` units from unit `skip` of (t, kvh) on
+    int t = 0, kvh = 0, skip = 0, left = 0;
+    long long total = 0, begin = 0, stretches = 0;
+    {
+        const int chunk = (a.tokens + kWarps * 32 - 1) / (kWarps * 32), t_lo = threadIdx.x * chunk, t_hi = min(a.tokens, t_lo + chunk);
+        int mine = 0;
+        for (int i = t_lo; i < t_hi; ++i) mine += span_of(a, i).units;
+        int upto = mine;                                            // with the lanes and warps before
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, s);
+            if (lane >= s) upto += v;
         }
-        return;
-    }
-    const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0, lo = split * a.split_keys;
-    if (lo > pos || lo + a.split_keys <= first) return;        // uniform for the CTA
-    const int32_t* table = a.table + static_cast<size_t>(seq) * a.table_width;
-    const int n_tiles = a.split_keys / kUnit;
-    auto tile_base = [&](int j) { return lo + j * kUnit + warp * kTile; };
-    // the bytes at which a key's row of this head lies, or all ones where there is no such page
-    auto row_at = [&](int key) {
-        const int index = key / a.page_size, page = index < a.table_width ? table[index] : -1;
-        if (page < 0 || page >= a.num_pages) {
-            complain(a.status, kCodeNoPage);
-            return ~size_t(0);
+        if (lane == 31) warp_sums[warp] = upto;
+        __syncthreads();
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) upto += sum;
+            sum += warp_sums[w];
         }
-        return ((static_cast<size_t>(page) * a.nkv + kvh) * a.page_size + key % a.page_size) * ROW;
-    };
-    // lane 2 j + h answers for half h of tile j
-    const int my_key = tile_base(lane >> 1) + (lane & 1) * kSub;
-    size_t my_row = ~size_t(0);
-    bool mine = lane < 2 * n_tiles && my_key <= pos && my_key + kSub > first;
-    if (BULK && mine) {
-        my_row = row_at(my_key);
-        mine = my_row != ~size_t(0);
+        total = static_cast<long long>(sum) * a.nkv;
+        // one unit a CTA while that leaves SMs idle, then two at least, since a part costs about as much as a unit
+        stretches = min(static_cast<long long>(gridDim.x), total <= 148 ? total : max(148LL, total / 2));
+        if (blockIdx.x < stretches) {
+            begin = blockIdx.x * total / stretches;
+            left = static_cast<int>((blockIdx.x + 1) * total / stretches - begin);
+            // units are counted token by token, key heads inside: the token whose heads hold unit `begin`
+            if (begin < static_cast<long long>(upto) * a.nkv && begin >= static_cast<long long>(upto - mine) * a.nkv) {
+                int before = upto - mine, i = t_lo;
+                for (;; ++i) {
+                    const int units = span_of(a, i).units;
+                    if (begin < static_cast<long long>(before + units) * a.nkv) break;
+                    before += units;
+                }
+                begin_token = i;
+                begin_units = before;
+            }
+        }
+        __syncthreads();
     }
-    const uint32_t live = __ballot_sync(0xffffffffu, mine);
+    for (int i = blockIdx.x; i < a.tokens; i += gridDim.x) {        // rows without keys: zeros
+        const int seq = a.seq_of_token[i], pos = a.positions[i];
+        if (seq >= 0 && pos >= 0 && pos < a.max_context) continue;
+        for (int d = threadIdx.x; d < a.nq * HD; d += blockDim.x) a.out[static_cast<size_t>(i) * a.nq * HD + d] = __float2bfloat16_rn(0.f);
+        if (seq >= 0 && threadIdx.x == 0) complain(a.status, kCodeBeyondBound);
+    }
+    if (left == 0) return;
+    t = begin_token;
+    long long item = static_cast<long long>(begin_units) * a.nkv;   // the first unit of (t, kvh)
+    Span span = span_of(a, t);
+    kvh = static_cast<int>((begin - item) / span.units);
+    item += static_cast<long long>(kvh) * span.units;
+    skip = static_cast<int>(begin - item);
+    auto stretch_of = [&](long long unit) { return static_cast<int>(((unit + 1) * stretches + total - 1) / total - 1); };
+
     unsigned char* ring = smem + warp * kStages * STAGE;
     if (BULK) {
         if (lane == 0)
@@ -172,22 +221,70 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         __syncwarp();
     }
+    const int row_a = token_of<G>(g), row_b = token_of<G>(g + 8);                                   // tokens of this lane's score rows
+    const int col[4] = {token_of<G>(2 * c), token_of<G>(2 * c + 1), token_of<G>(2 * c + 8), token_of<G>(2 * c + 9)};        // of its weights
+    const uint32_t pick = g < 4 ? 0x7632u : 0x5410u;            // rows of `cen`: centres or scales
+    const bool bent = a.cap_log2e > 0.f || a.slopes != nullptr;
+    bool alive = true;
+    uint32_t uses = 0, held = 0;            // per stage: the parity of its barrier, and which halves of its tile were copied
+    int stage = 0;
+
+    for (;;) {          // ---- a (token, key head), or what the stretch holds of one
+    const int n_tiles = min(left, span.units - skip), lo = (span.first + skip) * kUnit;
+    const int pos = a.positions[t], first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const int32_t* table = a.table + static_cast<size_t>(a.seq_of_token[t]) * a.table_width;
+    auto tile_base = [&](int j) { return lo + j * kUnit + warp * kTile; };
+    auto page_of = [&](int key) {
+        const int index = key / a.page_size;
+        return index < a.table_width ? table[index] : -1;
+    };
+    // the bytes at which a key's row of this head lies, or all ones where there is no such page
+    auto row_at = [&](int key, int page) {
+        if (page < 0 || page >= a.num_pages) {
+            complain(a.status, kCodeNoPage);
+            return ~size_t(0);
+        }
+        return ((static_cast<size_t>(page) * a.nkv + kvh) * a.page_size + key % a.page_size) * ROW;
+    };
+    // BULK: lane 2 i + h answers for half h of tile `window` + i: its row, and for the window after it the page
+    size_t my_row = ~size_t(0);
+    int my_page = -1;
+    uint32_t live = 0;
+    auto half_key = [&](int window) { return tile_base(window + (lane >> 1)) + (lane & 1) * kSub; };
+    auto wanted = [&](int window) {
+        const int key = half_key(window);
+        return window + (lane >> 1) < n_tiles && key <= pos && key + kSub > first;
+    };
+    if (BULK && wanted(0)) my_page = page_of(half_key(0));
     auto issue = [&](int j, int stage) {
+        if (j >= n_tiles) {
+            if (!BULK) cp_async_commit();
+            return;
+        }
         if (BULK) {
+            if (j % kWindow == 0) {
+                my_row = wanted(j) ? row_at(half_key(j), my_page) : ~size_t(0);
+                live = __ballot_sync(0xffffffffu, my_row != ~size_t(0));
+                if (wanted(j + kWindow)) my_page = page_of(half_key(j + kWindow));
+            }
+            const uint32_t halves = live >> (2 * (j % kWindow)) & 3u;
+            held = (held & ~(3u << (2 * stage))) | halves << (2 * stage);
             // (the barrier's one arrival, with the count of bytes, keeps the phase open whichever copy lands first)
-            if (j < n_tiles && (lane >> 1) == j && mine) {
+            if ((lane >> 1) == j % kWindow && my_row != ~size_t(0)) {
                 const uint32_t dst = tc::smem_u32(ring + stage * STAGE + (lane & 1) * 2 * HALF), bar = tc::smem_u32(&bars[warp][stage]);
-                const uint32_t halves = live >> (2 * j) & 3u;
                 if ((lane & 1) == (halves == 2u)) tc::mbar_expect_tx(bar, halves == 3u ? 4 * HALF : 2 * HALF);
                 bulk_copy(dst, a.k_pages + my_row, HALF, bar);
                 bulk_copy(dst + HALF, a.v_pages + my_row, HALF, bar);
             }
             return;
         }
-        if (j < n_tiles && (live >> (2 * j) & 3u)) {
+        const int base = tile_base(j);
+        const uint32_t halves = (base <= pos && base + kSub > first ? 1u : 0u) | (base + kSub <= pos && base + kTile > first ? 2u : 0u);
+        held = (held & ~(3u << (2 * stage))) | halves << (2 * stage);
+        if (halves) {
             size_t row = ~size_t(0);
-            const int key = tile_base(j) + lane;
-            if (key >= first && key <= pos) row = row_at(key);
+            const int key = base + lane;
+            if (key >= first && key <= pos) row = row_at(key, page_of(key));
             unsigned char* to = ring + stage * STAGE;
 #pragma unroll
             for (int i = 0; i < 5; ++i) {               // 32 rows of 5 pieces
@@ -204,8 +301,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         }
         cp_async_commit();
     };
+    {
+        int s = stage;
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) issue(s, s);
+        for (int i = 0; i < kStages; ++i) {
+            issue(i, s);
+            s = s + 1 == kStages ? 0 : s + 1;
+        }
+    }
 
     // ---- the query: lane (g, c) holds, of head 8 nt + g, entries 32 grp + 8 c .. + 7
     uint32_t qb[NT][G][2][2], cb[NT][2];            // B operands: of the numbers, of centres and scales
@@ -281,15 +384,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             for (int grp = 0; grp < G; ++grp) o[nt][grp][0][e] = o[nt][grp][1][e] = 0.f;
         }
     }
-    const int row_a = token_of<G>(g), row_b = token_of<G>(g + 8);                                   // tokens of this lane's score rows
-    const int col[4] = {token_of<G>(2 * c), token_of<G>(2 * c + 1), token_of<G>(2 * c + 8), token_of<G>(2 * c + 9)};        // of its weights
-    const uint32_t pick = g < 4 ? 0x7632u : 0x5410u;            // rows of `cen`: centres or scales
-    const bool bent = a.cap_log2e > 0.f || a.slopes != nullptr;
-    bool alive = true;
-    uint32_t uses = 0;
-    int stage = 0;
     for (int j = 0; j < n_tiles; ++j) {
-        const uint32_t halves = live >> (2 * j) & 3u;
+        const uint32_t halves = held >> (2 * stage) & 3u;
         if (BULK) {
             if (halves && alive) {
                 alive = __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&bars[warp][stage]), uses >> stage & 1u, a.status, kCodeCopyWait));
@@ -337,8 +433,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                 uint32_t vp[2][G];
                 load_words<G>(vp[0], ks + HALF + row_a * ROW + 16 * G);
                 load_words<G>(vp[1], ks + HALF + row_b * ROW + 16 * G);
-                amp[h][0] = amplitude<G>(vp[0]);
-                amp[h][1] = amplitude<G>(vp[1]);
+                amp[h][0] = largest_scale<G>(vp[0]);
+                amp[h][1] = largest_scale<G>(vp[1]);
             }
             // x becomes the score in units of log2
             if (bent) {
@@ -379,23 +475,36 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float high = 0.f;
+                float most_of[2][2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) P[nt][h][e] = exp2_quick(x[nt][h][e] - R[nt][e & 1]);
+                    most_of[h][0] = fmaxf(P[nt][h][0], P[nt][h][1]);
+                    most_of[h][1] = fmaxf(P[nt][h][2], P[nt][h][3]);
                 }
-                // (a maximum passes a NaN over: while R is -inf, in the first tile, every weight is infinite or none, and the sum shows it)
-                high = fmaxf(fmaxf(fmaxf(P[nt][0][0], P[nt][0][1]) * amp[0][0], fmaxf(P[nt][0][2], P[nt][0][3]) * amp[0][1]),
-                             fmaxf(fmaxf(P[nt][1][0], P[nt][1][1]) * amp[1][0], fmaxf(P[nt][1][2], P[nt][1][3]) * amp[1][1]));
-                if (__any_sync(0xffffffffu, !(high <= kLimit) || R[nt][0] == -INFINITY)) {
+                const float product = fmaxf(fmaxf(most_of[0][0] * amp[0][0], most_of[0][1] * amp[0][1]),
+                                            fmaxf(most_of[1][0] * amp[1][0], most_of[1][1] * amp[1][1]));
+                const float weight = fmaxf(fmaxf(most_of[0][0], most_of[0][1]), fmaxf(most_of[1][0], most_of[1][1]));
+                // (R is -inf until a tile with a key; then weights are infinite or, of masked keys, no numbers)
+                if (__any_sync(0xffffffffu, !(product <= kLimit && weight <= kMostWeight))) {
+                    float size[2][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t vp[2][G];
+                        load_words<G>(vp[0], at + h * 2 * HALF + HALF + row_a * ROW + 16 * G);
+                        load_words<G>(vp[1], at + h * 2 * HALF + HALF + row_b * ROW + 16 * G);
+                        size[h][0] = log2_size<G>(vp[0]);
+                        size[h][1] = log2_size<G>(vp[1]);
+                    }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float most = -INFINITY;
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int r = 0; r < 2; ++r) most = fmaxf(most, x[nt][h][2 * r + e] + fmaxf(__log2f(amp[h][r]), kLeastLog));
+                            for (int r = 0; r < 2; ++r)
+                                most = x[nt][h][2 * r + e] == -INFINITY ? most : fmaxf(most, x[nt][h][2 * r + e] + size[h][r]);
 #pragma unroll
                         for (int s = 4; s < 32; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
                         const float next = fmaxf(R[nt][e], most), by = R[nt][e] == -INFINITY ? 0.f : exp2_quick(R[nt][e] - next);
@@ -482,7 +591,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
     }
 
     // ---- the warps' results side by side in shared memory (the rings are no longer needed)
-    const int s_lo = first / a.split_keys, n = pos / a.split_keys - s_lo + 1;      // live splits
+    const int before = stretch_of(item), parts = stretch_of(item + span.units - 1) - before + 1;
     __syncthreads();
     float* red = reinterpret_cast<float*>(smem);
     constexpr int RS = HD + 2;
@@ -512,6 +621,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             }
         }
     __syncthreads();
+    __nv_bfloat16* out = a.out + (static_cast<size_t>(t) * a.nq + kvh * group) * HD;
+    // where a part lies: one that begins with the keys in the CTA's second place (it is its last), any other in its first
+    auto place = [&](int part) { return static_cast<size_t>(2 * (before + part) + (part == 0)) * group; };
     for (int idx = threadIdx.x; idx < group * HD; idx += blockDim.x) {
         const int row = idx / HD, d = idx - row * HD;
         float mm = -INFINITY;
@@ -525,109 +637,96 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             acc += f * src[d];
             sum += f * src[HD + 1];
         }
-        if (n == 1) {           // no other split
+        if (parts == 1) {
             if (a.sinks != nullptr && mm != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -mm));
             out[idx] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);      // 0: no key had a page
             continue;
         }
-        const size_t slot = (static_cast<size_t>(t) * a.nq + kvh * group + row) * a.num_splits + split;
-        a.part_o[slot * HD + d] = acc;
+        const size_t at = place(blockIdx.x - before) + row;
+        a.part_o[at * HD + d] = acc;
         if (d == 0) {
-            a.part_ml[slot * 2] = mm;
-            a.part_ml[slot * 2 + 1] = sum;
+            a.part_ml[at * 2] = mm;
+            a.part_ml[at * 2 + 1] = sum;
         }
     }
-    if (n == 1) return;
-    // ---- the CTA that finishes last for this (token, key head) merges the splits
-    __shared__ int is_last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int* ticket = a.tickets + static_cast<size_t>(t) * a.nkv + kvh;
-        is_last = atomicAdd(ticket, 1) == n - 1;
-        if (is_last) *ticket = 0;       // ready for the next launch; nobody else touches it before then
-    }
-    __syncthreads();
-    if (!is_last) return;
-    __threadfence();
-    float* weights = red;                       // [group][n]
-    float* total = red + group * n;             // [group]
-    for (int row = warp; row < group; row += kWarps) {
-        const size_t base = (static_cast<size_t>(t) * a.nq + kvh * group + row) * a.num_splits + s_lo;
-        float most = -INFINITY;
-        for (int sp = lane; sp < n; sp += 32) {
-            const float v = __ldcg(a.part_ml + (base + sp) * 2);
-            weights[row * n + sp] = v;
-            most = fmaxf(most, v);
+    if (parts > 1) {
+        // ---- the CTA that finishes last for this (token, key head) merges the parts
+        __shared__ int is_last;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int* ticket = a.tickets + static_cast<size_t>(t) * a.nkv + kvh;
+            is_last = atomicAdd(ticket, 1) == parts - 1;
+            if (is_last) *ticket = 0;       // ready for the next launch; nobody else touches it before then
         }
-        most = warp_max(most);
-        float sum = 0.f;
-        for (int sp = lane; sp < n; sp += 32) {
-            const float w = most == -INFINITY ? 0.f : exp2f(weights[row * n + sp] - most);
-            weights[row * n + sp] = w;
-            sum += w * __ldcg(a.part_ml + (base + sp) * 2 + 1);
-        }
-        sum = warp_sum(sum);
-        if (a.sinks != nullptr && most != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -most));
-        if (lane == 0) total[row] = sum;
-    }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < group * (HD / 4); idx += blockDim.x) {
-        const int row = idx / (HD / 4), d = (idx - row * (HD / 4)) * 4;
-        const size_t base = (static_cast<size_t>(t) * a.nq + kvh * group + row) * a.num_splits + s_lo;
-        const float4* column = reinterpret_cast<const float4*>(a.part_o + base * HD + d);
-        const float* w = weights + row * n;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncthreads();
+        if (is_last) {
+            __threadfence();
+            for (int idx = threadIdx.x; idx < group * (HD / 4); idx += blockDim.x) {
+                const int row = idx / (HD / 4), d = (idx - row * (HD / 4)) * 4;
+                float most = -INFINITY;
 #pragma unroll 8
-        for (int sp = 0; sp < n; ++sp) {
-            const float4 v = __ldcg(column + static_cast<size_t>(sp) * (HD / 4));
-            acc.x = fmaf(w[sp], v.x, acc.x);
-            acc.y = fmaf(w[sp], v.y, acc.y);
-            acc.z = fmaf(w[sp], v.z, acc.z);
-            acc.w = fmaf(w[sp], v.w, acc.w);
+                for (int i = 0; i < parts; ++i) most = fmaxf(most, __ldcg(a.part_ml + (place(i) + row) * 2));
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                float sum = 0.f;
+#pragma unroll 8
+                for (int i = 0; i < parts; ++i) {
+                    const size_t at = place(i) + row;
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + at * 2));
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + d));
+                    const float w = most == -INFINITY ? 0.f : exp2f(ml.x - most);
+                    sum = fmaf(w, ml.y, sum);
+                    acc.x = fmaf(w, v.x, acc.x);
+                    acc.y = fmaf(w, v.y, acc.y);
+                    acc.z = fmaf(w, v.z, acc.z);
+                    acc.w = fmaf(w, v.w, acc.w);
+                }
+                if (a.sinks != nullptr && most != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -most));
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+                if (reinterpret_cast<uintptr_t>(a.out) % 8 == 0) {
+                    *reinterpret_cast<uint2*>(out + row * HD + d) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[row * HD + d + i] = __float2bfloat16_rn(y[i]);
+                }
+            }
         }
-        const float inv = total[row] == 0.f ? 0.f : 1.f / total[row];
-        uint2 packed;
-        packed.x = pack_bf16(acc.x * inv, acc.y * inv);
-        packed.y = pack_bf16(acc.z * inv, acc.w * inv);
-        if (reinterpret_cast<uintptr_t>(a.out) % 8 == 0)
-            *reinterpret_cast<uint2*>(out + row * HD + d) = packed;
-        else
-            for (int i = 0; i < 4; ++i) out[row * HD + d + i] = __float2bfloat16_rn((&acc.x)[i] * inv);
+    }
+    // ---- on to the next
+    left -= n_tiles;
+    if (left == 0) return;
+    item += span.units;
+    skip = 0;
+    if (++kvh == a.nkv) {
+        kvh = 0;
+        do span = span_of(a, ++t);
+        while (span.units == 0);
+    }
+    tc::fence_proxy_async();        // the ring was written through the generic proxy: before the next copies into it
+    __syncthreads();
     }
 }
 
-// Keys per CTA, a multiple of 128 up to 2048: by the launch's sizes alone, so that a captured graph stays valid.
-inline int choose_split_keys(int tokens, int nkv, int max_context) {
-    static const int forced = [] {      // tuning hook: STRIDE_DECODE_INT4_SPLIT_KEYS=<multiple of 128>
-        const char* e = getenv("STRIDE_DECODE_INT4_SPLIT_KEYS");
-        const int v = e ? atoi(e) : 0;
-        return v > 0 ? (v < kMaxTiles * kUnit ? (v + kUnit - 1) / kUnit * kUnit : kMaxTiles * kUnit) : 0;
-    }();
-    if (forced) return forced;
-    const long long units = static_cast<long long>(tokens) * nkv * ((max_context + kUnit - 1) / kUnit);
-    long long u = (units + 820) / 821;
-    if (u < 4) u = (units + 206) / 207;
-    u = u < 1 ? 1 : (u > kMaxTiles ? kMaxTiles : u);
-    return static_cast<int>(u) * kUnit;
+// CTAs of a launch: as many as fit at once, no more than there can be units.
+inline int choose_ctas(int tokens, int nkv, int max_context, int group) {
+    const long long units = static_cast<long long>(tokens) * nkv * ((static_cast<long long>(max_context) + kUnit - 1) / kUnit);
+    const int fit = 148 * (group <= 8 ? 3 : 2);
+    return units < fit ? static_cast<int>(units) : fit;
 }
 
 template <int G, int NT>
-int launch_decode(const Decode& a, int tokens, cudaStream_t stream) {
+int launch_decode(const Decode& a, int ctas, cudaStream_t stream) {
     constexpr int smem = kWarps * kStages * 2 * kTile * 20 * G;        // 61 KB at head size 128
-    const int group = a.nq / a.nkv;
-    static_assert(kWarps * 8 * NT * (32 * G + 2) * 4 <= smem || NT > 1, "the merge fits into the rings");
-    const long long merge = static_cast<long long>(group) * (a.num_splits + 1) * 4, warps = static_cast<long long>(kWarps) * group * (32 * G + 2) * 4;
-    if (merge > smem || warps > smem) return STRIDE_UNSUPPORTED;
+    static_assert(kWarps * 8 * NT * (32 * G + 2) * 4 <= smem, "the warps' results fit into the rings");
     const bool bulk = a.page_size % kSub == 0;
     cudaError_t e = allow_shared<decode_kernel<G, NT, true>>(smem);
     if (e == cudaSuccess) e = allow_shared<decode_kernel<G, NT, false>>(smem);
     if (e != cudaSuccess) return static_cast<int>(e);
-    const dim3 grid(a.num_splits, a.nkv, tokens);
     if (bulk)
-        stride::launch(decode_kernel<G, NT, true>, grid, dim3(kWarps * 32), smem, stream, a);
+        stride::launch(decode_kernel<G, NT, true>, dim3(ctas), dim3(kWarps * 32), smem, stream, a);
     else
-        stride::launch(decode_kernel<G, NT, false>, grid, dim3(kWarps * 32), smem, stream, a);
+        stride::launch(decode_kernel<G, NT, false>, dim3(ctas), dim3(kWarps * 32), smem, stream, a);
     return STRIDE_LAUNCH_STATUS();
 }
 
@@ -641,9 +740,8 @@ extern "C" {
 // Number of float32 scratch elements the launcher needs for these sizes.
 long long stride_decode_int4_scratch_floats(int tokens, int nq, int nkv, int hd, int max_context) {
     if (tokens <= 0 || nq <= 0 || nkv <= 0 || max_context <= 0) return 0;
-    const int split_keys = four::choose_split_keys(tokens, nkv, max_context);
-    const long long splits = (static_cast<long long>(max_context) + split_keys - 1) / split_keys;
-    return four::kTicketInts + static_cast<long long>(tokens) * nq * splits * (hd + 2);
+    const int group = nq / nkv;
+    return four::kTicketInts + 2LL * four::choose_ctas(tokens, nkv, max_context, group) * group * (hd + 2);
 }
 
 struct DecodeCall {
@@ -669,21 +767,22 @@ static_assert(sizeof(DecodeCall) == 152, "the record that the caller packs");
 // One query token per row. `scratch` must be zero when it is first used (every launch leaves its tickets zero) and belongs to one stream at a
 // time. A row whose position does not lie below `max_context` gets zeros, and code 32 in the status word; a key whose page is none of the
 // cache's is left out, with code 33. Returns -2 for sizes it does not run: head sizes other than 64 and 128, groups above 16, more than
-// 65536 (token, key head) pairs, contexts of more than 8192 splits.
+// 65536 (token, key head) pairs.
 int stride_decode_int4(const void* record) {
     const DecodeCall r = read_record<DecodeCall>(record);
     if (r.tokens < 0 || r.nq <= 0 || r.nkv <= 0 || r.page_size <= 0 || r.table_width <= 0 || r.num_pages <= 0 || r.window < 0 || r.softcap < 0.f ||
         r.max_context <= 0 || r.nq % r.nkv || r.status == nullptr)
         return STRIDE_BAD_ARGUMENT;
-    if ((r.hd != 64 && r.hd != 128) || r.nq / r.nkv > 16 || r.tokens > 65535 || r.nkv > 65535 || r.max_context > (1 << 30)) return STRIDE_UNSUPPORTED;
+    if ((r.hd != 64 && r.hd != 128) || r.nq / r.nkv > 16 || r.max_context > (1 << 30)) return STRIDE_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(r.k_pages) | reinterpret_cast<uintptr_t>(r.v_pages) | reinterpret_cast<uintptr_t>(r.scratch)) % 16)
         return STRIDE_UNSUPPORTED;
     if (r.tokens == 0) return 0;
-    const int split_keys = four::choose_split_keys(r.tokens, r.nkv, r.max_context);
-    const int num_splits = (r.max_context + split_keys - 1) / split_keys;
-    if (num_splits > 8192 || static_cast<long long>(r.tokens) * r.nkv > four::kTicketInts) return STRIDE_UNSUPPORTED;
+    if (static_cast<long long>(r.tokens) * r.nkv > four::kTicketInts) return STRIDE_UNSUPPORTED;
+    // units are counted in 32 bits token by token
+    if (static_cast<long long>(r.tokens) * (r.max_context / four::kUnit + 1) > 2147483647LL) return STRIDE_UNSUPPORTED;
     if (r.scratch == nullptr || r.scratch_floats < stride_decode_int4_scratch_floats(r.tokens, r.nq, r.nkv, r.hd, r.max_context))
         return STRIDE_BAD_ARGUMENT;
+    const int ctas = four::choose_ctas(r.tokens, r.nkv, r.max_context, r.nq / r.nkv);
     static_assert(sizeof(int) == sizeof(float), "the tickets live in the float scratch");
     four::Decode a;
     a.q = r.q;
@@ -697,7 +796,7 @@ int stride_decode_int4(const void* record) {
     a.slopes = r.slopes;
     a.tickets = reinterpret_cast<int*>(r.scratch);
     a.part_o = r.scratch + four::kTicketInts;
-    a.part_ml = a.part_o + static_cast<long long>(r.tokens) * r.nq * num_splits * r.hd;
+    a.part_ml = a.part_o + 2LL * ctas * (r.nq / r.nkv) * r.hd;
     a.status = r.status;
     a.q_stride = r.q_stride;
     a.table_width = r.table_width;
@@ -706,14 +805,14 @@ int stride_decode_int4(const void* record) {
     a.nkv = r.nkv;
     a.page_size = r.page_size;
     a.window = r.window;
-    a.split_keys = split_keys;
-    a.num_splits = num_splits;
+    a.tokens = r.tokens;
+    a.max_context = r.max_context;
     a.scale_log2e = r.scale * 1.4426950408889634f;
     a.cap_log2e = r.softcap * 1.4426950408889634f;
     a.scale_over_cap = r.softcap > 0.f ? r.scale / r.softcap : 0.f;
     const bool wide = r.nq / r.nkv > 8;
-    if (r.hd == 64) return wide ? four::launch_decode<2, 2>(a, r.tokens, r.stream) : four::launch_decode<2, 1>(a, r.tokens, r.stream);
-    return wide ? four::launch_decode<4, 2>(a, r.tokens, r.stream) : four::launch_decode<4, 1>(a, r.tokens, r.stream);
+    if (r.hd == 64) return wide ? four::launch_decode<2, 2>(a, ctas, r.stream) : four::launch_decode<2, 1>(a, ctas, r.stream);
+    return wide ? four::launch_decode<4, 2>(a, ctas, r.stream) : four::launch_decode<4, 1>(a, ctas, r.stream);
 }
 
 }  // extern "C"

@@ -9,8 +9,8 @@
 //   keys    entry 8 a + i of group g: 32-bit word a G + g, bits 4 i      (a lane that takes part a = lane % 4 of every key finds it side by side)
 //   values  entry 4 a + i of group g: 16-bit word a G + g, bits 4 i      (a lane that takes part a = lane / 4 of every value, likewise)
 // A number that stands for nothing (behind a head's last entry) is 8.
-// A key or value that is no number or not below 2^102 makes its token no number for that key head: the key row gets s = c = NaN and the value
-// row zeros, so whoever sees the token gets NaN and whoever does not is left alone, whatever the mask multiplies. (Below 2^102 a weight
+// A key or value that is no number or not below 2^64 makes its token no number for that key head: the key row gets s = c = NaN and the value
+// row zeros, so whoever sees the token gets NaN and whoever does not is left alone, whatever the mask multiplies. (Below 2^64 a weight
 // can be scaled against a row's scales and centres without leaving the 32-bit range.)
 #pragma once
 
@@ -33,7 +33,7 @@ namespace four {
 constexpr int kGroup = 32;
 constexpr int kMaxHeadDim = 256;
 constexpr int kMaxGroups = kMaxHeadDim / kGroup;
-constexpr float kMaxEntry = 5.0706024e30f;      // 2^102
+constexpr float kMaxEntry = 1.8446744e19f;      // 2^64
 
 __host__ __device__ __forceinline__ int groups_of(int hd) { return (hd + kGroup - 1) / kGroup; }
 __host__ __device__ __forceinline__ int row_bytes(int hd) { return 20 * groups_of(hd); }
