@@ -162,6 +162,208 @@ __global__ void __launch_bounds__(kWriteWarps * 32) head_write_kernel(const Head
     }
 }
 
+// The same for head sizes 64, 128 and 256: HD / 8 lanes a head, a lane owns four neighbouring entries of either half, so the pairs that turn
+// together meet in one lane, a group of 32 is eight neighbouring lanes, and loads and stores are 8 (bfloat16) or 16 bytes. A CTA is a token;
+// a slot of HD / 8 lanes takes UNITS units, whose loads are all under way before the first is worked on, with one read of the angles.
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+    float4 raw;
+    __device__ __forceinline__ void load(const float* p) { raw = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void get(float (&x)[4]) const { x[0] = raw.x; x[1] = raw.y; x[2] = raw.z; x[3] = raw.w; }
+    static __device__ __forceinline__ void put(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+};
+template <>
+struct Four<__nv_bfloat16> {
+    uint2 raw;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { raw = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ void get(float (&x)[4]) const {
+        x[0] = four::bf16_low(raw.x); x[1] = four::bf16_high(raw.x); x[2] = four::bf16_low(raw.y); x[3] = four::bf16_high(raw.y);
+    }
+    static __device__ __forceinline__ void put(__nv_bfloat16* p, const float (&x)[4]) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(four::pack_params(x[0], x[1]), four::pack_params(x[2], x[3]));
+    }
+};
+
+constexpr int kMostWriteThreads = 512;
+
+template <typename T, bool FOUR, int HD, int UNITS>
+__global__ void __launch_bounds__(kMostWriteThreads) head_write_vec_kernel(const HeadWrite a) {
+    constexpr int L = HD / 8, HALF = HD / 2, G = HD / 32;
+    pdl_trigger();
+    pdl_wait();
+    const int t = blockIdx.x, lane = threadIdx.x & 31, i = threadIdx.x % L, slots = blockDim.x / L, heads = a.nq + 2 * a.nkv;
+    const uint32_t mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (lane / L * L);       // the lanes of this slot
+    const int pos = a.rotate ? a.positions[t] : 0;
+    if (a.rotate && (pos < 0 || pos >= a.num_positions)) {
+        if (threadIdx.x == 0) four::complain(a.status, four::kCodeNoPosition);
+        return;
+    }
+    const int place = a.slots != nullptr ? a.slots[t] : -1, page = place < 0 ? -1 : place / a.page_size;
+    if (page >= a.num_pages && threadIdx.x == 0) four::complain(a.status, four::kCodeNoSlot);
+    const bool stored = page >= 0 && page < a.num_pages;
+    const T* row = static_cast<const T*>(a.rows) + static_cast<size_t>(t) * heads * HD;
+    float cs[4], sn[4];
+    if (a.rotate) {
+        Four<float> c, s;
+        c.load(a.cos + static_cast<size_t>(pos) * HALF + 4 * i);
+        s.load(a.sin + static_cast<size_t>(pos) * HALF + 4 * i);
+        c.get(cs);
+        s.get(sn);
+    }
+    for (int u0 = threadIdx.x / L; u0 < a.nq + a.nkv; u0 += slots * UNITS) {
+        Four<T> in[UNITS][2], vin[UNITS][2];
+#pragma unroll
+        for (int k = 0; k < UNITS; ++k) {
+            const int u = u0 + k * slots;
+            if (u >= a.nq + a.nkv || (u >= a.nq && !stored)) continue;
+            in[k][0].load(row + static_cast<size_t>(u) * HD + 4 * i);
+            in[k][1].load(row + static_cast<size_t>(u) * HD + HALF + 4 * i);
+            if (u >= a.nq) {
+                vin[k][0].load(row + static_cast<size_t>(u + a.nkv) * HD + 4 * i);
+                vin[k][1].load(row + static_cast<size_t>(u + a.nkv) * HD + HALF + 4 * i);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < UNITS; ++k) {
+            const int u = u0 + k * slots;
+            if (u >= a.nq + a.nkv || (u >= a.nq && !stored)) continue;
+            const bool is_q = u < a.nq;
+            float x[2][4], v[2][4];
+            in[k][0].get(x[0]);
+            in[k][1].get(x[1]);
+            if (!is_q) {
+                vin[k][0].get(v[0]);
+                vin[k][1].get(v[1]);
+            }
+            if (a.bias != nullptr) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    Four<float> add;
+                    float b[4];
+                    add.load(a.bias + static_cast<size_t>(u) * HD + h * HALF + 4 * i);
+                    add.get(b);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[h][e] = __fadd_rn(x[h][e], b[e]);
+                    if (is_q) continue;
+                    add.load(a.bias + static_cast<size_t>(u + a.nkv) * HD + h * HALF + 4 * i);
+                    add.get(b);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[h][e] = __fadd_rn(v[h][e], b[e]);
+                }
+            }
+            const float* weight = is_q ? a.q_norm : a.k_norm;
+            if (weight != nullptr) {
+                float sum = 0.f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum = fmaf(x[h][e], x[h][e], sum);
+#pragma unroll
+                for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
+                const float inv = rsqrtf(__fadd_rn(__fdiv_rn(sum, static_cast<float>(HD)), a.eps));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    Four<float> of;
+                    float w[4];
+                    of.load(weight + h * HALF + 4 * i);
+                    of.get(w);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[h][e] = __fmul_rn(__fmul_rn(x[h][e], inv), w[e]);
+                }
+            }
+            if (a.rotate) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = x[0][e], q = x[1][e];
+                    x[0][e] = __fadd_rn(__fmul_rn(p, cs[e]), __fmul_rn(-q, sn[e]));
+                    x[1][e] = __fadd_rn(__fmul_rn(q, cs[e]), __fmul_rn(p, sn[e]));
+                }
+            }
+            if (is_q) {
+                T* out = static_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.q_out_stride + static_cast<size_t>(u) * HD + 4 * i;
+                Four<T>::put(out, x[0]);
+                Four<T>::put(out + HALF, x[1]);
+                continue;
+            }
+            const size_t at = (static_cast<size_t>(page) * a.nkv + (u - a.nq)) * a.page_size + place % a.page_size;
+            if constexpr (!FOUR) {
+                T* ko = static_cast<T*>(a.k_pages) + at * HD + 4 * i;
+                T* vo = static_cast<T*>(a.v_pages) + at * HD + 4 * i;
+                Four<T>::put(ko, x[0]);
+                Four<T>::put(ko + HALF, x[1]);
+                Four<T>::put(vo, v[0]);
+                Four<T>::put(vo + HALF, v[1]);
+            } else {
+                uint8_t* ko = static_cast<uint8_t*>(a.k_pages) + at * (20 * G);
+                uint8_t* vo = static_cast<uint8_t*>(a.v_pages) + at * (20 * G);
+                float s[2][2], c[2][2];             // [key, value][half]
+                bool fine = true;
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float(&y)[4] = w ? v[h] : x[h];
+                        float lo = fminf(fminf(y[0], y[1]), fminf(y[2], y[3])), hi = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) fine = fine && fabsf(y[e]) < four::kMaxEntry;
+#pragma unroll
+                        for (int o = 1; o < 8; o <<= 1) {
+                            lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+                            hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+                        }
+                        four::group_params(lo, hi, s[w][h], c[w][h]);
+                    }
+                fine = __all_sync(mask, fine);
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float(&y)[4] = w ? v[h] : x[h];
+                        const int g = h * (G / 2) + i / 8, r = i & 7;          // this lane: entries 4 r .. of group g
+                        float sg = s[w][h], cg = c[w][h];
+                        uint32_t n = 0x8888u;
+                        if (!fine) {
+                            sg = cg = w ? 0.f : __int_as_float(0x7fc00000);
+                        } else if (sg > 0.f) {
+                            const float inverse = __frcp_rn(sg);
+                            n = four::number_of(y[0], cg, inverse) | four::number_of(y[1], cg, inverse) << 4 | four::number_of(y[2], cg, inverse) << 8 |
+                                four::number_of(y[3], cg, inverse) << 12;
+                        }
+                        uint8_t* out = w ? vo : ko;
+                        // keys: half a word of entries 8 (r / 2) .., values: the 16 bits of entries 4 r ..
+                        const int half_word = w ? r * G + g : 2 * ((r >> 1) * G + g) + (r & 1);
+                        reinterpret_cast<uint16_t*>(out)[half_word] = static_cast<uint16_t>(n);
+                        if (r == 0) reinterpret_cast<uint32_t*>(out + 16 * G)[g] = four::pack_params(sg, cg);
+                    }
+            }
+        }
+    }
+}
+
+template <typename T, bool FOUR, int HD>
+void launch_vec(const HeadWrite& a) {
+    constexpr int L = HD / 8;
+    const int units = a.nq + a.nkv;
+    int threads = (units + 1) / 2 * L;
+    threads = threads > kMostWriteThreads ? kMostWriteThreads : (threads + 31) / 32 * 32;
+    stride::launch(head_write_vec_kernel<T, FOUR, HD, 2>, dim3(a.tokens), dim3(threads), 0, a.stream, a);
+}
+template <typename T, bool FOUR>
+bool launch_vec_of(const HeadWrite& a) {        // false: not these sizes, or not aligned
+    uintptr_t rows = reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(a.q_out);
+    if (!FOUR) rows |= reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages);
+    uintptr_t angles = reinterpret_cast<uintptr_t>(a.bias) | reinterpret_cast<uintptr_t>(a.q_norm) | reinterpret_cast<uintptr_t>(a.k_norm);
+    if (a.rotate) angles |= reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin);
+    if (rows % (4 * sizeof(T)) || angles % 16 || a.q_out_stride % 4) return false;
+    if (a.hd == 64) launch_vec<T, FOUR, 64>(a);
+    else if (a.hd == 128) launch_vec<T, FOUR, 128>(a);
+    else if (a.hd == 256) launch_vec<T, FOUR, 256>(a);
+    else return false;
+    return true;
+}
+
 // What the slots of a 4-bit cache stand for: k_out, v_out [n, nkv, hd]. A slot below zero reads as zeros. A warp a row.
 template <typename T>
 __global__ void __launch_bounds__(kWriteWarps * 32)
@@ -195,6 +397,47 @@ int4_read_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict_
         out[0][d] = from_f32<T>(four::value_of(kn, four::bf16_low(kp), four::bf16_high(kp)));
         out[1][d] = from_f32<T>(four::value_of(vn, four::bf16_low(vp), four::bf16_high(vp)));
     }
+}
+
+// The same for head sizes 64, 128 and 256: HD / 8 lanes a row, four neighbouring entries of either half a lane.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256)
+int4_read_vec_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const int32_t* __restrict__ slots, T* __restrict__ k_out,
+                     T* __restrict__ v_out, long long units, int nkv, int page_size, int num_pages, int* status) {
+    constexpr int L = HD / 8, HALF = HD / 2, G = HD / 32;
+    pdl_trigger();
+    pdl_wait();
+    const int i = threadIdx.x % L, r = i & 7;
+    const long long unit = static_cast<long long>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+    if (unit >= units) return;
+    const int slot = slots[unit / nkv], kvh = static_cast<int>(unit % nkv);
+    int page = slot < 0 ? -1 : slot / page_size;
+    if (page >= num_pages) {
+        if (i == 0) four::complain(status, four::kCodeNoSlot);
+        page = -1;
+    }
+    float y[4][4] = {};
+    if (page >= 0) {
+        const size_t at = ((static_cast<size_t>(page) * nkv + kvh) * page_size + slot % page_size) * (20 * G);
+        uint32_t n[4], p[4];
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint8_t* row = (w ? v_pages : k_pages) + at;
+                const int g = h * (G / 2) + i / 8;
+                n[2 * w + h] = reinterpret_cast<const uint16_t*>(row)[w ? r * G + g : 2 * ((r >> 1) * G + g) + (r & 1)];
+                p[2 * w + h] = reinterpret_cast<const uint32_t*>(row + 16 * G)[g];
+            }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[q][e] = four::value_of(n[q] >> (4 * e) & 15u, four::bf16_low(p[q]), four::bf16_high(p[q]));
+    }
+    Four<T>::put(k_out + unit * HD + 4 * i, y[0]);
+    Four<T>::put(k_out + unit * HD + HALF + 4 * i, y[1]);
+    Four<T>::put(v_out + unit * HD + 4 * i, y[2]);
+    Four<T>::put(v_out + unit * HD + HALF + 4 * i, y[3]);
 }
 
 // The keys of the first num_seqs requests as pages of 64 in bfloat16, for the attention of portions: a request's pages one after the other,
@@ -304,15 +547,18 @@ extern "C" int stride_head_write(const void* record) {
     const int units = a.nq + a.nkv, ctas_y = (units + kWriteWarps - 1) / kWriteWarps;
     if (ctas_y > 65535) return STRIDE_UNSUPPORTED;
     if (a.tokens == 0) return 0;
+    if (a.dtype != STRIDE_DTYPE_F32 && a.dtype != STRIDE_DTYPE_BF16) return STRIDE_BAD_ARGUMENT;
+    const bool wide = a.dtype == STRIDE_DTYPE_F32;
+    if (wide ? (a.bits4 ? launch_vec_of<float, true>(a) : launch_vec_of<float, false>(a))
+             : (a.bits4 ? launch_vec_of<__nv_bfloat16, true>(a) : launch_vec_of<__nv_bfloat16, false>(a)))
+        return STRIDE_LAUNCH_STATUS();
     const dim3 grid(a.tokens, ctas_y), block(kWriteWarps * 32);
-    if (a.dtype == STRIDE_DTYPE_F32)
+    if (wide)
         a.bits4 ? stride::launch(head_write_kernel<float, true>, grid, block, 0, a.stream, a)
                 : stride::launch(head_write_kernel<float, false>, grid, block, 0, a.stream, a);
-    else if (a.dtype == STRIDE_DTYPE_BF16)
+    else
         a.bits4 ? stride::launch(head_write_kernel<__nv_bfloat16, true>, grid, block, 0, a.stream, a)
                 : stride::launch(head_write_kernel<__nv_bfloat16, false>, grid, block, 0, a.stream, a);
-    else
-        return STRIDE_BAD_ARGUMENT;
     return STRIDE_LAUNCH_STATUS();
 }
 
@@ -334,17 +580,32 @@ extern "C" int stride_int4_read(const void* record) {
     if (a.n < 0 || a.nkv <= 0 || a.hd <= 0 || a.page_size <= 0 || a.num_pages <= 0) return STRIDE_BAD_ARGUMENT;
     if (a.hd > four::kMaxHeadDim || (reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4) return STRIDE_UNSUPPORTED;
     if (a.n == 0) return 0;
+    const long long units = static_cast<long long>(a.n) * a.nkv;
+    if (a.dtype != STRIDE_DTYPE_F32 && a.dtype != STRIDE_DTYPE_BF16) return STRIDE_BAD_ARGUMENT;
+    const bool aligned = (reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) % 16 == 0;
+    if (aligned && (a.hd == 64 || a.hd == 128 || a.hd == 256)) {
+        const int rows = 2048 / a.hd;       // of a CTA of 256 threads
+        if ((units + rows - 1) / rows > 2147483647LL) return STRIDE_UNSUPPORTED;
+        const dim3 grid(static_cast<unsigned>((units + rows - 1) / rows));
+#define STRIDE_READ(T_, HD_)                                                                                                                       \
+    stride::launch(int4_read_vec_kernel<T_, HD_>, grid, dim3(256), 0, a.stream, a.k_pages, a.v_pages, a.slots, static_cast<T_*>(a.k_out),           \
+                   static_cast<T_*>(a.v_out), units, a.nkv, a.page_size, a.num_pages, a.status)
+        if (a.dtype == STRIDE_DTYPE_F32)
+            a.hd == 64 ? STRIDE_READ(float, 64) : a.hd == 128 ? STRIDE_READ(float, 128) : STRIDE_READ(float, 256);
+        else
+            a.hd == 64 ? STRIDE_READ(__nv_bfloat16, 64) : a.hd == 128 ? STRIDE_READ(__nv_bfloat16, 128) : STRIDE_READ(__nv_bfloat16, 256);
+#undef STRIDE_READ
+        return STRIDE_LAUNCH_STATUS();
+    }
     const long long ctas = (static_cast<long long>(a.n) * a.nkv + kWriteWarps - 1) / kWriteWarps;
     if (ctas > 2147483647LL) return STRIDE_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(ctas)), block(kWriteWarps * 32);
     if (a.dtype == STRIDE_DTYPE_F32)
         stride::launch(int4_read_kernel<float>, grid, block, 0, a.stream, a.k_pages, a.v_pages, a.slots, static_cast<float*>(a.k_out),
                        static_cast<float*>(a.v_out), a.n, a.nkv, a.hd, a.page_size, a.num_pages, a.status);
-    else if (a.dtype == STRIDE_DTYPE_BF16)
+    else
         stride::launch(int4_read_kernel<__nv_bfloat16>, grid, block, 0, a.stream, a.k_pages, a.v_pages, a.slots, static_cast<__nv_bfloat16*>(a.k_out),
                        static_cast<__nv_bfloat16*>(a.v_out), a.n, a.nkv, a.hd, a.page_size, a.num_pages, a.status);
-    else
-        return STRIDE_BAD_ARGUMENT;
     return STRIDE_LAUNCH_STATUS();
 }
 
