@@ -163,8 +163,9 @@ __global__ void __launch_bounds__(kWriteWarps * 32) head_write_kernel(const Head
 }
 
 // The same for head sizes 64, 128 and 256: HD / 8 lanes a head, a lane owns four neighbouring entries of either half, so the pairs that turn
-// together meet in one lane, a group of 32 is eight neighbouring lanes, and loads and stores are 8 (bfloat16) or 16 bytes. A CTA is a token;
-// a slot of HD / 8 lanes takes UNITS units, whose loads are all under way before the first is worked on, with one read of the angles.
+// together meet in one lane, a group of 32 is eight neighbouring lanes, and loads and stores are 8 (bfloat16) or 16 bytes. HD / 8 lanes take
+// an item: kQueries query heads of a token, or kPairs of its key heads with their values, whose loads are all under way, beside the
+// position's and the slot's, before the first is worked on; the angles are read once an item.
 template <typename T>
 struct Four;
 template <>
@@ -186,169 +187,188 @@ struct Four<__nv_bfloat16> {
     }
 };
 
-constexpr int kMostWriteThreads = 512;
+constexpr int kItemThreads = 256, kQueries = 4, kPairs = 2;
 
-template <typename T, bool FOUR, int HD, int UNITS>
-__global__ void __launch_bounds__(kMostWriteThreads) head_write_vec_kernel(const HeadWrite a) {
+template <typename T, bool FOUR, int HD>
+__global__ void __launch_bounds__(kItemThreads, 4) head_write_vec_kernel(const HeadWrite a) {
     constexpr int L = HD / 8, HALF = HD / 2, G = HD / 32;
     pdl_trigger();
     pdl_wait();
-    const int t = blockIdx.x, lane = threadIdx.x & 31, i = threadIdx.x % L, slots = blockDim.x / L, heads = a.nq + 2 * a.nkv;
-    const uint32_t mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (lane / L * L);       // the lanes of this slot
+    const int lane = threadIdx.x & 31, i = threadIdx.x % L, heads = a.nq + 2 * a.nkv;
+    const uint32_t mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (lane / L * L);       // the lanes of this item
+    const int q_items = (a.nq + kQueries - 1) / kQueries, kv_items = (a.nkv + kPairs - 1) / kPairs;
+    long long item = static_cast<long long>(blockIdx.x) * (kItemThreads / L) + threadIdx.x / L;
+    const bool is_q = item < static_cast<long long>(a.tokens) * q_items;
+    if (!is_q) item -= static_cast<long long>(a.tokens) * q_items;
+    const int per = is_q ? q_items : kv_items, t = static_cast<int>(item / per), u0 = static_cast<int>(item % per);   // heads u0, u0 + per, ...
+    if (t >= a.tokens) return;
+    const T* row = static_cast<const T*>(a.rows) + static_cast<size_t>(t) * heads * HD + 4 * i;
     const int pos = a.rotate ? a.positions[t] : 0;
-    if (a.rotate && (pos < 0 || pos >= a.num_positions)) {
-        if (threadIdx.x == 0) four::complain(a.status, four::kCodeNoPosition);
-        return;
-    }
-    const int place = a.slots != nullptr ? a.slots[t] : -1, page = place < 0 ? -1 : place / a.page_size;
-    if (page >= a.num_pages && threadIdx.x == 0) four::complain(a.status, four::kCodeNoSlot);
-    const bool stored = page >= 0 && page < a.num_pages;
-    const T* row = static_cast<const T*>(a.rows) + static_cast<size_t>(t) * heads * HD;
+    const int place = !is_q && a.slots != nullptr ? a.slots[t] : -1;
     float cs[4], sn[4];
-    if (a.rotate) {
+    auto angles = [&]() {           // false: there are none for the token's position
+        if (!a.rotate) return true;
+        if (pos < 0 || pos >= a.num_positions) {
+            if (i == 0) four::complain(a.status, four::kCodeNoPosition);
+            return false;
+        }
         Four<float> c, s;
         c.load(a.cos + static_cast<size_t>(pos) * HALF + 4 * i);
         s.load(a.sin + static_cast<size_t>(pos) * HALF + 4 * i);
         c.get(cs);
         s.get(sn);
-    }
-    for (int u0 = threadIdx.x / L; u0 < a.nq + a.nkv; u0 += slots * UNITS) {
-        Four<T> in[UNITS][2], vin[UNITS][2];
+        return true;
+    };
+    auto add_bias = [&](float (&x)[2][4], int u) {
 #pragma unroll
-        for (int k = 0; k < UNITS; ++k) {
-            const int u = u0 + k * slots;
-            if (u >= a.nq + a.nkv || (u >= a.nq && !stored)) continue;
-            in[k][0].load(row + static_cast<size_t>(u) * HD + 4 * i);
-            in[k][1].load(row + static_cast<size_t>(u) * HD + HALF + 4 * i);
-            if (u >= a.nq) {
-                vin[k][0].load(row + static_cast<size_t>(u + a.nkv) * HD + 4 * i);
-                vin[k][1].load(row + static_cast<size_t>(u + a.nkv) * HD + HALF + 4 * i);
+        for (int h = 0; h < 2; ++h) {
+            Four<float> add;
+            float b[4];
+            add.load(a.bias + static_cast<size_t>(u) * HD + h * HALF + 4 * i);
+            add.get(b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[h][e] = __fadd_rn(x[h][e], b[e]);
+        }
+    };
+    auto norm_and_turn = [&](float (&x)[2][4], const float* weight) {
+        if (weight != nullptr) {
+            float sum = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = fmaf(x[h][e], x[h][e], sum);
+#pragma unroll
+            for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
+            const float inv = rsqrtf(__fadd_rn(__fdiv_rn(sum, static_cast<float>(HD)), a.eps));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                Four<float> of;
+                float w[4];
+                of.load(weight + h * HALF + 4 * i);
+                of.get(w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[h][e] = __fmul_rn(__fmul_rn(x[h][e], inv), w[e]);
             }
         }
+        if (a.rotate) {
 #pragma unroll
-        for (int k = 0; k < UNITS; ++k) {
-            const int u = u0 + k * slots;
-            if (u >= a.nq + a.nkv || (u >= a.nq && !stored)) continue;
-            const bool is_q = u < a.nq;
-            float x[2][4], v[2][4];
+            for (int e = 0; e < 4; ++e) {
+                const float p = x[0][e], q = x[1][e];
+                x[0][e] = __fadd_rn(__fmul_rn(p, cs[e]), __fmul_rn(-q, sn[e]));
+                x[1][e] = __fadd_rn(__fmul_rn(q, cs[e]), __fmul_rn(p, sn[e]));
+            }
+        }
+    };
+    if (is_q) {
+        Four<T> in[kQueries][2];
+#pragma unroll
+        for (int k = 0; k < kQueries; ++k)
+            if (u0 + k * per < a.nq) {
+                in[k][0].load(row + static_cast<size_t>(u0 + k * per) * HD);
+                in[k][1].load(row + static_cast<size_t>(u0 + k * per) * HD + HALF);
+            }
+        if (!angles()) return;
+        T* out = static_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.q_out_stride + 4 * i;
+#pragma unroll
+        for (int k = 0; k < kQueries; ++k) {
+            const int u = u0 + k * per;
+            if (u >= a.nq) break;
+            float x[2][4];
             in[k][0].get(x[0]);
             in[k][1].get(x[1]);
-            if (!is_q) {
-                vin[k][0].get(v[0]);
-                vin[k][1].get(v[1]);
-            }
-            if (a.bias != nullptr) {
+            if (a.bias != nullptr) add_bias(x, u);
+            norm_and_turn(x, a.q_norm);
+            Four<T>::put(out + static_cast<size_t>(u) * HD, x[0]);
+            Four<T>::put(out + static_cast<size_t>(u) * HD + HALF, x[1]);
+        }
+        return;
+    }
+    Four<T> in[kPairs][4];
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k)
+        if (u0 + k * per < a.nkv) {
+            const T* key = row + static_cast<size_t>(a.nq + u0 + k * per) * HD;
+            const T* value = key + static_cast<size_t>(a.nkv) * HD;
+            in[k][0].load(key);
+            in[k][1].load(key + HALF);
+            in[k][2].load(value);
+            in[k][3].load(value + HALF);
+        }
+    if (place < 0 || !angles()) return;
+    const int page = place / a.page_size;
+    if (page >= a.num_pages) {
+        if (i == 0) four::complain(a.status, four::kCodeNoSlot);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) {
+        const int u = u0 + k * per;
+        if (u >= a.nkv) break;
+        float x[2][2][4];                           // key, value
+#pragma unroll
+        for (int q = 0; q < 4; ++q) in[k][q].get(x[q >> 1][q & 1]);
+        if (a.bias != nullptr) {
+            add_bias(x[0], a.nq + u);
+            add_bias(x[1], a.nq + a.nkv + u);
+        }
+        norm_and_turn(x[0], a.k_norm);
+        const size_t at = (static_cast<size_t>(page) * a.nkv + u) * a.page_size + place % a.page_size;
+        if constexpr (!FOUR) {
+            T* ko = static_cast<T*>(a.k_pages) + at * HD + 4 * i;
+            T* vo = static_cast<T*>(a.v_pages) + at * HD + 4 * i;
+            Four<T>::put(ko, x[0][0]);
+            Four<T>::put(ko + HALF, x[0][1]);
+            Four<T>::put(vo, x[1][0]);
+            Four<T>::put(vo + HALF, x[1][1]);
+        } else {
+            float s[2][2], c[2][2];                 // [key, value][half]
+            bool fine = true;
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    Four<float> add;
-                    float b[4];
-                    add.load(a.bias + static_cast<size_t>(u) * HD + h * HALF + 4 * i);
-                    add.get(b);
+                    const float(&y)[4] = x[w][h];
+                    float lo = fminf(fminf(y[0], y[1]), fminf(y[2], y[3])), hi = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[h][e] = __fadd_rn(x[h][e], b[e]);
-                    if (is_q) continue;
-                    add.load(a.bias + static_cast<size_t>(u + a.nkv) * HD + h * HALF + 4 * i);
-                    add.get(b);
+                    for (int e = 0; e < 4; ++e) fine = fine && fabsf(y[e]) < four::kMaxEntry;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[h][e] = __fadd_rn(v[h][e], b[e]);
+                    for (int o = 1; o < 8; o <<= 1) {
+                        lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+                        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+                    }
+                    four::group_params(lo, hi, s[w][h], c[w][h]);
                 }
-            }
-            const float* weight = is_q ? a.q_norm : a.k_norm;
-            if (weight != nullptr) {
-                float sum = 0.f;
+            fine = __all_sync(mask, fine);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum = fmaf(x[h][e], x[h][e], sum);
-#pragma unroll
-                for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
-                const float inv = rsqrtf(__fadd_rn(__fdiv_rn(sum, static_cast<float>(HD)), a.eps));
+            for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    Four<float> of;
-                    float w[4];
-                    of.load(weight + h * HALF + 4 * i);
-                    of.get(w);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[h][e] = __fmul_rn(__fmul_rn(x[h][e], inv), w[e]);
-                }
-            }
-            if (a.rotate) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = x[0][e], q = x[1][e];
-                    x[0][e] = __fadd_rn(__fmul_rn(p, cs[e]), __fmul_rn(-q, sn[e]));
-                    x[1][e] = __fadd_rn(__fmul_rn(q, cs[e]), __fmul_rn(p, sn[e]));
-                }
-            }
-            if (is_q) {
-                T* out = static_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.q_out_stride + static_cast<size_t>(u) * HD + 4 * i;
-                Four<T>::put(out, x[0]);
-                Four<T>::put(out + HALF, x[1]);
-                continue;
-            }
-            const size_t at = (static_cast<size_t>(page) * a.nkv + (u - a.nq)) * a.page_size + place % a.page_size;
-            if constexpr (!FOUR) {
-                T* ko = static_cast<T*>(a.k_pages) + at * HD + 4 * i;
-                T* vo = static_cast<T*>(a.v_pages) + at * HD + 4 * i;
-                Four<T>::put(ko, x[0]);
-                Four<T>::put(ko + HALF, x[1]);
-                Four<T>::put(vo, v[0]);
-                Four<T>::put(vo + HALF, v[1]);
-            } else {
-                uint8_t* ko = static_cast<uint8_t*>(a.k_pages) + at * (20 * G);
-                uint8_t* vo = static_cast<uint8_t*>(a.v_pages) + at * (20 * G);
-                float s[2][2], c[2][2];             // [key, value][half]
-                bool fine = true;
-#pragma unroll
-                for (int w = 0; w < 2; ++w)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float(&y)[4] = w ? v[h] : x[h];
-                        float lo = fminf(fminf(y[0], y[1]), fminf(y[2], y[3])), hi = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) fine = fine && fabsf(y[e]) < four::kMaxEntry;
-#pragma unroll
-                        for (int o = 1; o < 8; o <<= 1) {
-                            lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-                            hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
-                        }
-                        four::group_params(lo, hi, s[w][h], c[w][h]);
+                    const float(&y)[4] = x[w][h];
+                    const int g = h * (G / 2) + i / 8, r = i & 7;              // this lane: entries 4 r .. of group g
+                    float sg = s[w][h], cg = c[w][h];
+                    uint32_t n = 0x8888u;
+                    if (!fine) {
+                        sg = cg = w ? 0.f : __int_as_float(0x7fc00000);
+                    } else if (sg > 0.f) {
+                        const float inverse = __frcp_rn(sg);
+                        n = four::number_of(y[0], cg, inverse) | four::number_of(y[1], cg, inverse) << 4 | four::number_of(y[2], cg, inverse) << 8 |
+                            four::number_of(y[3], cg, inverse) << 12;
                     }
-                fine = __all_sync(mask, fine);
-#pragma unroll
-                for (int w = 0; w < 2; ++w)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float(&y)[4] = w ? v[h] : x[h];
-                        const int g = h * (G / 2) + i / 8, r = i & 7;          // this lane: entries 4 r .. of group g
-                        float sg = s[w][h], cg = c[w][h];
-                        uint32_t n = 0x8888u;
-                        if (!fine) {
-                            sg = cg = w ? 0.f : __int_as_float(0x7fc00000);
-                        } else if (sg > 0.f) {
-                            const float inverse = __frcp_rn(sg);
-                            n = four::number_of(y[0], cg, inverse) | four::number_of(y[1], cg, inverse) << 4 | four::number_of(y[2], cg, inverse) << 8 |
-                                four::number_of(y[3], cg, inverse) << 12;
-                        }
-                        uint8_t* out = w ? vo : ko;
-                        // keys: half a word of entries 8 (r / 2) .., values: the 16 bits of entries 4 r ..
-                        const int half_word = w ? r * G + g : 2 * ((r >> 1) * G + g) + (r & 1);
-                        reinterpret_cast<uint16_t*>(out)[half_word] = static_cast<uint16_t>(n);
-                        if (r == 0) reinterpret_cast<uint32_t*>(out + 16 * G)[g] = four::pack_params(sg, cg);
-                    }
-            }
+                    uint8_t* out = static_cast<uint8_t*>(w ? a.v_pages : a.k_pages) + at * (20 * G);
+                    // keys: half a word of entries 8 (r / 2) .., values: the 16 bits of entries 4 r ..
+                    const int half_word = w ? r * G + g : 2 * ((r >> 1) * G + g) + (r & 1);
+                    reinterpret_cast<uint16_t*>(out)[half_word] = static_cast<uint16_t>(n);
+                    if (r == 0) reinterpret_cast<uint32_t*>(out + 16 * G)[g] = four::pack_params(sg, cg);
+                }
         }
     }
 }
 
 template <typename T, bool FOUR, int HD>
 void launch_vec(const HeadWrite& a) {
-    constexpr int L = HD / 8;
-    const int units = a.nq + a.nkv;
-    int threads = (units + 1) / 2 * L;
-    threads = threads > kMostWriteThreads ? kMostWriteThreads : (threads + 31) / 32 * 32;
-    stride::launch(head_write_vec_kernel<T, FOUR, HD, 2>, dim3(a.tokens), dim3(threads), 0, a.stream, a);
+    const long long items = static_cast<long long>(a.tokens) * ((a.nq + kQueries - 1) / kQueries + (a.nkv + kPairs - 1) / kPairs);
+    const long long per_cta = kItemThreads / (HD / 8);
+    stride::launch(head_write_vec_kernel<T, FOUR, HD>, dim3(static_cast<unsigned>((items + per_cta - 1) / per_cta)), dim3(kItemThreads), 0, a.stream, a);
 }
 template <typename T, bool FOUR>
 bool launch_vec_of(const HeadWrite& a) {        // false: not these sizes, or not aligned
@@ -356,7 +376,7 @@ bool launch_vec_of(const HeadWrite& a) {        // false: not these sizes, or no
     if (!FOUR) rows |= reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages);
     uintptr_t angles = reinterpret_cast<uintptr_t>(a.bias) | reinterpret_cast<uintptr_t>(a.q_norm) | reinterpret_cast<uintptr_t>(a.k_norm);
     if (a.rotate) angles |= reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin);
-    if (rows % (4 * sizeof(T)) || angles % 16 || a.q_out_stride % 4) return false;
+    if (rows % (4 * sizeof(T)) || angles % 16 || a.q_out_stride % 4 || static_cast<long long>(a.tokens) * (a.nq + a.nkv) > 2147483647LL) return false;
     if (a.hd == 64) launch_vec<T, FOUR, 64>(a);
     else if (a.hd == 128) launch_vec<T, FOUR, 128>(a);
     else if (a.hd == 256) launch_vec<T, FOUR, 256>(a);
