@@ -104,6 +104,213 @@ attention_int4_exact_kernel(const T* __restrict__ q, int q_stride, T* __restrict
         if (32 * j + lane < hd) out_row[32 * j + lane] = from_f32<T>(acc[j] * inv);
 }
 
+// The same, bit for bit, for head sizes up to 128, with 32 keys and values at a time in shared memory as the numbers they stand for: a CTA owns TQ
+// consecutive rows and up to kTileHeads query heads of one key head, a warp NR of those (row, head) pairs. A key is taken apart once for all
+// of them instead of once each, and what the next 32 hold is on its way while these are worked through.
+constexpr int kTileHeads = 4, kTileGroups = 4;
+
+template <typename T, int TQ, int NW, int NR>
+__global__ void __launch_bounds__(NW * 32)
+attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, const uint8_t* __restrict__ k_pages,
+                           const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table, int table_width,
+                           const int32_t* __restrict__ seq_of_token, const int32_t* __restrict__ positions, int tokens, int nq, int nkv, int hd,
+                           int page_size, float scale, int window, float softcap, const float* __restrict__ sinks, const float* __restrict__ slopes,
+                           int* status) {
+    static_assert(NW * NR == TQ * kTileHeads, "a pair of row and head for every place");
+    constexpr int THREADS = NW * 32, KW = (32 * 4 * kTileGroups + THREADS - 1) / THREADS, VW = 2 * KW;       // words and half words a thread at most
+    extern __shared__ __align__(16) float tile[];
+    __shared__ size_t row_at[2][32];                    // where a key's row lies, all ones for none
+    pdl_trigger();
+    pdl_wait();
+    const int G = four::groups_of(hd), width = 32 * G, kld = width + 4, bytes = four::row_bytes(hd);
+    float* const ks = tile;                             // [32][width + 4]
+    float* const vs = ks + 32 * kld;                    // [32][width]
+    float* const qs = vs + 32 * width;                  // [NW * NR][width]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = nq / nkv, parts = (group + kTileHeads - 1) / kTileHeads;
+    const int kvh = blockIdx.y / parts, head0 = kvh * group + (blockIdx.y % parts) * kTileHeads, heads = min(kTileHeads, (kvh + 1) * group - head0);
+    const int t0 = blockIdx.x * TQ, t_end = min(tokens, t0 + TQ);
+    auto row_token = [&](int row) { return t0 + row / kTileHeads; };
+    auto row_head = [&](int row) { return head0 + row % kTileHeads; };
+    auto row_used = [&](int row) { return row_token(row) < t_end && row % kTileHeads < heads; };
+    for (int i = threadIdx.x; i < NW * NR * width; i += THREADS) {
+        const int row = i / width, d = i - row * width;
+        qs[i] = d < hd && row_used(row) ? to_f32(q[static_cast<size_t>(row_token(row)) * q_stride + static_cast<size_t>(row_head(row)) * hd + d]) : 0.f;
+    }
+    for (int a = t0; a < t_end;) {                      // a run of rows of one request
+        const int seq = seq_of_token[a];
+        int b = a + 1, low = positions[a], high = low;
+        while (b < t_end && seq_of_token[b] == seq) {
+            low = min(low, positions[b]);
+            high = max(high, positions[b]);
+            ++b;
+        }
+        if (seq < 0) {                                  // padded tokens of a fixed-size batch
+            for (int row = warp; row < TQ * kTileHeads; row += NW)
+                if (row_used(row) && row_token(row) >= a && row_token(row) < b)
+                    for (int d = lane; d < hd; d += 32) out[(static_cast<size_t>(row_token(row)) * nq + row_head(row)) * hd + d] = from_f32<T>(0.f);
+            a = b;
+            continue;
+        }
+        const int32_t* table = block_table + static_cast<size_t>(seq) * table_width;
+        const int lowest = window > 0 ? max(0, low - window + 1) : 0, begin = lowest / 32 * 32;
+        int pos[NR];
+        float m[NR], l[NR], acc[NR][kTileGroups];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = warp * NR + r;
+            pos[r] = row_used(row) && row_token(row) >= a && row_token(row) < b ? positions[row_token(row)] : -1;      // -1: not of this run
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < kTileGroups; ++j) acc[r][j] = 0.f;
+        }
+        uint32_t kw[KW], kp[KW], vh[VW], vp[VW];
+        auto find = [&](int base, int buf) {            // warp 0: the rows of 32 keys
+            if (warp != 0) return;
+            const int key = base + lane;
+            size_t at = ~size_t(0);
+            if (key >= lowest && key <= high) {
+                const int index = key / page_size, page = index < table_width ? table[index] : -1;
+                if (page < 0 || page >= num_pages)
+                    four::complain(status, four::kCodeNoPage);
+                else
+                    at = ((static_cast<size_t>(page) * nkv + kvh) * page_size + key % page_size) * bytes;
+            }
+            row_at[buf][lane] = at;
+        };
+        auto fetch = [&](int buf) {                     // words of keys: 4 G a row; half words of values: 8 G
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+                const int w = threadIdx.x + i * THREADS, j = w / (4 * G);
+                if (w >= 32 * 4 * G || row_at[buf][j] == ~size_t(0)) continue;
+                const uint32_t* row = reinterpret_cast<const uint32_t*>(k_pages + row_at[buf][j]);
+                kw[i] = row[w % (4 * G)];
+                kp[i] = row[4 * G + w % G];
+            }
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const int w = threadIdx.x + i * THREADS, j = w / (8 * G);
+                if (w >= 32 * 8 * G || row_at[buf][j] == ~size_t(0)) continue;
+                const uint8_t* row = v_pages + row_at[buf][j];
+                vh[i] = reinterpret_cast<const uint16_t*>(row)[w % (8 * G)];
+                vp[i] = reinterpret_cast<const uint32_t*>(row + 16 * G)[w % G];
+            }
+        };
+        auto spread = [&](int buf) {                    // as the numbers they stand for; a key without a row is not looked at
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+                const int w = threadIdx.x + i * THREADS, j = w / (4 * G), in = w % (4 * G);
+                if (w >= 32 * 4 * G || row_at[buf][j] == ~size_t(0)) continue;
+                const float s = four::bf16_low(kp[i]), c = four::bf16_high(kp[i]);
+                float* to = ks + j * kld + 32 * (in % G) + 8 * (in / G);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<float4*>(to + 4 * h) =
+                        make_float4(four::value_of(kw[i] >> (16 * h) & 15u, s, c), four::value_of(kw[i] >> (16 * h + 4) & 15u, s, c),
+                                    four::value_of(kw[i] >> (16 * h + 8) & 15u, s, c), four::value_of(kw[i] >> (16 * h + 12) & 15u, s, c));
+            }
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const int w = threadIdx.x + i * THREADS, j = w / (8 * G), in = w % (8 * G);
+                if (w >= 32 * 8 * G || row_at[buf][j] == ~size_t(0)) continue;
+                const float s = four::bf16_low(vp[i]), c = four::bf16_high(vp[i]);
+                *reinterpret_cast<float4*>(vs + j * width + 32 * (in % G) + 4 * (in / G)) =
+                    make_float4(four::value_of(vh[i] & 15u, s, c), four::value_of(vh[i] >> 4 & 15u, s, c), four::value_of(vh[i] >> 8 & 15u, s, c),
+                                four::value_of(vh[i] >> 12, s, c));
+            }
+        };
+        __syncthreads();                                // the queries are there, the run before has left the tiles
+        find(begin, 0);
+        if (begin + 32 <= high) find(begin + 32, 1);
+        __syncthreads();
+        fetch(0);
+        int buf = 0;
+        for (int base = begin; base <= high; base += 32, buf ^= 1) {
+            spread(buf);
+            __syncthreads();
+            const bool there = row_at[buf][lane] != ~size_t(0);
+            if (base + 32 <= high) fetch(buf ^ 1);
+            const int key = base + lane;
+            const float* k_row = ks + lane * kld;
+            float s[NR];
+            unsigned valid[NR], any = 0;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const int first = window > 0 ? max(0, pos[r] - window + 1) : 0;
+                valid[r] = __ballot_sync(0xffffffffu, there && key >= first && key <= pos[r]);
+                any |= valid[r];
+                s[r] = 0.f;
+            }
+            if (any) {
+                const float* q_row = qs + warp * NR * width;
+                for (int d = 0; d < width; d += 4) {
+                    const float4 kv = *reinterpret_cast<const float4*>(k_row + d);
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        const float4 qv = *reinterpret_cast<const float4*>(q_row + r * width + d);
+                        s[r] = fmaf(qv.x, kv.x, s[r]);
+                        s[r] = fmaf(qv.y, kv.y, s[r]);
+                        s[r] = fmaf(qv.z, kv.z, s[r]);
+                        s[r] = fmaf(qv.w, kv.w, s[r]);
+                    }
+                }
+                float p[NR];
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    p[r] = 0.f;
+                    if (!valid[r]) continue;
+                    const bool ok = (valid[r] >> lane) & 1u;
+                    float z = s[r] * scale;
+                    if (softcap > 0.f) z = softcap * tanhf(z / softcap);
+                    if (slopes) z = __fadd_rn(z, -__fmul_rn(slopes[row_head(warp * NR + r)], static_cast<float>(pos[r] - key)));
+                    z = ok ? z : -INFINITY;
+                    const float m_new = fmaxf(m[r], warp_max(z));
+                    p[r] = ok ? expf(z - m_new) : 0.f;
+                    const float corr = expf(m[r] - m_new);
+                    l[r] = l[r] * corr + warp_sum(p[r]);
+#pragma unroll
+                    for (int j = 0; j < kTileGroups; ++j) acc[r][j] *= corr;
+                    m[r] = m_new;
+                }
+                for (unsigned left = any; left; left &= left - 1) {
+                    const int from = __ffs(left) - 1;
+                    float v[kTileGroups];
+#pragma unroll
+                    for (int j = 0; j < kTileGroups; ++j) v[j] = j < G ? vs[from * width + 32 * j + lane] : 0.f;
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        const float pj = __shfl_sync(0xffffffffu, p[r], from);
+                        if ((valid[r] >> from) & 1u) {
+#pragma unroll
+                            for (int j = 0; j < kTileGroups; ++j) acc[r][j] = fmaf(pj, v[j], acc[r][j]);
+                        }
+                    }
+                }
+            }
+            __syncthreads();                            // the tiles have been read, and the rows of this 32
+            if (base + 64 <= high) find(base + 64, buf);
+            // (the barrier of the next 32 comes before these rows are asked for)
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            if (pos[r] < 0) continue;
+            const int row = warp * NR + r;
+            if (sinks) {
+                const float sink = sinks[row_head(row)], m_new = fmaxf(m[r], sink), corr = expf(m[r] - m_new);
+                l[r] = l[r] * corr + expf(sink - m_new);
+#pragma unroll
+                for (int j = 0; j < kTileGroups; ++j) acc[r][j] *= corr;
+            }
+            const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+            T* out_row = out + (static_cast<size_t>(row_token(row)) * nq + row_head(row)) * hd;
+#pragma unroll
+            for (int j = 0; j < kTileGroups; ++j)
+                if (32 * j + lane < hd) out_row[32 * j + lane] = from_f32<T>(acc[r][j] * inv);
+        }
+        a = b;
+    }
+}
+
 }  // namespace stride
 
 using namespace stride;
@@ -122,10 +329,34 @@ struct Int4Attention {
     cudaStream_t stream;
     int q_stride, num_pages, table_width, tokens, nq, nkv, hd, page_size, window;
     float scale, softcap;
-    int dtype;
+    int dtype, neighbours;          // neighbours: rows next to each other are mostly of one request (only the time depends on it)
+    int unused;
 };
 
-static_assert(sizeof(Int4Attention) == 136, "the record that the caller packs");
+static_assert(sizeof(Int4Attention) == 144, "the record that the caller packs");
+
+template <typename T, int TQ, int NW, int NR>
+static int launch_tiles(const Int4Attention& a) {
+    const auto floats = [](int width) { return 32 * (width + 4) + 32 * width + NW * NR * width; };
+    const cudaError_t e = allow_shared<attention_int4_tile_kernel<T, TQ, NW, NR>>(floats(32 * kTileGroups) * 4);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const int group = a.nq / a.nkv, ctas_y = a.nkv * ((group + kTileHeads - 1) / kTileHeads);
+    if (ctas_y > 65535) return STRIDE_UNSUPPORTED;
+    stride::launch(attention_int4_tile_kernel<T, TQ, NW, NR>, dim3((a.tokens + TQ - 1) / TQ, ctas_y), dim3(NW * 32), floats(32 * four::groups_of(a.hd)) * 4,
+                   a.stream, static_cast<const T*>(a.q), a.q_stride, static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table,
+                   a.table_width, a.seq_of_token, a.positions, a.tokens, a.nq, a.nkv, a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks,
+                   a.slopes, a.status);
+    return STRIDE_LAUNCH_STATUS();
+}
+
+template <typename T>
+static int launch_exact(const Int4Attention& a, int ctas_y) {
+    if (a.hd <= 32 * kTileGroups) return a.neighbours ? launch_tiles<T, 4, 8, 2>(a) : launch_tiles<T, 1, 4, 1>(a);
+    stride::launch(attention_int4_exact_kernel<T>, dim3(a.tokens, ctas_y), dim3(kExactWarps * 32), 0, a.stream, static_cast<const T*>(a.q), a.q_stride,
+                   static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions, a.nq, a.nkv,
+                   a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
+    return STRIDE_LAUNCH_STATUS();
+}
 
 // A key whose page is none of the cache's is left out, and the status word says so.
 extern "C" int stride_attention_int4_exact(const void* record) {
@@ -137,16 +368,6 @@ extern "C" int stride_attention_int4_exact(const void* record) {
     if (a.hd > four::kMaxHeadDim || ctas_y > 65535 || (reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4)
         return STRIDE_UNSUPPORTED;
     if (a.tokens == 0) return 0;
-    const dim3 grid(a.tokens, ctas_y), block(kExactWarps * 32);
-    if (a.dtype == STRIDE_DTYPE_F32)
-        stride::launch(attention_int4_exact_kernel<float>, grid, block, 0, a.stream, static_cast<const float*>(a.q), a.q_stride,
-                       static_cast<float*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions, a.nq,
-                       a.nkv, a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
-    else if (a.dtype == STRIDE_DTYPE_BF16)
-        stride::launch(attention_int4_exact_kernel<__nv_bfloat16>, grid, block, 0, a.stream, static_cast<const __nv_bfloat16*>(a.q), a.q_stride,
-                       static_cast<__nv_bfloat16*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions,
-                       a.nq, a.nkv, a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
-    else
-        return STRIDE_BAD_ARGUMENT;
-    return STRIDE_LAUNCH_STATUS();
+    if (a.dtype == STRIDE_DTYPE_F32) return launch_exact<float>(a, ctas_y);
+    return a.dtype == STRIDE_DTYPE_BF16 ? launch_exact<__nv_bfloat16>(a, ctas_y) : STRIDE_BAD_ARGUMENT;
 }

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kWriteWarps * 32) head_write_kernel(const Head
 
 // The same for head sizes 64, 128 and 256: HD / 8 lanes a head, a lane owns four neighbouring entries of either half, so the pairs that turn
 // together meet in one lane, a group of 32 is eight neighbouring lanes, and loads and stores are 8 (bfloat16) or 16 bytes. HD / 8 lanes take
-// an item: kQueries query heads of a token, or kPairs of its key heads with their values, whose loads are all under way, beside the
+// an item: kQueries query heads of a token, or kPairs of its key heads with their values (two of them were slower), whose loads are all under way, beside the
 // position's and the slot's, before the first is worked on; the angles are read once an item.
 template <typename T>
 struct Four;
@@ -187,10 +187,10 @@ struct Four<__nv_bfloat16> {
     }
 };
 
-constexpr int kItemThreads = 256, kQueries = 4, kPairs = 2;
+constexpr int kItemThreads = 256, kQueries = 4, kPairs = 1;
 
 template <typename T, bool FOUR, int HD>
-__global__ void __launch_bounds__(kItemThreads, 4) head_write_vec_kernel(const HeadWrite a) {
+__global__ void __launch_bounds__(kItemThreads, 5) head_write_vec_kernel(const HeadWrite a) {
     constexpr int L = HD / 8, HALF = HD / 2, G = HD / 32;
     pdl_trigger();
     pdl_wait();

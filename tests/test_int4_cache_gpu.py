@@ -244,6 +244,10 @@ def test_exact_attention(ops, nq, nkv, hd, page, rules, dtype):
                              gpu(slopes))
     want, largest, value = plain.attention(q[:, :nq * hd].view(-1, nq, hd), k, v, pos, seq, hd ** -0.5, window, softcap, sinks, slopes)
     check(out.view(-1, nq, hd), want, score_error(hd, largest + 90), 90, value, dtype)
+    again = torch.full_like(out, 9.0)
+    ops.paged_attention_int4(q.cuda(), nq * hd + 3, again, *pages, table, seq.cuda(), pos.cuda(), nq, nkv, hd, page, hd ** -0.5, window, softcap, gpu(sinks),
+                             gpu(slopes), neighbours=True)
+    assert torch.equal(out, again)                          # rows of several requests side by side: only the time differs
     ops.check_kernel_status()
 
 
