@@ -119,7 +119,8 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
     static_assert(NW * NR == TQ * kTileHeads, "a pair of row and head for every place");
     constexpr int THREADS = NW * 32, KW = (32 * 4 * kTileGroups + THREADS - 1) / THREADS, VW = 2 * KW;       // words and half words a thread at most
     extern __shared__ __align__(16) float tile[];
-    __shared__ size_t row_at[2][32];                    // where a key's row lies, all ones for none
+    __shared__ size_t row_at[2][THREADS];               // where the rows of THREADS keys lie, and of those after them; all ones for none
+    __shared__ float4 weights[NW * NR][8];              // of a pair's 32 keys
     pdl_trigger();
     pdl_wait();
     const int G = four::groups_of(hd), width = 32 * G, kld = width + 4, bytes = four::row_bytes(hd);
@@ -165,9 +166,8 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
             for (int j = 0; j < kTileGroups; ++j) acc[r][j] = 0.f;
         }
         uint32_t kw[KW], kp[KW], vh[VW], vp[VW];
-        auto find = [&](int base, int buf) {            // warp 0: the rows of 32 keys
-            if (warp != 0) return;
-            const int key = base + lane;
+        auto find = [&](int base, int buf) {
+            const int key = base + threadIdx.x;
             size_t at = ~size_t(0);
             if (key >= lowest && key <= high) {
                 const int index = key / page_size, page = index < table_width ? table[index] : -1;
@@ -176,32 +176,34 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
                 else
                     at = ((static_cast<size_t>(page) * nkv + kvh) * page_size + key % page_size) * bytes;
             }
-            row_at[buf][lane] = at;
+            row_at[buf][threadIdx.x] = at;
         };
-        auto fetch = [&](int buf) {                     // words of keys: 4 G a row; half words of values: 8 G
+        auto rows_of = [&](int base) { return row_at[(base - begin) / THREADS & 1] + (base - begin) % THREADS; };
+        auto fetch = [&](const size_t* rows) {          // words of keys: 4 G a row; half words of values: 8 G
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
                 const int w = threadIdx.x + i * THREADS, j = w / (4 * G);
-                if (w >= 32 * 4 * G || row_at[buf][j] == ~size_t(0)) continue;
-                const uint32_t* row = reinterpret_cast<const uint32_t*>(k_pages + row_at[buf][j]);
+                if (w >= 32 * 4 * G || rows[j] == ~size_t(0)) continue;
+                const uint32_t* row = reinterpret_cast<const uint32_t*>(k_pages + rows[j]);
                 kw[i] = row[w % (4 * G)];
                 kp[i] = row[4 * G + w % G];
             }
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
                 const int w = threadIdx.x + i * THREADS, j = w / (8 * G);
-                if (w >= 32 * 8 * G || row_at[buf][j] == ~size_t(0)) continue;
-                const uint8_t* row = v_pages + row_at[buf][j];
+                if (w >= 32 * 8 * G || rows[j] == ~size_t(0)) continue;
+                const uint8_t* row = v_pages + rows[j];
                 vh[i] = reinterpret_cast<const uint16_t*>(row)[w % (8 * G)];
                 vp[i] = reinterpret_cast<const uint32_t*>(row + 16 * G)[w % G];
             }
         };
-        auto spread = [&](int buf) {                    // as the numbers they stand for; a key without a row is not looked at
+        auto spread = [&](const size_t* rows) {         // as the numbers they stand for; zeros for a key without a row
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
                 const int w = threadIdx.x + i * THREADS, j = w / (4 * G), in = w % (4 * G);
-                if (w >= 32 * 4 * G || row_at[buf][j] == ~size_t(0)) continue;
-                const float s = four::bf16_low(kp[i]), c = four::bf16_high(kp[i]);
+                if (w >= 32 * 4 * G) continue;
+                const bool there = rows[j] != ~size_t(0);
+                const float s = there ? four::bf16_low(kp[i]) : 0.f, c = there ? four::bf16_high(kp[i]) : 0.f;
                 float* to = ks + j * kld + 32 * (in % G) + 8 * (in / G);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -212,8 +214,9 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
                 const int w = threadIdx.x + i * THREADS, j = w / (8 * G), in = w % (8 * G);
-                if (w >= 32 * 8 * G || row_at[buf][j] == ~size_t(0)) continue;
-                const float s = four::bf16_low(vp[i]), c = four::bf16_high(vp[i]);
+                if (w >= 32 * 8 * G) continue;
+                const bool there = rows[j] != ~size_t(0);
+                const float s = there ? four::bf16_low(vp[i]) : 0.f, c = there ? four::bf16_high(vp[i]) : 0.f;
                 *reinterpret_cast<float4*>(vs + j * width + 32 * (in % G) + 4 * (in / G)) =
                     make_float4(four::value_of(vh[i] & 15u, s, c), four::value_of(vh[i] >> 4 & 15u, s, c), four::value_of(vh[i] >> 8 & 15u, s, c),
                                 four::value_of(vh[i] >> 12, s, c));
@@ -221,15 +224,16 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
         };
         __syncthreads();                                // the queries are there, the run before has left the tiles
         find(begin, 0);
-        if (begin + 32 <= high) find(begin + 32, 1);
+        if (begin + THREADS <= high) find(begin + THREADS, 1);
         __syncthreads();
-        fetch(0);
-        int buf = 0;
-        for (int base = begin; base <= high; base += 32, buf ^= 1) {
-            spread(buf);
+        fetch(rows_of(begin));
+        for (int base = begin; base <= high; base += 32) {
+            // (the rows before this THREADS keys' have been read by all)
+            if (base != begin && (base - begin) % THREADS == 0 && base + THREADS <= high) find(base + THREADS, ((base - begin) / THREADS + 1) & 1);
+            spread(rows_of(base));
             __syncthreads();
-            const bool there = row_at[buf][lane] != ~size_t(0);
-            if (base + 32 <= high) fetch(buf ^ 1);
+            const bool there = rows_of(base)[lane] != ~size_t(0);
+            if (base + 32 <= high) fetch(rows_of(base + 32));
             const int key = base + lane;
             const float* k_row = ks + lane * kld;
             float s[NR];
@@ -272,24 +276,28 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
                     for (int j = 0; j < kTileGroups; ++j) acc[r][j] *= corr;
                     m[r] = m_new;
                 }
-                for (unsigned left = any; left; left &= left - 1) {
-                    const int from = __ffs(left) - 1;
-                    float v[kTileGroups];
+                // a weight of 0 adds nothing: its key's values are numbers, or zeros
+                __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < kTileGroups; ++j) v[j] = j < G ? vs[from * width + 32 * j + lane] : 0.f;
+                for (int r = 0; r < NR; ++r) reinterpret_cast<float*>(weights[warp * NR + r])[lane] = p[r];
+                __syncwarp();
+                const int last = 31 - __clz(any);
+                for (int j4 = (__ffs(any) - 1) / 4; j4 <= last / 4; ++j4) {
+                    float4 w[NR];
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        const float pj = __shfl_sync(0xffffffffu, p[r], from);
-                        if ((valid[r] >> from) & 1u) {
+                    for (int r = 0; r < NR; ++r) w[r] = weights[warp * NR + r][j4];
 #pragma unroll
-                            for (int j = 0; j < kTileGroups; ++j) acc[r][j] = fmaf(pj, v[j], acc[r][j]);
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int j = 0; j < kTileGroups; ++j)
+                            if (j < G) {
+                                const float v = vs[(4 * j4 + e) * width + 32 * j + lane];
+#pragma unroll
+                                for (int r = 0; r < NR; ++r) acc[r][j] = fmaf((&w[r].x)[e], v, acc[r][j]);
+                            }
                 }
             }
-            __syncthreads();                            // the tiles have been read, and the rows of this 32
-            if (base + 64 <= high) find(base + 64, buf);
-            // (the barrier of the next 32 comes before these rows are asked for)
+            __syncthreads();                            // the tiles have been read
         }
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -351,7 +359,7 @@ static int launch_tiles(const Int4Attention& a) {
 
 template <typename T>
 static int launch_exact(const Int4Attention& a, int ctas_y) {
-    if (a.hd <= 32 * kTileGroups) return a.neighbours ? launch_tiles<T, 4, 8, 2>(a) : launch_tiles<T, 1, 4, 1>(a);
+    if (a.hd <= 32 * kTileGroups) return a.neighbours ? launch_tiles<T, 2, 8, 1>(a) : launch_tiles<T, 1, 4, 1>(a);
     stride::launch(attention_int4_exact_kernel<T>, dim3(a.tokens, ctas_y), dim3(kExactWarps * 32), 0, a.stream, static_cast<const T*>(a.q), a.q_stride,
                    static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions, a.nq, a.nkv,
                    a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
