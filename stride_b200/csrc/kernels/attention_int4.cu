@@ -107,9 +107,9 @@ attention_int4_exact_kernel(const T* __restrict__ q, int q_stride, T* __restrict
 // The same, bit for bit, for head sizes up to 128, with 32 keys and values at a time in shared memory as the numbers they stand for: a CTA owns TQ
 // consecutive rows and up to kTileHeads query heads of one key head, a warp NR of those (row, head) pairs. A key is taken apart once for all
 // of them instead of once each, and what the next 32 hold is on its way while these are worked through.
-constexpr int kTileHeads = 4, kTileGroups = 4;
+constexpr int kTileHeads = 4;
 
-template <typename T, int TQ, int NW, int NR>
+template <typename T, int G, int TQ, int NW, int NR>
 __global__ void __launch_bounds__(NW * 32)
 attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, const uint8_t* __restrict__ k_pages,
                            const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table, int table_width,
@@ -117,13 +117,13 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
                            int page_size, float scale, int window, float softcap, const float* __restrict__ sinks, const float* __restrict__ slopes,
                            int* status) {
     static_assert(NW * NR == TQ * kTileHeads, "a pair of row and head for every place");
-    constexpr int THREADS = NW * 32, KW = (32 * 4 * kTileGroups + THREADS - 1) / THREADS, VW = 2 * KW;       // words and half words a thread at most
+    constexpr int THREADS = NW * 32, KW = (32 * 4 * G + THREADS - 1) / THREADS, VW = (32 * 8 * G + THREADS - 1) / THREADS;       // words, half words a thread
     extern __shared__ __align__(16) float tile[];
     __shared__ size_t row_at[2][THREADS];               // where the rows of THREADS keys lie, and of those after them; all ones for none
     __shared__ float4 weights[NW * NR][8];              // of a pair's 32 keys
-    pdl_trigger();
+    // (no early start for the next kernel: its waiting CTAs would take the places of this one's, which run for long and are few)
     pdl_wait();
-    const int G = four::groups_of(hd), width = 32 * G, kld = width + 4, bytes = four::row_bytes(hd);
+    constexpr int width = 32 * G, kld = width + 4, bytes = 20 * G;
     float* const ks = tile;                             // [32][width + 4]
     float* const vs = ks + 32 * kld;                    // [32][width]
     float* const qs = vs + 32 * width;                  // [NW * NR][width]
@@ -155,7 +155,7 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
         const int32_t* table = block_table + static_cast<size_t>(seq) * table_width;
         const int lowest = window > 0 ? max(0, low - window + 1) : 0, begin = lowest / 32 * 32;
         int pos[NR];
-        float m[NR], l[NR], acc[NR][kTileGroups];
+        float m[NR], l[NR], acc[NR][G];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const int row = warp * NR + r;
@@ -163,7 +163,7 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
             m[r] = -INFINITY;
             l[r] = 0.f;
 #pragma unroll
-            for (int j = 0; j < kTileGroups; ++j) acc[r][j] = 0.f;
+            for (int j = 0; j < G; ++j) acc[r][j] = 0.f;
         }
         uint32_t kw[KW], kp[KW], vh[VW], vp[VW];
         auto find = [&](int base, int buf) {
@@ -247,6 +247,7 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
             }
             if (any) {
                 const float* q_row = qs + warp * NR * width;
+#pragma unroll
                 for (int d = 0; d < width; d += 4) {
                     const float4 kv = *reinterpret_cast<const float4*>(k_row + d);
 #pragma unroll
@@ -273,7 +274,7 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
                     const float corr = expf(m[r] - m_new);
                     l[r] = l[r] * corr + warp_sum(p[r]);
 #pragma unroll
-                    for (int j = 0; j < kTileGroups; ++j) acc[r][j] *= corr;
+                    for (int j = 0; j < G; ++j) acc[r][j] *= corr;
                     m[r] = m_new;
                 }
                 // a weight of 0 adds nothing: its key's values are numbers, or zeros
@@ -289,8 +290,8 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int j = 0; j < kTileGroups; ++j)
-                            if (j < G) {
+                        for (int j = 0; j < G; ++j)
+                            {
                                 const float v = vs[(4 * j4 + e) * width + 32 * j + lane];
 #pragma unroll
                                 for (int r = 0; r < NR; ++r) acc[r][j] = fmaf((&w[r].x)[e], v, acc[r][j]);
@@ -307,12 +308,12 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
                 const float sink = sinks[row_head(row)], m_new = fmaxf(m[r], sink), corr = expf(m[r] - m_new);
                 l[r] = l[r] * corr + expf(sink - m_new);
 #pragma unroll
-                for (int j = 0; j < kTileGroups; ++j) acc[r][j] *= corr;
+                for (int j = 0; j < G; ++j) acc[r][j] *= corr;
             }
             const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
             T* out_row = out + (static_cast<size_t>(row_token(row)) * nq + row_head(row)) * hd;
 #pragma unroll
-            for (int j = 0; j < kTileGroups; ++j)
+            for (int j = 0; j < G; ++j)
                 if (32 * j + lane < hd) out_row[32 * j + lane] = from_f32<T>(acc[r][j] * inv);
         }
         a = b;
@@ -343,23 +344,33 @@ struct Int4Attention {
 
 static_assert(sizeof(Int4Attention) == 144, "the record that the caller packs");
 
-template <typename T, int TQ, int NW, int NR>
+template <typename T, int G, int TQ, int NW, int NR>
 static int launch_tiles(const Int4Attention& a) {
-    const auto floats = [](int width) { return 32 * (width + 4) + 32 * width + NW * NR * width; };
-    const cudaError_t e = allow_shared<attention_int4_tile_kernel<T, TQ, NW, NR>>(floats(32 * kTileGroups) * 4);
+    constexpr int width = 32 * G, bytes = (32 * (width + 4) + 32 * width + NW * NR * width) * 4;
+    const auto kernel = attention_int4_tile_kernel<T, G, TQ, NW, NR>;
+    const cudaError_t e = allow_shared<attention_int4_tile_kernel<T, G, TQ, NW, NR>>(bytes);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int group = a.nq / a.nkv, ctas_y = a.nkv * ((group + kTileHeads - 1) / kTileHeads);
     if (ctas_y > 65535) return STRIDE_UNSUPPORTED;
-    stride::launch(attention_int4_tile_kernel<T, TQ, NW, NR>, dim3((a.tokens + TQ - 1) / TQ, ctas_y), dim3(NW * 32), floats(32 * four::groups_of(a.hd)) * 4,
-                   a.stream, static_cast<const T*>(a.q), a.q_stride, static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table,
-                   a.table_width, a.seq_of_token, a.positions, a.tokens, a.nq, a.nkv, a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks,
-                   a.slopes, a.status);
+    stride::launch(kernel, dim3((a.tokens + TQ - 1) / TQ, ctas_y), dim3(NW * 32), bytes, a.stream, static_cast<const T*>(a.q), a.q_stride,
+                   static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions, a.tokens, a.nq,
+                   a.nkv, a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
     return STRIDE_LAUNCH_STATUS();
+}
+
+template <typename T, int G>
+static int launch_tiles_of(const Int4Attention& a) {
+    return a.neighbours ? launch_tiles<T, G, 2, 8, 1>(a) : launch_tiles<T, G, 1, 4, 1>(a);
 }
 
 template <typename T>
 static int launch_exact(const Int4Attention& a, int ctas_y) {
-    if (a.hd <= 32 * kTileGroups) return a.neighbours ? launch_tiles<T, 2, 8, 1>(a) : launch_tiles<T, 1, 4, 1>(a);
+    switch (four::groups_of(a.hd)) {
+        case 1: return launch_tiles_of<T, 1>(a);
+        case 2: return launch_tiles_of<T, 2>(a);
+        case 3: return launch_tiles_of<T, 3>(a);
+        case 4: return launch_tiles_of<T, 4>(a);
+    }
     stride::launch(attention_int4_exact_kernel<T>, dim3(a.tokens, ctas_y), dim3(kExactWarps * 32), 0, a.stream, static_cast<const T*>(a.q), a.q_stride,
                    static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions, a.nq, a.nkv,
                    a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
