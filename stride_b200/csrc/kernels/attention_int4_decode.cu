@@ -149,7 +149,7 @@ __device__ __forceinline__ float log2_size(const uint32_t (&p)[G]) {
 // G: groups of a head (head size 32 G). NT: tiles of 8 query heads.
 template <int G, int NT, bool BULK>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(const Decode a) {
-    constexpr int HD = 32 * G, ROW = 20 * G, HALF = kSub * ROW, STAGE = 4 * HALF;      // a stage: keys and values of either half
+    constexpr int HD = 32 * G, ROW = 20 * G, HALF = kSub * ROW, STAGE = 4 * HALF;      // a stage: the keys of either half, then their values
     pdl_trigger();
     pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];
@@ -271,10 +271,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             held = (held & ~(3u << (2 * stage))) | halves << (2 * stage);
             // (the barrier's one arrival, with the count of bytes, keeps the phase open whichever copy lands first)
             if ((lane >> 1) == j % kWindow && my_row != ~size_t(0)) {
-                const uint32_t dst = tc::smem_u32(ring + stage * STAGE + (lane & 1) * 2 * HALF), bar = tc::smem_u32(&bars[warp][stage]);
+                const uint32_t dst = tc::smem_u32(ring + stage * STAGE + (lane & 1) * HALF), bar = tc::smem_u32(&bars[warp][stage]);
                 if ((lane & 1) == (halves == 2u)) tc::mbar_expect_tx(bar, halves == 3u ? 4 * HALF : 2 * HALF);
-                bulk_copy(dst, a.k_pages + my_row, HALF, bar);
-                bulk_copy(dst + HALF, a.v_pages + my_row, HALF, bar);
+                if (halves == 3u && a.page_size % kTile == 0) {
+                    if ((lane & 1) == 0) {
+                        bulk_copy(dst, a.k_pages + my_row, 2 * HALF, bar);
+                        bulk_copy(dst + 2 * HALF, a.v_pages + my_row, 2 * HALF, bar);
+                    }
+                } else {
+                    bulk_copy(dst, a.k_pages + my_row, HALF, bar);
+                    bulk_copy(dst + 2 * HALF, a.v_pages + my_row, HALF, bar);
+                }
             }
             return;
         }
@@ -288,14 +295,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             unsigned char* to = ring + stage * STAGE;
 #pragma unroll
             for (int i = 0; i < 5; ++i) {               // 32 rows of 5 pieces
-                const int piece = i * 32 + lane, r = piece / 5, at = (r >> 4) * 2 * HALF + (r & 15) * ROW + (piece - r * 5) * 4 * G;
+                const int piece = i * 32 + lane, r = piece / 5, at = r * ROW + (piece - r * 5) * 4 * G;
                 const size_t from = __shfl_sync(0xffffffffu, row, r);
                 if (from != ~size_t(0)) {
                     small_copy<4 * G>(tc::smem_u32(to + at), a.k_pages + from + (piece - r * 5) * 4 * G);
-                    small_copy<4 * G>(tc::smem_u32(to + HALF + at), a.v_pages + from + (piece - r * 5) * 4 * G);
+                    small_copy<4 * G>(tc::smem_u32(to + 2 * HALF + at), a.v_pages + from + (piece - r * 5) * 4 * G);
                 } else {
                     for (int b = 0; b < 4 * G; b += 4)
-                        *reinterpret_cast<uint32_t*>(to + at + b) = *reinterpret_cast<uint32_t*>(to + HALF + at + b) = 0u;
+                        *reinterpret_cast<uint32_t*>(to + at + b) = *reinterpret_cast<uint32_t*>(to + 2 * HALF + at + b) = 0u;
                 }
             }
         }
@@ -403,7 +410,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             float x[NT][2][4], P[NT][2][4], amp[2][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const unsigned char* ks = at + h * 2 * HALF;
+                const unsigned char* ks = at + h * HALF;
                 uint32_t kw[2][G], kp[2][G];
                 load_words<G>(kw[0], ks + row_a * ROW + c * 4 * G);
                 load_words<G>(kw[1], ks + row_b * ROW + c * 4 * G);
@@ -431,8 +438,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                     }
                 }
                 uint32_t vp[2][G];
-                load_words<G>(vp[0], ks + HALF + row_a * ROW + 16 * G);
-                load_words<G>(vp[1], ks + HALF + row_b * ROW + 16 * G);
+                load_words<G>(vp[0], ks + 2 * HALF + row_a * ROW + 16 * G);
+                load_words<G>(vp[1], ks + 2 * HALF + row_b * ROW + 16 * G);
                 amp[h][0] = largest_scale<G>(vp[0]);
                 amp[h][1] = largest_scale<G>(vp[1]);
             }
@@ -492,8 +499,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t vp[2][G];
-                        load_words<G>(vp[0], at + h * 2 * HALF + HALF + row_a * ROW + 16 * G);
-                        load_words<G>(vp[1], at + h * 2 * HALF + HALF + row_b * ROW + 16 * G);
+                        load_words<G>(vp[0], at + (2 + h) * HALF + row_a * ROW + 16 * G);
+                        load_words<G>(vp[1], at + (2 + h) * HALF + row_b * ROW + 16 * G);
                         size[h][0] = log2_size<G>(vp[0]);
                         size[h][1] = log2_size<G>(vp[1]);
                     }
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const unsigned char* vs = at + h * 2 * HALF + HALF;
+                const unsigned char* vs = at + (2 + h) * HALF;
                 uint32_t vp[2][G], vw[4][G / 2], vc[4];
                 load_words<G>(vp[0], vs + row_a * ROW + 16 * G);
                 load_words<G>(vp[1], vs + row_b * ROW + 16 * G);
@@ -652,16 +659,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
     if (parts > 1) {
         // ---- the CTA that finishes last for this (token, key head) merges the parts
         __shared__ int is_last;
-        __threadfence();
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0) {             // (the barriers order the CTA's stores before this thread's fence, and its loads behind it)
+            __threadfence();
             int* ticket = a.tickets + static_cast<size_t>(t) * a.nkv + kvh;
             is_last = atomicAdd(ticket, 1) == parts - 1;
             if (is_last) *ticket = 0;       // ready for the next launch; nobody else touches it before then
+            __threadfence();
         }
         __syncthreads();
         if (is_last) {
-            __threadfence();
             for (int idx = threadIdx.x; idx < group * (HD / 4); idx += blockDim.x) {
                 const int row = idx / (HD / 4), d = (idx - row * (HD / 4)) * 4;
                 float most = -INFINITY;
