@@ -12,9 +12,9 @@
 // * Keys are the A operand (16 tokens by 16 entries), the 8 columns of B are the group's query heads; the products of a group of 32 entries end in
 //   an accumulator of their own, which the token's scale multiplies. Values are the A operand of the second product (16 entries by 16 tokens),
 //   the weights P_t s_tg its B operand: a transpose of 8 x 8 in the warp.
-// * Scales and centres themselves go through products in bfloat16, which they are exact in: with the sums of the query (in two parts, 16 bits) on
-//   the side of the keys, with P on the side of the values. P is rounded to bfloat16 once, P s to 16 bits from that, so what the offset of 8
-//   adds in one product the other takes off to 2^-12.
+// * Scales and centres themselves go through products in bfloat16, which they are exact in: with the sums of the query on the side of the keys,
+//   with P on the side of the values, both in two parts, 16 bits. P s is rounded to 16 bits (2^-11 at most), so what the offset of 8 adds in
+//   one product the other takes off but for that. The sum of the weights comes from the same product, from rows of ones.
 // * The query is scaled by a power of two to below 2^15. The reference R of a weight 2^(score - R) is the running maximum of score + log2 of the
 //   token's largest scale or centre, so that what is rounded to 16 bits lies below 2^8 and its largest near 1 whatever the values' size; R moves
 //   only when a product passes 2^8 (a vote per tile), and then everything is rescaled.
@@ -379,11 +379,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             slope[nt][e] = a.slopes != nullptr && 8 * nt + 2 * c + e < group ? a.slopes[kvh * group + 8 * nt + 2 * c + e] * 1.4426950408889634f : 0.f;
     }
 
-    float R[NT][2], l[NT][2], o[NT][G][2][4], cen[NT][4];       // cen: rows 0 .. G - 1 for the centres, from 4 on for the scales
+    // cen: rows 0 .. G - 1 for the centres, from 4 on for the scales, 8 .. 15 (all alike) for the sum of the weights
+    float R[NT][2], o[NT][G][2][4], cen[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         R[nt][0] = R[nt][1] = -INFINITY;
-        l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             cen[nt][e] = 0.f;
@@ -443,7 +443,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                 amp[h][0] = largest_scale<G>(vp[0]);
                 amp[h][1] = largest_scale<G>(vp[1]);
             }
-            // x becomes the score in units of log2
+            // where something bends the score, x becomes the score in units of log2 here; else it stays as it is, `unit` of them
+            float unit[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) unit[nt][e] = bent ? 1.f : factor[nt][e];
             if (bent) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -455,13 +460,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                             if (a.cap_log2e > 0.f) y = a.cap_log2e * tanh_quick(y);
                             x[nt][h][e] = fmaf(slope[nt][e & 1], static_cast<float>(base + h * kSub + (e < 2 ? row_a : row_b) - pos), y);
                         }
-            } else {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[nt][h][e] *= factor[nt][e & 1];
             }
             uint32_t seen = 0xfu;           // of the score rows: half 0 row_a, row_b, half 1 row_a, row_b
             if (edge) {
@@ -486,7 +484,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) P[nt][h][e] = exp2_quick(x[nt][h][e] - R[nt][e & 1]);
+                    for (int e = 0; e < 4; ++e) P[nt][h][e] = exp2_quick(fmaf(x[nt][h][e], unit[nt][e & 1], -R[nt][e & 1]));
                     most_of[h][0] = fmaxf(P[nt][h][0], P[nt][h][1]);
                     most_of[h][1] = fmaxf(P[nt][h][2], P[nt][h][3]);
                 }
@@ -511,13 +509,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
                             for (int r = 0; r < 2; ++r)
-                                most = x[nt][h][2 * r + e] == -INFINITY ? most : fmaxf(most, x[nt][h][2 * r + e] + size[h][r]);
+                                most = x[nt][h][2 * r + e] == -INFINITY ? most : fmaxf(most, fmaf(x[nt][h][2 * r + e], unit[nt][e], size[h][r]));
 #pragma unroll
                         for (int s = 4; s < 32; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
                         const float next = fmaxf(R[nt][e], most), by = R[nt][e] == -INFINITY ? 0.f : exp2_quick(R[nt][e] - next);
                         R[nt][e] = next;
-                        l[nt][e] *= by;
                         cen[nt][e] *= by;
+                        cen[nt][e + 2] *= by;
 #pragma unroll
                         for (int grp = 0; grp < G; ++grp)
 #pragma unroll
@@ -529,7 +527,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int r = 0; r < 2; ++r) P[nt][h][2 * r + e] = exp2_quick(x[nt][h][2 * r + e] - (next == -INFINITY ? 0.f : next));
+                            for (int r = 0; r < 2; ++r) P[nt][h][2 * r + e] = exp2_quick(fmaf(x[nt][h][2 * r + e], unit[nt][e], next == -INFINITY ? 0.f : -next));
                     }
                 }
             }
@@ -565,15 +563,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                 const uint32_t a0 = __byte_perm(vc[0], vc[1], pick), a2 = __byte_perm(vc[2], vc[3], pick);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const uint32_t pa = pack_bf16(P[nt][h][0], P[nt][h][1]), pb = pack_bf16(P[nt][h][2], P[nt][h][3]);
-                    P[nt][h][0] = bf16_low(pa);
-                    P[nt][h][1] = bf16_high(pa);
-                    P[nt][h][2] = bf16_low(pb);
-                    P[nt][h][3] = bf16_high(pb);
-                    l[nt][0] += P[nt][h][0] + P[nt][h][2];
-                    l[nt][1] += P[nt][h][1] + P[nt][h][3];
-                    const uint32_t b[2] = {transposed(pa), transposed(pb)};
-                    mma_bf16(cen[nt], a0, 0u, a2, 0u, b, cen[nt][0], cen[nt][1], cen[nt][2], cen[nt][3]);
+                    float rest[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) rest[e] = P[nt][h][e] - bf16_high(__float_as_uint(P[nt][h][e]));
+                    const uint32_t high[2] = {transposed(__byte_perm(__float_as_uint(P[nt][h][0]), __float_as_uint(P[nt][h][1]), 0x7632)),
+                                              transposed(__byte_perm(__float_as_uint(P[nt][h][2]), __float_as_uint(P[nt][h][3]), 0x7632))};
+                    const uint32_t low[2] = {transposed(pack_bf16(rest[0], rest[1])), transposed(pack_bf16(rest[2], rest[3]))};
+                    float(&d)[4] = cen[nt];
+                    mma_bf16(d, a0, 0x3f803f80u, a2, 0x3f803f80u, high, d[0], d[1], d[2], d[3]);
+                    mma_bf16(d, a0, 0x3f803f80u, a2, 0x3f803f80u, low, d[0], d[1], d[2], d[3]);
                 }
 #pragma unroll
                 for (int grp = 0; grp < G; ++grp) {
@@ -607,9 +605,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int head = 8 * nt + 2 * c + e;
-            float sum = l[nt][e];
-#pragma unroll
-            for (int s = 4; s < 32; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
             float* dst = red + (warp * group + head) * RS;
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
@@ -624,7 +619,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             }
             if (head < group && g == 0) {
                 dst[HD] = R[nt][e];
-                dst[HD + 1] = sum;
+                dst[HD + 1] = cen[nt][e + 2];
             }
         }
     __syncthreads();
