@@ -40,10 +40,110 @@
 // head 0 (warp 7 fetches Q first), warps 8-15 do the softmax and the final store, four per head.
 // CTAs are dispatched longest first (the grid's fast dimension is the head, the slow one the query tile,
 // last tile first). Every mbarrier wait is bounded; a wait that runs out sets *status.
+#include "int4_cache.cuh"
 #include "tcgen05.cuh"
 #include "mma.cuh"
 
 namespace stride {
+
+// The keys of the first num_seqs requests of a cache held in 4 bits (int4_cache.cuh) as pages of 64 in 16-bit floating point, for the attention of
+// portions: a request's pages one after the other, the requests' too, and the table that says so. A key is expanded once for all query tiles
+// that read it, which costs little beside them: 8192 keys of 8 heads of 128 take as long as 2 % of 2,048 queries' attention to them, and what it
+// writes is read back from L2. The format has 11 bits where bfloat16 has 8, which an entry's place between two of its sixteen numbers
+// needs; an entry beyond its range, 65504, counts as that. CTA (page, key head).
+__device__ __forceinline__ uint32_t pack_half_in_range(float lo, float hi) {
+    uint32_t y;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {        // (a NaN stays one)
+    return pack_half_in_range(fabsf(lo) > 65504.f ? copysignf(65504.f, lo) : lo, fabsf(hi) > 65504.f ? copysignf(65504.f, hi) : hi);
+}
+constexpr int kExpandKeys = 64, kExpandThreads = 256;
+
+template <int G>
+__global__ void __launch_bounds__(kExpandThreads)
+int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table,
+                   int table_width, const int32_t* __restrict__ q_len, const int32_t* __restrict__ ctx_len, int num_seqs, int nkv, int page_size,
+                   int window, uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int32_t* __restrict__ table_out, int out_pages,
+                   int* status) {
+    pdl_trigger();
+    constexpr int HD = 32 * G, BYTES = 20 * G;
+    __shared__ size_t row_at[kExpandKeys];
+    pdl_wait();
+    int seq = -1, index = 0, at = 0;                        // this page is number `index` of request `seq`
+    for (int s = 0; s < num_seqs; ++s) {
+        const int pages = (ctx_len[s] + kExpandKeys - 1) / kExpandKeys;
+        if (static_cast<int>(blockIdx.x) < at + pages) {
+            seq = s;
+            index = blockIdx.x - at;
+            break;
+        }
+        at += pages;
+    }
+    if (seq < 0) return;
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && threadIdx.x == 0) {      // the last page there is room for
+        bool more = (index + 1) * kExpandKeys < ctx_len[seq];
+        for (int s = seq + 1; s < num_seqs; ++s) more = more || ctx_len[s] > 0;
+        if (more) four::complain(status, four::kCodeTooManyKeys);
+    }
+    const int ctx = ctx_len[seq], kvh = blockIdx.y, key0 = index * kExpandKeys;
+    const int first = window > 0 ? max(0, ctx - q_len[seq] - window + 1) : 0;
+    if (kvh == 0 && threadIdx.x == 0) table_out[static_cast<size_t>(seq) * out_pages + index] = blockIdx.x;
+    if (key0 + kExpandKeys <= first) return;                // behind every window
+    if (threadIdx.x < kExpandKeys) {
+        const int key = key0 + threadIdx.x;
+        size_t row = ~size_t(0);
+        if (key >= first && key < ctx) {
+            const int page = key / page_size < table_width ? block_table[static_cast<size_t>(seq) * table_width + key / page_size] : -1;
+            if (page < 0 || page >= num_pages)
+                four::complain(status, four::kCodeNoPage);
+            else
+                row = ((static_cast<size_t>(page) * nkv + kvh) * page_size + key % page_size) * BYTES;
+        }
+        row_at[threadIdx.x] = row;
+    }
+    __syncthreads();
+    const size_t out_row = (static_cast<size_t>(blockIdx.x) * nkv + kvh) * kExpandKeys;
+    // a key without a page (before the windows, behind the end) becomes zeros: attention masks it
+    for (int i = threadIdx.x; i < kExpandKeys * 4; i += kExpandThreads) {           // keys: part a of a row, 8 entries of every group
+        const int r = i >> 2, a = i & 3;
+        const bool there = row_at[r] != ~size_t(0);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pages + (there ? row_at[r] : 0));
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint4 out = make_uint4(0, 0, 0, 0);
+            if (there) {
+                const uint32_t w = words[a * G + g], p = words[4 * G + g];
+                const float s = four::bf16_low(p), c = four::bf16_high(p);
+                uint32_t pair[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    pair[e] = pack_half(four::value_of(w >> (8 * e) & 15u, s, c), four::value_of(w >> (8 * e + 4) & 15u, s, c));
+                }
+                out = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+            }
+            *reinterpret_cast<uint4*>(k_out + (out_row + r) * HD + 32 * g + 8 * a) = out;
+        }
+    }
+    for (int i = threadIdx.x; i < kExpandKeys * 8; i += kExpandThreads) {           // values: part a of a row, 4 entries of every group
+        const int r = i >> 3, a = i & 7;
+        const bool there = row_at[r] != ~size_t(0);
+        const uint8_t* row = v_pages + (there ? row_at[r] : 0);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint2 out = make_uint2(0, 0);
+            if (there) {
+                const uint32_t w = reinterpret_cast<const uint16_t*>(row)[a * G + g], p = reinterpret_cast<const uint32_t*>(row + 16 * G)[g];
+                const float s = four::bf16_low(p), c = four::bf16_high(p);
+                out = make_uint2(pack_half(four::value_of(w & 15u, s, c), four::value_of(w >> 4 & 15u, s, c)),
+                                 pack_half(four::value_of(w >> 8 & 15u, s, c), four::value_of(w >> 12, s, c)));
+            }
+            *reinterpret_cast<uint2*>(v_out + (out_row + r) * HD + 32 * g + 4 * a) = out;
+        }
+    }
+}
+
 namespace tc {
 
 constexpr int kQRows = 128;
@@ -67,12 +167,15 @@ constexpr long long kStaggerCycles = 1000;
 // for two CTAs per SM, and the scores run two tiles ahead, which hides the one stage. An optional gate (LatentGate) multiplies the
 // result. 2,048 tokens of 16 heads: 42 us, beside 20 us for the product that expands (moe_tc.cu) and 4 us for the
 // gather; on the latents themselves (latent_attention_tc.cu and two products a head) 745 + 24 + 19 us.
+// F16: keys and values are 16-bit floating point of 11 bits, as the expanded form of a cache held in 4 bits has them (at the end of this file).
+// Both operands of a product are of one type, so the softmax warps turn the query tiles, bfloat16 in the projection's output, in place
+// (a query beyond 65504 counts as that, one below 2^-14 loses bits that a score does not show) and write P so.
 struct LatentGate {
     const __nv_bfloat16* values;        // null: none
     int ld, per_output;                 // row stride; one number an output (else one a head)
     int head_stride, v_off;             // of an expanded row: head h's key at column h * head_stride, its value v_off behind it
 };
-template <int HD, int HEADS, bool TMA_KV, bool REL, bool LATENT = false>
+template <int HD, int HEADS, bool TMA_KV, bool REL, bool LATENT = false, bool F16 = false>
 __global__ void __launch_bounds__(HEADS == 1 ? 256 : 512, HEADS == 1 ? 2 : 1)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const __nv_bfloat16* __restrict__ k_pages,
@@ -103,7 +206,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     unsigned char* q_s = smem;                            // HEADS query tiles
     unsigned char* k_s = q_s + HEADS * Q_BYTES;           // KS key tiles, then KSV value tiles
     unsigned char* v_s = k_s + KS * K_BYTES;
-    __shared__ __align__(8) uint64_t q_full;
+    __shared__ __align__(8) uint64_t q_full, q_turned;           // q_turned: F16 alone
     __shared__ __align__(8) uint64_t s_full[HEADS][2], p_full[HEADS][2], s_free[HEADS][2], k_full[KS], k_empty[KS], v_full[KSV], v_empty[KSV];
     __shared__ uint32_t tmem_base_slot;
 
@@ -141,6 +244,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&q_full), 1);
+        if (F16) mbar_init(smem_u32(&q_turned), 4 * HEADS);
         for (int h = 0; h < HEADS; ++h) {
             for (int s = 0; s < 2; ++s) {
                 mbar_init(smem_u32(&s_full[h][s]), 1);
@@ -286,7 +390,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
         __syncwarp();
         const bool issuer = elect_one();
-        constexpr uint32_t idesc_pv = instr_desc_bf16(kQRows, HD, true);
+        constexpr uint32_t idesc_pv = instr_desc_16(kQRows, HD, true, F16);
         const uint32_t tmem_h = tmem_base + h * HEAD_COLS;
         bool ok = true;
         for (int j = 0; j < n_tiles && ok; ++j) {
@@ -312,9 +416,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         // into the buffer that held P of tile j as soon as the output product of tile j has read it.
         const int h = MMA_WARP - warp;
         const bool issuer = elect_one();
-        constexpr uint32_t idesc_qk = instr_desc_bf16(kQRows, kKeys, false);
+        constexpr uint32_t idesc_qk = instr_desc_16(kQRows, kKeys, false, F16);
         const uint32_t q_addr = smem_u32(q_s + h * Q_BYTES);
-        bool ok = mbar_wait(smem_u32(&q_full), 0, status, 12);
+        bool ok = mbar_wait(smem_u32(F16 ? &q_turned : &q_full), 0, status, 12);
         for (int j = 0; j < n_tiles && ok; ++j) {
             const int st = j % KS;
             if (j >= 2) ok = mbar_wait(smem_u32(&s_free[h][j & 1]), static_cast<uint32_t>((j - 2) >> 1) & 1u, status, 22);
@@ -361,7 +465,24 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             return mbar_wait(smem_u32(&s_free[hh][x & 1]), static_cast<uint32_t>(x >> 1) & 1u, status, code);
         };
         uint32_t sr[64];                                     // the scores of the row, requested one tile ahead
-        bool ok = mbar_wait(smem_u32(&s_full[hh][0]), 0, status, 15);
+        bool ok = true;
+        if constexpr (F16) {
+            ok = mbar_wait(smem_u32(&q_full), 0, status, 23);
+            if (ok) {
+                for (int i = threadIdx.x - SERVICE_WARPS * 32; i < HEADS * Q_BYTES / 16; i += 128 * HEADS) {
+                    uint4* at = reinterpret_cast<uint4*>(q_s) + i;
+                    uint4 w = *at;
+                    uint32_t* p = &w.x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = pack_half(four::bf16_low(p[e]), four::bf16_high(p[e]));
+                    *at = w;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&q_turned));
+            }
+        }
+        ok = ok && mbar_wait(smem_u32(&s_full[hh][0]), 0, status, 15);
         tc_fence_after();
         if (ok) tmem_ld64_issue(tmem_s + lane_base, sr);
         if (hh == 1) {
@@ -447,7 +568,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     const float p0 = ex2_approx(fmaf(sv[i], scale_log2e, neg_m));
                     const float p1 = ex2_approx(fmaf(sv[i + 1], scale_log2e, neg_m));
                     l4[(i / 2) & 3] += p0 + p1;
-                    packed[i / 2] = __uint_as_float(pack_bf16(p0, p1));
+                    packed[i / 2] = __uint_as_float(F16 ? pack_half_in_range(p0, p1) : pack_bf16(p0, p1))       /* at most 2^8 */;
                 }
                 tmem_st32(tmem_sj, packed);   // over S columns 0-31, all of which have been read
                 l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
@@ -528,7 +649,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     if (warp == MMA_WARP) tmem_dealloc(tmem_base_slot, TMEM_COLS);
 }
 
-template <int HD, int HEADS>
+template <int HD, int HEADS, bool F16 = false>
 int launch_attn(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const __nv_bfloat16* k_pages, const __nv_bfloat16* v_pages, __nv_bfloat16* out,
                 const int32_t* block_table, int table_width, const int32_t* q_start, const int32_t* q_len, const int32_t* ctx_len,
                 int num_seqs, int max_tiles, int nq, int nkv, int page_shift, float scale, int window, float softcap,
@@ -538,6 +659,15 @@ int launch_attn(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtens
     static bool configured[64] = {};        // the shared-memory limit is set per kernel and device
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return STRIDE_BAD_ARGUMENT;
+    if constexpr (F16) {
+        const cudaError_t e = allow_shared<attn_prefill_tc_kernel<HD, HEADS, true, false, false, true>>(smem);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        stride::launch(attn_prefill_tc_kernel<HD, HEADS, true, false, false, true>, dim3(nq / HEADS, max_tiles), dim3(HEADS == 1 ? 256 : 512), smem, stream,
+                       *map_q, *map_k, *map_v, k_pages, v_pages, out, block_table, table_width, q_start, q_len, ctx_len, num_seqs, nq, nkv, page_shift,
+                       (softcap != 0.f ? fabsf(softcap) : scale) * 1.4426950408889634f, window, softcap != 0.f ? scale / softcap : 0.f, sinks, slopes,
+                       nullptr, 0, status, *map_q, *map_q, LatentGate{}, 0);
+        return STRIDE_LAUNCH_STATUS();
+    }
     if (!configured[device]) {
         const void* kernels[4] = {reinterpret_cast<const void*>(attn_prefill_tc_kernel<HD, HEADS, true, false>),
                                   reinterpret_cast<const void*>(attn_prefill_tc_kernel<HD, HEADS, false, false>),
@@ -683,4 +813,67 @@ extern "C" int stride_latent_prefill_tc(const void* q, int q_ld, const void* q_r
                    nullptr, 0, q_start, q_len, ctx_len, num_seqs, heads, heads, 0, scale * 1.4426950408889634f, 0, 0.f, sinks, nullptr, nullptr, 0,
                    status, *map_q2, *map_k2, tc::LatentGate{static_cast<const __nv_bfloat16*>(gate), gate_ld, gate_per_output, kv_head_stride, kv_v_off}, q_rot_stride);
     return STRIDE_LAUNCH_STATUS();
+}
+
+namespace stride {
+
+struct Int4Prefill {                // a record that the caller packs
+    const void* q;                  // [tokens, q_stride] bfloat16, head h at columns h hd
+    void* out;                      // [tokens, nq hd]
+    const uint8_t* k_pages;         // [num_pages, nkv, page_size, 20 hd / 32]
+    const uint8_t* v_pages;
+    const int32_t* block_table;     // [num_seqs at least, table_width]
+    const int32_t* q_start;
+    const int32_t* q_len;
+    const int32_t* ctx_len;
+    uint16_t* k_wide;               // [wide_pages, nkv, 64, hd]
+    uint16_t* v_wide;
+    int32_t* table_wide;            // [num_seqs, wide_pages]
+    const float* sinks;
+    const float* slopes;
+    int* status;
+    cudaStream_t stream;
+    int q_stride, num_pages, table_width, wide_pages, num_seqs, tokens, nq, nkv, hd, page_size, window;
+    float scale, softcap;
+    int unused;
+};
+static_assert(sizeof(Int4Prefill) == 176, "the record that the caller packs");
+
+}  // namespace stride
+
+// Attention over a cache held in 4 bits for the first `num_seqs` requests of the step, which own the first `tokens` rows of the flat batch: the keys
+// and values that they see are expanded to pages of 64, and attended to from there. wide_pages: at least the sum over the requests of
+// ceil(ctx_len / 64) (else code 36 in the status word). softcap as for stride_paged_prefill_attention_tc. Returns -2 for head sizes other than
+// 64 and 128 and for unaligned rows.
+extern "C" int stride_int4_prefill(const void* record) {
+    const Int4Prefill a = read_record<Int4Prefill>(record);
+    if (a.tokens < 0 || a.num_seqs < 0 || a.nq <= 0 || a.nkv <= 0 || a.page_size <= 0 || a.num_pages <= 0 || a.table_width <= 0 || a.window < 0 ||
+        a.wide_pages <= 0 || a.nq % a.nkv || a.status == nullptr)
+        return STRIDE_BAD_ARGUMENT;
+    if ((a.hd != 64 && a.hd != 128) || a.nkv > 65535 || a.nq > 65535 || a.q_stride % 8) return STRIDE_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4 ||
+        (reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.k_wide) | reinterpret_cast<uintptr_t>(a.v_wide)) % 16)
+        return STRIDE_UNSUPPORTED;
+    if (a.tokens == 0 || a.num_seqs == 0) return 0;
+    const int max_tiles = (a.tokens + tc::kQRows - 1) / tc::kQRows + a.num_seqs;
+    if (max_tiles > 65535) return STRIDE_UNSUPPORTED;
+    const CUtensorMap* map_q = tc::cached_map(a.q, a.tokens, a.q_stride, a.q_stride, tc::kQRows);
+    const long long wide_rows = static_cast<long long>(a.wide_pages) * a.nkv * kExpandKeys;
+    const CUtensorMap* map_k = tc::cached_map(a.k_wide, wide_rows, a.hd, a.hd, tc::kKeys);
+    const CUtensorMap* map_v = tc::cached_map(a.v_wide, wide_rows, a.hd, a.hd, tc::kKeys);
+    if (!map_q || !map_k || !map_v) return STRIDE_UNSUPPORTED;
+    stride::launch(a.hd == 64 ? int4_expand_kernel<2> : int4_expand_kernel<4>, dim3(a.wide_pages, a.nkv), dim3(kExpandThreads), 0, a.stream, a.k_pages,
+                   a.v_pages, a.num_pages, a.block_table, a.table_width, a.q_len, a.ctx_len, a.num_seqs, a.nkv, a.page_size, a.window, a.k_wide, a.v_wide,
+                   a.table_wide, a.wide_pages, a.status);
+    const int code = STRIDE_LAUNCH_STATUS();
+    if (code) return code;
+    const bool pair = (a.nq / a.nkv) % 2 == 0 && pair_heads();
+    static_assert(kExpandKeys == tc::kKeys && kExpandKeys == 1 << 6, "a page is a key tile");
+#define STRIDE_INT4_LAUNCH(HD_, HEADS_)                                                                                                                 \
+    tc::launch_attn<HD_, HEADS_, true>(map_q, map_k, map_v, nullptr, nullptr, static_cast<__nv_bfloat16*>(a.out), a.table_wide, a.wide_pages, a.q_start, \
+                                       a.q_len, a.ctx_len, a.num_seqs, max_tiles, a.nq, a.nkv, 6, a.scale, a.window, a.softcap, a.sinks, a.slopes, nullptr, 0, \
+                                       a.status, a.stream)
+    if (a.hd == 64) return pair ? STRIDE_INT4_LAUNCH(64, 2) : STRIDE_INT4_LAUNCH(64, 1);
+    return pair ? STRIDE_INT4_LAUNCH(128, 2) : STRIDE_INT4_LAUNCH(128, 1);
+#undef STRIDE_INT4_LAUNCH
 }

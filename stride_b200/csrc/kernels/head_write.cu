@@ -460,95 +460,6 @@ int4_read_vec_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restr
     Four<T>::put(v_out + unit * HD + HALF + 4 * i, y[3]);
 }
 
-// The keys of the first num_seqs requests as pages of 64 in bfloat16, for the attention of portions: a request's pages one after the other,
-// the requests' too, and the table that says so. A key is expanded once for all query tiles that read it. CTA (page, key head).
-constexpr int kExpandKeys = 64, kExpandThreads = 256;
-
-template <int G>
-__global__ void __launch_bounds__(kExpandThreads)
-int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table,
-                   int table_width, const int32_t* __restrict__ q_len, const int32_t* __restrict__ ctx_len, int num_seqs, int nkv, int page_size,
-                   int window, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int32_t* __restrict__ table_out, int out_pages,
-                   int* status) {
-    pdl_trigger();
-    constexpr int HD = 32 * G, BYTES = 20 * G;
-    __shared__ size_t row_at[kExpandKeys];
-    pdl_wait();
-    int seq = -1, index = 0, at = 0;                        // this page is number `index` of request `seq`
-    for (int s = 0; s < num_seqs; ++s) {
-        const int pages = (ctx_len[s] + kExpandKeys - 1) / kExpandKeys;
-        if (static_cast<int>(blockIdx.x) < at + pages) {
-            seq = s;
-            index = blockIdx.x - at;
-            break;
-        }
-        at += pages;
-    }
-    if (seq < 0) return;
-    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && threadIdx.x == 0) {      // the last page there is room for
-        bool more = (index + 1) * kExpandKeys < ctx_len[seq];
-        for (int s = seq + 1; s < num_seqs; ++s) more = more || ctx_len[s] > 0;
-        if (more) four::complain(status, four::kCodeTooManyKeys);
-    }
-    const int ctx = ctx_len[seq], kvh = blockIdx.y, key0 = index * kExpandKeys;
-    const int first = window > 0 ? max(0, ctx - q_len[seq] - window + 1) : 0;
-    if (kvh == 0 && threadIdx.x == 0) table_out[static_cast<size_t>(seq) * out_pages + index] = blockIdx.x;
-    if (key0 + kExpandKeys <= first) return;                // behind every window
-    if (threadIdx.x < kExpandKeys) {
-        const int key = key0 + threadIdx.x;
-        size_t row = ~size_t(0);
-        if (key >= first && key < ctx) {
-            const int page = key / page_size < table_width ? block_table[static_cast<size_t>(seq) * table_width + key / page_size] : -1;
-            if (page < 0 || page >= num_pages)
-                four::complain(status, four::kCodeNoPage);
-            else
-                row = ((static_cast<size_t>(page) * nkv + kvh) * page_size + key % page_size) * BYTES;
-        }
-        row_at[threadIdx.x] = row;
-    }
-    __syncthreads();
-    const size_t out_row = (static_cast<size_t>(blockIdx.x) * nkv + kvh) * kExpandKeys;
-    // a key without a page (before the windows, behind the end) becomes zeros: attention masks it
-    for (int i = threadIdx.x; i < kExpandKeys * 4; i += kExpandThreads) {           // keys: part a of a row, 8 entries of every group
-        const int r = i >> 2, a = i & 3;
-        const bool there = row_at[r] != ~size_t(0);
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pages + (there ? row_at[r] : 0));
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            uint4 out = make_uint4(0, 0, 0, 0);
-            if (there) {
-                const uint32_t w = words[a * G + g], p = words[4 * G + g];
-                const float s = four::bf16_low(p), c = four::bf16_high(p);
-                uint32_t pair[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const __nv_bfloat162 v = __floats2bfloat162_rn(four::value_of(w >> (8 * e) & 15u, s, c), four::value_of(w >> (8 * e + 4) & 15u, s, c));
-                    pair[e] = *reinterpret_cast<const uint32_t*>(&v);
-                }
-                out = make_uint4(pair[0], pair[1], pair[2], pair[3]);
-            }
-            *reinterpret_cast<uint4*>(k_out + (out_row + r) * HD + 32 * g + 8 * a) = out;
-        }
-    }
-    for (int i = threadIdx.x; i < kExpandKeys * 8; i += kExpandThreads) {           // values: part a of a row, 4 entries of every group
-        const int r = i >> 3, a = i & 7;
-        const bool there = row_at[r] != ~size_t(0);
-        const uint8_t* row = v_pages + (there ? row_at[r] : 0);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            uint2 out = make_uint2(0, 0);
-            if (there) {
-                const uint32_t w = reinterpret_cast<const uint16_t*>(row)[a * G + g], p = reinterpret_cast<const uint32_t*>(row + 16 * G)[g];
-                const float s = four::bf16_low(p), c = four::bf16_high(p);
-                const __nv_bfloat162 x = __floats2bfloat162_rn(four::value_of(w & 15u, s, c), four::value_of(w >> 4 & 15u, s, c));
-                const __nv_bfloat162 y = __floats2bfloat162_rn(four::value_of(w >> 8 & 15u, s, c), four::value_of(w >> 12, s, c));
-                out = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-            }
-            *reinterpret_cast<uint2*>(v_out + (out_row + r) * HD + 32 * g + 4 * a) = out;
-        }
-    }
-}
-
 }  // namespace stride
 
 using namespace stride;
@@ -626,38 +537,5 @@ extern "C" int stride_int4_read(const void* record) {
     else
         stride::launch(int4_read_kernel<__nv_bfloat16>, grid, block, 0, a.stream, a.k_pages, a.v_pages, a.slots, static_cast<__nv_bfloat16*>(a.k_out),
                        static_cast<__nv_bfloat16*>(a.v_out), a.n, a.nkv, a.hd, a.page_size, a.num_pages, a.status);
-    return STRIDE_LAUNCH_STATUS();
-}
-
-struct Int4Expand {
-    const uint8_t* k_pages;
-    const uint8_t* v_pages;
-    const int32_t* block_table;
-    const int32_t* q_len;
-    const int32_t* ctx_len;
-    __nv_bfloat16* k_out;           // [out_pages, nkv, 64, hd]
-    __nv_bfloat16* v_out;
-    int32_t* table_out;             // [num_seqs, out_pages]
-    int* status;
-    cudaStream_t stream;
-    int num_pages, table_width, num_seqs, nkv, hd, page_size, window, out_pages;
-};
-
-static_assert(sizeof(Int4Expand) == 112, "the record that the caller packs");
-
-// out_pages: at least the sum over the requests of ceil(ctx_len / 64) (else code 36 in the status word). Pages that no query of its request's
-// portion can see are left as they were. Head sizes 64 and 128.
-extern "C" int stride_int4_expand(const void* record) {
-    const Int4Expand a = read_record<Int4Expand>(record);
-    if (a.num_seqs < 0 || a.nkv <= 0 || a.page_size <= 0 || a.num_pages <= 0 || a.table_width <= 0 || a.window < 0 || a.out_pages <= 0)
-        return STRIDE_BAD_ARGUMENT;
-    if ((a.hd != 64 && a.hd != 128) || a.nkv > 65535) return STRIDE_UNSUPPORTED;
-    if ((reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4 ||
-        (reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) % 16)
-        return STRIDE_UNSUPPORTED;
-    if (a.num_seqs == 0) return 0;
-    const auto kernel = a.hd == 64 ? int4_expand_kernel<2> : int4_expand_kernel<4>;
-    stride::launch(kernel, dim3(a.out_pages, a.nkv), dim3(kExpandThreads), 0, a.stream, a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width,
-                   a.q_len, a.ctx_len, a.num_seqs, a.nkv, a.page_size, a.window, a.k_out, a.v_out, a.table_out, a.out_pages, a.status);
     return STRIDE_LAUNCH_STATUS();
 }

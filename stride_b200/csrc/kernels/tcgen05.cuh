@@ -239,6 +239,11 @@ __host__ __device__ constexpr uint32_t instr_desc_bf16(int m, int n, bool b_mn_m
            (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// The same for operands of either 16-bit type (`f16`: 11 bits, else bfloat16), both of one.
+__host__ __device__ constexpr uint32_t instr_desc_16(int m, int n, bool b_mn_major, bool f16) {
+    return instr_desc_bf16(m, n, b_mn_major) & ~(f16 ? (1u << 7) | (1u << 10) : 0u);
+}
+
 // ------------------------------------------------------------------------- host
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,

@@ -70,7 +70,7 @@ _SIGNATURES = {
                                                          c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "stride_head_write": ("head_write", [c_char_p]),
     "stride_int4_read": ("head_write", [c_char_p]),
-    "stride_int4_expand": ("head_write", [c_char_p]),
+    "stride_int4_prefill": ("attention_prefill_tc", [c_char_p]),
     "stride_attention_int4_exact": ("attention_int4", [c_char_p]),
     "stride_decode_int4": ("attention_int4_decode", [c_char_p]),
     "stride_copy_pages": ("page_copy", [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
@@ -221,7 +221,7 @@ _SIGNATURES = {
 _RECORDS = {
     "stride_head_write": _struct.Struct("@13Pq10if4x"),
     "stride_int4_read": _struct.Struct("@7P6i"),
-    "stride_int4_expand": _struct.Struct("@10P8i"),
+    "stride_int4_prefill": _struct.Struct("@15P11i2f4x"),
     "stride_attention_int4_exact": _struct.Struct("@11P9i2f2i4x"),
     "stride_decode_int4": _struct.Struct("@12Pq10i2f"),
 }
@@ -279,7 +279,7 @@ _CLASS_OF = {
     "stride_ssm_step": "state space: recurrence", "stride_ssm_chunks": "state space: recurrence",
     "stride_gated_group_norm": "gate + norm of parts",
     "stride_paged_decode_attention_biased": "attention (decode)",
-    "stride_head_write": "rotation + head norms + cache write", "stride_int4_read": "4-bit cache: values", "stride_int4_expand": "4-bit cache: values",
+    "stride_head_write": "rotation + head norms + cache write", "stride_int4_read": "4-bit cache: values", "stride_int4_prefill": "attention (prefill, tcgen05)",
     "stride_attention_int4_exact": "attention (exact kernel)", "stride_decode_int4": "attention (decode)", "stride_copy_pages": "copies of pages",
 }
 
@@ -1551,7 +1551,7 @@ _WAIT_CODES = {1: "matrix product: producer", 2: "matrix product: tensor-core is
                53: "tokens-as-rows product: tensor-core issuer", 54: "tokens-as-rows product: epilogue",
                61: "float32 product: copies", 62: "float32 product: tensor-core issuer", 63: "float32 product: cutting warps",
                71: "latent attention: copies of keys", 72: "latent attention: tensor-core issuer", 73: "latent attention: softmax", 81: "decode attention over a 4-bit cache: a tile copy"}
-_WAIT_CODES.update({c: "prefill attention (attention_prefill_tc.cu)" for c in range(11, 22)})
+_WAIT_CODES.update({c: "prefill attention (attention_prefill_tc.cu)" for c in range(11, 24)})
 _OTHER_CODES = {32: "decode attention was given a token whose position is not below the context bound of its launch",
                 33: "attention over a 4-bit cache met a key whose block-table entry names no page of the cache",
                 34: "a cache write or read was given a slot behind the cache's last page",
@@ -2254,7 +2254,7 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     """``paged_attention_prefill_tc`` over pages held in 4 bits, for the first ``num_seqs`` requests of the step (portions of any length), which own
     the rows of ``out``: bfloat16, head sizes 64 and 128. ``keys``: at least what those requests hold together; ``scratch``: int32, at least
     ``prefill_int4_scratch_ints`` elements, for one stream at a time. The keys and values that the portions see are expanded once, to pages
-    of 64 in bfloat16 (a rounding of 2^-9 of an entry, as a bfloat16 cache has it), and attended to from there."""
+    of 64 in 16-bit floating point (a rounding of 2^-11 of an entry at most; 65504 is the largest), and attended to from there."""
     device, qp, op, k, v, pages, rows, width = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
                                                                     softcap, torch.bfloat16)
     if not fast_attention_supported(q.dtype, nq, nkv, hd):
@@ -2272,12 +2272,10 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     wide_v, table = wide_k + half, wide_k + 2 * half
     starts, lens, held = (_covers(t, name, device, num_seqs) for t, name in ((q_start, "q_start"), (q_len, "q_len"), (ctx_len, "ctx_len")))
     sink, slope = _here_opt(sinks, "sinks", device, nq), _here_opt(slopes, "slopes", device, nq)
-    status, stream = _status_here(device), _stream_here(device)
-    _launch("stride_int4_expand", "paged_attention_prefill_int4", k, v, rows, lens, held, wide_k, wide_v, table, status, stream, pages, width, num_seqs, nkv,
-            hd, page_size, window, out_pages)
-    _check(_fn("stride_paged_prefill_attention_tc")(
-        qp, q_stride, op, wide_k, wide_v, out_pages, table, out_pages, starts, lens, held, num_seqs, tokens, nq, nkv, hd, INT4_EXPANDED_PAGE, scale,
-        window, -softcap if precise_cap else softcap, sink or None, slope or None, None, 0, status, stream), "paged_attention_prefill_int4")
+    _launch("stride_int4_prefill", "paged_attention_prefill_int4", qp, op, k, v, rows, starts, lens, held, wide_k, wide_v, table, sink, slope,
+            _status_here(device), _stream_here(device), q_stride, pages, width, out_pages, num_seqs, tokens, nq, nkv, hd, page_size, window, scale,
+            -softcap if precise_cap else softcap)
+    counters["launches"] += 1           # two kernels
 
 
 # ------------------------------------------------------------------- copies of pages

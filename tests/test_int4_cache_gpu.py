@@ -437,6 +437,21 @@ def test_attention_of_portions(ops, nq, nkv, hd, page, rules):
     ops.check_kernel_status()
 
 
+def test_portions_count_entries_beyond_the_16_bit_range_as_its_end(ops):
+    nq, nkv, hd, page, n = 4, 1, 64, 16, 40
+    pages, table, (k, v) = made_cache(5, [n], nkv, hd, page, spread=3e4)
+    clipped = v[0].clamp(-65504, 65504)
+    assert bool((clipped != v[0]).any())
+    q = (torch.randn(n, nq * hd, generator=torch.Generator().manual_seed(9)) * 1e-5).to(BF16)
+    pos, seq = torch.arange(n, dtype=torch.int32), torch.zeros(n, dtype=torch.int32)
+    out = torch.empty(n, nq * hd, dtype=BF16, device="cuda")
+    run_portion(ops, q.cuda(), out, pages, table, [n], [n], nq, nkv, hd, page)
+    want, largest, value = plain.attention(q.view(n, nq, hd), [k[0].clamp(-65504, 65504)], [clipped], pos, seq, hd ** -0.5)
+    # keys, values and weights to 11 bits; queries of 1e-5 are below the smallest normal 16-bit number, 2^-14, and keep multiples of 2^-24
+    ds = score_error(hd, largest) + 2.0 ** -11 * largest + hd * 2.0 ** -25 * 65504 * hd ** -0.5
+    check(out.view(n, nq, hd), want, ds, n, value, BF16, weight_error=2.0 ** -10, value_error=2.0 ** -11)
+
+
 def test_too_many_keys_for_a_portions_scratch_are_reported(ops):
     nq, nkv, hd, page = 4, 1, 64, 16
     held, lens = [2300, 10], [1, 1]
