@@ -10,10 +10,18 @@ namespace stride {
 
 constexpr int kExactWarps = 4;
 
+// The request of a row: -1 for a padded one, and for one whose request or position the block table does not hold (the status word says so).
+__device__ __forceinline__ int request_of(int seq, int pos, int table_rows, int table_width, int page_size, int* status) {
+    if (seq < 0) return -1;
+    if (seq < table_rows && pos >= 0 && pos < static_cast<long long>(table_width) * page_size) return seq;
+    four::complain(status, four::kCodeNoPage);
+    return -1;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kExactWarps * 32)
 attention_int4_exact_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, const uint8_t* __restrict__ k_pages,
-                            const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table, int table_width,
+                            const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table, int table_rows, int table_width,
                             const int32_t* __restrict__ seq_of_token, const int32_t* __restrict__ positions, int nq, int nkv, int hd, int page_size,
                             float scale, int window, float softcap, const float* __restrict__ sinks, const float* __restrict__ slopes, int* status) {
     pdl_trigger();
@@ -23,12 +31,11 @@ attention_int4_exact_kernel(const T* __restrict__ q, int q_stride, T* __restrict
     if (head >= nq) return;
     const int G = four::groups_of(hd), bytes = four::row_bytes(hd);
     T* out_row = out + (static_cast<size_t>(t) * nq + head) * hd;
-    const int seq = seq_of_token[t];
+    const int pos = positions[t], kvh = head / (nq / nkv), seq = request_of(seq_of_token[t], pos, table_rows, table_width, page_size, status);
     if (seq < 0) {      // a padded token of a fixed-size batch
         for (int d = lane; d < hd; d += 32) out_row[d] = from_f32<T>(0.f);
         return;
     }
-    const int pos = positions[t], kvh = head / (nq / nkv);
     const int first = window > 0 ? max(0, pos - window + 1) : 0;
     const int32_t* table = block_table + static_cast<size_t>(seq) * table_width;
     float* qs = q_smem[warp];
@@ -112,7 +119,7 @@ constexpr int kTileHeads = 4;
 template <typename T, int G, int TQ, int NW, int NR>
 __global__ void __launch_bounds__(NW * 32)
 attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, const uint8_t* __restrict__ k_pages,
-                           const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table, int table_width,
+                           const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table, int table_rows, int table_width,
                            const int32_t* __restrict__ seq_of_token, const int32_t* __restrict__ positions, int tokens, int nq, int nkv, int hd,
                            int page_size, float scale, int window, float softcap, const float* __restrict__ sinks, const float* __restrict__ slopes,
                            int* status) {
@@ -138,9 +145,10 @@ attention_int4_tile_kernel(const T* __restrict__ q, int q_stride, T* __restrict_
         qs[i] = d < hd && row_used(row) ? to_f32(q[static_cast<size_t>(row_token(row)) * q_stride + static_cast<size_t>(row_head(row)) * hd + d]) : 0.f;
     }
     for (int a = t0; a < t_end;) {                      // a run of rows of one request
-        const int seq = seq_of_token[a];
+        auto request = [&](int t) { return request_of(seq_of_token[t], positions[t], table_rows, table_width, page_size, status); };
+        const int seq = request(a);
         int b = a + 1, low = positions[a], high = low;
-        while (b < t_end && seq_of_token[b] == seq) {
+        while (b < t_end && request(b) == seq) {
             low = min(low, positions[b]);
             high = max(high, positions[b]);
             ++b;
@@ -339,7 +347,7 @@ struct Int4Attention {
     int q_stride, num_pages, table_width, tokens, nq, nkv, hd, page_size, window;
     float scale, softcap;
     int dtype, neighbours;          // neighbours: rows next to each other are mostly of one request (only the time depends on it)
-    int unused;
+    int table_rows;
 };
 
 static_assert(sizeof(Int4Attention) == 144, "the record that the caller packs");
@@ -353,7 +361,7 @@ static int launch_tiles(const Int4Attention& a) {
     const int group = a.nq / a.nkv, ctas_y = a.nkv * ((group + kTileHeads - 1) / kTileHeads);
     if (ctas_y > 65535) return STRIDE_UNSUPPORTED;
     stride::launch(kernel, dim3((a.tokens + TQ - 1) / TQ, ctas_y), dim3(NW * 32), bytes, a.stream, static_cast<const T*>(a.q), a.q_stride,
-                   static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions, a.tokens, a.nq,
+                   static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_rows, a.table_width, a.seq_of_token, a.positions, a.tokens, a.nq,
                    a.nkv, a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
     return STRIDE_LAUNCH_STATUS();
 }
@@ -372,7 +380,7 @@ static int launch_exact(const Int4Attention& a, int ctas_y) {
         case 4: return launch_tiles_of<T, 4>(a);
     }
     stride::launch(attention_int4_exact_kernel<T>, dim3(a.tokens, ctas_y), dim3(kExactWarps * 32), 0, a.stream, static_cast<const T*>(a.q), a.q_stride,
-                   static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_width, a.seq_of_token, a.positions, a.nq, a.nkv,
+                   static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_rows, a.table_width, a.seq_of_token, a.positions, a.nq, a.nkv,
                    a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
     return STRIDE_LAUNCH_STATUS();
 }
@@ -380,7 +388,7 @@ static int launch_exact(const Int4Attention& a, int ctas_y) {
 // A key whose page is none of the cache's is left out, and the status word says so.
 extern "C" int stride_attention_int4_exact(const void* record) {
     const Int4Attention a = read_record<Int4Attention>(record);
-    if (a.tokens < 0 || a.nq <= 0 || a.nkv <= 0 || a.hd <= 0 || a.page_size <= 0 || a.table_width <= 0 || a.num_pages <= 0 || a.window < 0 ||
+    if (a.tokens < 0 || a.nq <= 0 || a.nkv <= 0 || a.hd <= 0 || a.page_size <= 0 || a.table_width <= 0 || a.table_rows <= 0 || a.num_pages <= 0 || a.window < 0 ||
         a.softcap < 0.f || a.nq % a.nkv)
         return STRIDE_BAD_ARGUMENT;
     const int ctas_y = (a.nq + kExactWarps - 1) / kExactWarps;

@@ -58,17 +58,19 @@ struct Decode {
     float* part_ml;         // [2 CTAs][group][2]: R, sum of weights
     int* tickets;           // [token][key head]
     int* status;
-    int q_stride, table_width, num_pages, nq, nkv, page_size, window, tokens, max_context;
+    int q_stride, table_width, table_rows, num_pages, nq, nkv, page_size, window, tokens, max_context;
     float scale_log2e, cap_log2e, scale_over_cap;        // cap_log2e 0: no cap
 };
 
-// The keys of a token in units: first unit and how many; none for a padded row or one beyond the bound.
+// Whether a token reads keys: not a padded row, nor one of a request or position that the table or the launch's bound does not hold.
+__device__ __forceinline__ bool reads(const Decode& a, int seq, int pos) { return seq >= 0 && seq < a.table_rows && pos >= 0 && pos < a.max_context; }
+// The keys of a token in units: first unit and how many; none where it reads none.
 struct Span {
     int first, units;
 };
 __device__ __forceinline__ Span span_of(const Decode& a, int t) {
     const int seq = a.seq_of_token[t], pos = a.positions[t];
-    if (seq < 0 || pos < 0 || pos >= a.max_context) return {0, 0};
+    if (!reads(a, seq, pos)) return {0, 0};
     const int first = a.window > 0 ? max(0, pos - a.window + 1) / kUnit : 0;
     return {first, pos / kUnit - first + 1};
 }
@@ -201,9 +203,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
     }
     for (int i = blockIdx.x; i < a.tokens; i += gridDim.x) {        // rows without keys: zeros
         const int seq = a.seq_of_token[i], pos = a.positions[i];
-        if (seq >= 0 && pos >= 0 && pos < a.max_context) continue;
+        if (reads(a, seq, pos)) continue;
         for (int d = threadIdx.x; d < a.nq * HD; d += blockDim.x) a.out[static_cast<size_t>(i) * a.nq * HD + d] = __float2bfloat16_rn(0.f);
-        if (seq >= 0 && threadIdx.x == 0) complain(a.status, kCodeBeyondBound);
+        if (seq >= 0 && threadIdx.x == 0) complain(a.status, seq < a.table_rows ? kCodeBeyondBound : kCodeNoPage);
     }
     if (left == 0) return;
     t = begin_token;
@@ -760,11 +762,12 @@ struct DecodeCall {
     int* status;
     cudaStream_t stream;
     long long scratch_floats;
-    int q_stride, num_pages, table_width, tokens, nq, nkv, hd, page_size, window, max_context;
+    int q_stride, num_pages, table_width, table_rows, tokens, nq, nkv, hd, page_size, window, max_context;
     float scale, softcap;
+    int unused;
 };
 
-static_assert(sizeof(DecodeCall) == 152, "the record that the caller packs");
+static_assert(sizeof(DecodeCall) == 160, "the record that the caller packs");
 
 // One query token per row. `scratch` must be zero when it is first used (every launch leaves its tickets zero) and belongs to one stream at a
 // time. A row whose position does not lie below `max_context` gets zeros, and code 32 in the status word; a key whose page is none of the
@@ -772,7 +775,7 @@ static_assert(sizeof(DecodeCall) == 152, "the record that the caller packs");
 // 65536 (token, key head) pairs.
 int stride_decode_int4(const void* record) {
     const DecodeCall r = read_record<DecodeCall>(record);
-    if (r.tokens < 0 || r.nq <= 0 || r.nkv <= 0 || r.page_size <= 0 || r.table_width <= 0 || r.num_pages <= 0 || r.window < 0 || r.softcap < 0.f ||
+    if (r.tokens < 0 || r.nq <= 0 || r.nkv <= 0 || r.page_size <= 0 || r.table_width <= 0 || r.table_rows <= 0 || r.num_pages <= 0 || r.window < 0 || r.softcap < 0.f ||
         r.max_context <= 0 || r.nq % r.nkv || r.status == nullptr)
         return STRIDE_BAD_ARGUMENT;
     if ((r.hd != 64 && r.hd != 128) || r.nq / r.nkv > 16 || r.max_context > (1 << 30)) return STRIDE_UNSUPPORTED;
@@ -802,6 +805,7 @@ int stride_decode_int4(const void* record) {
     a.status = r.status;
     a.q_stride = r.q_stride;
     a.table_width = r.table_width;
+    a.table_rows = r.table_rows;
     a.num_pages = r.num_pages;
     a.nq = r.nq;
     a.nkv = r.nkv;

@@ -67,13 +67,13 @@ int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restric
                    int table_width, const int32_t* __restrict__ q_len, const int32_t* __restrict__ ctx_len, int num_seqs, int nkv, int page_size,
                    int window, uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int32_t* __restrict__ table_out, int out_pages,
                    int* status) {
-    pdl_trigger();
     constexpr int HD = 32 * G, BYTES = 20 * G;
     __shared__ size_t row_at[kExpandKeys];
     pdl_wait();
+    pdl_trigger();          // the attention reads the requests' lengths before it waits: only now are they what the kernels before made them
     int seq = -1, index = 0, at = 0;                        // this page is number `index` of request `seq`
     for (int s = 0; s < num_seqs; ++s) {
-        const int pages = (ctx_len[s] + kExpandKeys - 1) / kExpandKeys;
+        const int pages = (max(0, ctx_len[s]) + kExpandKeys - 1) / kExpandKeys;
         if (static_cast<int>(blockIdx.x) < at + pages) {
             seq = s;
             index = blockIdx.x - at;
@@ -184,7 +184,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                        const int32_t* __restrict__ q_len, const int32_t* __restrict__ ctx_len, int num_seqs, int nq, int nkv,
                        int page_shift, float scale_log2e, int window, float cap_in, const float* __restrict__ sinks,
                        const float* __restrict__ slopes, const float* __restrict__ rel, int rel_len, int* __restrict__ status,
-                       const __grid_constant__ CUtensorMap map_q2, const __grid_constant__ CUtensorMap map_k2, LatentGate gate, int q2_stride) {
+                       const __grid_constant__ CUtensorMap map_q2, const __grid_constant__ CUtensorMap map_k2, LatentGate gate, int q2_stride, int out_rows) {
     static_assert(!LATENT || (HEADS == 1 && TMA_KV && !REL), "the latent form");
     constexpr int HALVES = HD / 64;                       // 64-column boxes per row
     constexpr int HALF_BYTES = kQRows * 128;              // a [128 rows x 64 columns] bf16 box of Q
@@ -241,6 +241,10 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int n_tiles = last_pos / kKeys - kt_first + 1;
     const int q_row0 = q_start[seq] + row0;                // row of the projection output that holds query 0 of this tile
     const int32_t* table = LATENT ? nullptr : block_table + static_cast<size_t>(seq) * table_width;
+    if (F16 && (q_start[seq] < 0 || static_cast<long long>(q_start[seq]) + n_q > out_rows || n_q > ctx_len[seq])) {     // rows that are not the output's, or keys that are not there
+        if (threadIdx.x == 0) four::complain(status, four::kCodeTooManyKeys);
+        return;
+    }
 
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&q_full), 1);
@@ -649,6 +653,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     if (warp == MMA_WARP) tmem_dealloc(tmem_base_slot, TMEM_COLS);
 }
 
+// F16: rel is null and rel_len the rows of the output.
 template <int HD, int HEADS, bool F16 = false>
 int launch_attn(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const __nv_bfloat16* k_pages, const __nv_bfloat16* v_pages, __nv_bfloat16* out,
                 const int32_t* block_table, int table_width, const int32_t* q_start, const int32_t* q_len, const int32_t* ctx_len,
@@ -665,7 +670,7 @@ int launch_attn(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtens
         stride::launch(attn_prefill_tc_kernel<HD, HEADS, true, false, false, true>, dim3(nq / HEADS, max_tiles), dim3(HEADS == 1 ? 256 : 512), smem, stream,
                        *map_q, *map_k, *map_v, k_pages, v_pages, out, block_table, table_width, q_start, q_len, ctx_len, num_seqs, nq, nkv, page_shift,
                        (softcap != 0.f ? fabsf(softcap) : scale) * 1.4426950408889634f, window, softcap != 0.f ? scale / softcap : 0.f, sinks, slopes,
-                       nullptr, 0, status, *map_q, *map_q, LatentGate{}, 0);
+                       nullptr, 0, status, *map_q, *map_q, LatentGate{}, 0, rel_len);
         return STRIDE_LAUNCH_STATUS();
     }
     if (!configured[device]) {
@@ -686,7 +691,7 @@ int launch_attn(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtens
     stride::launch(kernel, grid, block, smem, stream, *map_q, tma ? *map_k : *map_q, tma ? *map_v : *map_q, k_pages, v_pages, out,
                    block_table, table_width, q_start, q_len, ctx_len, num_seqs, nq, nkv, page_shift,
                    (softcap != 0.f ? fabsf(softcap) : scale) * 1.4426950408889634f, window, softcap != 0.f ? scale / softcap : 0.f, sinks, slopes, rel,
-                   rel_len, status, *map_q, *map_q, LatentGate{}, 0);
+                   rel_len, status, *map_q, *map_q, LatentGate{}, 0, 0);
     return STRIDE_LAUNCH_STATUS();
 }
 
@@ -811,7 +816,7 @@ extern "C" int stride_latent_prefill_tc(const void* q, int q_ld, const void* q_r
     if (!map_q || !map_q2 || !map_kv || !map_k2) return STRIDE_UNSUPPORTED;
     stride::launch(kernel, dim3(heads, max_tiles), dim3(256), smem, stream, *map_q, *map_kv, *map_kv, nullptr, nullptr, static_cast<__nv_bfloat16*>(out),
                    nullptr, 0, q_start, q_len, ctx_len, num_seqs, heads, heads, 0, scale * 1.4426950408889634f, 0, 0.f, sinks, nullptr, nullptr, 0,
-                   status, *map_q2, *map_k2, tc::LatentGate{static_cast<const __nv_bfloat16*>(gate), gate_ld, gate_per_output, kv_head_stride, kv_v_off}, q_rot_stride);
+                   status, *map_q2, *map_k2, tc::LatentGate{static_cast<const __nv_bfloat16*>(gate), gate_ld, gate_per_output, kv_head_stride, kv_v_off}, q_rot_stride, 0);
     return STRIDE_LAUNCH_STATUS();
 }
 
@@ -871,8 +876,8 @@ extern "C" int stride_int4_prefill(const void* record) {
     static_assert(kExpandKeys == tc::kKeys && kExpandKeys == 1 << 6, "a page is a key tile");
 #define STRIDE_INT4_LAUNCH(HD_, HEADS_)                                                                                                                 \
     tc::launch_attn<HD_, HEADS_, true>(map_q, map_k, map_v, nullptr, nullptr, static_cast<__nv_bfloat16*>(a.out), a.table_wide, a.wide_pages, a.q_start, \
-                                       a.q_len, a.ctx_len, a.num_seqs, max_tiles, a.nq, a.nkv, 6, a.scale, a.window, a.softcap, a.sinks, a.slopes, nullptr, 0, \
-                                       a.status, a.stream)
+                                       a.q_len, a.ctx_len, a.num_seqs, max_tiles, a.nq, a.nkv, 6, a.scale, a.window, a.softcap, a.sinks, a.slopes, nullptr,    \
+                                       a.tokens, a.status, a.stream)
     if (a.hd == 64) return pair ? STRIDE_INT4_LAUNCH(64, 2) : STRIDE_INT4_LAUNCH(64, 1);
     return pair ? STRIDE_INT4_LAUNCH(128, 2) : STRIDE_INT4_LAUNCH(128, 1);
 #undef STRIDE_INT4_LAUNCH

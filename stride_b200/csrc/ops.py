@@ -222,8 +222,8 @@ _RECORDS = {
     "stride_head_write": _struct.Struct("@13Pq10if4x"),
     "stride_int4_read": _struct.Struct("@7P6i"),
     "stride_int4_prefill": _struct.Struct("@15P11i2f4x"),
-    "stride_attention_int4_exact": _struct.Struct("@11P9i2f2i4x"),
-    "stride_decode_int4": _struct.Struct("@12Pq10i2f"),
+    "stride_attention_int4_exact": _struct.Struct("@11P9i2f3i"),
+    "stride_decode_int4": _struct.Struct("@12Pq11i2f4x"),
 }
 
 
@@ -1556,7 +1556,7 @@ _OTHER_CODES = {32: "decode attention was given a token whose position is not be
                 33: "attention over a 4-bit cache met a key whose block-table entry names no page of the cache",
                 34: "a cache write or read was given a slot behind the cache's last page",
                 35: "a rotation was given a position behind its tables",
-                36: "attention of portions over a 4-bit cache: the requests hold more keys than the call said"}
+                36: "attention of portions over a 4-bit cache: the requests hold more keys than the call said, or bring rows that are not the output's"}
 
 
 def reset_kernel_status(device=None) -> None:
@@ -2174,7 +2174,7 @@ def read_int4(k_pages, v_pages, slots, k_out, v_out, nkv: int, hd: int, page_siz
 
 
 def _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window, softcap, dtype=None) -> tuple:
-    """(number of the device, q, out, keys, values, number of pages, block table, its width) of the attention kernels over a cache held in 4
+    """(number of the device, q, out, keys, values, number of pages, block table, its width and rows) of the attention kernels over a cache held in 4
     bits, checked."""
     if nq <= 0 or nkv <= 0 or hd <= 0 or page_size <= 0 or nq % nkv:
         raise KernelError(f"{nq} query heads of {hd} do not group into {nkv} key heads")
@@ -2190,7 +2190,8 @@ def _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nk
         raise KernelError("block_table must be [requests, pages]")
     device = _device_of(q, "q")
     k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd), device, torch.uint8)
-    return (device, _here(q, "q", device, dtype), _here(out, "out", device), k, v, pages, _here(block_table, "block_table", device, torch.int32), table[1])
+    return (device, _here(q, "q", device, dtype), _here(out, "out", device), k, v, pages, _here(block_table, "block_table", device, torch.int32), table[1],
+            table[0])
 
 
 def paged_attention_int4(q, q_stride: int, out, k_pages, v_pages, block_table, seq_of_token, positions, nq: int, nkv: int, hd: int, page_size: int,
@@ -2198,14 +2199,14 @@ def paged_attention_int4(q, q_stride: int, out, k_pages, v_pages, block_table, s
     """``paged_attention`` over pages held in 4 bits: any mix of rows, any head size up to 256, float32 or bfloat16. The exact kernel: the
     result of a row has the same bits however the work is cut. ``neighbours``: whether rows next to each other are mostly of one request
     (None: where there are four rows or more for each row of the block table); only the time depends on it."""
-    device, qp, op, k, v, pages, table, width = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
-                                                                     softcap)
+    device, qp, op, k, v, pages, table, width, requests = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size,
+                                                                               window, softcap)
     tokens = out.shape[0]
     if neighbours is None:
-        neighbours = tokens >= 4 * block_table.shape[0]
+        neighbours = tokens >= 4 * requests
     _launch("stride_attention_int4_exact", "paged_attention_int4", qp, op, k, v, table, _covers(seq_of_token, "seq_of_token", device, tokens),
             _covers(positions, "positions", device, tokens), _here_opt(sinks, "sinks", device, nq), _here_opt(slopes, "slopes", device, nq),
-            _status_here(device), _stream_here(device), q_stride, pages, width, tokens, nq, nkv, hd, page_size, window, scale, softcap, _code(q.dtype), neighbours)
+            _status_here(device), _stream_here(device), q_stride, pages, width, tokens, nq, nkv, hd, page_size, window, scale, softcap, _code(q.dtype), neighbours, requests)
 
 
 def decode_int4_scratch_floats(tokens: int, nq: int, nkv: int, hd: int, max_context: int) -> int:
@@ -2223,13 +2224,13 @@ def paged_attention_decode_int4(q, q_stride: int, out, k_pages, v_pages, block_t
                                 page_size: int, scale: float, window: int, max_context: int, softcap: float = 0.0, sinks=None, slopes=None) -> None:
     """``paged_attention_decode`` over pages held in 4 bits: one query per row, bfloat16, head sizes 64 and 128. ``max_context`` exceeds every
     position; ``scratch``: float32, zero when it is first used, at least ``decode_int4_scratch_floats`` elements, for one stream at a time."""
-    device, qp, op, k, v, pages, table, width = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
-                                                                     softcap, torch.bfloat16)
+    device, qp, op, k, v, pages, table, width, requests = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size,
+                                                                               window, softcap, torch.bfloat16)
     tokens = out.shape[0]
     _launch("stride_decode_int4", "paged_attention_decode_int4", qp, op, k, v, table, _covers(seq_of_token, "seq_of_token", device, tokens),
             _covers(positions, "positions", device, tokens), _here(scratch, "scratch", device, torch.float32), _here_opt(sinks, "sinks", device, nq),
-            _here_opt(slopes, "slopes", device, nq), _status_here(device), _stream_here(device), scratch.numel(), q_stride, pages, width, tokens, nq, nkv, hd,
-            page_size, window, max_context, scale, softcap)
+            _here_opt(slopes, "slopes", device, nq), _status_here(device), _stream_here(device), scratch.numel(), q_stride, pages, width, requests, tokens, nq,
+            nkv, hd, page_size, window, max_context, scale, softcap)
 
 
 INT4_EXPANDED_PAGE = 64     # keys of a page of the expanded keys and values
@@ -2255,8 +2256,8 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     the rows of ``out``: bfloat16, head sizes 64 and 128. ``keys``: at least what those requests hold together; ``scratch``: int32, at least
     ``prefill_int4_scratch_ints`` elements, for one stream at a time. The keys and values that the portions see are expanded once, to pages
     of 64 in 16-bit floating point (a rounding of 2^-11 of an entry at most; 65504 is the largest), and attended to from there."""
-    device, qp, op, k, v, pages, rows, width = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size, window,
-                                                                    softcap, torch.bfloat16)
+    device, qp, op, k, v, pages, rows, width, requests = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size,
+                                                                              window, softcap, torch.bfloat16)
     if not fast_attention_supported(q.dtype, nq, nkv, hd):
         raise KernelError(f"paged_attention_prefill_int4: {nq} heads of {hd} on {nkv} are not supported (paged_attention_int4 takes them)")
     if num_seqs < 0 or keys < 0 or scratch.numel() < prefill_int4_scratch_ints(num_seqs, keys, nkv, hd):
@@ -2265,7 +2266,7 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     if tokens == 0 or num_seqs == 0:
         return
     out_pages = _int4_expanded_pages(num_seqs, keys)
-    if block_table.shape[0] < num_seqs:
+    if requests < num_seqs:
         raise KernelError("block_table must have a row a request")
     half = out_pages * nkv * INT4_EXPANDED_PAGE * hd * 2
     wide_k = _here(scratch, "scratch", device, torch.int32)

@@ -325,9 +325,13 @@ class Engine:
         if self._ahead is not None:
             raise RuntimeError("a step of the engine's own requests is in flight; call step() until they are done")
         copies, state = self.cache.fork(int(parent), int(child), int(num_tokens))
-        for group, src, dst in copies:
-            self.device_cache.copy_pages(group, [src], [dst])
-        self.device_cache.copy_state(*state)
+        try:
+            for group, src, dst in copies:
+                self.device_cache.copy_pages(group, [src], [dst])
+            self.device_cache.copy_state(*state)
+        except Exception:
+            self.cache.close(int(child))        # what its pages hold is not the parent's
+            raise
 
     def get_weight(self, name: str) -> torch.Tensor:
         return self.model.get_weight(name)

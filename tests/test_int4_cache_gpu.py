@@ -483,6 +483,40 @@ def test_a_key_without_a_page_is_reported(ops, call, entry):
     assert bool(out.isfinite().all())
 
 
+@pytest.mark.parametrize("call", ["exact", "neighbours", "decode"])
+@pytest.mark.parametrize("seq,pos", [(1, 5), (7, 5), (0, 64), (0, 2 ** 31 - 1), (0, -1)])
+def test_a_row_whose_request_or_position_there_is_not_is_reported(ops, call, seq, pos):
+    """Beside rows that are in order, which keep their results."""
+    nq, nkv, hd, page = 4, 1, 64, 16
+    pages, table, (k, v) = made_cache(2, [60], nkv, hd, page)
+    q = torch.randn(3, nq * hd, generator=torch.Generator().manual_seed(3)).to(BF16)
+    seqs, poss = torch.tensor([0, seq, 0], dtype=torch.int32), torch.tensor([40, pos, 59], dtype=torch.int32)
+    out = torch.full((3, nq * hd), math.nan, dtype=BF16, device="cuda")
+    if call == "decode":
+        run_decode(ops, q.cuda(), nq * hd, out, pages, table, seqs.cuda(), poss.cuda(), nq, nkv, hd, page, 0, 0.0, None, None, 64)
+    else:
+        ops.paged_attention_int4(q.cuda(), nq * hd, out, *pages, table, seqs.cuda(), poss.cuda(), nq, nkv, hd, page, 0.125, neighbours=call == "neighbours")
+    with pytest.raises(ops.KernelError, match="names no page|context bound"):
+        ops.check_kernel_status()
+    assert not bool(out[1].any())
+    want, largest, value = plain.attention(q[::2].view(2, nq, hd), k, v, poss[::2], seqs[::2], hd ** -0.5)
+    check_decode(out[::2].view(2, nq, hd), want, hd, largest, 60, value)
+
+
+@pytest.mark.parametrize("start,length,held", [(9, 4, 30), (-1, 4, 30), (2 ** 31 - 2, 4, 30), (0, 31, 30)])
+def test_portions_that_are_not_the_outputs_are_reported(ops, start, length, held):
+    nq, nkv, hd, page = 4, 1, 64, 16
+    pages, table, _values = made_cache(2, [30], nkv, hd, page)
+    q = torch.randn(12, nq * hd).to(BF16).cuda()
+    out = torch.full_like(q, 7.0)
+    ints = lambda v: torch.tensor([v], dtype=torch.int32, device="cuda")  # noqa: E731
+    scratch = torch.zeros(ops.prefill_int4_scratch_ints(1, 64, nkv, hd), dtype=torch.int32, device="cuda")
+    ops.paged_attention_prefill_int4(q, nq * hd, out, *pages, table, ints(start), ints(length), ints(held), scratch, 1, 64, nq, nkv, hd, page, 0.125, 0)
+    with pytest.raises(ops.KernelError, match="portions"):
+        ops.check_kernel_status()
+    assert bool((out == 7.0).all())
+
+
 def test_empty_calls(ops):
     nq, nkv, hd, page = 4, 1, 64, 16
     pages, table, _values = made_cache(2, [10], nkv, hd, page)
