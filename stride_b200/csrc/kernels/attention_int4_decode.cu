@@ -38,6 +38,7 @@ constexpr int kUnit = kTile * kWarps;   // keys that a CTA's warps cover with a 
 constexpr int kStages = 3;
 constexpr int kWindow = 16;             // tiles whose pages the lanes look up at once, a half each
 constexpr int kTicketInts = 65536;      // ticket counters at the start of the scratch, one per (token, key head)
+constexpr int kMostCtas = 148 * 3;      // of a launch: what fits at once
 constexpr int kCodeBeyondBound = 32;    // as in attention_decode.cu
 constexpr int kCodeCopyWait = 81;       // a wait for a tile's copies ran out
 constexpr float kLimit = 256.f;         // what a weight's product with a scale may reach before R moves
@@ -158,6 +159,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
     __shared__ int warp_sums[kWarps];
     __shared__ int begin_token, begin_units;
+    __shared__ Span begin_span;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, group = a.nq / a.nkv;
 
     // ---- this CTA's stretch: `left` units from unit `skip` of (t, kvh) on
@@ -165,8 +167,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
     long long total = 0, begin = 0, stretches = 0;
     {
         const int chunk = (a.tokens + kWarps * 32 - 1) / (kWarps * 32), t_lo = threadIdx.x * chunk, t_hi = min(a.tokens, t_lo + chunk);
+        Span span = {0, 0};                                         // of the thread's last token
         int mine = 0;
-        for (int i = t_lo; i < t_hi; ++i) mine += span_of(a, i).units;
+        bool idle = false;                                          // a token without keys is among them
+        for (int i = t_lo; i < t_hi; ++i) {
+            span = span_of(a, i);
+            mine += span.units;
+            idle = idle || span.units == 0;
+        }
         int upto = mine;                                            // with the lanes and warps before
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             if (lane >= s) upto += v;
         }
         if (lane == 31) warp_sums[warp] = upto;
-        __syncthreads();
+        idle = __syncthreads_or(idle);
         int sum = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
@@ -182,39 +190,50 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             sum += warp_sums[w];
         }
         total = static_cast<long long>(sum) * a.nkv;
-        // one unit a CTA while that leaves SMs idle, then two at least, since a part costs about as much as a unit
-        stretches = min(static_cast<long long>(gridDim.x), total <= 148 ? total : max(148LL, total / 2));
+        stretches = min(static_cast<long long>(gridDim.x), total);
         if (blockIdx.x < stretches) {
-            begin = blockIdx.x * total / stretches;
-            left = static_cast<int>((blockIdx.x + 1) * total / stretches - begin);
+            if (total < (1LL << 31) / gridDim.x) {                  // 32-bit divisions, a tenth of the time
+                begin = static_cast<uint32_t>(blockIdx.x) * static_cast<uint32_t>(total) / static_cast<uint32_t>(stretches);
+                left = static_cast<int>((blockIdx.x + 1u) * static_cast<uint32_t>(total) / static_cast<uint32_t>(stretches) - static_cast<uint32_t>(begin));
+            } else {
+                begin = blockIdx.x * total / stretches;
+                left = static_cast<int>((blockIdx.x + 1) * total / stretches - begin);
+            }
             // units are counted token by token, key heads inside: the token whose heads hold unit `begin`
             if (begin < static_cast<long long>(upto) * a.nkv && begin >= static_cast<long long>(upto - mine) * a.nkv) {
                 int before = upto - mine, i = t_lo;
-                for (;; ++i) {
-                    const int units = span_of(a, i).units;
-                    if (begin < static_cast<long long>(before + units) * a.nkv) break;
-                    before += units;
+                for (; chunk > 1; ++i) {
+                    span = span_of(a, i);
+                    if (begin < static_cast<long long>(before + span.units) * a.nkv) break;
+                    before += span.units;
                 }
                 begin_token = i;
                 begin_units = before;
+                begin_span = span;
             }
         }
         __syncthreads();
-    }
-    for (int i = blockIdx.x; i < a.tokens; i += gridDim.x) {        // rows without keys: zeros
-        const int seq = a.seq_of_token[i], pos = a.positions[i];
-        if (reads(a, seq, pos)) continue;
-        for (int d = threadIdx.x; d < a.nq * HD; d += blockDim.x) a.out[static_cast<size_t>(i) * a.nq * HD + d] = __float2bfloat16_rn(0.f);
-        if (seq >= 0 && threadIdx.x == 0) complain(a.status, seq < a.table_rows ? kCodeBeyondBound : kCodeNoPage);
+        if (idle) {
+            for (int i = blockIdx.x; i < a.tokens; i += gridDim.x) {        // rows without keys: zeros
+                const int seq = a.seq_of_token[i], pos = a.positions[i];
+                if (reads(a, seq, pos)) continue;
+                for (int d = threadIdx.x; d < a.nq * HD; d += blockDim.x) a.out[static_cast<size_t>(i) * a.nq * HD + d] = __float2bfloat16_rn(0.f);
+                if (seq >= 0 && threadIdx.x == 0) complain(a.status, seq < a.table_rows ? kCodeBeyondBound : kCodeNoPage);
+            }
+        }
     }
     if (left == 0) return;
     t = begin_token;
     long long item = static_cast<long long>(begin_units) * a.nkv;   // the first unit of (t, kvh)
-    Span span = span_of(a, t);
-    kvh = static_cast<int>((begin - item) / span.units);
+    Span span = begin_span;
+    kvh = static_cast<int>(begin - item) / span.units;
     item += static_cast<long long>(kvh) * span.units;
     skip = static_cast<int>(begin - item);
-    auto stretch_of = [&](long long unit) { return static_cast<int>(((unit + 1) * stretches + total - 1) / total - 1); };
+    auto stretch_of = [&](long long unit) {
+        if (total < (1LL << 31) / gridDim.x)
+            return static_cast<int>((static_cast<uint32_t>(unit + 1) * static_cast<uint32_t>(stretches) + static_cast<uint32_t>(total) - 1) / static_cast<uint32_t>(total)) - 1;
+        return static_cast<int>(((unit + 1) * stretches + total - 1) / total - 1);
+    };
 
     unsigned char* ring = smem + warp * kStages * STAGE;
     if (BULK) {
@@ -666,26 +685,40 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         }
         __syncthreads();
         if (is_last) {
+            // a warp a head works out the weights, then a thread sums four columns, many parts on their way at once
+            float* weights = reinterpret_cast<float*>(smem);        // [group][parts], then [group] sums
+            for (int row = warp; row < group; row += kWarps) {
+                float most = -INFINITY;
+                for (int i = lane; i < parts; i += 32) {
+                    const float v = __ldcg(a.part_ml + (place(i) + row) * 2);
+                    weights[row * parts + i] = v;
+                    most = fmaxf(most, v);
+                }
+                most = warp_max(most);
+                float sum = 0.f;
+                for (int i = lane; i < parts; i += 32) {
+                    const float w = most == -INFINITY ? 0.f : exp2f(weights[row * parts + i] - most);
+                    weights[row * parts + i] = w;
+                    sum = fmaf(w, __ldcg(a.part_ml + (place(i) + row) * 2 + 1), sum);
+                }
+                sum = warp_sum(sum);
+                if (a.sinks != nullptr && most != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -most));
+                if (lane == 0) weights[group * parts + row] = sum;
+            }
+            __syncthreads();
             for (int idx = threadIdx.x; idx < group * (HD / 4); idx += blockDim.x) {
                 const int row = idx / (HD / 4), d = (idx - row * (HD / 4)) * 4;
-                float most = -INFINITY;
-#pragma unroll 8
-                for (int i = 0; i < parts; ++i) most = fmaxf(most, __ldcg(a.part_ml + (place(i) + row) * 2));
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                float sum = 0.f;
-#pragma unroll 8
+#pragma unroll 16
                 for (int i = 0; i < parts; ++i) {
-                    const size_t at = place(i) + row;
-                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + at * 2));
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + d));
-                    const float w = most == -INFINITY ? 0.f : exp2f(ml.x - most);
-                    sum = fmaf(w, ml.y, sum);
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (place(i) + row) * HD + d));
+                    const float w = weights[row * parts + i];
                     acc.x = fmaf(w, v.x, acc.x);
                     acc.y = fmaf(w, v.y, acc.y);
                     acc.z = fmaf(w, v.z, acc.z);
                     acc.w = fmaf(w, v.w, acc.w);
                 }
-                if (a.sinks != nullptr && most != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -most));
+                const float sum = weights[group * parts + row];
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
                 const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
                 if (reinterpret_cast<uintptr_t>(a.out) % 8 == 0) {
@@ -715,14 +748,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 // CTAs of a launch: as many as fit at once, no more than there can be units.
 inline int choose_ctas(int tokens, int nkv, int max_context, int group) {
     const long long units = static_cast<long long>(tokens) * nkv * ((static_cast<long long>(max_context) + kUnit - 1) / kUnit);
-    const int fit = 148 * (group <= 8 ? 3 : 2);
+    const int fit = group <= 8 ? kMostCtas : 148 * 2;
     return units < fit ? static_cast<int>(units) : fit;
 }
 
 template <int G, int NT>
 int launch_decode(const Decode& a, int ctas, cudaStream_t stream) {
     constexpr int smem = kWarps * kStages * 2 * kTile * 20 * G;        // 61 KB at head size 128
-    static_assert(kWarps * 8 * NT * (32 * G + 2) * 4 <= smem, "the warps' results fit into the rings");
+    static_assert(kWarps * 8 * NT * (32 * G + 2) * 4 <= smem && 8 * NT * (kMostCtas + 1) * 4 <= smem, "the warps' results and the parts' weights fit into the rings");
     const bool bulk = a.page_size % kSub == 0;
     cudaError_t e = allow_shared<decode_kernel<G, NT, true>>(smem);
     if (e == cudaSuccess) e = allow_shared<decode_kernel<G, NT, false>>(smem);
