@@ -267,6 +267,25 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         }
         return ((static_cast<size_t>(page) * a.nkv + kvh) * a.page_size + key % a.page_size) * ROW;
     };
+    // the query's rows, on their way beside the pages: lane (g, c) holds, of head 8 nt + g, entries 32 grp + 8 c .. + 7
+    uint4 rows[NT][G];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+            const int head = 8 * nt + g;
+            const __nv_bfloat16* src = a.q + static_cast<size_t>(t) * a.q_stride + static_cast<size_t>(kvh * group + head) * HD + 32 * grp + 8 * c;
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (head < group) {
+                if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+                    raw = *reinterpret_cast<const uint4*>(src);
+                } else {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+                    raw = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                }
+            }
+            rows[nt][grp] = raw;
+        }
     // BULK: lane 2 i + h answers for half h of tile `window` + i: its row, and for the window after it the page
     size_t my_row = ~size_t(0);
     int my_page = -1;
@@ -338,25 +357,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         }
     }
 
-    // ---- the query: lane (g, c) holds, of head 8 nt + g, entries 32 grp + 8 c .. + 7
+    // ---- the query
     uint32_t qb[NT][G][2][2], cb[NT][2];            // B operands: of the numbers, of centres and scales
     float factor[NT][2], slope[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int head = 8 * nt + g;
         float x[G][8], most = 0.f;
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
-            const __nv_bfloat16* src = a.q + static_cast<size_t>(t) * a.q_stride + static_cast<size_t>(kvh * group + head) * HD + 32 * grp + 8 * c;
-            uint4 raw = make_uint4(0, 0, 0, 0);
-            if (head < group) {
-                if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
-                    raw = *reinterpret_cast<const uint4*>(src);
-                } else {
-                    const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-                    raw = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-                }
-            }
+            const uint4 raw = rows[nt][grp];
             const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -676,12 +685,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
         // ---- the CTA that finishes last for this (token, key head) merges the parts
         __shared__ int is_last;
         __syncthreads();
-        if (threadIdx.x == 0) {             // (the barriers order the CTA's stores before this thread's fence, and its loads behind it)
-            __threadfence();
+        if (threadIdx.x == 0) {             // (the barriers order the CTA's stores before this thread's release, and its loads behind its acquire)
             int* ticket = a.tickets + static_cast<size_t>(t) * a.nkv + kvh;
-            is_last = atomicAdd(ticket, 1) == parts - 1;
+            int drawn;
+            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(drawn) : "l"(ticket) : "memory");
+            is_last = drawn == parts - 1;
             if (is_last) *ticket = 0;       // ready for the next launch; nobody else touches it before then
-            __threadfence();
         }
         __syncthreads();
         if (is_last) {
