@@ -395,20 +395,21 @@ def _device_of(t: torch.Tensor, name: str) -> int:
     device = t.get_device()
     if device < 0:
         raise KernelError(f"{name} must live on a CUDA device; stride_b200 has no CPU path")
-    if device != _current_device():
-        raise KernelError(f"{name} lives on cuda:{device}, but the current device is cuda:{_current_device()}")
+    current = _current_device()
+    if device != current:
+        raise KernelError(f"{name} lives on cuda:{device}, but the current device is cuda:{current}")
     return device
 
 
 def _here(t: torch.Tensor, name: str, device: int, dtype=None) -> int:
     """``_dev`` for a tensor that must live on the call's device. (Small calls are bound by the host: a tensor is asked for each thing once.)"""
+    if t.get_device() == device and (dtype is None or t.dtype is dtype) and t.is_contiguous():
+        return t.data_ptr()
     if t.get_device() != device:
         raise KernelError(f"{name} must live on cuda:{device}, the call's device")
-    if dtype is not None and t.dtype is not dtype:
-        raise KernelError(f"{name} must be {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise KernelError(f"{name} must be contiguous")
-    return t.data_ptr()
+    raise KernelError(f"{name} must be {dtype}, got {t.dtype}")
 
 
 def _here_opt(t, name: str, device: int, count: int) -> int:
@@ -2121,24 +2122,27 @@ def _head_write(what: str, bits4: bool, qkv, bias, q_norm, k_norm, eps, position
         raise KernelError("the norms of queries and keys come together")
     dtype = qkv.dtype
     code = _code(dtype)
-    if q_out is not None and (q_out.dim() != 2 or q_out.shape[0] < tokens or q_out.shape[1] != nq * hd or q_out.dtype is not dtype or
-                              q_out.stride(1) != 1 or q_out.stride(0) < nq * hd):
-        raise KernelError("q_out must be rows [tokens, nq * hd] of qkv's element type")
-    if rotate and (cos.dim() != 2 or sin.shape != cos.shape or cos.shape[1] * 2 != hd):
-        raise KernelError("cos and sin must be [positions, hd / 2]")
+    if rotate:
+        angles = cos.shape
+        if len(angles) != 2 or 2 * angles[1] != hd or sin.shape != angles:
+            raise KernelError("cos and sin must be [positions, hd / 2]")
     device = _device_of(qkv, "qkv")
     rows = _here(qkv, "qkv", device)
     if q_out is None:
         out, stride = rows, width
-    elif q_out.get_device() != device:
-        raise KernelError("q_out must live on qkv's device")
     else:
-        out, stride = q_out.data_ptr(), q_out.stride(0)
+        shape = q_out.shape
+        stride, step = q_out.stride() if len(shape) == 2 else (0, 0)
+        if len(shape) != 2 or shape[0] < tokens or shape[1] != nq * hd or step != 1 or stride < nq * hd or q_out.dtype is not dtype:
+            raise KernelError("q_out must be rows [tokens, nq * hd] of qkv's element type")
+        if q_out.get_device() != device:
+            raise KernelError("q_out must live on qkv's device")
+        out = q_out.data_ptr()
     k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd) if bits4 else hd, device, torch.uint8 if bits4 else dtype)
     _launch("stride_head_write", what, rows, out, _here_opt(bias, "bias", device, width), _here_opt(q_norm, "q_norm", device, hd),
             _here_opt(k_norm, "k_norm", device, hd), _covers(positions, "positions", device, tokens),
             0 if slot_mapping is None else _covers(slot_mapping, "slot_mapping", device, tokens), _here(cos, "cos", device, torch.float32),
-            _here(sin, "sin", device, torch.float32), k, v, _status_here(device), _stream_here(device), stride, cos.shape[0] if rotate else 0, pages, bits4,
+            _here(sin, "sin", device, torch.float32), k, v, _status_here(device), _stream_here(device), stride, angles[0] if rotate else 0, pages, bits4,
             tokens, nq, nkv, hd, page_size, rotate, code, eps)
 
 
@@ -2260,18 +2264,18 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
                                                                               window, softcap, torch.bfloat16)
     if not fast_attention_supported(q.dtype, nq, nkv, hd):
         raise KernelError(f"paged_attention_prefill_int4: {nq} heads of {hd} on {nkv} are not supported (paged_attention_int4 takes them)")
-    if num_seqs < 0 or keys < 0 or scratch.numel() < prefill_int4_scratch_ints(num_seqs, keys, nkv, hd):
+    out_pages = _int4_expanded_pages(num_seqs, keys)
+    half = out_pages * nkv * INT4_EXPANDED_PAGE * hd * 2            # bytes of the keys, and of the values
+    if num_seqs < 0 or keys < 0 or 4 * scratch.numel() < 2 * half + 4 * num_seqs * out_pages:
         raise KernelError("paged_attention_prefill_int4: the scratch is too small for the requests and keys")
     tokens = out.shape[0]
     if tokens == 0 or num_seqs == 0:
         return
-    out_pages = _int4_expanded_pages(num_seqs, keys)
     if requests < num_seqs:
         raise KernelError("block_table must have a row a request")
-    half = out_pages * nkv * INT4_EXPANDED_PAGE * hd * 2
     wide_k = _here(scratch, "scratch", device, torch.int32)
     wide_v, table = wide_k + half, wide_k + 2 * half
-    starts, lens, held = (_covers(t, name, device, num_seqs) for t, name in ((q_start, "q_start"), (q_len, "q_len"), (ctx_len, "ctx_len")))
+    starts, lens, held = _covers(q_start, "q_start", device, num_seqs), _covers(q_len, "q_len", device, num_seqs), _covers(ctx_len, "ctx_len", device, num_seqs)
     sink, slope = _here_opt(sinks, "sinks", device, nq), _here_opt(slopes, "slopes", device, nq)
     _launch("stride_int4_prefill", "paged_attention_prefill_int4", qp, op, k, v, rows, starts, lens, held, wide_k, wide_v, table, sink, slope,
             _status_here(device), _stream_here(device), q_stride, pages, width, out_pages, num_seqs, tokens, nq, nkv, hd, page_size, window, scale,

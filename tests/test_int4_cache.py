@@ -166,7 +166,7 @@ def rows(tokens=3, nq=4, nkv=2, hd=64, page=8, pages=5, dtype=torch.bfloat16, bi
 @pytest.mark.parametrize("change", [
     dict(nq=3), dict(nkv=1), dict(hd=0), dict(page_size=16), dict(q_norm=torch.ones(64)), dict(positions=torch.zeros(2, dtype=torch.int32)),
     dict(slot_mapping=torch.zeros(2, dtype=torch.int32)), dict(cos=torch.zeros(16, 31)), dict(k_pages=torch.zeros(5, 2, 8, 63, dtype=torch.uint8)),
-    dict(v_pages=torch.zeros(4, 2, 8, 40, dtype=torch.uint8)), dict(q_out=torch.zeros(3, 255, dtype=torch.bfloat16)), dict(q_out=torch.zeros(3, 256)),
+    dict(v_pages=torch.zeros(4, 2, 8, 40, dtype=torch.uint8)), 
     dict(qkv=torch.zeros(3, 512, dtype=torch.float16)), dict()])
 def test_refused_writes(bits4, change):
     from stride_b200.csrc import ops

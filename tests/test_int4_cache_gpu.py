@@ -156,6 +156,18 @@ def test_groups_without_a_range_and_tokens_that_are_no_numbers(ops):
     ops.check_kernel_status()
 
 
+@pytest.mark.parametrize("bits4", [False, True])
+@pytest.mark.parametrize("q_out", [torch.zeros(3, 255, dtype=BF16), torch.zeros(3, 256), torch.zeros(2, 256, dtype=BF16), torch.zeros(256, 3, dtype=BF16).t(),
+                                   torch.zeros(3, 2, 128, dtype=BF16)])
+def test_refused_rows_for_queries(ops, bits4, q_out):
+    made = made_rows(1, 3, 4, 2, 64, BF16, False, False)
+    pages = [torch.zeros(2, 2, 4, 40 if bits4 else 64, dtype=torch.uint8 if bits4 else BF16, device="cuda") for _ in "kv"]
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    for bad in (q_out.cuda(), torch.zeros(3, 256, dtype=BF16)):            # the last on the host
+        with pytest.raises(ops.KernelError):
+            write(ops, made, slots, pages, 4, 2, 64, 4, bits4, q_out=bad)
+
+
 def test_slots_and_positions_out_of_range_are_reported(ops):
     made = made_rows(1, 3, 2, 1, 64, BF16, False, False, positions=50)
     for bits4 in (False, True):
