@@ -222,7 +222,7 @@ _RECORDS = {
     "stride_head_write": _struct.Struct("@13Pq10if4x"),
     "stride_int4_read": _struct.Struct("@7P6i"),
     "stride_int4_prefill": _struct.Struct("@15P11i2f4x"),
-    "stride_attention_int4_exact": _struct.Struct("@11P9i2f3i"),
+    "stride_attention_int4_exact": _struct.Struct("@11P9i2f4i4x"),
     "stride_decode_int4": _struct.Struct("@12Pq11i2f4x"),
 }
 
@@ -2199,10 +2199,12 @@ def _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nk
 
 
 def paged_attention_int4(q, q_stride: int, out, k_pages, v_pages, block_table, seq_of_token, positions, nq: int, nkv: int, hd: int, page_size: int,
-                         scale: float, window: int = 0, softcap: float = 0.0, sinks=None, slopes=None, neighbours: bool | None = None) -> None:
+                         scale: float, window: int = 0, softcap: float = 0.0, sinks=None, slopes=None, neighbours: bool | None = None,
+                         context_bound: int | None = None) -> None:
     """``paged_attention`` over pages held in 4 bits: any mix of rows, any head size up to 256, float32 or bfloat16. The exact kernel: the
     result of a row has the same bits however the work is cut. ``neighbours``: whether rows next to each other are mostly of one request
-    (None: where there are four rows or more for each row of the block table); only the time depends on it."""
+    (None: where there are four rows or more for each row of the block table); ``context_bound``: about the most keys that a row has (None: what
+    the block table has room for). Only the time depends on these two."""
     device, qp, op, k, v, pages, table, width, requests = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size,
                                                                                window, softcap)
     tokens = out.shape[0]
@@ -2210,7 +2212,8 @@ def paged_attention_int4(q, q_stride: int, out, k_pages, v_pages, block_table, s
         neighbours = tokens >= 4 * requests
     _launch("stride_attention_int4_exact", "paged_attention_int4", qp, op, k, v, table, _covers(seq_of_token, "seq_of_token", device, tokens),
             _covers(positions, "positions", device, tokens), _here_opt(sinks, "sinks", device, nq), _here_opt(slopes, "slopes", device, nq),
-            _status_here(device), _stream_here(device), q_stride, pages, width, tokens, nq, nkv, hd, page_size, window, scale, softcap, _code(q.dtype), neighbours, requests)
+            _status_here(device), _stream_here(device), q_stride, pages, width, tokens, nq, nkv, hd, page_size, window, scale, softcap, _code(q.dtype),
+            neighbours, requests, max(1, min(context_bound or width * page_size, 2 ** 31 - 1)))
 
 
 def decode_int4_scratch_floats(tokens: int, nq: int, nkv: int, hd: int, max_context: int) -> int:

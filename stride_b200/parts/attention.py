@@ -554,7 +554,7 @@ class PagedAttention(Mixer):
         if not self._fast or (split > 0 and not ctx.portion_keys):
             # the exact kernel: the whole 32-bit path, sizes the tensor-core kernels refuse, and a step that does not say what its portions hold
             ops.paged_attention_int4(qkv[:split], self.qkv_dim, attn[:split], *pages, ctx.seq_of_token[:split], ctx.positions[:split], *geometry, *rules,
-                                     neighbours=ctx.decode_tail_start >= split // 2 and ctx.max_q_len >= 4)
+                                     neighbours=ctx.decode_tail_start >= split // 2 and ctx.max_q_len >= 4, context_bound=ctx.context_bound)
         elif split > 0:
             seqs, keys = ctx.decode_tail_seq, ctx.portion_keys
             scratch = self.rt.scratch("int4_expanded", ops.prefill_int4_scratch_ints(seqs, keys, self.nkv, self.hd), torch.int32)

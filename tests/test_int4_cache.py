@@ -218,4 +218,4 @@ def test_records_are_as_long_as_the_launchers_read():
     """sizeof of the C records, which the sources assert."""
     from stride_b200.csrc import ops
     assert {n: r.size for n, r in ops._RECORDS.items()} == {"stride_head_write": 160, "stride_int4_read": 80, "stride_int4_prefill": 176,
-                                                            "stride_attention_int4_exact": 144, "stride_decode_int4": 160}
+                                                            "stride_attention_int4_exact": 152, "stride_decode_int4": 160}

@@ -260,6 +260,36 @@ def test_exact_attention(ops, nq, nkv, hd, page, rules, dtype):
     ops.paged_attention_int4(q.cuda(), nq * hd + 3, again, *pages, table, seq.cuda(), pos.cuda(), nq, nkv, hd, page, hd ** -0.5, window, softcap, gpu(sinks),
                              gpu(slopes), neighbours=True)
     assert torch.equal(out, again)                          # rows of several requests side by side: only the time differs
+    for neighbours in (False, True):
+        for bound in (1, 5000):                             # one CTA for a row's keys, eight of them
+            again = torch.full_like(out, 9.0)
+            ops.paged_attention_int4(q.cuda(), nq * hd + 3, again, *pages, table, seq.cuda(), pos.cuda(), nq, nkv, hd, page, hd ** -0.5, window, softcap,
+                                     gpu(sinks), gpu(slopes), neighbours, bound)
+            assert torch.equal(out, again)
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("hd", [64, 112, 160])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=str)
+def test_exact_attention_over_rounds_of_streams(ops, dtype, hd, window):
+    """1900 keys: each of the eight streams comes round more than seven times; a portion of 70 rows, and rows of two requests in one tile."""
+    nq, nkv, page = 10, 2, 48
+    lengths = [1900, 517]
+    pages, table, (k, v) = made_cache(9, lengths, nkv, hd, page)
+    at = [(0, p) for p in range(1830, 1900)] + [(1, 516), (0, 255), (0, 256), (1, 0), (-1, 0), (1, 300)]
+    seq, pos = (torch.tensor(c, dtype=torch.int32) for c in zip(*at))
+    q = torch.randn(len(at), nq * hd, generator=torch.Generator().manual_seed(5)).to(dtype)
+    sinks = torch.randn(nq, generator=torch.Generator().manual_seed(6))
+    outs = []
+    for neighbours in (False, True):
+        for bound in (1, 5000):
+            outs.append(torch.full((len(at), nq * hd), 9.0, dtype=dtype, device="cuda"))
+            ops.paged_attention_int4(q.cuda(), nq * hd, outs[-1], *pages, table, seq.cuda(), pos.cuda(), nq, nkv, hd, page, hd ** -0.5, window, 0.0,
+                                     sinks.cuda(), None, neighbours, bound)
+    want, largest, value = plain.attention(q.view(-1, nq, hd), k, v, pos, seq, hd ** -0.5, window, 0.0, sinks, None)
+    check(outs[0].view(-1, nq, hd), want, score_error(hd, largest), 1900, value, dtype)
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
     ops.check_kernel_status()
 
 
