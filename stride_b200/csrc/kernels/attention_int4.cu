@@ -6,9 +6,10 @@
 // joined in order. So every sum depends on p alone: a token's result has the same bits in a whole prompt, in a portion or alone, on
 // whatever pages, and eight CTAs can work on a row at once.
 //
-// Tensor cores have no 32-bit products, so 4 q d operations a key and head go through the FMA units, whose rate bounds a long prompt: 2048 rows
-// of 32 heads of 128 take 2.79 ms, 25 TFLOP/s of the causal half's 69 GFLOP. A few rows are bound by the chain of their keys: 2 portions of 50
-// rows at 1000 keys, 12 heads of 64, 38 us (102 without the streams side by side), one row at 8000 keys 110 us (707).
+// Tensor cores have no 32-bit products, so the 4 hd operations a row, head and key go through the FMA units. What bounds a long prompt is shared
+// memory: every key is read from it once a warp, for the warp's rows. 2048 rows of 32 heads of 128 take 2.28 ms, 15 TFLOP/s. A few rows are
+// bound by the chain of their keys: 2 portions of 50 rows at 1000 keys, 12 heads of 64, 38 us (102 without the streams side by side), one row
+// at 8000 keys 110 us (707).
 #include "int4_cache.cuh"
 
 namespace stride {
@@ -470,6 +471,9 @@ static int launch_tiles_of(const Int4Attention& a) {
     const long long keys = a.window > 0 ? min(a.window, a.bound) : a.bound;
     const long long ctas = static_cast<long long>((a.tokens + tile - 1) / tile) * a.nkv * ((a.nq / a.nkv + kTileHeads - 1) / kTileHeads);
     if (keys > 4 * kStretch && keys > ctas) return a.neighbours ? launch_tiles<T, G, 4, 8, 2, kStreams>(a) : launch_tiles<T, G, 1, 4, 1, kStreams>(a);
+    // Eight rows a CTA, four to a warp, where that still leaves four CTAs an SM: a key read from shared memory meets twice the rows (2048 rows in a
+    // prompt 2794 / 2276 us, 8 x 100 at 700 364 / 359, but 32 x 16 at 200 with 512 CTAs 35 / 41).
+    if (a.neighbours && ctas >= 8 * 148) return launch_tiles<T, G, 8, 8, 4, 1>(a);
     return a.neighbours ? launch_tiles<T, G, 4, 8, 2, 1>(a) : launch_tiles<T, G, 1, 4, 1, 1>(a);
 }
 

@@ -269,6 +269,28 @@ def test_exact_attention(ops, nq, nkv, hd, page, rules, dtype):
     ops.check_kernel_status()
 
 
+def test_exact_attention_of_a_long_prompt_has_the_bits_of_its_portions(ops):
+    """1190 rows of 16 key heads: enough for eight rows a CTA; a last tile of six; against portions of other sizes and rows alone."""
+    nq, nkv, hd, page, n = 16, 16, 64, 16, 1190
+    pages, table, (k, v) = made_cache(12, [n], nkv, hd, page)
+    q = torch.randn(n, nq * hd, generator=torch.Generator().manual_seed(8)).cuda()
+    pos, seq = torch.arange(n, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+
+    def run(lo, hi, **cut):
+        into = torch.full((hi - lo, nq * hd), 9.0, device="cuda")
+        ops.paged_attention_int4(q[lo:hi], nq * hd, into, *pages, table, seq[lo:hi], pos[lo:hi], nq, nkv, hd, page, hd ** -0.5, **cut)
+        return into
+
+    out = run(0, n)
+    for lo, hi in ((0, 37), (500, 503), (1100, n)):
+        assert torch.equal(run(lo, hi), out[lo:hi])
+        assert torch.equal(run(lo, hi, neighbours=False, context_bound=1), out[lo:hi])
+    some = [0, 31, 32, 255, 256, 257, 700, n - 1]
+    want, largest, value = plain.attention(q.cpu()[some].view(-1, nq, hd), k, v, pos.cpu()[some], seq.cpu()[some], hd ** -0.5)
+    check(out[some].view(-1, nq, hd), want, score_error(hd, largest), n, value, torch.float32)
+    ops.check_kernel_status()
+
+
 @pytest.mark.parametrize("window", [0, 300])
 @pytest.mark.parametrize("hd", [64, 112, 160])
 @pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=str)
