@@ -2157,8 +2157,9 @@ def qk_norm_rope_write(qkv, bias, q_norm, k_norm, eps: float, positions, slot_ma
 
 def rope_kv_write_int4(qkv, bias, q_norm, k_norm, eps: float, positions, slot_mapping, cos, sin, k_pages, v_pages, nq: int, nkv: int, hd: int,
                        page_size: int, rotate: bool = True, q_out=None) -> None:
-    """``qk_norm_rope_write`` into pages held in 4 bits, uint8 [num_pages, nkv, page_size, int4_row_bytes(hd)]: an entry is rounded once, to a
-    sixteenth of the range of its group of 32. A token with a key or value that is not finite reads as no number in that key head."""
+    """``qk_norm_rope_write`` into pages held in 4 bits, uint8 [num_pages, nkv, page_size, int4_row_bytes(hd)]: an entry is rounded once, to
+    the nearest of sixteen numbers over the range of its group of 32. A token with a key or value that is no number, or not below 2^64, reads as
+    no number in that key head."""
     _head_write("rope_kv_write_int4", True, qkv, bias, q_norm, k_norm, eps, positions, slot_mapping, cos, sin, k_pages, v_pages, nq, nkv, hd, page_size,
                 rotate, q_out)
 
