@@ -8,13 +8,11 @@
 //
 // Tensor cores have no 32-bit products, so the 4 hd operations a row, head and key go through the FMA units. What bounds a long prompt is shared
 // memory: every key is read from it once a warp, for the warp's rows. 2048 rows of 32 heads of 128 take 2.28 ms, 15 TFLOP/s. A few rows are
-// bound by the chain of their keys: 2 portions of 50 rows at 1000 keys, 12 heads of 64, 38 us (102 without the streams side by side), one row
+// bound by the chain of their keys: 2 portions of 50 rows at 1000 keys, 12 heads of 64, 38 us (103 without the streams side by side), one row
 // at 8000 keys 110 us (707).
 #include "int4_cache.cuh"
 
 namespace stride {
-
-constexpr int kExactWarps = 4;
 
 constexpr int kStreams = 8, kStretch = 32, kRound = kStreams * kStretch;
 
@@ -46,109 +44,10 @@ __device__ __forceinline__ int request_of(int seq, int pos, int table_rows, int 
     return -1;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kExactWarps * 32)
-attention_int4_exact_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, const uint8_t* __restrict__ k_pages,
-                            const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table, int table_rows, int table_width,
-                            const int32_t* __restrict__ seq_of_token, const int32_t* __restrict__ positions, int nq, int nkv, int hd, int page_size,
-                            float scale, int window, float softcap, const float* __restrict__ sinks, const float* __restrict__ slopes, int* status) {
-    pdl_trigger();
-    pdl_wait();
-    __shared__ float q_smem[kExactWarps][four::kMaxHeadDim];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.x, head = blockIdx.y * kExactWarps + warp;
-    if (head >= nq) return;
-    const int G = four::groups_of(hd), bytes = four::row_bytes(hd);
-    T* out_row = out + (static_cast<size_t>(t) * nq + head) * hd;
-    const int pos = positions[t], kvh = head / (nq / nkv), seq = request_of(seq_of_token[t], pos, table_rows, table_width, page_size, status);
-    if (seq < 0) {      // a padded token of a fixed-size batch
-        for (int d = lane; d < hd; d += 32) out_row[d] = from_f32<T>(0.f);
-        return;
-    }
-    const int first = window > 0 ? max(0, pos - window + 1) : 0;
-    const int32_t* table = block_table + static_cast<size_t>(seq) * table_width;
-    float* qs = q_smem[warp];
-    const T* q_row = q + static_cast<size_t>(t) * q_stride + static_cast<size_t>(head) * hd;
-    for (int d = lane; d < 32 * G; d += 32) qs[d] = d < hd ? to_f32(q_row[d]) : 0.f;
-    __syncwarp();
-
-    const float slope = slopes ? slopes[head] : 0.f;
-    float M = -INFINITY, L = 0.f, A[four::kMaxGroups];
-#pragma unroll
-    for (int j = 0; j < four::kMaxGroups; ++j) A[j] = 0.f;
-    for (int stream = 0; stream < kStreams; ++stream) {
-        float m = -INFINITY, l = 0.f, acc[four::kMaxGroups];
-#pragma unroll
-        for (int j = 0; j < four::kMaxGroups; ++j) acc[j] = 0.f;
-        for (int index = 0, begin = stream_begin(first, stream); stream_key(begin, index) <= pos; index += 32) {
-            const int key = stream_key(begin, index) + lane;
-            bool ok = key >= first && key <= pos;
-            size_t row = 0;
-            if (ok) {
-                const int index = key / page_size, page = index < table_width ? table[index] : -1;
-                if (page < 0 || page >= num_pages) {
-                    four::complain(status, four::kCodeNoPage);
-                    ok = false;
-                } else {
-                    row = ((static_cast<size_t>(page) * nkv + kvh) * page_size + key % page_size) * bytes;
-                }
-            }
-            float s = -INFINITY;
-            if (ok) {
-                const uint32_t* words = reinterpret_cast<const uint32_t*>(k_pages + row);
-                float dot = 0.f;
-                for (int g = 0; g < G; ++g) {
-                    const uint32_t p = words[4 * G + g];
-                    const float gs = four::bf16_low(p), gc = four::bf16_high(p);
-                    for (int a = 0; a < 4; ++a) {
-                        const uint32_t w = words[a * G + g];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) dot = fmaf(qs[32 * g + 8 * a + i], four::value_of(w >> (4 * i) & 15u, gs, gc), dot);
-                    }
-                }
-                s = dot * scale;
-                if (softcap > 0.f) s = softcap * tanhf(s / softcap);
-                if (slopes) s = __fadd_rn(s, -__fmul_rn(slope, static_cast<float>(pos - key)));
-            }
-            unsigned valid = __ballot_sync(0xffffffffu, ok);
-            if (!valid) continue;
-            const float m_new = fmaxf(m, warp_max(s));
-            const float p = ok ? expf(s - m_new) : 0.f;
-            const float corr = expf(m - m_new);
-            l = l * corr + warp_sum(p);
-#pragma unroll
-            for (int j = 0; j < four::kMaxGroups; ++j) acc[j] *= corr;
-            for (; valid; valid &= valid - 1) {
-                const int from = __ffs(valid) - 1;
-                const float pj = __shfl_sync(0xffffffffu, p, from);
-                const uint8_t* v_row = v_pages + __shfl_sync(0xffffffffu, row, from);
-#pragma unroll
-                for (int j = 0; j < four::kMaxGroups; ++j)
-                    if (j < G) {
-                        const uint32_t n = static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(v_row)[(lane >> 2) * G + j]) >> (4 * (lane & 3)) & 15u;
-                        const uint32_t params = reinterpret_cast<const uint32_t*>(v_row + 16 * G)[j];
-                        acc[j] = fmaf(pj, four::value_of(n, four::bf16_low(params), four::bf16_high(params)), acc[j]);
-                    }
-            }
-            m = m_new;
-        }
-        join(M, L, A, m, l, acc);
-    }
-    if (sinks) {
-        const float sink = sinks[head], m_new = fmaxf(M, sink), corr = expf(M - m_new);
-        L = L * corr + expf(sink - m_new);
-#pragma unroll
-        for (int j = 0; j < four::kMaxGroups; ++j) A[j] *= corr;
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;         // 0: no key had a page
-#pragma unroll
-    for (int j = 0; j < four::kMaxGroups; ++j)
-        if (32 * j + lane < hd) out_row[32 * j + lane] = from_f32<T>(A[j] * inv);
-}
-
-// The same, bit for bit, for head sizes up to 128, with 32 keys and values at a time in shared memory as the numbers they stand for: one CTA, or a
-// cluster of eight, one a stream, owns TQ consecutive rows and up to kTileHeads query heads of one key head, a warp NR of those (row, head)
-// pairs. A key is taken apart once for all of them instead of once each, and what the next 32 hold is on its way while these are worked
-// through. The streams of a pair meet in the shared memory of one of the CTAs, each of which joins an eighth of the pairs.
+// 32 keys and values at a time lie in shared memory as the numbers they stand for: one CTA, or a cluster of eight, one a stream, owns TQ consecutive
+// rows and up to kTileHeads query heads of one key head, a warp NR of those (row, head) pairs. A key is taken apart once for all of them
+// instead of once each, and what the next 32 hold is on its way while these are worked through. The streams of a pair meet in the shared
+// memory of one of the CTAs, each of which joins an eighth of the pairs.
 __device__ __forceinline__ void store_cluster(uint32_t local, uint32_t rank, float x) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
@@ -473,22 +372,24 @@ static int launch_tiles_of(const Int4Attention& a) {
     if (keys > 4 * kStretch && keys > ctas) return a.neighbours ? launch_tiles<T, G, 4, 8, 2, kStreams>(a) : launch_tiles<T, G, 1, 4, 1, kStreams>(a);
     // Eight rows a CTA, four to a warp, where that still leaves four CTAs an SM: a key read from shared memory meets twice the rows (2048 rows in a
     // prompt 2794 / 2276 us, 8 x 100 at 700 364 / 359, but 32 x 16 at 200 with 512 CTAs 35 / 41).
-    if (a.neighbours && ctas >= 8 * 148) return launch_tiles<T, G, 8, 8, 4, 1>(a);
+    if constexpr (G <= 4)           // (the registers' sake)
+        if (a.neighbours && ctas >= 8 * 148) return launch_tiles<T, G, 8, 8, 4, 1>(a);
     return a.neighbours ? launch_tiles<T, G, 4, 8, 2, 1>(a) : launch_tiles<T, G, 1, 4, 1, 1>(a);
 }
 
 template <typename T>
-static int launch_exact(const Int4Attention& a, int ctas_y) {
+static int launch_exact(const Int4Attention& a) {
     switch (four::groups_of(a.hd)) {
         case 1: return launch_tiles_of<T, 1>(a);
         case 2: return launch_tiles_of<T, 2>(a);
         case 3: return launch_tiles_of<T, 3>(a);
         case 4: return launch_tiles_of<T, 4>(a);
+        case 5: return launch_tiles_of<T, 5>(a);
+        case 6: return launch_tiles_of<T, 6>(a);
+        case 7: return launch_tiles_of<T, 7>(a);
+        case 8: return launch_tiles_of<T, 8>(a);
     }
-    stride::launch(attention_int4_exact_kernel<T>, dim3(a.tokens, ctas_y), dim3(kExactWarps * 32), 0, a.stream, static_cast<const T*>(a.q), a.q_stride,
-                   static_cast<T*>(a.out), a.k_pages, a.v_pages, a.num_pages, a.block_table, a.table_rows, a.table_width, a.seq_of_token, a.positions, a.nq, a.nkv,
-                   a.hd, a.page_size, a.scale, a.window, a.softcap, a.sinks, a.slopes, a.status);
-    return STRIDE_LAUNCH_STATUS();
+    return STRIDE_UNSUPPORTED;
 }
 
 // A key whose page is none of the cache's is left out, and the status word says so.
@@ -497,10 +398,8 @@ extern "C" int stride_attention_int4_exact(const void* record) {
     if (a.tokens < 0 || a.nq <= 0 || a.nkv <= 0 || a.hd <= 0 || a.page_size <= 0 || a.table_width <= 0 || a.table_rows <= 0 || a.num_pages <= 0 || a.window < 0 ||
         a.softcap < 0.f || a.nq % a.nkv)
         return STRIDE_BAD_ARGUMENT;
-    const int ctas_y = (a.nq + kExactWarps - 1) / kExactWarps;
-    if (a.hd > four::kMaxHeadDim || ctas_y > 65535 || (reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4)
-        return STRIDE_UNSUPPORTED;
+    if (a.hd > four::kMaxHeadDim || (reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4) return STRIDE_UNSUPPORTED;
     if (a.tokens == 0) return 0;
-    if (a.dtype == STRIDE_DTYPE_F32) return launch_exact<float>(a, ctas_y);
-    return a.dtype == STRIDE_DTYPE_BF16 ? launch_exact<__nv_bfloat16>(a, ctas_y) : STRIDE_BAD_ARGUMENT;
+    if (a.dtype == STRIDE_DTYPE_F32) return launch_exact<float>(a);
+    return a.dtype == STRIDE_DTYPE_BF16 ? launch_exact<__nv_bfloat16>(a) : STRIDE_BAD_ARGUMENT;
 }

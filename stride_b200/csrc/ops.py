@@ -229,7 +229,11 @@ _RECORDS = {
 
 def _launch(name: str, what: str, *args) -> None:
     """Calls a launcher of ``_RECORDS``; None stands for no address."""
-    _check(_fn(name)(_RECORDS[name].pack(*args)), what)
+    try:
+        record = _RECORDS[name].pack(*args)
+    except (_struct.error, OverflowError) as e:
+        raise KernelError(f"{what}: a number does not fit the launch ({e})") from None
+    _check(_fn(name)(record), what)
 
 
 def _fn(name: str, what: str | None = None):
@@ -2138,6 +2142,8 @@ def _head_write(what: str, bits4: bool, qkv, bias, q_norm, k_norm, eps, position
         if q_out.get_device() != device:
             raise KernelError("q_out must live on qkv's device")
         out = q_out.data_ptr()
+        if out < rows + qkv.nbytes and rows < out + (tokens * stride * qkv.itemsize) and (out != rows or stride != width):
+            raise KernelError("q_out must be the queries of qkv or lie apart from it")
     k, v, pages = _pages_args(k_pages, v_pages, nkv, page_size, int4_row_bytes(hd) if bits4 else hd, device, torch.uint8 if bits4 else dtype)
     _launch("stride_head_write", what, rows, out, _here_opt(bias, "bias", device, width), _here_opt(q_norm, "q_norm", device, hd),
             _here_opt(k_norm, "k_norm", device, hd), _covers(positions, "positions", device, tokens),

@@ -219,3 +219,10 @@ def test_records_are_as_long_as_the_launchers_read():
     from stride_b200.csrc import ops
     assert {n: r.size for n, r in ops._RECORDS.items()} == {"stride_head_write": 160, "stride_int4_read": 80, "stride_int4_prefill": 176,
                                                             "stride_attention_int4_exact": 152, "stride_decode_int4": 160}
+
+
+@pytest.mark.parametrize("number", [2 ** 31, -2 ** 31 - 1])
+def test_numbers_that_no_launch_holds_are_refused(number):
+    from stride_b200.csrc import ops
+    with pytest.raises(ops.KernelError, match="read_int4: a number does not fit"):
+        ops._launch("stride_int4_read", "read_int4", 0, 0, 0, 0, 0, 0, 0, number, 1, 64, 16, 1, 0)

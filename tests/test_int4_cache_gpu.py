@@ -157,6 +157,23 @@ def test_groups_without_a_range_and_tokens_that_are_no_numbers(ops):
 
 
 @pytest.mark.parametrize("bits4", [False, True])
+@pytest.mark.parametrize("columns", [(64, 320), (256, 512)])
+def test_rows_for_queries_among_those_of_the_call_are_refused(ops, bits4, columns):
+    """A block of qkv other than its queries is still to be read when queries are written."""
+    nq, nkv, hd, page = 4, 2, 64, 4
+    qkv = torch.zeros(3, (nq + 2 * nkv) * hd, dtype=BF16, device="cuda")
+    row = ops.int4_row_bytes(hd) if bits4 else hd
+    pages = [torch.zeros(2, nkv, page, row, dtype=torch.uint8 if bits4 else BF16, device="cuda") for _ in "kv"]
+    at = torch.zeros(3, dtype=torch.int32, device="cuda")
+    angles = torch.zeros(8, hd // 2, device="cuda")
+    call = ops.rope_kv_write_int4 if bits4 else ops.qk_norm_rope_write
+    with pytest.raises(ops.KernelError, match="lie apart"):
+        call(qkv, None, None, None, 1e-5, at, None, angles, angles, *pages, nq, nkv, hd, page, q_out=qkv[:, columns[0]:columns[1]])
+    call(qkv, None, None, None, 1e-5, at, None, angles, angles, *pages, nq, nkv, hd, page, q_out=qkv[:, :nq * hd])
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("bits4", [False, True])
 @pytest.mark.parametrize("q_out", [torch.zeros(3, 255, dtype=BF16), torch.zeros(3, 256), torch.zeros(2, 256, dtype=BF16), torch.zeros(256, 3, dtype=BF16).t(),
                                    torch.zeros(3, 2, 128, dtype=BF16)])
 def test_refused_rows_for_queries(ops, bits4, q_out):
@@ -292,7 +309,7 @@ def test_exact_attention_of_a_long_prompt_has_the_bits_of_its_portions(ops):
 
 
 @pytest.mark.parametrize("window", [0, 300])
-@pytest.mark.parametrize("hd", [64, 112, 160])
+@pytest.mark.parametrize("hd", [64, 112, 160, 200, 256])
 @pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=str)
 def test_exact_attention_over_rounds_of_streams(ops, dtype, hd, window):
     """1900 keys: each of the eight streams comes round more than seven times; a portion of 70 rows, and rows of two requests in one tile."""
