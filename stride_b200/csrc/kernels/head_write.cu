@@ -4,9 +4,9 @@
 // Everything is 32-bit between the load and the store: a query, key or value is rounded once, to the element type or to 4 bits.
 //
 // Every row is read and written once, and nothing is reduced over more than a head, so the bytes are the floor: 2048 tokens of 32 + 8 heads of 128
-// in bfloat16 move 51 MB, 7.9 us; the launch takes 13.9 us. Its loads come from L2 or memory with a single item in flight a lane group: the
-// warps wait for them (long_scoreboard), instruction issue at 62 %. In 4 bits the same tokens with norms and a bias take 16 us: the extra
-// time is the search of each group's extremes and the rounding. A step of 64 tokens takes 2.5 us, a launch's latency.
+// in bfloat16 move 51 MB, 7.9 us; the launch takes 11.4 us. Its loads come from L2 or memory with a single item in flight a lane group, so warps
+// wait for them, and instructions issue in 60 % of the cycles. In 4 bits the same tokens with norms and a bias take 14.5 us: the extra time
+// is the search of each group's extremes and the rounding. A step of 64 tokens takes 2.3 us, a launch's latency.
 #include "int4_cache.cuh"
 
 namespace stride {
@@ -36,7 +36,7 @@ static_assert(sizeof(HeadWrite) == 160, "the record that the caller packs");
 
 // A warp a unit: a query head, or a key head with its value head. Lane l holds entry 32 j + l of the head in x[j], so a group of 32 is
 // one register of the warp. The form for every even head size: its loads are 2 or 4 bytes a lane, and where the one below can run it takes three
-// times as long (a prompt of 2048 tokens 42 us for 14, in 4 bits 81 with the read back for 24); 333 tokens of 32 bits with heads of 96 take 4.3.
+// times as long (a prompt of 2048 tokens 42 us for 11, in 4 bits 81 with the read back for 22); 333 tokens of 32 bits with heads of 96 take 4.3.
 template <typename T, bool FOUR>
 __global__ void __launch_bounds__(kWriteWarps * 32) head_write_kernel(const HeadWrite a) {
     pdl_trigger();
@@ -171,8 +171,9 @@ __global__ void __launch_bounds__(kWriteWarps * 32) head_write_kernel(const Head
 // The same for head sizes 64, 128 and 256: HD / 8 lanes a head, a lane owns four neighbouring entries of either half, so the pairs that turn
 // together meet in one lane, a group of 32 is eight neighbouring lanes, and loads and stores are 8 (bfloat16) or 16 bytes. HD / 8 lanes take
 // an item: kQueries query heads of a token, or kPairs of its key heads with their values, whose loads are all under way, beside the position's and
-// the slot's, before the first is worked on; the angles are read once an item. Four query heads an item: 21 us with one, 13.6 with four (2048
-// tokens, 32 + 8 heads of 128); two pairs of keys and values instead of one are slower, for their registers.
+// the slot's, before the first is worked on; angles and weights are read once an item. 2048 tokens of 32 + 8 heads of 128: 21 us with one query
+// head an item, 14.3 with two, 11.4 with four, 12.5 with eight; two pairs of keys and values are slower than one, for their registers. CTAs of
+// 128 threads, nine an SM: 256 threads, five an SM, take 12.9, 64 threads 12.3.
 template <typename T>
 struct Four;
 template <>
@@ -194,20 +195,20 @@ struct Four<__nv_bfloat16> {
     }
 };
 
-constexpr int kItemThreads = 256, kQueries = 4, kPairs = 1;
+constexpr int kItemThreads = 128, kQueries = 4, kPairs = 1;
 
 template <typename T, bool FOUR, int HD>
-__global__ void __launch_bounds__(kItemThreads, 5) head_write_vec_kernel(const HeadWrite a) {
+__global__ void __launch_bounds__(kItemThreads, 9) head_write_vec_kernel(const HeadWrite a) {
     constexpr int L = HD / 8, HALF = HD / 2, G = HD / 32;
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31, i = threadIdx.x % L, heads = a.nq + 2 * a.nkv;
     const uint32_t mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u) << (lane / L * L);       // the lanes of this item
-    const int q_items = (a.nq + kQueries - 1) / kQueries, kv_items = (a.nkv + kPairs - 1) / kPairs;
-    long long item = static_cast<long long>(blockIdx.x) * (kItemThreads / L) + threadIdx.x / L;
-    const bool is_q = item < static_cast<long long>(a.tokens) * q_items;
-    if (!is_q) item -= static_cast<long long>(a.tokens) * q_items;
-    const int per = is_q ? q_items : kv_items, t = static_cast<int>(item / per), u0 = static_cast<int>(item % per);   // heads u0, u0 + per, ...
+    const uint32_t q_items = (a.nq + kQueries - 1) / kQueries, kv_items = (a.nkv + kPairs - 1) / kPairs;
+    uint32_t item = blockIdx.x * (kItemThreads / L) + threadIdx.x / L;             // (the launch sees to it that items fit 31 bits)
+    const bool is_q = item < a.tokens * q_items;
+    if (!is_q) item -= a.tokens * q_items;
+    const int per = is_q ? q_items : kv_items, t = item / static_cast<uint32_t>(per), u0 = item - t * per;      // heads u0, u0 + per, ...
     if (t >= a.tokens) return;
     const T* row = static_cast<const T*>(a.rows) + static_cast<size_t>(t) * heads * HD + 4 * i;
     const int pos = a.rotate ? a.positions[t] : 0;
@@ -237,8 +238,17 @@ __global__ void __launch_bounds__(kItemThreads, 5) head_write_vec_kernel(const H
             for (int e = 0; e < 4; ++e) x[h][e] = __fadd_rn(x[h][e], b[e]);
         }
     };
-    auto norm_and_turn = [&](float (&x)[2][4], const float* weight) {
-        if (weight != nullptr) {
+    float w[2][4];
+    auto weights = [&](const float* from) {     // once an item: behind a head's store they would be read again
+#pragma unroll
+        for (int h = 0; h < 2 && from != nullptr; ++h) {
+            Four<float> of;
+            of.load(from + h * HALF + 4 * i);
+            of.get(w[h]);
+        }
+    };
+    auto norm_and_turn = [&](float (&x)[2][4], bool norm) {
+        if (norm) {
             float sum = 0.f;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -246,16 +256,11 @@ __global__ void __launch_bounds__(kItemThreads, 5) head_write_vec_kernel(const H
                 for (int e = 0; e < 4; ++e) sum = fmaf(x[h][e], x[h][e], sum);
 #pragma unroll
             for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
-            const float inv = rsqrtf(__fadd_rn(__fdiv_rn(sum, static_cast<float>(HD)), a.eps));
+            const float inv = rsqrtf(__fadd_rn(__fmul_rn(sum, 1.f / HD), a.eps));       // (HD is a power of two: the quotient's bits)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                Four<float> of;
-                float w[4];
-                of.load(weight + h * HALF + 4 * i);
-                of.get(w);
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[h][e] = __fmul_rn(__fmul_rn(x[h][e], inv), w[e]);
-            }
+                for (int e = 0; e < 4; ++e) x[h][e] = __fmul_rn(__fmul_rn(x[h][e], inv), w[h][e]);
         }
         if (a.rotate) {
 #pragma unroll
@@ -274,6 +279,7 @@ __global__ void __launch_bounds__(kItemThreads, 5) head_write_vec_kernel(const H
                 in[k][0].load(row + static_cast<size_t>(u0 + k * per) * HD);
                 in[k][1].load(row + static_cast<size_t>(u0 + k * per) * HD + HALF);
             }
+        weights(a.q_norm);
         if (!angles()) return;
         T* out = static_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.q_out_stride + 4 * i;
 #pragma unroll
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(kItemThreads, 5) head_write_vec_kernel(const H
             in[k][0].get(x[0]);
             in[k][1].get(x[1]);
             if (a.bias != nullptr) add_bias(x, u);
-            norm_and_turn(x, a.q_norm);
+            norm_and_turn(x, a.q_norm != nullptr);
             Four<T>::put(out + static_cast<size_t>(u) * HD, x[0]);
             Four<T>::put(out + static_cast<size_t>(u) * HD + HALF, x[1]);
         }
@@ -301,6 +307,7 @@ __global__ void __launch_bounds__(kItemThreads, 5) head_write_vec_kernel(const H
             in[k][2].load(value);
             in[k][3].load(value + HALF);
         }
+    weights(a.k_norm);
     if (place < 0 || !angles()) return;
     const int page = place / a.page_size;
     if (page >= a.num_pages) {
@@ -318,7 +325,7 @@ __global__ void __launch_bounds__(kItemThreads, 5) head_write_vec_kernel(const H
             add_bias(x[0], a.nq + u);
             add_bias(x[1], a.nq + a.nkv + u);
         }
-        norm_and_turn(x[0], a.k_norm);
+        norm_and_turn(x[0], a.k_norm != nullptr);
         const size_t at = (static_cast<size_t>(page) * a.nkv + u) * a.page_size + place % a.page_size;
         if constexpr (!FOUR) {
             T* ko = static_cast<T*>(a.k_pages) + at * HD + 4 * i;
@@ -431,14 +438,14 @@ int4_read_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict_
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
 int4_read_vec_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const int32_t* __restrict__ slots, T* __restrict__ k_out,
-                     T* __restrict__ v_out, long long units, int nkv, int page_size, int num_pages, int* status) {
+                     T* __restrict__ v_out, uint32_t units, int nkv, int page_size, int num_pages, int* status) {
     constexpr int L = HD / 8, HALF = HD / 2, G = HD / 32;
     pdl_trigger();
     pdl_wait();
     const int i = threadIdx.x % L, r = i & 7;
-    const long long unit = static_cast<long long>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+    const uint32_t unit = blockIdx.x * (256 / L) + threadIdx.x / L, token = unit / nkv;
     if (unit >= units) return;
-    const int slot = slots[unit / nkv], kvh = static_cast<int>(unit % nkv);
+    const int slot = slots[token], kvh = unit - token * nkv;
     int page = slot < 0 ? -1 : slot / page_size;
     if (page >= num_pages) {
         if (i == 0) four::complain(status, four::kCodeNoSlot);
@@ -462,10 +469,11 @@ int4_read_vec_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restr
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[q][e] = four::value_of(n[q] >> (4 * e) & 15u, four::bf16_low(p[q]), four::bf16_high(p[q]));
     }
-    Four<T>::put(k_out + unit * HD + 4 * i, y[0]);
-    Four<T>::put(k_out + unit * HD + HALF + 4 * i, y[1]);
-    Four<T>::put(v_out + unit * HD + 4 * i, y[2]);
-    Four<T>::put(v_out + unit * HD + HALF + 4 * i, y[3]);
+    const size_t to = static_cast<size_t>(unit) * HD + 4 * i;
+    Four<T>::put(k_out + to, y[0]);
+    Four<T>::put(k_out + to + HALF, y[1]);
+    Four<T>::put(v_out + to, y[2]);
+    Four<T>::put(v_out + to + HALF, y[3]);
 }
 
 }  // namespace stride
@@ -524,11 +532,11 @@ extern "C" int stride_int4_read(const void* record) {
     const bool aligned = (reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) % 16 == 0;
     if (aligned && (a.hd == 64 || a.hd == 128 || a.hd == 256)) {
         const int rows = 2048 / a.hd;       // of a CTA of 256 threads
-        if ((units + rows - 1) / rows > 2147483647LL) return STRIDE_UNSUPPORTED;
+        if (units > 2147483647LL) return STRIDE_UNSUPPORTED;
         const dim3 grid(static_cast<unsigned>((units + rows - 1) / rows));
 #define STRIDE_READ(T_, HD_)                                                                                                                       \
     stride::launch(int4_read_vec_kernel<T_, HD_>, grid, dim3(256), 0, a.stream, a.k_pages, a.v_pages, a.slots, static_cast<T_*>(a.k_out),           \
-                   static_cast<T_*>(a.v_out), units, a.nkv, a.page_size, a.num_pages, a.status)
+                   static_cast<T_*>(a.v_out), static_cast<uint32_t>(units), a.nkv, a.page_size, a.num_pages, a.status)
         if (a.dtype == STRIDE_DTYPE_F32)
             a.hd == 64 ? STRIDE_READ(float, 64) : a.hd == 128 ? STRIDE_READ(float, 128) : STRIDE_READ(float, 256);
         else
