@@ -18,12 +18,16 @@
 // * The query is scaled by a power of two to below 2^15. The reference R of a weight 2^(score - R) is the running maximum of score + log2 of the
 //   token's largest scale or centre, so that what is rounded to 16 bits lies below 2^8 and its largest near 1 whatever the values' size; R moves
 //   only when a product passes 2^8 (a vote per tile), and then everything is rescaled.
+// * What falls below 2^-24 is lost in 16-bit floating point, which a group does not notice whose own products reach near 1. The row that R comes
+//   from vouches for them: where its smallest group is within a factor of 64 of its largest, every group has a product of 2^-6. Where it is not
+//   (a value channel that stands out), the products of the second kind run in bfloat16, which has the range, with P s in two parts and the numbers
+//   made whole, until R comes from a row that vouches for its groups again: 64 requests of such values take 121 us for 95.
 //
 // The work of a launch is a row of units, 128 keys of one (token, key head) each, in the order of tokens and key heads; every CTA takes an equal
 // stretch of it (it works out from the positions where its own begins), so requests of any lengths keep all SMs busy to the end and a
 // (token, key head) is cut only where a stretch ends. Parts of one are merged by the CTA that draws its last ticket, in the order of the keys.
 //
-// Measured: 64 requests of up to 8192 keys, 8 key heads of 128, group 4: 345 MB in 93 us, 3.7 TB/s, 0.57 of the copy rate; 8 requests 26 us; one
+// Measured: 64 requests of up to 8192 keys, 8 key heads of 128, group 4: 345 MB in 95 us, 3.6 TB/s, 0.56 of the copy rate; 8 requests 26 us; one
 // request of 2048 keys 9.6 us. What bounds a full batch is the instructions between the copies and the products: 168 registers let three warps
 // run on a scheduler, which issue in 0.50 of the cycles and wait for their own last instruction in most others; of a warp's cycles on 32
 // keys 700 go to the scores, 350 to the softmax, 880 to the values, 230 to waiting for copies. Whole units instead of equal stretches took 97
@@ -51,6 +55,7 @@ constexpr int kCodeBeyondBound = 32;    // as in attention_decode.cu
 constexpr int kCodeCopyWait = 81;       // a wait for a tile's copies ran out
 constexpr float kLimit = 256.f;         // what a weight's product with a scale may reach before R moves
 constexpr float kMostWeight = 1.1529215e18f;    // 2^60, what a weight may (its product with a centre, below 2^64, stays a number)
+constexpr float kMostUneven = 64.f;     // how far apart the groups of a row may be for 16-bit floating point
 constexpr float kLeastLog = -90.f;      // log2 of the least size that R counts: a weight stays below 2^98
 
 struct Decode {
@@ -148,13 +153,26 @@ __device__ __forceinline__ float largest_scale(const uint32_t (&p)[G]) {
     for (int g = 1; g < G; ++g) m = __vmaxu2(m, p[g]);
     return bf16_low(m);
 }
-// log2 of the largest of a row's scales and its centres' sizes, 0 of them counted as 2^kLeastLog.
+// log2 of the largest of a row's scales and its centres' sizes, 0 of them counted as 2^kLeastLog. uneven: some group's lies below it
+// by more than kMostUneven, or all of it below 2^kLeastLog.
 template <int G>
-__device__ __forceinline__ float log2_size(const uint32_t (&p)[G]) {
-    float m = 0.f;
+__device__ __forceinline__ float log2_size(const uint32_t (&p)[G], bool& uneven) {
+    float m = 0.f, least = INFINITY;
 #pragma unroll
-    for (int g = 0; g < G; ++g) m = fmaxf(m, fmaxf(bf16_low(p[g]), fabsf(bf16_high(p[g]))));
-    return fmaxf(__log2f(m), kLeastLog);
+    for (int g = 0; g < G; ++g) {
+        const float size = fmaxf(bf16_low(p[g]), fabsf(bf16_high(p[g])));
+        m = fmaxf(m, size);
+        least = fminf(least, size);
+    }
+    const float log2 = __log2f(m);
+    uneven = !(least * kMostUneven >= m && log2 >= kLeastLog);
+    return fmaxf(log2, kLeastLog);
+}
+// Two numbers in 16-bit halves under 0x000f000f, times `by` (a power of two up to 16), in bfloat16: 128 + n is exact there, and so are both steps.
+__device__ __forceinline__ uint32_t whole_numbers(uint32_t n, float by) {
+    const uint32_t biased = n | 0x43004300u;
+    const __nv_bfloat162 y = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&biased), __float2bfloat162_rn(by), __float2bfloat162_rn(-128.f * by));
+    return *reinterpret_cast<const uint32_t*>(&y);
 }
 
 // G: groups of a head (head size 32 G). NT: tiles of 8 query heads.
@@ -419,6 +437,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 
     // cen: rows 0 .. G - 1 for the centres, from 4 on for the scales, 8 .. 15 (all alike) for the sum of the weights
     float R[NT][2], o[NT][G][2][4], cen[NT][4];
+    uint32_t uneven_cols = 0;               // bit 2 nt + e: the row that R[nt][e] comes from is uneven (alike in all lanes of a column)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         R[nt][0] = R[nt][1] = -INFINITY;
@@ -532,13 +551,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                 // (R is -inf until a tile with a key; then weights are infinite or, of masked keys, no numbers)
                 if (__any_sync(0xffffffffu, !(product <= kLimit && weight <= kMostWeight))) {
                     float size[2][2];
+                    bool uneven[2][2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t vp[2][G];
                         load_words<G>(vp[0], at + (2 + h) * HALF + row_a * ROW + 16 * G);
                         load_words<G>(vp[1], at + (2 + h) * HALF + row_b * ROW + 16 * G);
-                        size[h][0] = log2_size<G>(vp[0]);
-                        size[h][1] = log2_size<G>(vp[1]);
+                        size[h][0] = log2_size<G>(vp[0], uneven[h][0]);
+                        size[h][1] = log2_size<G>(vp[1], uneven[h][1]);
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -550,6 +570,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                                 most = x[nt][h][2 * r + e] == -INFINITY ? most : fmaxf(most, fmaf(x[nt][h][2 * r + e], unit[nt][e], size[h][r]));
 #pragma unroll
                         for (int s = 4; s < 32; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+                        bool from_uneven = false;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+                                from_uneven = from_uneven || (uneven[h][r] && fmaf(x[nt][h][2 * r + e], unit[nt][e], size[h][r]) >= most);
+                        const uint32_t lanes = __ballot_sync(0xffffffffu, from_uneven) & 0x11111111u << c, bit = 1u << (2 * nt + e);
+                        if (most > R[nt][e] && 8 * nt + 2 * c + static_cast<int>(e) < group) uneven_cols = lanes ? uneven_cols | bit : uneven_cols & ~bit;
                         const float next = fmaxf(R[nt][e], most), by = R[nt][e] == -INFINITY ? 0.f : exp2_quick(R[nt][e] - next);
                         R[nt][e] = next;
                         cen[nt][e] *= by;
@@ -569,6 +597,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                     }
                 }
             }
+            const bool wide = __any_sync(0xffffffffu, uneven_cols != 0u);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const unsigned char* vs = at + (2 + h) * HALF;
@@ -610,6 +639,35 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                     float(&d)[4] = cen[nt];
                     mma_bf16(d, a0, 0x3f803f80u, a2, 0x3f803f80u, high, d[0], d[1], d[2], d[3]);
                     mma_bf16(d, a0, 0x3f803f80u, a2, 0x3f803f80u, low, d[0], d[1], d[2], d[3]);
+                }
+                if (wide) {                         // P s 2^-24 in two parts of 8 bits beside whole numbers: the same units
+#pragma unroll
+                    for (int grp = 0; grp < G; ++grp) {
+                        const uint32_t x0 = __byte_perm(vw[0][grp >> 1], vw[1][grp >> 1], grp & 1 ? 0x7632 : 0x5410),
+                                       x1 = __byte_perm(vw[2][grp >> 1], vw[3][grp >> 1], grp & 1 ? 0x7632 : 0x5410), y0 = x0 >> 8, y1 = x1 >> 8;
+                        const float s0 = bf16_low(vp[0][grp]), s1 = bf16_low(vp[1][grp]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const float y[4] = {P[nt][h][0] * s0 * 5.9604644775390625e-08f, P[nt][h][1] * s0 * 5.9604644775390625e-08f,
+                                                P[nt][h][2] * s1 * 5.9604644775390625e-08f, P[nt][h][3] * s1 * 5.9604644775390625e-08f};
+                            float rest[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) rest[e] = y[e] - bf16_high(__float_as_uint(y[e]));
+                            const uint32_t parts[2][2] = {{transposed(__byte_perm(__float_as_uint(y[0]), __float_as_uint(y[1]), 0x7632)),
+                                                           transposed(__byte_perm(__float_as_uint(y[2]), __float_as_uint(y[3]), 0x7632))},
+                                                          {transposed(pack_bf16(rest[0], rest[1])), transposed(pack_bf16(rest[2], rest[3]))}};
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const uint32_t u0 = k ? y0 : x0, u1 = k ? y1 : x1;
+                                const uint32_t n0 = whole_numbers(u0 & 0x000f000fu, 1.f), n1 = whole_numbers(u0 >> 4 & 0x000f000fu, 16.f),
+                                               n2 = whole_numbers(u1 & 0x000f000fu, 1.f), n3 = whole_numbers(u1 >> 4 & 0x000f000fu, 16.f);
+                                float(&d)[4] = o[nt][grp][k];
+                                mma_bf16(d, n0, n1, n2, n3, parts[0], d[0], d[1], d[2], d[3]);
+                                mma_bf16(d, n0, n1, n2, n3, parts[1], d[0], d[1], d[2], d[3]);
+                            }
+                        }
+                    }
+                    continue;
                 }
 #pragma unroll
                 for (int grp = 0; grp < G; ++grp) {

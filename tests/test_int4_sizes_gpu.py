@@ -1,0 +1,88 @@
+"""Attention over a cache held in 4 bits where sizes differ: groups of a row, rows of a cache, queries."""
+
+import pytest
+import torch
+
+import plain_int4 as plain
+
+pytestmark = pytest.mark.gpu
+BF16, F64 = torch.bfloat16, torch.float64
+HALF_STEP = 2.0 ** -8                   # of a bfloat16 result, relative
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from stride_b200.csrc import ops
+    ops.check_kernel_status()
+    yield ops
+    ops.check_kernel_status()
+
+
+def cache_of(keys, values, page):
+    """Pages of one request's keys and values [n, nkv, hd], its table, and what the pages stand for (float64)."""
+    n, nkv, hd = keys.shape
+    count = -(-n // page)
+    pages, stored = [], []
+    for which, x in (("k", keys), ("v", values)):
+        rows = plain.pack(which, *plain.quantise(x.float()))
+        stored.append(plain.unpack(which, rows, hd))
+        full = torch.full((count * page, nkv, rows.shape[-1]), 255, dtype=torch.uint8)
+        full[:n] = rows
+        pages.append(full.view(count, page, nkv, -1).transpose(1, 2).contiguous().cuda())
+    return pages, torch.arange(count, dtype=torch.int32, device="cuda")[None], stored
+
+
+def decode(ops, q, pages, table, n, nq, nkv, hd, page):
+    out = torch.empty(q.shape[0], nq * hd, dtype=BF16, device="cuda")
+    at = torch.full((q.shape[0],), n - 1, dtype=torch.int32, device="cuda")
+    scratch = torch.zeros(ops.decode_int4_scratch_floats(q.shape[0], nq, nkv, hd, n), device="cuda")
+    ops.paged_attention_decode_int4(q.cuda(), nq * hd, out, *pages, table, torch.zeros_like(at), at, scratch, nq, nkv, hd, page, hd ** -0.5, 0, n)
+    return out.view(-1, nq, hd).double().cpu()
+
+
+def group_errors(got, want):
+    """Of every group of 32 of every head: the error's norm over the result's."""
+    return ((got - want).unflatten(-1, (-1, 32)).norm(dim=-1) / want.unflatten(-1, (-1, 32)).norm(dim=-1)).amax()
+
+
+def positive(g, *shape):
+    """Values that do not cancel: a sum of them with weights is as large as they are."""
+    return 0.5 + torch.rand(*shape, generator=g)
+
+
+SHAPES = [(8, 2, 128, 16), (16, 1, 64, 16), (3, 1, 128, 5), (4, 1, 64, 32)]
+
+
+@pytest.mark.parametrize("large", [0, 1])
+@pytest.mark.parametrize("log_ratio", [4, 9, 12, 16, 20, 24, 40])
+@pytest.mark.parametrize("nq,nkv,hd,page", SHAPES)
+def test_decode_of_values_whose_groups_differ_in_size(ops, nq, nkv, hd, page, log_ratio, large):
+    n, g = 500, torch.Generator().manual_seed(hd + log_ratio)
+    values = positive(g, n, nkv, hd)
+    values[..., 32 * large:32 * large + 32] *= 2.0 ** log_ratio
+    pages, table, (k, v) = cache_of(torch.randn(n, nkv, hd, generator=g), values, page)
+    q = torch.randn(2, nq * hd, generator=g).to(BF16)
+    want, _l, _v = plain.attention(q.view(2, nq, hd), [k], [v], torch.tensor([n - 1] * 2), torch.tensor([0, 0]), hd ** -0.5)
+    # the result's rounding; a weight's, 2^-11 of its product with a scale, and what it drops below 2^-24 of the largest such product, times
+    # the numbers up to 15, where a row's groups are so near in size that 16-bit floating point takes them (a factor of 64)
+    floor = 15 * n * 2.0 ** (log_ratio - 25) if log_ratio <= 6 else 0.0
+    assert group_errors(decode(ops, q, pages, table, n, nq, nkv, hd, page), want) <= HALF_STEP + 2.0 ** -10 + floor
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("weight", [0.0, 3.0])
+@pytest.mark.parametrize("at", [0, 3, 130, 299])
+@pytest.mark.parametrize("nq,nkv,hd,page", SHAPES)
+def test_decode_beside_one_token_with_a_group_that_stands_out(ops, nq, nkv, hd, page, at, weight):
+    """One value's first group is 2^20 times the others'; what the rest of the head holds comes from all tokens."""
+    n, g = 300, torch.Generator().manual_seed(hd + at)
+    keys, values = 0.3 * torch.randn(n, nkv, hd, generator=g), positive(g, n, nkv, hd)
+    values[at, :, :32] *= 2.0 ** 20
+    q = torch.randn(1, nq * hd, generator=g).to(BF16)
+    keys[at] += weight * q.float().view(nkv, nq // nkv, hd).mean(1) / hd ** 0.5
+    pages, table, (k, v) = cache_of(keys, values, page)
+    want, _l, _v = plain.attention(q.view(1, nq, hd), [k], [v], torch.tensor([n - 1]), torch.tensor([0]), hd ** -0.5)
+    assert group_errors(decode(ops, q, pages, table, n, nq, nkv, hd, page), want) <= HALF_STEP + 2.0 ** -10
+    ops.check_kernel_status()
