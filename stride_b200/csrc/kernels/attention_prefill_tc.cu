@@ -49,26 +49,33 @@ namespace stride {
 // The keys of the first num_seqs requests of a cache held in 4 bits (int4_cache.cuh) as pages of 64 in 16-bit floating point, for the attention of
 // portions: a request's pages one after the other, the requests' too, and the table that says so. A key is expanded once for all query tiles
 // that read it, which costs little beside them: 8192 keys of 8 heads of 128 take 14 us, 2,048 queries' attention to them 295, and what it writes,
-// 34 MB, is read back from L2 (no byte of it reached memory in a profile of 4096 keys). The format has 11 bits where bfloat16 has 8, which an entry's place between two of its sixteen numbers
-// needs; an entry beyond its range, 65504, counts as that. CTA (page, key head).
-__device__ __forceinline__ uint32_t pack_half_in_range(float lo, float hi) {
+// 34 MB, is read back from L2 (no byte of it reached memory in a profile of 4096 keys). The format has 11 bits where bfloat16 has 8, which an entry's place
+// between two of its sixteen numbers needs, but few exponents: the keys of a page are multiplied by the power of two that brings the largest of
+// their entries near 2^15, the values by another, and the attention takes both off again. So an entry keeps 11 bits down to 2^-29 of the
+// page's largest, and the rest of them down to 2^-40. CTA (page, key head).
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {        // (an infinity stays one, and what is no number)
     uint32_t y;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
     return y;
 }
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {        // (a NaN stays one)
-    return pack_half_in_range(fabsf(lo) > 65504.f ? copysignf(65504.f, lo) : lo, fabsf(hi) > 65504.f ? copysignf(65504.f, hi) : hi);
-}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }      // -126 .. 127
+// e, so that x 2^-e lies in [2^14, 2^15), where that is one of -112 .. most.
+__device__ __forceinline__ int half_exponent(float x, int most) { return max(-112, min(most, static_cast<int>(__float_as_uint(x) >> 23) - 127 - 14)); }
+constexpr int kMostEntry = 60, kMostQuery = 112;        // (entries lie below 2^64)
+struct WidePage {                   // of a page and key head
+    int keys, values;               // the exponents
+};
 constexpr int kExpandKeys = 64, kExpandThreads = 256;
 
 template <int G>
 __global__ void __launch_bounds__(kExpandThreads)
 int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, int num_pages, const int32_t* __restrict__ block_table,
                    int table_width, const int32_t* __restrict__ q_len, const int32_t* __restrict__ ctx_len, int num_seqs, int nkv, int page_size,
-                   int window, uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int32_t* __restrict__ table_out, int out_pages,
-                   int* status) {
+                   int window, uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out,
+                   int32_t* __restrict__ table_out, int out_pages, WidePage* __restrict__ about, int* status) {
     constexpr int HD = 32 * G, BYTES = 20 * G;
     __shared__ size_t row_at[kExpandKeys];
+    __shared__ float most[kExpandThreads / 32];
     pdl_wait();
     pdl_trigger();          // the attention reads the requests' lengths before it waits: only now are they what the kernels before made them
     int seq = -1, index = 0, at = 0;                        // this page is number `index` of request `seq`
@@ -104,6 +111,25 @@ int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restric
         row_at[threadIdx.x] = row;
     }
     __syncthreads();
+    {       // no entry exceeds |c| + 8 s of its group: the first half of the threads look through the keys, the other through the values, two to a row
+        const int i = threadIdx.x & 127, r = i >> 1;
+        float x = 0.f;
+        if (row_at[r] != ~size_t(0)) {
+            const uint32_t* params = reinterpret_cast<const uint32_t*>((threadIdx.x < 128 ? k_pages : v_pages) + row_at[r] + 16 * G);
+#pragma unroll
+            for (int g = 0; g < G / 2; ++g) {       // (fmaxf passes by what is no number)
+                const uint32_t p = params[(i & 1) * (G / 2) + g];
+                x = fmaxf(x, fmaf(8.f, four::bf16_low(p), fabsf(four::bf16_high(p))));
+            }
+        }
+        x = warp_max(x);
+        if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = x;
+    }
+    __syncthreads();
+    const int k_exponent = half_exponent(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), kMostEntry);
+    const int v_exponent = half_exponent(fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])), kMostEntry);
+    const float k_by = power_of_two(-k_exponent), v_by = power_of_two(-v_exponent);
+    if (threadIdx.x == 0) about[static_cast<size_t>(blockIdx.x) * nkv + kvh] = {k_exponent, v_exponent};
     const size_t out_row = (static_cast<size_t>(blockIdx.x) * nkv + kvh) * kExpandKeys;
     // a key without a page (before the windows, behind the end) becomes zeros: attention masks it
     for (int i = threadIdx.x; i < kExpandKeys * 4; i += kExpandThreads) {           // keys: part a of a row, 8 entries of every group
@@ -115,7 +141,7 @@ int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restric
             uint4 out = make_uint4(0, 0, 0, 0);
             if (there) {
                 const uint32_t w = words[a * G + g], p = words[4 * G + g];
-                const float s = four::bf16_low(p), c = four::bf16_high(p);
+                const float s = four::bf16_low(p) * k_by, c = four::bf16_high(p) * k_by;
                 uint32_t pair[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -135,7 +161,7 @@ int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restric
             uint2 out = make_uint2(0, 0);
             if (there) {
                 const uint32_t w = reinterpret_cast<const uint16_t*>(row)[a * G + g], p = reinterpret_cast<const uint32_t*>(row + 16 * G)[g];
-                const float s = four::bf16_low(p), c = four::bf16_high(p);
+                const float s = four::bf16_low(p) * v_by, c = four::bf16_high(p) * v_by;
                 out = make_uint2(pack_half(four::value_of(w & 15u, s, c), four::value_of(w >> 4 & 15u, s, c)),
                                  pack_half(four::value_of(w >> 8 & 15u, s, c), four::value_of(w >> 12, s, c)));
             }
@@ -167,9 +193,19 @@ constexpr long long kStaggerCycles = 1000;
 // for two CTAs per SM, and the scores run two tiles ahead, which hides the one stage. An optional gate (LatentGate) multiplies the
 // result. 2,048 tokens of 16 heads: 42 us, beside 20 us for the product that expands (moe_tc.cu) and 4 us for the
 // gather; on the latents themselves (latent_attention_tc.cu and two products a head) 745 + 24 + 19 us.
-// F16: keys and values are 16-bit floating point of 11 bits, as the expanded form of a cache held in 4 bits has them (at the end of this file).
-// Both operands of a product are of one type, so the softmax warps turn the query tiles, bfloat16 in the projection's output, in place
-// (a query beyond 65504 counts as that, one below 2^-14 loses bits that a score does not show) and write P so.
+// F16: keys and values are 16-bit floating point of 11 bits, as the expanded form of a cache held in 4 bits has them (in front of this kernel).
+// Both operands of a product are of one type, so the softmax warps turn the query tiles, bfloat16 in the projection's output, in place,
+// every row times the power of two that brings its largest entry near 2^15. That and the exponent of a tile's keys go into the factor of its raw
+// scores. The exponent of its values goes into the scores that the reference m_ref is taken from, and into P: what is rounded to 16 bits is
+// a weight times the size of the values it meets, at most 2^8 times its reference and 2^kLift on top, so that what falls below 2^-32 of the
+// reference is lost and nothing else, whatever the values' size. The sum of the weights is kept without it, in units of 2^kSumUnit: beside
+// values of 2^-98 a weight may reach 2^120.
+struct WideCache {                      // F16 alone
+    const WidePage* about;              // of the expanded pages [table_width, nkv]
+    int out_rows;                       // rows of q and out
+};
+constexpr int kLift = 7;                // (2^15 in all: the largest number is 65504)
+constexpr int kSumUnit = 40;
 struct LatentGate {
     const __nv_bfloat16* values;        // null: none
     int ld, per_output;                 // row stride; one number an output (else one a head)
@@ -184,7 +220,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                        const int32_t* __restrict__ q_len, const int32_t* __restrict__ ctx_len, int num_seqs, int nq, int nkv,
                        int page_shift, float scale_log2e, int window, float cap_in, const float* __restrict__ sinks,
                        const float* __restrict__ slopes, const float* __restrict__ rel, int rel_len, int* __restrict__ status,
-                       const __grid_constant__ CUtensorMap map_q2, const __grid_constant__ CUtensorMap map_k2, LatentGate gate, int q2_stride, int out_rows) {
+                       const __grid_constant__ CUtensorMap map_q2, const __grid_constant__ CUtensorMap map_k2, LatentGate gate, int q2_stride, WideCache wide) {
     static_assert(!LATENT || (HEADS == 1 && TMA_KV && !REL), "the latent form");
     constexpr int HALVES = HD / 64;                       // 64-column boxes per row
     constexpr int HALF_BYTES = kQRows * 128;              // a [128 rows x 64 columns] bf16 box of Q
@@ -241,7 +277,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int n_tiles = last_pos / kKeys - kt_first + 1;
     const int q_row0 = q_start[seq] + row0;                // row of the projection output that holds query 0 of this tile
     const int32_t* table = LATENT ? nullptr : block_table + static_cast<size_t>(seq) * table_width;
-    if (F16 && (q_start[seq] < 0 || static_cast<long long>(q_start[seq]) + n_q > out_rows || n_q > ctx_len[seq])) {     // rows that are not the output's, or keys that are not there
+    if (F16 && (q_start[seq] < 0 || static_cast<long long>(q_start[seq]) + n_q > wide.out_rows || n_q > ctx_len[seq])) {     // rows that are not the output's, or keys that are not there
         if (threadIdx.x == 0) four::complain(status, four::kCodeTooManyKeys);
         return;
     }
@@ -470,16 +506,36 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         };
         uint32_t sr[64];                                     // the scores of the row, requested one tile ahead
         bool ok = true;
+        int q_exponent = 0;
+        WidePage tile = {0, 0}, next_tile = {0, 0};          // F16: of the tile that is worked on, and the one after
+        const WidePage* about = nullptr;                     // of the first tile's page; a request's pages lie side by side
+        int pages_there = 0;
         if constexpr (F16) {
+            const int page = kt_first < table_width ? table[kt_first] : -1;
+            pages_there = page < 0 ? 0 : table_width - page; // (a request whose keys found no room may have any page here)
+            about = wide.about + static_cast<size_t>(max(page, 0)) * nkv + kvh;
+            if (pages_there > 0) tile = *about;
             ok = mbar_wait(smem_u32(&q_full), 0, status, 23);
-            if (ok) {
-                for (int i = threadIdx.x - SERVICE_WARPS * 32; i < HEADS * Q_BYTES / 16; i += 128 * HEADS) {
-                    uint4* at = reinterpret_cast<uint4*>(q_s) + i;
-                    uint4 w = *at;
-                    uint32_t* p = &w.x;
+            if (ok) {       // a thread turns its row; chunks in an order that lets eight rows be read at once (they are swizzled, which does not matter here)
+                unsigned char* q_row = q_s + hh * Q_BYTES + row * 128;
+                auto chunk = [&](int i) { return reinterpret_cast<uint4*>(q_row + (i >> 3) * HALF_BYTES + (((i ^ row) & 7) << 4)); };
+                uint4 w[HALVES * 8];
+                uint32_t most = 0u;                          // sizes of bfloat16 numbers order as integers do
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[e] = pack_half(four::bf16_low(p[e]), four::bf16_high(p[e]));
-                    *at = w;
+                for (int i = 0; i < HALVES * 8; ++i) {
+                    w[i] = *chunk(i);
+                    const uint32_t* p = &w[i].x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) most = __vmaxu2(most, p[e] & 0x7fff7fffu);
+                }
+                q_exponent = half_exponent(__uint_as_float(max(most << 16, most & 0xffff0000u)), kMostQuery);
+                const float by = power_of_two(-q_exponent);
+#pragma unroll
+                for (int i = 0; i < HALVES * 8; ++i) {
+                    uint32_t* p = &w[i].x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = pack_half(four::bf16_low(p[e]) * by, four::bf16_high(p[e]) * by);
+                    *chunk(i) = w[i];
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -497,6 +553,18 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const int st = j & 1;
             const int k0 = (kt_first + j) * kKeys;
             const uint32_t tmem_sj = tmem_s + st * kKeys + lane_base;
+            // what raw scores are multiplied by for units of log2 (a cap takes them out of their raw units), a cap's and a slope's share of it
+            float unit = scale_log2e, cap_unit = cap_in, slope_unit = slope_raw, lean = 0.f;
+            if constexpr (F16) {
+                const int e = max(-80, min(100, q_exponent + tile.keys));       // (beyond it scores are below 2^-40, or no 32-bit numbers)
+                cap_unit = cap_in * power_of_two(e);
+                if (cap_in == 0.f) {
+                    unit = fmaxf(scale_log2e * power_of_two(e), 1.17549435e-38f);
+                    slope_unit = slope_raw * power_of_two(-e);
+                }
+                lean = static_cast<float>(tile.values);
+                next_tile = j + 1 < pages_there ? about[static_cast<size_t>(j + 1) * nkv] : WidePage{0, 0};
+            }
             tmem_ld64_wait(sr);
             const bool edge = k0 + kKeys - 1 > pos0 || (window > 0 && k0 <= last_pos - window);   // some (row, key) is masked
             float sv[64];                                    // raw scores; a masked one is -inf
@@ -504,15 +572,15 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             for (int i = 0; i < 64; ++i) sv[i] = __uint_as_float(sr[i]);
             if (cap_in > 0.f) {     // capped scores: c tanh(scale s / c); scale_log2e then holds c log2(e)
 #pragma unroll
-                for (int i = 0; i < 64; ++i) sv[i] = tanh_approx(sv[i] * cap_in);
+                for (int i = 0; i < 64; ++i) sv[i] = tanh_approx(sv[i] * cap_unit);
             } else if (!REL && cap_in < 0.f) {      // the same, tanh in 32-bit accuracy (not beside a table of distances)
 #pragma unroll
-                for (int i = 0; i < 64; ++i) sv[i] = tanh_quick(sv[i] * -cap_in);
+                for (int i = 0; i < 64; ++i) sv[i] = tanh_quick(sv[i] * -cap_unit);
             }
             if (slopes != nullptr) {
                 const float d0 = static_cast<float>(k0 - pos_r);
 #pragma unroll
-                for (int i = 0; i < 64; ++i) sv[i] = fmaf(slope_raw, d0 + static_cast<float>(i), sv[i]);
+                for (int i = 0; i < 64; ++i) sv[i] = fmaf(slope_unit, d0 + static_cast<float>(i), sv[i]);
             }
             if (REL) {
                 if (pos0 - (k0 + kKeys - 1) >= rel_len - 1) {
@@ -539,7 +607,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
                     for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], sv[i + 2 * c], sv[i + 2 * c + 1]);
                 }
-                mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale_log2e;   // the scale is positive
+                mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * unit;   // the scale is positive
+                if (F16) mx += lean;
             }
             const bool grow = mx > m_ref + kRescaleThreshold;      // also true for the first finite maximum
             if (__any_sync(0xffffffffu, grow)) {
@@ -564,19 +633,21 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             {
                 // A masked score is -inf and gives exactly 0. A row that has seen no key yet has m_ref = -inf and
                 // only masked scores: subtract 0 there, or -inf - -inf would make a NaN.
-                const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+                const float neg_m = m_ref == -INFINITY ? 0.f : (F16 ? lean + static_cast<float>(kLift) : 0.f) - m_ref;
                 float l4[4] = {0.f, 0.f, 0.f, 0.f};       // independent partial sums
                 float packed[32];             // bfloat16 pairs, carried as 32-bit words: P's columns hold two keys each
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
-                    const float p0 = ex2_approx(fmaf(sv[i], scale_log2e, neg_m));
-                    const float p1 = ex2_approx(fmaf(sv[i + 1], scale_log2e, neg_m));
+                    const float p0 = ex2_approx(fmaf(sv[i], unit, neg_m));
+                    const float p1 = ex2_approx(fmaf(sv[i + 1], unit, neg_m));
                     l4[(i / 2) & 3] += p0 + p1;
-                    packed[i / 2] = __uint_as_float(F16 ? pack_half_in_range(p0, p1) : pack_bf16(p0, p1))       /* at most 2^8 */;
+                    packed[i / 2] = __uint_as_float(F16 ? pack_half(p0, p1) : pack_bf16(p0, p1));
                 }
                 tmem_st32(tmem_sj, packed);   // over S columns 0-31, all of which have been read
-                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                const float sum = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                l = F16 ? fmaf(sum, power_of_two(-kLift - kSumUnit - tile.values), l) : l + sum;
             }
+            if (F16) tile = next_tile;
             // The scores of the next tile were issued two tiles ago: ask for them now, so that they travel while this
             // tile is handed over.
             if (j + 1 < n_tiles) {
@@ -612,9 +683,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         tc_fence_after();
         if (ok) {
             // a sink joins the denominator: exp(sink - m), with m in log2 units
-            if (sinks != nullptr && m_ref != -INFINITY) l += ex2_approx(fmaf(sinks[head], 1.4426950408889634f, -m_ref));
+            if (sinks != nullptr && m_ref != -INFINITY) l += ex2_approx(fmaf(sinks[head], 1.4426950408889634f, -m_ref - (F16 ? static_cast<float>(kSumUnit) : 0.f)));
             // tcgen05.ld is a warp-wide instruction: rows past the portion's end take part and store nothing
-            const float inv = 1.f / l;
+            const float inv = F16 ? power_of_two(-kLift - kSumUnit) / l : 1.f / l;
             __nv_bfloat16* dst = out + (static_cast<size_t>(q_row0 + row) * nq + head) * HD;
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) {
@@ -653,12 +724,11 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     if (warp == MMA_WARP) tmem_dealloc(tmem_base_slot, TMEM_COLS);
 }
 
-// F16: rel is null and rel_len the rows of the output.
 template <int HD, int HEADS, bool F16 = false>
 int launch_attn(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const __nv_bfloat16* k_pages, const __nv_bfloat16* v_pages, __nv_bfloat16* out,
                 const int32_t* block_table, int table_width, const int32_t* q_start, const int32_t* q_len, const int32_t* ctx_len,
                 int num_seqs, int max_tiles, int nq, int nkv, int page_shift, float scale, int window, float softcap,
-                const float* sinks, const float* slopes, const float* rel, int rel_len, int* status, cudaStream_t stream) {
+                const float* sinks, const float* slopes, const float* rel, int rel_len, int* status, cudaStream_t stream, const WideCache& wide = {}) {
     constexpr int stages = HEADS == 1 ? 2 : 4;
     constexpr int smem = (HD / 64) * (HEADS * kQRows * 128 + 2 * stages * kKeys * 128) + 1024;      // Q tiles, key ring, value ring
     static bool configured[64] = {};        // the shared-memory limit is set per kernel and device
@@ -670,7 +740,7 @@ int launch_attn(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtens
         stride::launch(attn_prefill_tc_kernel<HD, HEADS, true, false, false, true>, dim3(nq / HEADS, max_tiles), dim3(HEADS == 1 ? 256 : 512), smem, stream,
                        *map_q, *map_k, *map_v, k_pages, v_pages, out, block_table, table_width, q_start, q_len, ctx_len, num_seqs, nq, nkv, page_shift,
                        (softcap != 0.f ? fabsf(softcap) : scale) * 1.4426950408889634f, window, softcap != 0.f ? scale / softcap : 0.f, sinks, slopes,
-                       nullptr, 0, status, *map_q, *map_q, LatentGate{}, 0, rel_len);
+                       nullptr, 0, status, *map_q, *map_q, LatentGate{}, 0, wide);
         return STRIDE_LAUNCH_STATUS();
     }
     if (!configured[device]) {
@@ -691,7 +761,7 @@ int launch_attn(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtens
     stride::launch(kernel, grid, block, smem, stream, *map_q, tma ? *map_k : *map_q, tma ? *map_v : *map_q, k_pages, v_pages, out,
                    block_table, table_width, q_start, q_len, ctx_len, num_seqs, nq, nkv, page_shift,
                    (softcap != 0.f ? fabsf(softcap) : scale) * 1.4426950408889634f, window, softcap != 0.f ? scale / softcap : 0.f, sinks, slopes, rel,
-                   rel_len, status, *map_q, *map_q, LatentGate{}, 0, 0);
+                   rel_len, status, *map_q, *map_q, LatentGate{}, 0, wide);
     return STRIDE_LAUNCH_STATUS();
 }
 
@@ -816,7 +886,7 @@ extern "C" int stride_latent_prefill_tc(const void* q, int q_ld, const void* q_r
     if (!map_q || !map_q2 || !map_kv || !map_k2) return STRIDE_UNSUPPORTED;
     stride::launch(kernel, dim3(heads, max_tiles), dim3(256), smem, stream, *map_q, *map_kv, *map_kv, nullptr, nullptr, static_cast<__nv_bfloat16*>(out),
                    nullptr, 0, q_start, q_len, ctx_len, num_seqs, heads, heads, 0, scale * 1.4426950408889634f, 0, 0.f, sinks, nullptr, nullptr, 0,
-                   status, *map_q2, *map_k2, tc::LatentGate{static_cast<const __nv_bfloat16*>(gate), gate_ld, gate_per_output, kv_head_stride, kv_v_off}, q_rot_stride, 0);
+                   status, *map_q2, *map_k2, tc::LatentGate{static_cast<const __nv_bfloat16*>(gate), gate_ld, gate_per_output, kv_head_stride, kv_v_off}, q_rot_stride, tc::WideCache{});
     return STRIDE_LAUNCH_STATUS();
 }
 
@@ -833,7 +903,7 @@ struct Int4Prefill {                // a record that the caller packs
     const int32_t* ctx_len;
     uint16_t* k_wide;               // [wide_pages, nkv, 64, hd]
     uint16_t* v_wide;
-    int32_t* table_wide;            // [num_seqs, wide_pages]
+    int32_t* table_wide;            // [num_seqs, wide_pages], then (at an even place) WidePage [wide_pages, nkv]
     const float* sinks;
     const float* slopes;
     int* status;
@@ -867,9 +937,10 @@ extern "C" int stride_int4_prefill(const void* record) {
     const CUtensorMap* map_k = tc::cached_map(a.k_wide, wide_rows, a.hd, a.hd, tc::kKeys);
     const CUtensorMap* map_v = tc::cached_map(a.v_wide, wide_rows, a.hd, a.hd, tc::kKeys);
     if (!map_q || !map_k || !map_v) return STRIDE_UNSUPPORTED;
+    auto about = reinterpret_cast<WidePage*>(a.table_wide + (static_cast<size_t>(a.num_seqs) * a.wide_pages + 1) / 2 * 2);
     stride::launch(a.hd == 64 ? int4_expand_kernel<2> : int4_expand_kernel<4>, dim3(a.wide_pages, a.nkv), dim3(kExpandThreads), 0, a.stream, a.k_pages,
                    a.v_pages, a.num_pages, a.block_table, a.table_width, a.q_len, a.ctx_len, a.num_seqs, a.nkv, a.page_size, a.window, a.k_wide, a.v_wide,
-                   a.table_wide, a.wide_pages, a.status);
+                   a.table_wide, a.wide_pages, about, a.status);
     const int code = STRIDE_LAUNCH_STATUS();
     if (code) return code;
     const bool pair = (a.nq / a.nkv) % 2 == 0 && pair_heads();
@@ -877,7 +948,7 @@ extern "C" int stride_int4_prefill(const void* record) {
 #define STRIDE_INT4_LAUNCH(HD_, HEADS_)                                                                                                                 \
     tc::launch_attn<HD_, HEADS_, true>(map_q, map_k, map_v, nullptr, nullptr, static_cast<__nv_bfloat16*>(a.out), a.table_wide, a.wide_pages, a.q_start, \
                                        a.q_len, a.ctx_len, a.num_seqs, max_tiles, a.nq, a.nkv, 6, a.scale, a.window, a.softcap, a.sinks, a.slopes, nullptr,    \
-                                       a.tokens, a.status, a.stream)
+                                       0, a.status, a.stream, tc::WideCache{about, a.tokens})
     if (a.hd == 64) return pair ? STRIDE_INT4_LAUNCH(64, 2) : STRIDE_INT4_LAUNCH(64, 1);
     return pair ? STRIDE_INT4_LAUNCH(128, 2) : STRIDE_INT4_LAUNCH(128, 1);
 #undef STRIDE_INT4_LAUNCH

@@ -2260,7 +2260,8 @@ def _int4_expanded_pages(num_seqs: int, keys: int) -> int:
 def prefill_int4_scratch_ints(num_seqs: int, keys: int, nkv: int, hd: int) -> int:
     """int32 elements of scratch that ``paged_attention_prefill_int4`` needs for ``num_seqs`` requests that hold at most ``keys`` keys together."""
     pages = _int4_expanded_pages(num_seqs, keys)
-    return pages * nkv * INT4_EXPANDED_PAGE * hd + num_seqs * pages
+    # keys and values of two bytes; the table of the pages; two exponents of every page and key head
+    return pages * nkv * INT4_EXPANDED_PAGE * hd + (num_seqs * pages + 1) // 2 * 2 + 2 * pages * nkv
 
 
 def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_table, q_start, q_len, ctx_len, scratch, num_seqs: int, keys: int,
@@ -2269,14 +2270,16 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     """``paged_attention_prefill_tc`` over pages held in 4 bits, for the first ``num_seqs`` requests of the step (portions of any length), which own
     the rows of ``out``: bfloat16, head sizes 64 and 128. ``keys``: at least what those requests hold together; ``scratch``: int32, at least
     ``prefill_int4_scratch_ints`` elements, for one stream at a time. The keys and values that the portions see are expanded once, to pages
-    of 64 in 16-bit floating point (a rounding of 2^-11 of an entry at most; 65504 is the largest), and attended to from there."""
+    of 64 in 16-bit floating point, scaled by a power of two for each page and key head (a rounding of 2^-11 of an entry at most, or of
+    2^-40 of the page's largest), and attended to from there. A weight whose product with its page's largest value lies below 2^-32 of the
+    largest such product of the row counts in the denominator alone."""
     device, qp, op, k, v, pages, rows, width, requests = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size,
                                                                               window, softcap, torch.bfloat16)
     if not fast_attention_supported(q.dtype, nq, nkv, hd):
         raise KernelError(f"paged_attention_prefill_int4: {nq} heads of {hd} on {nkv} are not supported (paged_attention_int4 takes them)")
     out_pages = _int4_expanded_pages(num_seqs, keys)
     half = out_pages * nkv * INT4_EXPANDED_PAGE * hd * 2            # bytes of the keys, and of the values
-    if num_seqs < 0 or keys < 0 or 4 * scratch.numel() < 2 * half + 4 * num_seqs * out_pages:
+    if num_seqs < 0 or keys < 0 or scratch.numel() < prefill_int4_scratch_ints(num_seqs, keys, nkv, hd):
         raise KernelError("paged_attention_prefill_int4: the scratch is too small for the requests and keys")
     tokens = out.shape[0]
     if tokens == 0 or num_seqs == 0:

@@ -86,3 +86,70 @@ def test_decode_beside_one_token_with_a_group_that_stands_out(ops, nq, nkv, hd, 
     want, _l, _v = plain.attention(q.view(1, nq, hd), [k], [v], torch.tensor([n - 1]), torch.tensor([0]), hd ** -0.5)
     assert group_errors(decode(ops, q, pages, table, n, nq, nkv, hd, page), want) <= HALF_STEP + 2.0 ** -10
     ops.check_kernel_status()
+
+
+def portion(ops, q, pages, table, n, nq, nkv, hd, page, **rules):
+    """The last q.shape[0] tokens of a request of n keys."""
+    p = q.shape[0]
+    ints = lambda x: torch.tensor([x], dtype=torch.int32, device="cuda")  # noqa: E731
+    out = torch.full((p, nq * hd), 9.0, dtype=BF16, device="cuda")
+    scratch = torch.full((ops.prefill_int4_scratch_ints(1, n, nkv, hd),), -1, dtype=torch.int32, device="cuda")
+    ops.paged_attention_prefill_int4(q.cuda(), nq * hd, out, *pages, table, ints(0), ints(p), ints(n), scratch, 1, n, nq, nkv, hd, page, hd ** -0.5, 0, **rules)
+    return out.view(p, nq, hd).double().cpu()
+
+
+def rows_of(n, p):
+    return torch.arange(n - p, n), torch.zeros(p, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("large", [0, 1])
+@pytest.mark.parametrize("log_ratio", [12, 20, 24])
+@pytest.mark.parametrize("nq,nkv,hd,page", SHAPES)
+def test_portions_of_values_whose_groups_differ_in_size(ops, nq, nkv, hd, page, log_ratio, large):
+    n, p, g = 300, 5, torch.Generator().manual_seed(hd + log_ratio)
+    values = positive(g, n, nkv, hd)
+    values[..., 32 * large:32 * large + 32] *= 2.0 ** log_ratio
+    pages, table, (k, v) = cache_of(0.3 * torch.randn(n, nkv, hd, generator=g), values, page)
+    q = torch.randn(p, nq * hd, generator=g).to(BF16)
+    want, largest, _v = plain.attention(q.view(p, nq, hd), [k], [v], *rows_of(n, p), hd ** -0.5)
+    # the result's rounding, a weight's and a value's of 2^-11, a key's of 2^-11 in every product of a score; of the largest value 2^-40
+    limit = HALF_STEP + 2 * 2.0 ** -11 + 2 * 2.0 ** -11 * largest + 2.0 ** (log_ratio - 40)
+    assert group_errors(portion(ops, q, pages, table, n, nq, nkv, hd, page), want) <= limit
+    ops.check_kernel_status()
+
+
+SIZES = [(1e-6, 1.0, 1.0), (1e-8, 1.0, 1.0), (1e-30, 1e-3, 1e3), (1e5, 1.0, 1.0), (1e15, 1e6, 1e-6), (1.0, 1e-20, 1e20), (3.0, 1e15, 1e-15), (1.0, 1.0, 1e-30),
+         (1e-33, 1e-33, 1e33)]
+
+
+@pytest.mark.parametrize("rules", [dict(), dict(softcap=4.0, precise_cap=True), dict(slopes=True), dict(softcap=4.0, precise_cap=True, slopes=True, sinks=True)], ids=str)
+@pytest.mark.parametrize("of_values,of_keys,of_queries", SIZES)
+@pytest.mark.parametrize("nq,nkv,hd,page", SHAPES[:2])
+def test_portions_of_keys_values_and_queries_of_any_size(ops, nq, nkv, hd, page, of_values, of_keys, of_queries, rules):
+    """Rows of queries of very different sizes beside one another, tokens of different sizes in one head, scores of the usual size."""
+    n, p, g = 200, 130, torch.Generator().manual_seed(7)
+    keys = torch.randn(n, nkv, hd, generator=g, dtype=F64) * of_keys
+    values = positive(g, n, nkv, hd).double() * of_values * torch.logspace(-2, 0, n, dtype=F64)[:, None, None]
+    pages, table, (k, v) = cache_of(keys, values, page)
+    q = torch.randn(p, nq * hd, generator=g, dtype=F64) * of_queries * 0.3
+    q[::2] *= 2.0 ** -20                                    # rows whose scores are all alike
+    q = q.to(BF16)
+    sinks = torch.randn(nq, generator=g) if rules.get("sinks") else None
+    slopes = torch.full((nq,), 0.01) if rules.get("slopes") else None
+    want, largest, _v = plain.attention(q.view(p, nq, hd), [k], [v], *rows_of(n, p), hd ** -0.5, softcap=rules.get("softcap", 0.0), sinks=sinks, slopes=slopes)
+    given = dict(rules, sinks=None if sinks is None else sinks.cuda(), slopes=None if slopes is None else slopes.cuda())
+    got = portion(ops, q, pages, table, n, nq, nkv, hd, page, **given)
+    # as above; the penalty of up to 200 positions of 0.01 in 32 bits counts nothing, the capped score's tanh a few 2^-24 of the cap
+    assert group_errors(got, want) <= HALF_STEP + 2 * 2.0 ** -11 + 2 * 2.0 ** -11 * largest
+    ops.check_kernel_status()
+
+
+def test_a_portion_reads_entries_beyond_the_16_bit_range_as_they_are(ops):
+    """The first token sees itself alone: its result is its value. (The largest number of 16-bit floating point is 65504.)"""
+    n, nq, nkv, hd, page, g = 40, 4, 1, 64, 16, torch.Generator().manual_seed(5)
+    values = torch.randn(n, nkv, hd, generator=g) * 3e4
+    values[0, 0, :4] = torch.tensor([84760.0, -1e5, 1e6, 7e4])
+    pages, table, (k, v) = cache_of(torch.randn(n, nkv, hd, generator=g), values, page)
+    got = portion(ops, torch.randn(n, nq * hd, generator=g).to(BF16), pages, table, n, nq, nkv, hd, page)
+    assert bool(((got[0] - v[0]).abs() <= (HALF_STEP + 2.0 ** -10) * v[0].abs()).all())
+    ops.check_kernel_status()
