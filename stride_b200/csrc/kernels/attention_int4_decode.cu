@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
     pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
+    __shared__ uint32_t copied[kWarps][BULK ? 1 : kStages];         // small copies: the keys of a stage's tile that have a page, a bit each
     __shared__ int warp_sums[kWarps];
     __shared__ int begin_token, begin_units;
     __shared__ Span begin_span;
@@ -358,6 +359,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             size_t row = ~size_t(0);
             const int key = base + lane;
             if (key >= first && key <= pos) row = row_at(key, page_of(key));
+            const uint32_t have = __ballot_sync(0xffffffffu, row != ~size_t(0));
+            if (lane == 0) copied[warp][stage] = have;
             unsigned char* to = ring + stage * STAGE;
 #pragma unroll
             for (int i = 0; i < 5; ++i) {               // 32 rows of 5 pieces
@@ -463,7 +466,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             const unsigned char* at = ring + stage * STAGE;
             const int base = tile_base(j);
             // some key of the tile is behind the token, before its window or without a page: what its row holds counts for nothing
-            const bool edge = halves != 3u || base + kTile - 1 > pos || base < first;
+            const uint32_t there = BULK ? ~0u : copied[warp][stage];
+            const bool edge = halves != 3u || base + kTile - 1 > pos || base < first || there != ~0u;
             float x[NT][2][4], P[NT][2][4], amp[2][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -526,7 +530,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const int key = base + h * kSub + (r ? row_b : row_a);
-                        const bool ok = (halves >> h & 1u) && key <= pos && key >= first;
+                        const bool ok = (halves >> h & 1u) && key <= pos && key >= first && (there >> (key - base) & 1u);
                         seen |= ok ? 1u << (2 * h + r) : 0u;
                         if (!ok) {
                             amp[h][r] = 0.f;
@@ -624,7 +628,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = base + h * kSub + col[i];
-                        if (!(halves >> h & 1u) || key > pos || key < first) vc[i] = 0u;
+                        if (!(halves >> h & 1u) || key > pos || key < first || !(there >> (key - base) & 1u)) vc[i] = 0u;
                     }
                 }
                 const uint32_t a0 = __byte_perm(vc[0], vc[1], pick), a2 = __byte_perm(vc[2], vc[3], pick);

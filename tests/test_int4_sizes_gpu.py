@@ -153,3 +153,52 @@ def test_a_portion_reads_entries_beyond_the_16_bit_range_as_they_are(ops):
     got = portion(ops, torch.randn(n, nq * hd, generator=g).to(BF16), pages, table, n, nq, nkv, hd, page)
     assert bool(((got[0] - v[0]).abs() <= (HALF_STEP + 2.0 ** -10) * v[0].abs()).all())
     ops.check_kernel_status()
+
+
+# ------------------------------------------------------------------------------------------------------- keys without a page
+def without(q, k, v, pos, keep, scale):
+    """Attention of every row to those of its keys that ``keep`` names; zeros where there are none."""
+    p, nq, hd = q.shape
+    nkv = k.shape[1]
+    out = torch.zeros(p, nq, hd, dtype=F64)
+    for t in range(p):
+        on = keep & (torch.arange(k.shape[0]) <= int(pos[t]))
+        for h in range(nq if bool(on.any()) else 0):
+            kv = h // (nq // nkv)
+            out[t, h] = torch.softmax(k[on, kv] @ q[t, h].double() * scale, 0) @ v[on, kv]
+    return out
+
+
+GONE = [[2], [0, 1], [4, 9], "last", "all"]
+
+
+def with_holes(page, gone, entry):
+    n, nq, nkv, hd, g = 190, 4, 2, 64, torch.Generator().manual_seed(page)
+    pages, table, (k, v) = cache_of(torch.randn(n, nkv, hd, generator=g), positive(g, n, nkv, hd), page)
+    at = [table.shape[1] - 1] if gone == "last" else list(range(table.shape[1])) if gone == "all" else sorted({i % table.shape[1] for i in gone})
+    keep = torch.ones(n, dtype=torch.bool)
+    for i in at:
+        table[0, i] = entry
+        keep[i * page:(i + 1) * page] = False
+    q = torch.randn(6, nq * hd, generator=g).to(BF16)
+    want = without(q.view(6, nq, hd), k, v, torch.arange(n - 6, n), keep, hd ** -0.5)
+    return n, nq, nkv, hd, pages, table, q, want
+
+
+def close(got, want):
+    # values between 0.5 and 1.5: the result's rounding, and some 2^-9 for weights and scores of 11 bits
+    assert bool(((got - want).abs() <= HALF_STEP * want.abs() + 2.0 ** -8 * (want != 0)).all()), float((got - want).abs().max())
+
+
+@pytest.mark.parametrize("entry", [-1, 9999])
+@pytest.mark.parametrize("gone", GONE, ids=str)
+@pytest.mark.parametrize("page", [1, 5, 8, 16, 48, 64])
+def test_decode_leaves_out_keys_without_a_page(ops, page, gone, entry):
+    n, nq, nkv, hd, pages, table, q, want = with_holes(page, gone, entry)
+    out = torch.full((6, nq * hd), 9.0, dtype=BF16, device="cuda")
+    at, seq = torch.arange(n - 6, n, dtype=torch.int32, device="cuda"), torch.zeros(6, dtype=torch.int32, device="cuda")
+    scratch = torch.zeros(ops.decode_int4_scratch_floats(6, nq, nkv, hd, n), device="cuda")
+    ops.paged_attention_decode_int4(q.cuda(), nq * hd, out, *pages, table, seq, at, scratch, nq, nkv, hd, page, hd ** -0.5, 0, n)
+    with pytest.raises(ops.KernelError, match="names no page"):
+        ops.check_kernel_status()
+    close(out.view(6, nq, hd).double().cpu(), want)
