@@ -62,9 +62,14 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(st
 // e, so that x 2^-e lies in [2^14, 2^15), where that is one of -112 .. most.
 __device__ __forceinline__ int half_exponent(float x, int most) { return max(-112, min(most, static_cast<int>(__float_as_uint(x) >> 23) - 127 - 14)); }
 constexpr int kMostEntry = 60, kMostQuery = 112;        // (entries lie below 2^64)
-struct WidePage {                   // of a page and key head
-    int keys, values;               // the exponents
+struct __align__(16) WidePage {     // of a page and key head
+    int exponents;                  // of the values, times 2^16, and of the keys, kMostEntry at the most, plus kLost where `there` lacks one
+    uint32_t there[2];              // a bit a key: 0 where the request holds the key and the cache has no page for it
+    int unused;
 };
+constexpr int kLost = 1024;
+__device__ __forceinline__ int values_exponent(int exponents) { return exponents >> 16; }
+__device__ __forceinline__ int keys_exponent(int exponents) { return static_cast<short>(exponents); }
 constexpr int kExpandKeys = 64, kExpandThreads = 256;
 
 template <int G>
@@ -76,6 +81,7 @@ int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restric
     constexpr int HD = 32 * G, BYTES = 20 * G;
     __shared__ size_t row_at[kExpandKeys];
     __shared__ float most[kExpandThreads / 32];
+    __shared__ uint32_t lost[2];
     pdl_wait();
     pdl_trigger();          // the attention reads the requests' lengths before it waits: only now are they what the kernels before made them
     int seq = -1, index = 0, at = 0;                        // this page is number `index` of request `seq`
@@ -101,7 +107,8 @@ int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restric
     if (threadIdx.x < kExpandKeys) {
         const int key = key0 + threadIdx.x;
         size_t row = ~size_t(0);
-        if (key >= first && key < ctx) {
+        const bool wanted = key >= first && key < ctx;
+        if (wanted) {
             const int page = key / page_size < table_width ? block_table[static_cast<size_t>(seq) * table_width + key / page_size] : -1;
             if (page < 0 || page >= num_pages)
                 four::complain(status, four::kCodeNoPage);
@@ -109,6 +116,8 @@ int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restric
                 row = ((static_cast<size_t>(page) * nkv + kvh) * page_size + key % page_size) * BYTES;
         }
         row_at[threadIdx.x] = row;
+        const uint32_t without = __ballot_sync(0xffffffffu, wanted && row == ~size_t(0));
+        if ((threadIdx.x & 31) == 0) lost[threadIdx.x >> 5] = without;
     }
     __syncthreads();
     {       // no entry exceeds |c| + 8 s of its group: the first half of the threads look through the keys, the other through the values, two to a row
@@ -129,9 +138,10 @@ int4_expand_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restric
     const int k_exponent = half_exponent(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), kMostEntry);
     const int v_exponent = half_exponent(fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])), kMostEntry);
     const float k_by = power_of_two(-k_exponent), v_by = power_of_two(-v_exponent);
-    if (threadIdx.x == 0) about[static_cast<size_t>(blockIdx.x) * nkv + kvh] = {k_exponent, v_exponent};
+    if (threadIdx.x == 0)
+        about[static_cast<size_t>(blockIdx.x) * nkv + kvh] = {v_exponent * 65536 + ((k_exponent + (lost[0] | lost[1] ? kLost : 0)) & 0xffff), {~lost[0], ~lost[1]}, 0};
     const size_t out_row = (static_cast<size_t>(blockIdx.x) * nkv + kvh) * kExpandKeys;
-    // a key without a page (before the windows, behind the end) becomes zeros: attention masks it
+    // a key without a row (before the windows, behind the end, without a page) becomes zeros: attention masks it
     for (int i = threadIdx.x; i < kExpandKeys * 4; i += kExpandThreads) {           // keys: part a of a row, 8 entries of every group
         const int r = i >> 2, a = i & 3;
         const bool there = row_at[r] != ~size_t(0);
@@ -180,7 +190,8 @@ constexpr int kServiceRegs = 48, kSoftmaxRegs = 208;     // per thread, after th
 // of what a tile takes them), so that one head's exponentials, which queue for the special-function unit, fall into
 // the other head's loads, maxima and hand-over. Left to themselves both heads run in step and the unit is contended
 // for in one half of the time and idle in the other (measured: 56 us against 50 us for 2,048 tokens).
-constexpr long long kStaggerCycles = 1000;
+// Of 16-bit floating point's tiles, which take longer, half is 1400 (2,048 queries at 8192 keys: 700 cycles 317 us, 1000 309, 1400 301 to 305).
+constexpr long long kStaggerCycles = 1000, kStaggerCyclesF16 = 1400;
 
 // HEADS query heads of one key head per CTA (1 or 2). One head: 4 service warps (keys, products, values, Q) and 4
 // softmax warps, two CTAs per SM. Two heads: 8 service warps (three for keys, products, three for values, Q) and
@@ -507,14 +518,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         uint32_t sr[64];                                     // the scores of the row, requested one tile ahead
         bool ok = true;
         int q_exponent = 0;
-        WidePage tile = {0, 0}, next_tile = {0, 0};          // F16: of the tile that is worked on, and the one after
-        const WidePage* about = nullptr;                     // of the first tile's page; a request's pages lie side by side
-        int pages_there = 0;
+        int window_of = 0;                                   // F16: the exponents of 32 tiles, one a lane
+        int about_at = 0;                                    // the WidePage of the first tile; a request's pages lie side by side
+        auto exponents_at = [&](int at) { return at < table_width * nkv ? wide.about[at].exponents : 0; };
         if constexpr (F16) {
             const int page = kt_first < table_width ? table[kt_first] : -1;
-            pages_there = page < 0 ? 0 : table_width - page; // (a request whose keys found no room may have any page here)
-            about = wide.about + static_cast<size_t>(max(page, 0)) * nkv + kvh;
-            if (pages_there > 0) tile = *about;
+            about_at = page < 0 || page >= table_width ? table_width * nkv : page * nkv + kvh;      // (a request whose keys found no room: anything)
+            window_of = exponents_at(about_at + lane * nkv);
             ok = mbar_wait(smem_u32(&q_full), 0, status, 23);
             if (ok) {       // a thread turns its row; chunks in an order that lets eight rows be read at once (they are swizzled, which does not matter here)
                 unsigned char* q_row = q_s + hh * Q_BYTES + row * 128;
@@ -547,7 +557,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         if (ok) tmem_ld64_issue(tmem_s + lane_base, sr);
         if (hh == 1) {
             const long long t0 = clock64();
-            while (clock64() - t0 < kStaggerCycles) {}
+            while (clock64() - t0 < (F16 ? kStaggerCyclesF16 : kStaggerCycles)) {}
         }
         for (int j = 0; j < n_tiles && ok; ++j) {
             const int st = j & 1;
@@ -555,18 +565,19 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const uint32_t tmem_sj = tmem_s + st * kKeys + lane_base;
             // what raw scores are multiplied by for units of log2 (a cap takes them out of their raw units), a cap's and a slope's share of it
             float unit = scale_log2e, cap_unit = cap_in, slope_unit = slope_raw, lean = 0.f;
+            const int tile = F16 ? __shfl_sync(0xffffffffu, window_of, j & 31) : 0;
+            const bool some_lost = F16 && keys_exponent(tile) > kMostEntry;
             if constexpr (F16) {
-                const int e = max(-80, min(100, q_exponent + tile.keys));       // (beyond it scores are below 2^-40, or no 32-bit numbers)
+                const int e = max(-80, min(100, q_exponent + keys_exponent(tile) - (some_lost ? kLost : 0)));       // (beyond it scores are below 2^-40, or no 32-bit numbers)
                 cap_unit = cap_in * power_of_two(e);
                 if (cap_in == 0.f) {
                     unit = fmaxf(scale_log2e * power_of_two(e), 1.17549435e-38f);
                     slope_unit = slope_raw * power_of_two(-e);
                 }
-                lean = static_cast<float>(tile.values);
-                next_tile = j + 1 < pages_there ? about[static_cast<size_t>(j + 1) * nkv] : WidePage{0, 0};
+                lean = static_cast<float>(values_exponent(tile));
             }
             tmem_ld64_wait(sr);
-            const bool edge = k0 + kKeys - 1 > pos0 || (window > 0 && k0 <= last_pos - window);   // some (row, key) is masked
+            const bool edge = k0 + kKeys - 1 > pos0 || (window > 0 && k0 <= last_pos - window) || some_lost;   // some (row, key) is masked
             float sv[64];                                    // raw scores; a masked one is -inf
 #pragma unroll
             for (int i = 0; i < 64; ++i) sv[i] = __uint_as_float(sr[i]);
@@ -592,7 +603,19 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     for (int i = 0; i < 64; ++i) sv[i] = fmaf(__ldg(rel_h + max(0, min(n0 - i, rel_len - 1))), rel_unit, sv[i]);
                 }
             }
-            if (edge) {
+            if (F16 && edge) {
+                auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };        // a bit for each of the n lowest places
+                const int end = pos_r + 1 - k0, begin = window > 0 ? end - window : 0;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t seen = below(end - 32 * half) & ~below(begin - 32 * half);
+                    if (some_lost) seen &= wide.about[about_at + j * nkv].there[half];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!(seen >> i & 1u)) sv[32 * half + i] = -INFINITY;
+                }
+            }
+            if (!F16 && edge) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i) {
                     const int key = k0 + i;
@@ -645,9 +668,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 tmem_st32(tmem_sj, packed);   // over S columns 0-31, all of which have been read
                 const float sum = (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                l = F16 ? fmaf(sum, power_of_two(-kLift - kSumUnit - tile.values), l) : l + sum;
+                l = F16 ? fmaf(sum, power_of_two(-kLift - kSumUnit - values_exponent(tile)), l) : l + sum;
             }
-            if (F16) tile = next_tile;
+            if (F16 && (j & 31) == 31) window_of = exponents_at(about_at + (j + 1 + lane) * nkv);
             // The scores of the next tile were issued two tiles ago: ask for them now, so that they travel while this
             // tile is handed over.
             if (j + 1 < n_tiles) {
@@ -685,7 +708,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             // a sink joins the denominator: exp(sink - m), with m in log2 units
             if (sinks != nullptr && m_ref != -INFINITY) l += ex2_approx(fmaf(sinks[head], 1.4426950408889634f, -m_ref - (F16 ? static_cast<float>(kSumUnit) : 0.f)));
             // tcgen05.ld is a warp-wide instruction: rows past the portion's end take part and store nothing
-            const float inv = F16 ? power_of_two(-kLift - kSumUnit) / l : 1.f / l;
+            const float inv = F16 ? (l == 0.f ? 0.f : power_of_two(-kLift - kSumUnit) / l) : 1.f / l;     // (0: no key had a page)
             __nv_bfloat16* dst = out + (static_cast<size_t>(q_row0 + row) * nq + head) * HD;
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) {
@@ -903,7 +926,7 @@ struct Int4Prefill {                // a record that the caller packs
     const int32_t* ctx_len;
     uint16_t* k_wide;               // [wide_pages, nkv, 64, hd]
     uint16_t* v_wide;
-    int32_t* table_wide;            // [num_seqs, wide_pages], then (at an even place) WidePage [wide_pages, nkv]
+    int32_t* table_wide;            // [num_seqs, wide_pages], then (at a multiple of 16 bytes) WidePage [wide_pages, nkv]
     const float* sinks;
     const float* slopes;
     int* status;
@@ -918,8 +941,8 @@ static_assert(sizeof(Int4Prefill) == 176, "the record that the caller packs");
 
 // Attention over a cache held in 4 bits for the first `num_seqs` requests of the step, which own the first `tokens` rows of the flat batch: the keys
 // and values that they see are expanded to pages of 64, and attended to from there. wide_pages: at least the sum over the requests of
-// ceil(ctx_len / 64) (else code 36 in the status word). softcap as for stride_paged_prefill_attention_tc. Returns -2 for head sizes other than
-// 64 and 128 and for unaligned rows.
+// ceil(ctx_len / 64) (else code 36 in the status word). A key whose page is none of the cache's is left out, with code 33. softcap as for
+// stride_paged_prefill_attention_tc. Returns -2 for head sizes other than 64 and 128 and for unaligned rows.
 extern "C" int stride_int4_prefill(const void* record) {
     const Int4Prefill a = read_record<Int4Prefill>(record);
     if (a.tokens < 0 || a.num_seqs < 0 || a.nq <= 0 || a.nkv <= 0 || a.page_size <= 0 || a.num_pages <= 0 || a.table_width <= 0 || a.window < 0 ||
@@ -927,7 +950,8 @@ extern "C" int stride_int4_prefill(const void* record) {
         return STRIDE_BAD_ARGUMENT;
     if ((a.hd != 64 && a.hd != 128) || a.nkv > 65535 || a.nq > 65535 || a.q_stride % 8) return STRIDE_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 4 ||
-        (reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.k_wide) | reinterpret_cast<uintptr_t>(a.v_wide)) % 16)
+        (reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.k_wide) | reinterpret_cast<uintptr_t>(a.v_wide) |
+         reinterpret_cast<uintptr_t>(a.table_wide)) % 16)
         return STRIDE_UNSUPPORTED;
     if (a.tokens == 0 || a.num_seqs == 0) return 0;
     const int max_tiles = (a.tokens + tc::kQRows - 1) / tc::kQRows + a.num_seqs;
@@ -937,7 +961,7 @@ extern "C" int stride_int4_prefill(const void* record) {
     const CUtensorMap* map_k = tc::cached_map(a.k_wide, wide_rows, a.hd, a.hd, tc::kKeys);
     const CUtensorMap* map_v = tc::cached_map(a.v_wide, wide_rows, a.hd, a.hd, tc::kKeys);
     if (!map_q || !map_k || !map_v) return STRIDE_UNSUPPORTED;
-    auto about = reinterpret_cast<WidePage*>(a.table_wide + (static_cast<size_t>(a.num_seqs) * a.wide_pages + 1) / 2 * 2);
+    auto about = reinterpret_cast<WidePage*>(a.table_wide + (static_cast<size_t>(a.num_seqs) * a.wide_pages + 3) / 4 * 4);
     stride::launch(a.hd == 64 ? int4_expand_kernel<2> : int4_expand_kernel<4>, dim3(a.wide_pages, a.nkv), dim3(kExpandThreads), 0, a.stream, a.k_pages,
                    a.v_pages, a.num_pages, a.block_table, a.table_width, a.q_len, a.ctx_len, a.num_seqs, a.nkv, a.page_size, a.window, a.k_wide, a.v_wide,
                    a.table_wide, a.wide_pages, about, a.status);

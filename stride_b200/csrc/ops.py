@@ -2260,8 +2260,8 @@ def _int4_expanded_pages(num_seqs: int, keys: int) -> int:
 def prefill_int4_scratch_ints(num_seqs: int, keys: int, nkv: int, hd: int) -> int:
     """int32 elements of scratch that ``paged_attention_prefill_int4`` needs for ``num_seqs`` requests that hold at most ``keys`` keys together."""
     pages = _int4_expanded_pages(num_seqs, keys)
-    # keys and values of two bytes; the table of the pages; two exponents of every page and key head
-    return pages * nkv * INT4_EXPANDED_PAGE * hd + (num_seqs * pages + 1) // 2 * 2 + 2 * pages * nkv
+    # keys and values of two bytes; the table of the pages; exponents and missing keys of every page and key head
+    return pages * nkv * INT4_EXPANDED_PAGE * hd + (num_seqs * pages + 3) // 4 * 4 + 4 * pages * nkv
 
 
 def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_table, q_start, q_len, ctx_len, scratch, num_seqs: int, keys: int,

@@ -202,3 +202,26 @@ def test_decode_leaves_out_keys_without_a_page(ops, page, gone, entry):
     with pytest.raises(ops.KernelError, match="names no page"):
         ops.check_kernel_status()
     close(out.view(6, nq, hd).double().cpu(), want)
+
+
+@pytest.mark.parametrize("entry", [-1, 9999])
+@pytest.mark.parametrize("gone", GONE, ids=str)
+@pytest.mark.parametrize("page", [1, 5, 8, 16, 48, 64])
+def test_portions_leave_out_keys_without_a_page(ops, page, gone, entry):
+    n, nq, nkv, hd, pages, table, q, want = with_holes(page, gone, entry)
+    got = portion(ops, q, pages, table, n, nq, nkv, hd, page)
+    with pytest.raises(ops.KernelError, match="names no page"):
+        ops.check_kernel_status()
+    close(got, want)
+
+
+@pytest.mark.parametrize("gone", GONE, ids=str)
+@pytest.mark.parametrize("page", [5, 16])
+def test_the_exact_kernel_leaves_out_keys_without_a_page(ops, page, gone):
+    n, nq, nkv, hd, pages, table, q, want = with_holes(page, gone, -1)
+    out = torch.full((6, nq * hd), 9.0, dtype=BF16, device="cuda")
+    at, seq = torch.arange(n - 6, n, dtype=torch.int32, device="cuda"), torch.zeros(6, dtype=torch.int32, device="cuda")
+    ops.paged_attention_int4(q.cuda(), nq * hd, out, *pages, table, seq, at, nq, nkv, hd, page, hd ** -0.5)
+    with pytest.raises(ops.KernelError, match="names no page"):
+        ops.check_kernel_status()
+    close(out.view(6, nq, hd).double().cpu(), want)
