@@ -288,7 +288,10 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int n_tiles = last_pos / kKeys - kt_first + 1;
     const int q_row0 = q_start[seq] + row0;                // row of the projection output that holds query 0 of this tile
     const int32_t* table = LATENT ? nullptr : block_table + static_cast<size_t>(seq) * table_width;
-    if (F16 && (q_start[seq] < 0 || static_cast<long long>(q_start[seq]) + n_q > wide.out_rows || n_q > ctx_len[seq])) {     // rows that are not the output's, or keys that are not there
+    // rows that are not the output's, keys that are not there, more keys than there is room for (each a wait on a key tile, so a length far beyond
+    // the room would keep the launch busy for minutes)
+    if (F16 && (q_start[seq] < 0 || static_cast<long long>(q_start[seq]) + n_q > wide.out_rows || n_q > ctx_len[seq] ||
+                ctx_len[seq] > static_cast<long long>(table_width) * kKeys)) {
         if (threadIdx.x == 0) four::complain(status, four::kCodeTooManyKeys);
         return;
     }

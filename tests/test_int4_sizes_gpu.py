@@ -225,3 +225,15 @@ def test_the_exact_kernel_leaves_out_keys_without_a_page(ops, page, gone):
     with pytest.raises(ops.KernelError, match="names no page"):
         ops.check_kernel_status()
     close(out.view(6, nq, hd).double().cpu(), want)
+
+
+@pytest.mark.parametrize("held", [2 ** 31 - 1, 2 ** 30, 64 * 32 + 1])
+def test_a_portion_of_a_request_beyond_the_room_for_its_keys_is_reported_and_not_run(ops, held):
+    n, nq, nkv, hd, pages, table, q, _want = with_holes(16, "last", -1)
+    ints = lambda x: torch.tensor([x], dtype=torch.int32, device="cuda")  # noqa: E731
+    out = torch.full((6, nq * hd), 9.0, dtype=BF16, device="cuda")
+    scratch = torch.zeros(ops.prefill_int4_scratch_ints(1, n, nkv, hd), dtype=torch.int32, device="cuda")       # 32 pages of 64
+    ops.paged_attention_prefill_int4(q.cuda(), nq * hd, out, *pages, table, ints(0), ints(6), ints(held), scratch, 1, n, nq, nkv, hd, 16, 0.125, 0)
+    with pytest.raises(ops.KernelError, match="more keys|names no page"):       # (both are so; the first report stays)
+        ops.check_kernel_status()
+    assert bool((out == 9.0).all())
