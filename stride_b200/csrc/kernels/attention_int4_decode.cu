@@ -835,7 +835,8 @@ template <int G, int NT>
 int launch_decode(const Decode& a, int ctas, cudaStream_t stream) {
     constexpr int smem = kWarps * kStages * 2 * kTile * 20 * G;        // 61 KB at head size 128
     static_assert(kWarps * 8 * NT * (32 * G + 2) * 4 <= smem && 8 * NT * (kMostCtas + 1) * 4 <= smem, "the warps' results and the parts' weights fit into the rings");
-    const bool bulk = a.page_size % kSub == 0;
+    // bulk copies: whole sixteens of keys side by side, from addresses that are multiples of 16 (rows of 40 bytes need not lie so)
+    const bool bulk = a.page_size % kSub == 0 && (reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) % 16 == 0;
     cudaError_t e = allow_shared<decode_kernel<G, NT, true>>(smem);
     if (e == cudaSuccess) e = allow_shared<decode_kernel<G, NT, false>>(smem);
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -884,15 +885,15 @@ static_assert(sizeof(DecodeCall) == 160, "the record that the caller packs");
 // One query token per row. `scratch` must be zero when it is first used (every launch leaves its tickets zero) and belongs to one stream at a
 // time. A row whose position does not lie below `max_context` gets zeros, and code 32 in the status word; a key whose page is none of the
 // cache's is left out, with code 33. Returns -2 for sizes it does not run: head sizes other than 64 and 128, groups above 16, more than
-// 65536 (token, key head) pairs.
+// 65536 (token, key head) pairs, pages at addresses that are no multiples of hd / 8.
 int stride_decode_int4(const void* record) {
     const DecodeCall r = read_record<DecodeCall>(record);
     if (r.tokens < 0 || r.nq <= 0 || r.nkv <= 0 || r.page_size <= 0 || r.table_width <= 0 || r.table_rows <= 0 || r.num_pages <= 0 || r.window < 0 || r.softcap < 0.f ||
         r.max_context <= 0 || r.nq % r.nkv || r.status == nullptr)
         return STRIDE_BAD_ARGUMENT;
     if ((r.hd != 64 && r.hd != 128) || r.nq / r.nkv > 16 || r.max_context > (1 << 30)) return STRIDE_UNSUPPORTED;
-    if ((reinterpret_cast<uintptr_t>(r.k_pages) | reinterpret_cast<uintptr_t>(r.v_pages) | reinterpret_cast<uintptr_t>(r.scratch)) % 16)
-        return STRIDE_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(r.k_pages) | reinterpret_cast<uintptr_t>(r.v_pages)) % (r.hd / 8) || reinterpret_cast<uintptr_t>(r.scratch) % 16)
+        return STRIDE_UNSUPPORTED;                      // (the pieces that small copies take of a row)
     if (r.tokens == 0) return 0;
     if (static_cast<long long>(r.tokens) * r.nkv > four::kTicketInts) return STRIDE_UNSUPPORTED;
     // units are counted in 32 bits token by token

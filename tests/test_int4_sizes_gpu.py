@@ -237,3 +237,43 @@ def test_a_portion_of_a_request_beyond_the_room_for_its_keys_is_reported_and_not
     with pytest.raises(ops.KernelError, match="more keys|names no page"):       # (both are so; the first report stays)
         ops.check_kernel_status()
     assert bool((out == 9.0).all())
+
+
+# --------------------------------------------------------------------------------------------------- where pages may begin
+@pytest.mark.parametrize("nq,nkv,hd,page,pages_of", [(4, 1, 64, 5, 41), (6, 3, 64, 1, 201), (4, 1, 64, 16, 13), (2, 1, 128, 5, 41), (2, 2, 128, 16, 13)])
+def test_every_layer_of_an_odd_pool_is_read(ops, nq, nkv, hd, page, pages_of):
+    """A layer's pages begin behind the layer before: heads of 64 have rows of 40 bytes, so that is any multiple of 8. Pages of 16 are moved to one, too."""
+    n, g = 200, torch.Generator().manual_seed(page)
+    pages, table, (k, v) = cache_of(torch.randn(n, nkv, hd, generator=g), positive(g, n, nkv, hd), page)
+    shift = 8 if page == 16 and hd == 64 else 0
+    moved = []
+    for t in pages:
+        pool = torch.zeros(2 * pages_of * t[0].numel() + shift, dtype=torch.uint8, device="cuda")[shift:].view(2, pages_of, *t.shape[1:])
+        pool[1, :t.shape[0]] = t
+        moved.append(pool[1])
+    if hd == 64:
+        assert moved[0].data_ptr() % 16 == 8
+    q = torch.randn(3, nq * hd, generator=g).to(BF16)
+    want, largest, _v = plain.attention(q.view(3, nq, hd), [k], [v], torch.tensor([n - 1] * 3), torch.zeros(3, dtype=torch.int32), hd ** -0.5)
+    got = decode(ops, q, moved, table, n, nq, nkv, hd, page)
+    assert group_errors(got, want) <= HALF_STEP + 2.0 ** -10
+    assert torch.equal(got, decode(ops, q, pages, table, n, nq, nkv, hd, page)) or page == 16       # (of the same copies: the same bits)
+    q = q.repeat(4, 1)
+    want, largest, _v = plain.attention(q.view(12, nq, hd), [k], [v], *rows_of(n, 12), hd ** -0.5)
+    assert group_errors(portion(ops, q, moved, table, n, nq, nkv, hd, page), want) <= HALF_STEP + 2 * 2.0 ** -11 + 2 * 2.0 ** -11 * largest
+    exact = torch.empty(12, nq * hd, dtype=BF16, device="cuda")
+    at, seq = (x.int().cuda() for x in rows_of(n, 12))
+    ops.paged_attention_int4(q.cuda(), nq * hd, exact, *moved, table, seq, at, nq, nkv, hd, page, hd ** -0.5)
+    assert group_errors(exact.view(12, nq, hd).double().cpu(), want) <= HALF_STEP + 2.0 ** -12
+    ops.check_kernel_status()
+
+
+def test_decode_over_pages_at_odd_addresses_is_refused(ops):
+    n, nq, nkv, hd, page, g = 60, 4, 1, 64, 5, torch.Generator().manual_seed(1)
+    pages, table, _stored = cache_of(torch.randn(n, nkv, hd, generator=g), positive(g, n, nkv, hd), page)
+    moved = []
+    for t in pages:
+        pool = torch.zeros(t.numel() + 4, dtype=torch.uint8, device="cuda")[4:].view(t.shape)
+        moved.append(pool)
+    with pytest.raises(ops.KernelError):
+        decode(ops, torch.zeros(1, nq * hd, dtype=BF16), moved, table, n, nq, nkv, hd, page)
