@@ -100,6 +100,12 @@ PYBIND11_MODULE(_runtime, m) {
              py::arg("parent"), py::arg("child"), py::arg("num_tokens"),
              "Opens `child` with the parent's first tokens. Returns ([(group, page to copy, page to copy to)], (the parent's state slot, the child's)).")
         .def("adopt_prefix", &CacheManager::adopt_prefix)
+        .def("note_run",
+             [](CacheManager& c, const StepBatch& batch) {
+                 for (auto& it : batch.items()) c.note_run(it.request, it.position, it.position + it.tokens.size());
+             },
+             py::arg("batch"), "The tokens of a step that has been launched count as run.")
+        .def("run_tokens", &CacheManager::run_tokens, py::arg("request"))
         .def("ensure", &CacheManager::ensure, py::arg("request"), py::arg("num_tokens"), py::arg("reserve") = 0)
         .def("pages_missing", &CacheManager::pages_missing)
         .def("trim", &CacheManager::trim)

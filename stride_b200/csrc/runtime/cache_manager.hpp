@@ -34,6 +34,7 @@ struct RequestPages {
     // Per group: how many leading pages were given back to the pool.
     std::vector<size_t> trimmed;
     size_t shared_prefix_tokens = 0;
+    size_t run_tokens = 0;          // leading tokens that steps have run, or that came with a prefix or a fork
 };
 
 class CacheManager {
@@ -129,6 +130,7 @@ public:
             e.trimmed[g] = std::min(from.trimmed[g], need);
         }
         e.shared_prefix_tokens = std::min(from.shared_prefix_tokens, whole * page_size_);
+        e.run_tokens = num_tokens;
         return copies;
     }
 
@@ -139,7 +141,7 @@ public:
         if (!prefix_caching_) return 0;
         if (!e.tables[0].empty()) throw std::invalid_argument("a prefix can only be adopted by an empty table");
         e.tables[0] = pools_[0].acquire_prefix(e.tenant, tokens);
-        e.shared_prefix_tokens = e.tables[0].size() * page_size_;
+        e.shared_prefix_tokens = e.run_tokens = e.tables[0].size() * page_size_;
         return e.shared_prefix_tokens;
     }
 
@@ -198,6 +200,14 @@ public:
         if (!prefix_caching_) return;
         pools_[0].publish(e.tenant, tokens, written_tokens, e.tables[0]);
     }
+
+    // A step has run tokens begin .. end of the request: its keys and values up to there are in the cache and its state is the one behind
+    // them, unless tokens before `begin` have not been run. What was run behind `end` before is no longer its continuation.
+    void note_run(RequestKey r, size_t begin, size_t end) {
+        auto& e = entry(r);
+        if (begin <= e.run_tokens) e.run_tokens = end;
+    }
+    size_t run_tokens(RequestKey r) const { return entry(r).run_tokens; }
 
     // Gives back every page and the state slot.
     void close(RequestKey r) {

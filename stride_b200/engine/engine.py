@@ -320,10 +320,16 @@ class Engine:
 
     def fork(self, parent: int, child: int, num_tokens: int) -> None:
         """Opens request ``child`` (a key like those of ``forward``) with the first ``num_tokens`` tokens of request ``parent``: whole
-        pages are shared, a page in part is copied, the state of mixers that keep some is copied as it stands, so with such mixers
-        ``num_tokens`` is what the parent has run. The caller manages both requests' pages from there on."""
+        pages are shared, a page in part is copied, the state of mixers that keep some is copied as it stands. The parent must have run
+        those tokens, and with mixers that keep state no others (ValueError). The caller manages both requests' pages from there on, and
+        runs neither again at positions that lie in shared pages."""
         if self._ahead is not None:
             raise RuntimeError("a step of the engine's own requests is in flight; call step() until they are done")
+        run = self.cache.run_tokens(int(parent))
+        if num_tokens > run:
+            raise ValueError(f"request {parent} has run {run} tokens, not {num_tokens}")
+        if self.device_cache.states and num_tokens not in (0, run):
+            raise ValueError(f"the model's layers keep a state, which is that behind the {run} tokens request {parent} has run, not behind {num_tokens}")
         copies, state = self.cache.fork(int(parent), int(child), int(num_tokens))
         try:
             for group, src, dst in copies:

@@ -106,11 +106,12 @@ class ModelRunner:
             raise ValueError(f"a request would reach position {batch.max_ctx - 1}; max_model_len is {self.max_model_len}")
         if self.cuda_graphs and batch.decode_only and batch.num_rows == batch.num_seqs:
             logits = self._step_graph(batch)
-            return logits.cpu() if to_host else logits
-        if self.cuda_graphs and batch.num_seqs == 1 and batch.num_tokens == self.token_capacity and batch.num_rows <= 1:
+        elif self.cuda_graphs and batch.num_seqs == 1 and batch.num_tokens == self.token_capacity and batch.num_rows <= 1:
             logits = self._step_full_portion(batch)
-            return logits.cpu() if to_host else logits
-        return self._step_eager(batch, to_host)
+        else:
+            logits = self._step_eager(batch, to_host)
+        self.cache.note_run(batch)
+        return logits.cpu() if to_host else logits
 
     def timed_step(self, batch):
         """The same step run eagerly with CUDA events around every launch: ``(logits, {class of kernel:
@@ -120,6 +121,7 @@ class ModelRunner:
             raise ValueError("the step does not fit the runner")
         with ops.KernelTimer() as timer:
             logits = self._step_eager(batch, to_host=False)
+        self.cache.note_run(batch)
         return logits, timer.milliseconds()
 
     # ------------------------------------------------------------------- eager

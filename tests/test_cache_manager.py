@@ -242,3 +242,36 @@ def test_packed_step_arrays():
         other.add(9, [1], 5, [1])
     with pytest.raises(ValueError, match="holds no cache"):
         other.add(5, [1], 0, [0])
+
+
+def test_tokens_that_steps_have_run():
+    rt = runtime()
+    cache = CacheManager(4, [(12, 0)], 3, False)
+    cache.open(1)
+    cache.ensure(1, 30, 0)
+
+    def step(request, position, count):
+        batch = rt.StepBatch(cache)
+        batch.add(request, list(range(count)), position, [])
+        cache.note_run(batch)
+        return cache.run_tokens(request)
+    assert cache.run_tokens(1) == 0                         # pages alone are no tokens
+    assert step(1, 0, 10) == 10 and step(1, 10, 1) == 11
+    assert step(1, 15, 3) == 11                             # what lies between has not been run
+    assert step(1, 6, 2) == 8                               # a request taken back to 6
+    cache.fork(1, 2, 8)
+    assert cache.run_tokens(2) == 8
+    cache.close(1)
+    cache.open(1)
+    assert cache.run_tokens(1) == 0
+    with pytest.raises(ValueError):
+        cache.run_tokens(9)
+
+
+def test_a_prefix_counts_as_run():
+    cache = CacheManager(4, [(12, 0)], 3, True)
+    cache.open(1)
+    cache.ensure(1, 8, 0)
+    cache.publish(1, list(range(8)), 8)
+    cache.open(2)
+    assert cache.run_tokens(2) == 0 and cache.adopt_prefix(2, list(range(12))) == 8 and cache.run_tokens(2) == 8
