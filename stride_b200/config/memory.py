@@ -64,7 +64,8 @@ def plan_memory(config, dtype: str = "bfloat16", memory_bytes: int = B200_MEMORY
     own parts (the tensors they declare, what their mixers keep per token and per request), not from arithmetic
     on the configuration class. ``activation_fraction`` of what the weights leave is held back for activations,
     workspace and fragmentation (the worker's ``--activation-reserve``, python/stride_worker/worker.py:182-225);
-    state of fixed size is set aside for ``max_requests`` requests; ``cache_dtype`` ``int4`` counts pages held in 4 bits. Raises ``PlanError`` when the weights do not
+    state of fixed size is set aside for ``max_requests`` requests; ``cache_dtype`` ``int4`` counts pages held in 4 bits, and sets aside
+    what attention of portions expands out of them. Raises ``PlanError`` when the weights do not
     fit or not even one page is left."""
     if dtype not in ITEMSIZE:
         raise PlanError(f"dtype must be one of {sorted(ITEMSIZE)}, got {dtype!r}")
@@ -74,7 +75,7 @@ def plan_memory(config, dtype: str = "bfloat16", memory_bytes: int = B200_MEMORY
         raise PlanError("activation_fraction must be in [0, 1)")
     from ..engine.loading import footprint      # the parts live above this package; asked for only when a plan is made
     try:
-        sizes = footprint(config, dtype, cache_dtype)
+        sizes = footprint(config, dtype, cache_dtype, max_requests)
     except ValueError as e:
         if cache_dtype is None:
             raise
@@ -85,7 +86,7 @@ def plan_memory(config, dtype: str = "bfloat16", memory_bytes: int = B200_MEMORY
         raise PlanError(f"{name}: the weights need {weight_bytes / GIB:.1f} GiB in {dtype} but the device has "
                         f"{memory_bytes / GIB:.1f} GiB")
     after_weights = memory_bytes - weight_bytes
-    reserve = int(after_weights * activation_fraction)
+    reserve = int(after_weights * activation_fraction) + sizes["expanded_bytes"]
     kv_bytes = after_weights - reserve
     per_token = max(1, sizes["kv_bytes_per_token"])
     num_blocks = kv_bytes // (per_token * block_size)

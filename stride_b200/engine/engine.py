@@ -112,7 +112,7 @@ class Engine:
         spec = self.model.spec
         self.max_model_len = min(self.cfg.max_model_len, spec.max_positions)
         plan = plan_cache(self.model, self.cfg.block_size, self.cfg.num_blocks, self.cfg.activation_reserve,
-                          self.cfg.max_batch_seqs, self.model.rt.dtype)
+                          self.cfg.max_batch_seqs, self.model.rt.dtype, self.max_model_len)
         self.device_cache, self.cache = attach_cache(self.model, plan, self.cfg.prefix_caching)
         self.runner = ModelRunner(self.model, self.cache, token_capacity=token_cap, seq_capacity=self.cfg.max_batch_seqs,
                                   row_capacity=row_cap, max_model_len=self.max_model_len, cuda_graphs=self.cfg.cuda_graphs)

@@ -82,11 +82,12 @@ def _declarations(config) -> dict:
     return DecoderModel(config.to_model_spec(), runtime).declare()
 
 
-def footprint(config, dtype: str = "bfloat16", cache_dtype: str | None = None) -> dict:
+def footprint(config, dtype: str = "bfloat16", cache_dtype: str | None = None, max_requests: int = 256, max_context: int | None = None) -> dict:
     """What a model of this configuration needs in bytes, read from its own parts without touching a device: the
     declared tensors (matrices in the compute dtype, vectors and tables in 32 bits, as the loader keeps them),
-    what its mixers keep per token in pages, and the state of fixed size per request. Works for any registered
-    architecture, since it asks the parts and not the configuration class."""
+    what its mixers keep per token in pages, the state of fixed size per request, and what a step expands out of the cache (for
+    ``max_requests`` requests of up to ``max_context`` tokens, None: the positions that the model has). Works for any
+    registered architecture, since it asks the parts and not the configuration class."""
     import math
 
     from ..cache import plan_groups
@@ -96,7 +97,8 @@ def footprint(config, dtype: str = "bfloat16", cache_dtype: str | None = None) -
     requests = model.cache_requests()
     per_token = sum(g.bytes_per_token(item) for g in plan_groups(requests))
     state = sum(math.prod(s.shape) * torch.empty((), dtype=s.dtype).element_size() for _r, s in requests if s is not None)
-    return {"weight_bytes": int(weights), "kv_bytes_per_token": int(per_token), "state_bytes_per_request": int(state)}
+    return {"weight_bytes": int(weights), "kv_bytes_per_token": int(per_token), "state_bytes_per_request": int(state),
+            "expanded_bytes": model.expanded_bytes(int(max_context or model.spec.max_positions), int(max_requests))}
 
 
 @dataclass
@@ -107,15 +109,16 @@ class CachePlan:
 
 
 def plan_cache(model, page_size: int, num_pages: int | None, activation_reserve: float, num_state_slots: int,
-               dtype: torch.dtype) -> CachePlan:
+               dtype: torch.dtype, max_context: int = 0) -> CachePlan:
     """Pool size: given, or what fits into the free device memory after the
-    reserve (python/stride_worker/worker.py:182-225)."""
+    reserve (python/stride_worker/worker.py:182-225) and after what a step expands out of the cache for requests of up to ``max_context``
+    tokens."""
     if num_pages is None:
         from ..cache import plan_groups
         item = torch.empty((), dtype=dtype).element_size()
         per_page = sum(g.bytes_per_page(page_size, item) for g in plan_groups(model.cache_requests()))
         free_bytes, _total = torch.cuda.mem_get_info(model.rt.device)
-        usable = int(free_bytes * (1.0 - activation_reserve))
+        usable = int(free_bytes * (1.0 - activation_reserve)) - model.expanded_bytes(max_context, num_state_slots)
         num_pages = usable // max(per_page, 1) if per_page else 1
         if num_pages < 1:
             raise RuntimeError(f"no room for even one KV page: {free_bytes / 2**30:.1f} GiB free, "

@@ -66,6 +66,8 @@ class ModelRunner:
                              "position tables hold")
         self.max_model_len = int(max_model_len)
         self.table_width = max(1, cache_manager.pages_for(max_model_len))
+        self.rt.longest_request = self.table_width * cache_manager.page_size
+        self.rt.most_requests = int(seq_capacity)
         self._rt_mod = load_runtime()
         self._eager = _Staging(self._rt_mod.packed_layout(self.groups, token_capacity, seq_capacity, row_capacity,
                                                           self.table_width), self.device)

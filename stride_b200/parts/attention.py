@@ -548,6 +548,28 @@ class PagedAttention(Mixer):
         return tokens
 
 
+    MAX_EXPANDED_BYTES = 1 << 28        # of keys and values expanded for a step's portions, where one request does not take more
+
+    def expanded_keys(self, longest, requests) -> int:
+        """Keys that are expanded at once, where a request holds up to ``longest`` and a step up to ``requests`` of them."""
+        return min(longest * requests, max(longest, self.MAX_EXPANDED_BYTES // (4 * self.nkv * self.hd)))
+
+    def expanded_bytes(self, longest, requests) -> int:
+        """Device memory that portions over a cache in 4 bits take beside the activations (one buffer for all layers of a shape)."""
+        return 4 * ops.prefill_int4_scratch_ints(requests, self.expanded_keys(longest, requests), self.nkv, self.hd) if self.int4 and self._fast else 0
+
+    def _portion_groups(self, ctx, room) -> list:
+        """The requests in front of the decode tail in groups of neighbours that hold at most ``room`` keys: (first, past the last, keys)."""
+        if ctx.portion_keys <= room or not ctx.host_items:
+            return [(0, ctx.decode_tail_seq, ctx.portion_keys)]
+        groups, first, held = [], 0, 0
+        for i, (_request, _row, n, position, _slot) in enumerate(ctx.host_items[:ctx.decode_tail_seq]):
+            if held and held + position + n > room:
+                groups.append((first, i, held))
+                first, held = i, 0
+            held += position + n
+        return groups + [(first, ctx.decode_tail_seq, held)]
+
     def _attend_int4(self, qkv, attn, table, ctx, cache, tokens, geometry):
         pages, rules = (cache.k_pages, cache.v_pages, table), (self.softcap, self.sinks, self.slopes)
         split = min(ctx.decode_tail_start, tokens) if self._fast else tokens        # portions before, single decoded tokens after
@@ -556,10 +578,16 @@ class PagedAttention(Mixer):
             ops.paged_attention_int4(qkv[:split], self.qkv_dim, attn[:split], *pages, ctx.seq_of_token[:split], ctx.positions[:split], *geometry, *rules,
                                      neighbours=ctx.decode_tail_start >= split // 2 and ctx.max_q_len >= 4, context_bound=ctx.context_bound)
         elif split > 0:
+            # one buffer for as long as the runner lives: what a step's portions read is expanded as many requests at a time as it holds
             seqs, keys = ctx.decode_tail_seq, ctx.portion_keys
-            scratch = self.rt.scratch("int4_expanded", ops.prefill_int4_scratch_ints(seqs, keys, self.nkv, self.hd), torch.int32)
-            ops.paged_attention_prefill_int4(qkv[:split], self.qkv_dim, attn[:split], *pages, ctx.q_start, ctx.q_len, ctx.ctx_len, scratch, seqs, keys,
-                                             *geometry, *rules, self.precise_cap)
+            most = self.rt.most_requests or seqs
+            room = self.expanded_keys(self.rt.longest_request, most) or keys
+            scratch = self.rt.scratch("int4_expanded", ops.prefill_int4_scratch_ints(most, room, self.nkv, self.hd), torch.int32)
+            for first, last, held in self._portion_groups(ctx, room):
+                of = (table, ctx.q_start, ctx.q_len, ctx.ctx_len)
+                rows, *lens = (t[first:] for t in of) if first else of
+                ops.paged_attention_prefill_int4(qkv[:split], self.qkv_dim, attn[:split], cache.k_pages, cache.v_pages, rows, *lens, scratch, last - first, held,
+                                                 *geometry, *rules, self.precise_cap)
         if tokens > split:
             n = tokens - split
             scratch = self.rt.scratch("attention_splits_int4", ops.decode_int4_scratch_floats(n, self.nq, self.nkv, self.hd, ctx.context_bound))

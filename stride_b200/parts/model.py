@@ -164,6 +164,12 @@ class DecoderModel:
         """True when a part sizes the launches of a prompt's portion by the keys that the requests hold."""
         return any(getattr(p, "sizes_by_context", False) for layer in self.layers for p in getattr(layer, "parts", lambda: ())())
 
+    def expanded_bytes(self, longest: int, requests: int) -> int:
+        """Device memory beside the activations for what parts expand out of the cache (one buffer for all layers), where a request holds up
+        to ``longest`` tokens and a step brings up to ``requests`` requests."""
+        parts = [p for layer in self.layers for p in getattr(layer, "parts", lambda: ())()]
+        return max((getattr(p, "expanded_bytes", lambda *_: 0)(longest, requests) for p in parts), default=0)
+
     @property
     def graph_safe(self) -> bool:
         """False when a part needs the host's view of the step and therefore cannot

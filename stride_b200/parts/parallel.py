@@ -42,6 +42,9 @@ class ParallelMixer(Mixer):
         self.graph_safe = all(getattr(m, "graph_safe", True) for m, _ in self.branches)
         self.sizes_by_context = any(getattr(m, "sizes_by_context", False) for m, _ in self.branches)
 
+    def expanded_bytes(self, longest, requests) -> int:
+        return max(getattr(m, "expanded_bytes", lambda *_: 0)(longest, requests) for m, _ in self.branches)
+
     def declare(self):
         d = {}
         for m, _ in self.branches:

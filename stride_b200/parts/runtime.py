@@ -24,6 +24,9 @@ def sequence_slots(ctx) -> int:
 class Runtime:
     # Kinds of the model's mixers (those inside a parallel mixer too), for a part whose form depends on what else the model holds.
     mixer_kinds: frozenset = frozenset()
+    # The most tokens that a request may hold, and the most requests of a step, for as long as the runner lives; 0: not known.
+    longest_request: int = 0
+    most_requests: int = 0
 
     def __init__(self, device, dtype: torch.dtype, token_capacity: int, row_capacity: int, cache_dtype: str | None = None):
         if cache_dtype not in (None, "int4"):

@@ -226,3 +226,44 @@ def test_numbers_that_no_launch_holds_are_refused(number):
     from stride_b200.csrc import ops
     with pytest.raises(ops.KernelError, match="read_int4: a number does not fit"):
         ops._launch("stride_int4_read", "read_int4", 0, 0, 0, 0, 0, 0, 0, number, 1, 64, 16, 1, 0)
+
+
+# ------------------------------------------------------------------------------------- what portions expand out of the cache
+def mixer_of(name="llama3.1-8b"):
+    return [p for p in model_for(config_from_dict(preset(name))).layers[0].parts() if hasattr(p, "expanded_keys")][0]
+
+
+def test_what_portions_expand_is_bounded():
+    mixer = mixer_of()
+    of_key = 2 * 8 * 128 * 2
+    for longest, requests in ((8192, 256), (131072, 256), (131072, 1), (300, 4), (65536, 2), (1, 1)):
+        keys = mixer.expanded_keys(longest, requests)
+        assert longest <= keys <= longest * requests            # one request always fits, and no more than a step can hold
+        assert keys * of_key <= max(mixer.MAX_EXPANDED_BYTES, longest * of_key)
+        # the buffer: pages in quarters of an octave, a table and a record a page
+        assert mixer.expanded_bytes(longest, requests) <= 1.25 * (keys + 64 * requests) * of_key * 1.02 + 32 * 64 * of_key
+    assert model_for(config_from_dict(preset("tiny-a")), torch.float32).expanded_bytes(8192, 16) == 0
+
+
+def test_requests_are_expanded_in_groups_that_fit():
+    from types import SimpleNamespace
+    mixer = mixer_of()
+
+    def groups(held, room):
+        items = [(i, 0, 5, n - 5, 0) for i, n in enumerate(held)] + [(99, 0, 1, 700, 0)] * 3       # and single tokens behind them
+        return mixer._portion_groups(SimpleNamespace(portion_keys=sum(held), decode_tail_seq=len(held), host_items=items), room)
+    assert groups([50, 60, 70], 180) == [(0, 3, 180)]
+    assert groups([50, 60, 70], 179) == [(0, 2, 110), (2, 3, 70)]
+    assert groups([100, 100, 100], 100) == [(0, 1, 100), (1, 2, 100), (2, 3, 100)]
+    for room in range(40, 200):
+        found = groups([40, 7, 33, 39, 12, 12, 40], room)
+        assert [g[0] for g in found][1:] == [g[1] for g in found][:-1] and found[0][0] == 0 and found[-1][1] == 7
+        assert all(g[2] <= max(room, 40) for g in found) and sum(g[2] for g in found) == 183
+
+
+def test_the_planner_sets_aside_what_portions_expand():
+    cfg = config_from_dict(preset("llama3.1-8b"))
+    four = plan_memory(cfg, cache_dtype="int4", max_requests=64)
+    wide = plan_memory(cfg, max_requests=64)
+    expanded = model_for(cfg).expanded_bytes(cfg.max_position_embeddings, 64)
+    assert expanded > 0 and four.activation_reserve_bytes - wide.activation_reserve_bytes == expanded == wide.kv_bytes - four.kv_bytes
