@@ -277,3 +277,56 @@ def test_decode_over_pages_at_odd_addresses_is_refused(ops):
         moved.append(pool)
     with pytest.raises(ops.KernelError):
         decode(ops, torch.zeros(1, nq * hd, dtype=BF16), moved, table, n, nq, nkv, hd, page)
+
+
+# ------------------------------------------------------------------------------------------------------------ how near to 64 bits
+# A bfloat16 result has 8 bits: a rounding is off by up to 2^-8 of the power of two below the value, evenly, 2^-8 / sqrt(3) of it in the mean square,
+# and a value's mean square is 2.16 of that power's where mantissas are spread as logarithms are: 1.53e-3 in the norm, up to 1.7e-3 for
+# sums of random values. What 11 bits of weights, keys and values (2^-11 / sqrt(3) / 1.47 = 1.9e-4 each) and 16 of a centre's weights add
+# stays below 8e-4 together, and sqrt(1.7^2 + 0.8^2) = 1.9. Keys, values or a centre's weights in 8 bits come to 2.4e-3 and more.
+NEAR = 2.1e-3
+
+
+def norm_error(got, want):
+    return float((got - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("nq,nkv,hd,page", [(32, 8, 128, 16), (16, 4, 64, 16), (16, 1, 128, 8)])
+def test_decode_is_as_near_as_its_result_can_be(ops, nq, nkv, hd, page):
+    n, g = 1500, torch.Generator().manual_seed(hd)
+    pages, table, (k, v) = cache_of(torch.randn(n, nkv, hd, generator=g), torch.randn(n, nkv, hd, generator=g), page)
+    q = torch.randn(4, nq * hd, generator=g).to(BF16)
+    want, _l, _v = plain.attention(q.view(4, nq, hd), [k], [v], torch.tensor([n - 1] * 4), torch.zeros(4, dtype=torch.int32), hd ** -0.5)
+    assert norm_error(decode(ops, q, pages, table, n, nq, nkv, hd, page), want) < NEAR
+
+
+@pytest.mark.parametrize("nq,nkv,hd,page", [(8, 2, 128, 16), (12, 4, 64, 16), (3, 1, 128, 8)])
+def test_portions_are_as_near_as_their_result_can_be(ops, nq, nkv, hd, page):
+    n, p, g = 700, 60, torch.Generator().manual_seed(hd)
+    pages, table, (k, v) = cache_of(torch.randn(n, nkv, hd, generator=g), torch.randn(n, nkv, hd, generator=g), page)
+    q = torch.randn(p, nq * hd, generator=g).to(BF16)
+    want, _l, _v = plain.attention(q.view(p, nq, hd), [k], [v], *rows_of(n, p), hd ** -0.5)
+    assert norm_error(portion(ops, q, pages, table, n, nq, nkv, hd, page), want) < NEAR
+
+
+def test_calls_on_the_same_inputs_have_the_same_bits(ops):
+    """Parts of a request are merged in the order of its keys, whichever CTA comes last."""
+    nq, nkv, hd, page, g = 32, 8, 128, 16, torch.Generator().manual_seed(3)
+    lengths = [3000, 1, 700, 1200]
+    kept = [cache_of(torch.randn(n, nkv, hd, generator=g), torch.randn(n, nkv, hd, generator=g), page)[0] for n in lengths]
+    pages = [torch.cat([made[w] for made in kept]) for w in (0, 1)]
+    table = torch.full((4, -(-3000 // page)), -1, dtype=torch.int32)
+    first = 0
+    for r, n in enumerate(lengths):
+        table[r, :-(-n // page)] = torch.arange(first, first - (-n // page))
+        first -= -n // page
+    table = table.cuda()
+    q = torch.randn(4, nq * hd, generator=g).to(BF16).cuda()
+    at, seq = torch.tensor([n - 1 for n in lengths], dtype=torch.int32, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda")
+    scratch = torch.zeros(ops.decode_int4_scratch_floats(4, nq, nkv, hd, 3000), device="cuda")
+    outs = []
+    for _ in range(20):
+        outs.append(torch.empty(4, nq * hd, dtype=BF16, device="cuda"))
+        ops.paged_attention_decode_int4(q, nq * hd, outs[-1], *pages, table, seq, at, scratch, nq, nkv, hd, page, hd ** -0.5, 0, 3000)
+    assert all(torch.equal(outs[0], o) for o in outs)
+    ops.check_kernel_status()
