@@ -582,10 +582,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                                 from_uneven = from_uneven || (uneven[h][r] && fmaf(x[nt][h][2 * r + e], unit[nt][e], size[h][r]) >= most);
                         const uint32_t lanes = __ballot_sync(0xffffffffu, from_uneven) & 0x11111111u << c, bit = 1u << (2 * nt + e);
                         if (most > R[nt][e] && 8 * nt + 2 * c + static_cast<int>(e) < group) uneven_cols = lanes ? uneven_cols | bit : uneven_cols & ~bit;
-                        const float next = fmaxf(R[nt][e], most), by = R[nt][e] == -INFINITY ? 0.f : exp2_quick(R[nt][e] - next);
+                        // (the weights' sum goes down in two steps: their values' sizes are in R, and the factor may be below any number)
+                        const float next = fmaxf(R[nt][e], most), half = R[nt][e] == -INFINITY ? 0.f : exp2_quick(0.5f * (R[nt][e] - next)), by = half * half;
                         R[nt][e] = next;
                         cen[nt][e] *= by;
-                        cen[nt][e + 2] *= by;
+                        cen[nt][e + 2] = cen[nt][e + 2] * half * half;
 #pragma unroll
                         for (int grp = 0; grp < G; ++grp)
 #pragma unroll
@@ -735,9 +736,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float* src = red + (w * group + row) * RS;
-            const float f = mm == -INFINITY ? 0.f : exp2f(src[HD] - mm);       // a warp without keys has weight 0
-            acc += f * src[d];
-            sum += f * src[HD + 1];
+            const float half = mm == -INFINITY ? 0.f : exp2f(0.5f * (src[HD] - mm));       // a warp without keys has weight 0
+            acc += half * half * src[d];
+            sum += src[HD + 1] * half * half;
         }
         if (parts == 1) {
             if (a.sinks != nullptr && mm != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -mm));
@@ -776,9 +777,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
                 most = warp_max(most);
                 float sum = 0.f;
                 for (int i = lane; i < parts; i += 32) {
-                    const float w = most == -INFINITY ? 0.f : exp2f(weights[row * parts + i] - most);
-                    weights[row * parts + i] = w;
-                    sum = fmaf(w, __ldcg(a.part_ml + (place(i) + row) * 2 + 1), sum);
+                    const float half = most == -INFINITY ? 0.f : exp2f(0.5f * (weights[row * parts + i] - most));
+                    weights[row * parts + i] = half * half;
+                    sum += __ldcg(a.part_ml + (place(i) + row) * 2 + 1) * half * half;
                 }
                 sum = warp_sum(sum);
                 if (a.sinks != nullptr && most != -INFINITY) sum += exp2f(fmaf(a.sinks[kvh * group + row], 1.4426950408889634f, -most));

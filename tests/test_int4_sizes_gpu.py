@@ -330,3 +330,42 @@ def test_calls_on_the_same_inputs_have_the_same_bits(ops):
         ops.paged_attention_decode_int4(q, nq * hd, outs[-1], *pages, table, seq, at, scratch, nq, nkv, hd, page, hd ** -0.5, 0, 3000)
     assert all(torch.equal(outs[0], o) for o in outs)
     ops.check_kernel_status()
+
+
+# sizes of the values of the pages, one after another over and over
+MIXES = [(0.0, 1e15), (1e15, 0.0), (1e-25, 1e10), (1e18, 1e-25, 0.0, 1.0), (0.0, 1e-28), (1e-28, 0.0, 1e-24)]
+
+
+@pytest.mark.parametrize("run", [16, 64, 128])
+@pytest.mark.parametrize("mix", MIXES, ids=str)
+@pytest.mark.parametrize("call", ["decode"])
+def test_pages_of_values_of_very_different_sizes(ops, call, mix, run):
+    """The sum of the weights is that of all tokens, whatever their values' size."""
+    n, nq, nkv, hd, page, g = 520, 4, 2, 64, 16, torch.Generator().manual_seed(run)
+    size = torch.tensor([mix[i // run % len(mix)] for i in range(n)], dtype=F64)
+    pages, table, (k, v) = cache_of(0.3 * torch.randn(n, nkv, hd, generator=g), positive(g, n, nkv, hd) * size[:, None, None], page)
+    q = torch.randn(7, nq * hd, generator=g).to(BF16)
+    if call == "decode":
+        want, largest, _v = plain.attention(q.view(7, nq, hd), [k], [v], torch.tensor([n - 1] * 7), torch.zeros(7, dtype=torch.int32), hd ** -0.5)
+        got = decode(ops, q, pages, table, n, nq, nkv, hd, page)
+    else:
+        want, largest, _v = plain.attention(q.view(7, nq, hd), [k], [v], *rows_of(n, 7), hd ** -0.5)
+        got = portion(ops, q, pages, table, n, nq, nkv, hd, page)
+    assert group_errors(got, want) <= HALF_STEP + 2 * 2.0 ** -11 + 2 * 2.0 ** -11 * largest
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("call", ["decode"])
+def test_large_values_that_weigh_nothing_do_not_drown_the_others(ops, call):
+    n, nq, nkv, hd, page, g = 320, 2, 2, 64, 16, torch.Generator().manual_seed(4)
+    far = (torch.arange(n) // 64) % 2 == 1                   # tokens whose scores are about -280 below the others'
+    q = torch.full((5, nq * hd), 2.0).to(BF16)
+    keys = 0.05 * torch.randn(n, nkv, hd, generator=g) - 17.5 * far[:, None, None]
+    values = positive(g, n, nkv, hd) * torch.where(far, 1e12, 1e-3)[:, None, None]
+    pages, table, (k, v) = cache_of(keys, values, page)
+    rows = rows_of(n, 5) if call == "portion" else (torch.tensor([n - 1] * 5), torch.zeros(5, dtype=torch.int32))
+    want, _l, _v = plain.attention(q.view(5, nq, hd), [k], [v], *rows, hd ** -0.5)
+    got = (portion if call == "portion" else decode)(ops, q, pages, table, n, nq, nkv, hd, page)
+    # keys near -17.5 are of no weight; the others' scores, of up to 0.2 times 16 in all, are off by 2^-11 of that
+    assert group_errors(got, want) <= HALF_STEP + 2 * 2.0 ** -11 + 4 * 2.0 ** -11
+    ops.check_kernel_status()
