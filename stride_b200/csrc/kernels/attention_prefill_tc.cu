@@ -190,7 +190,7 @@ constexpr int kServiceRegs = 48, kSoftmaxRegs = 208;     // per thread, after th
 // of what a tile takes them), so that one head's exponentials, which queue for the special-function unit, fall into
 // the other head's loads, maxima and hand-over. Left to themselves both heads run in step and the unit is contended
 // for in one half of the time and idle in the other (measured: 56 us against 50 us for 2,048 tokens).
-// Of 16-bit floating point's tiles, which take longer, half is 1400 (2,048 queries at 8192 keys: 700 cycles 317 us, 1000 309, 1400 301 to 305).
+// Of 16-bit floating point's tiles, which take longer, half is 1400 (2,048 queries at 8192 keys: 1000 cycles 313 us, 1400 305).
 constexpr long long kStaggerCycles = 1000, kStaggerCyclesF16 = 1400;
 
 // HEADS query heads of one key head per CTA (1 or 2). One head: 4 service warps (keys, products, values, Q) and 4
@@ -639,8 +639,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const bool grow = mx > m_ref + kRescaleThreshold;      // also true for the first finite maximum
             if (__any_sync(0xffffffffu, grow)) {
                 const float factor = grow ? (m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - mx)) : 1.f;
+                if (F16 && grow && m_ref != -INFINITY) {       // in two steps: the values' sizes are in the references, and the factor may be below any number
+                    const float half = ex2_approx(0.5f * (m_ref - mx));
+                    l = l * half * half;
+                } else {
+                    l *= factor;
+                }
                 if (grow) m_ref = mx;
-                l *= factor;
                 if (j > 0) {
                     // O belongs to the output product of the tile before until that has finished
                     ok = output_done(j - 1, 16);
@@ -659,7 +664,11 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             {
                 // A masked score is -inf and gives exactly 0. A row that has seen no key yet has m_ref = -inf and
                 // only masked scores: subtract 0 there, or -inf - -inf would make a NaN.
-                const float neg_m = m_ref == -INFINITY ? 0.f : (F16 ? lean + static_cast<float>(kLift) : 0.f) - m_ref;
+                // F16: where a tile's values are so far below others that P is all zeros (below 2^-94), the weights still count in their sum and
+                // must not vanish with P: they go up by 2^60, which leaves P zeros.
+                const int up = F16 && mx < m_ref - (94.f + kLift) ? 60 : 0;
+                float neg_m = (F16 ? lean + static_cast<float>(kLift + up) : 0.f) - m_ref;
+                if (m_ref == -INFINITY) neg_m = 0.f;
                 float l4[4] = {0.f, 0.f, 0.f, 0.f};       // independent partial sums
                 float packed[32];             // bfloat16 pairs, carried as 32-bit words: P's columns hold two keys each
 #pragma unroll
@@ -671,7 +680,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 tmem_st32(tmem_sj, packed);   // over S columns 0-31, all of which have been read
                 const float sum = (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                l = F16 ? fmaf(sum, power_of_two(-kLift - kSumUnit - values_exponent(tile)), l) : l + sum;
+                l = F16 ? fmaf(sum, power_of_two(max(-126, -kLift - kSumUnit - values_exponent(tile) - up)), l) : l + sum;
             }
             if (F16 && (j & 31) == 31) window_of = exponents_at(about_at + (j + 1 + lane) * nkv);
             // The scores of the next tile were issued two tiles ago: ask for them now, so that they travel while this

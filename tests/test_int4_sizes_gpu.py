@@ -338,7 +338,7 @@ MIXES = [(0.0, 1e15), (1e15, 0.0), (1e-25, 1e10), (1e18, 1e-25, 0.0, 1.0), (0.0,
 
 @pytest.mark.parametrize("run", [16, 64, 128])
 @pytest.mark.parametrize("mix", MIXES, ids=str)
-@pytest.mark.parametrize("call", ["decode"])
+@pytest.mark.parametrize("call", ["decode", "portion"])
 def test_pages_of_values_of_very_different_sizes(ops, call, mix, run):
     """The sum of the weights is that of all tokens, whatever their values' size."""
     n, nq, nkv, hd, page, g = 520, 4, 2, 64, 16, torch.Generator().manual_seed(run)
@@ -355,7 +355,7 @@ def test_pages_of_values_of_very_different_sizes(ops, call, mix, run):
     ops.check_kernel_status()
 
 
-@pytest.mark.parametrize("call", ["decode"])
+@pytest.mark.parametrize("call", ["decode", "portion"])
 def test_large_values_that_weigh_nothing_do_not_drown_the_others(ops, call):
     n, nq, nkv, hd, page, g = 320, 2, 2, 64, 16, torch.Generator().manual_seed(4)
     far = (torch.arange(n) // 64) % 2 == 1                   # tokens whose scores are about -280 below the others'
