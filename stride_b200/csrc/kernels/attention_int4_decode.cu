@@ -28,10 +28,10 @@
 // (token, key head) is cut only where a stretch ends. Parts of one are merged by the CTA that draws its last ticket, in the order of the keys.
 //
 // Measured: 64 requests of up to 8192 keys, 8 key heads of 128, group 4: 345 MB in 95 us, 3.6 TB/s, 0.56 of the copy rate; 8 requests 26 us; one
-// request of 2048 keys 9.6 us. What bounds a full batch is the instructions between the copies and the products: 168 registers let three warps
-// run on a scheduler, which issue in 0.50 of the cycles and wait for their own last instruction in most others; of a warp's cycles on 32
-// keys 700 go to the scores, 350 to the softmax, 880 to the values, 230 to waiting for copies. Whole units instead of equal stretches took 97
-// us; cp.async instead of bulk copies 104; one ring for the CTA instead of one a warp 100; four CTAs an SM with two stages and four lanes
+// request of 2048 keys 10.3 us. What bounds a full batch is the instructions between the copies and the products: 168 registers let three warps
+// run on a scheduler, which issue in 0.51 of the cycles and wait for their own last instruction in most others; of a warp's cycles on 32
+// keys 700 go to the scores, 350 to the softmax, 880 to the values, 230 to waiting for copies. Before the products in bfloat16 came beside those in 16-bit floating point
+// it took 93; measured against that: whole units instead of equal stretches 97 us; cp.async instead of bulk copies 104; one ring for the CTA instead of one a warp 100; four CTAs an SM with two stages and four lanes
 // asking for copies the same; P in one part instead of two 90, with an error of 2.4e-3 instead of 1.8e-3. One request is a chain of latencies:
 // prologue 3.0 thousand cycles, the first pages and copies 3 to 5, a few tiles, the parts' sums 2.4, ticket and merge 3.5.
 // A warp owns tiles of 32 keys and a ring of copies: a bulk copy for each 16 keys and one for their values where pages hold whole sixteens (a page's

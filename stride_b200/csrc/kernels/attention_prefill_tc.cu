@@ -48,7 +48,7 @@ namespace stride {
 
 // The keys of the first num_seqs requests of a cache held in 4 bits (int4_cache.cuh) as pages of 64 in 16-bit floating point, for the attention of
 // portions: a request's pages one after the other, the requests' too, and the table that says so. A key is expanded once for all query tiles
-// that read it, which costs little beside them: 8192 keys of 8 heads of 128 take 14 us, 2,048 queries' attention to them 295, and what it writes,
+// that read it, which costs little beside them: 8192 keys of 8 heads of 128 take 13 us, 2,048 queries' attention to them 293, and what it writes,
 // 34 MB, is read back from L2 (no byte of it reached memory in a profile of 4096 keys). The format has 11 bits where bfloat16 has 8, which an entry's place
 // between two of its sixteen numbers needs, but few exponents: the keys of a page are multiplied by the power of two that brings the largest of
 // their entries near 2^15, the values by another, and the attention takes both off again. So an entry keeps 11 bits down to 2^-29 of the

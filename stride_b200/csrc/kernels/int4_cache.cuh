@@ -3,7 +3,9 @@
 // A row (one head of one token) is cut into groups of 32 neighbouring entries, the last one possibly shorter. A group has a scale s and
 // a centre c, both bfloat16, and a number n in 0 .. 15 for each entry, which stands for c + s (n - 8):
 //     s = bf16((max - min) / 15)      c = bf16(min + 8 s)      n = clamp(rint((x - c) / s) + 8, 0, 15)      (s = 0: n = 8)
-// so an entry is off by half a step, plus at most 15 / 2 steps times the 2^-9 that s is rounded by at the ends of the range. 5 bits an entry.
+// so an entry is off by half a step, and at the ends of the range by what c is rounded by, up to 2^-8 |c|, and at the upper one by 15 times what s
+// is, up to 2^-8 s each: a group whose entries lie close together far from zero (100 to 100.1: c = 100, s = 0.0067) keeps few of its 4 bits.
+// 5 bits an entry.
 // A row of G groups is 16 G bytes of numbers, then (s, c) of each group, 4 bytes a group: 20 G bytes, whatever the head size.
 // The numbers lie as the lanes of a matrix instruction want them, without a shuffle:
 //   keys    entry 8 a + i of group g: 32-bit word a G + g, bits 4 i      (a lane that takes part a = lane % 4 of every key finds it side by side)
