@@ -430,7 +430,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) decode_kernel(co
             cb[nt][0] = pack_bf16(high, own - high);
             cb[nt][1] = pack_bf16(-8.f * high, -8.f * (own - high));
         }
-        const float down = __uint_as_float(static_cast<uint32_t>(254 - up) << 23) * ((a.cap_log2e > 0.f ? a.scale_over_cap : a.scale_log2e) * 16777216.f);
+        // (not 0, which would make masked scores no numbers)
+        const float down = fmaxf(__uint_as_float(static_cast<uint32_t>(254 - up) << 23) * ((a.cap_log2e > 0.f ? a.scale_over_cap : a.scale_log2e) * 16777216.f),
+                                 1.17549435e-38f);
         factor[nt][0] = __shfl_sync(0xffffffffu, down, 8 * c);
         factor[nt][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
 #pragma unroll

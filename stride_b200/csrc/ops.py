@@ -2240,6 +2240,8 @@ def paged_attention_decode_int4(q, q_stride: int, out, k_pages, v_pages, block_t
     position; ``scratch``: float32, zero when it is first used, at least ``decode_int4_scratch_floats`` elements, for one stream at a time."""
     device, qp, op, k, v, pages, table, width, requests = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size,
                                                                                window, softcap, torch.bfloat16)
+    if not scale > 0:
+        raise KernelError("paged_attention_decode_int4: the scale of the scores must be positive (paged_attention_int4 takes any)")
     tokens = out.shape[0]
     _launch("stride_decode_int4", "paged_attention_decode_int4", qp, op, k, v, table, _covers(seq_of_token, "seq_of_token", device, tokens),
             _covers(positions, "positions", device, tokens), _here(scratch, "scratch", device, torch.float32), _here_opt(sinks, "sinks", device, nq),
@@ -2277,6 +2279,8 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
                                                                               window, softcap, torch.bfloat16)
     if not fast_attention_supported(q.dtype, nq, nkv, hd):
         raise KernelError(f"paged_attention_prefill_int4: {nq} heads of {hd} on {nkv} are not supported (paged_attention_int4 takes them)")
+    if not scale > 0:
+        raise KernelError("paged_attention_prefill_int4: the scale of the scores must be positive (paged_attention_int4 takes any)")
     out_pages = _int4_expanded_pages(num_seqs, keys)
     half = out_pages * nkv * INT4_EXPANDED_PAGE * hd * 2            # bytes of the keys, and of the values
     if num_seqs < 0 or keys < 0 or scratch.numel() < prefill_int4_scratch_ints(num_seqs, keys, nkv, hd):

@@ -34,11 +34,12 @@ def cache_of(keys, values, page):
     return pages, torch.arange(count, dtype=torch.int32, device="cuda")[None], stored
 
 
-def decode(ops, q, pages, table, n, nq, nkv, hd, page):
+def decode(ops, q, pages, table, n, nq, nkv, hd, page, scale=None):
     out = torch.empty(q.shape[0], nq * hd, dtype=BF16, device="cuda")
     at = torch.full((q.shape[0],), n - 1, dtype=torch.int32, device="cuda")
     scratch = torch.zeros(ops.decode_int4_scratch_floats(q.shape[0], nq, nkv, hd, n), device="cuda")
-    ops.paged_attention_decode_int4(q.cuda(), nq * hd, out, *pages, table, torch.zeros_like(at), at, scratch, nq, nkv, hd, page, hd ** -0.5, 0, n)
+    ops.paged_attention_decode_int4(q.cuda(), nq * hd, out, *pages, table, torch.zeros_like(at), at, scratch, nq, nkv, hd, page,
+                                    hd ** -0.5 if scale is None else scale, 0, n)
     return out.view(-1, nq, hd).double().cpu()
 
 
@@ -88,13 +89,14 @@ def test_decode_beside_one_token_with_a_group_that_stands_out(ops, nq, nkv, hd, 
     ops.check_kernel_status()
 
 
-def portion(ops, q, pages, table, n, nq, nkv, hd, page, **rules):
+def portion(ops, q, pages, table, n, nq, nkv, hd, page, scale=None, **rules):
     """The last q.shape[0] tokens of a request of n keys."""
     p = q.shape[0]
     ints = lambda x: torch.tensor([x], dtype=torch.int32, device="cuda")  # noqa: E731
     out = torch.full((p, nq * hd), 9.0, dtype=BF16, device="cuda")
     scratch = torch.full((ops.prefill_int4_scratch_ints(1, n, nkv, hd),), -1, dtype=torch.int32, device="cuda")
-    ops.paged_attention_prefill_int4(q.cuda(), nq * hd, out, *pages, table, ints(0), ints(p), ints(n), scratch, 1, n, nq, nkv, hd, page, hd ** -0.5, 0, **rules)
+    ops.paged_attention_prefill_int4(q.cuda(), nq * hd, out, *pages, table, ints(0), ints(p), ints(n), scratch, 1, n, nq, nkv, hd, page,
+                                     hd ** -0.5 if scale is None else scale, 0, **rules)
     return out.view(p, nq, hd).double().cpu()
 
 
@@ -368,4 +370,40 @@ def test_large_values_that_weigh_nothing_do_not_drown_the_others(ops, call):
     got = (portion if call == "portion" else decode)(ops, q, pages, table, n, nq, nkv, hd, page)
     # keys near -17.5 are of no weight; the others' scores, of up to 0.2 times 16 in all, are off by 2^-11 of that
     assert group_errors(got, want) <= HALF_STEP + 2 * 2.0 ** -11 + 4 * 2.0 ** -11
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan")])
+@pytest.mark.parametrize("call", [decode, portion])
+def test_scales_that_are_not_positive_are_refused(ops, call, scale):
+    """The largest score is looked for before the scale, and a masked one is -inf."""
+    n, nq, nkv, hd, page, g = 60, 4, 2, 64, 16, torch.Generator().manual_seed(2)
+    pages, table, _stored = cache_of(torch.randn(n, nkv, hd, generator=g), positive(g, n, nkv, hd), page)
+    with pytest.raises(ops.KernelError, match="positive"):
+        call(ops, torch.zeros(6, nq * hd, dtype=BF16), pages, table, n, nq, nkv, hd, page, scale)
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-40])
+def test_the_exact_kernel_takes_any_scale(ops, scale):
+    n, nq, nkv, hd, page, g = 190, 4, 2, 64, 16, torch.Generator().manual_seed(2)
+    pages, table, (k, v) = cache_of(torch.randn(n, nkv, hd, generator=g), positive(g, n, nkv, hd), page)
+    q = torch.randn(6, nq * hd, generator=g).to(BF16)
+    want, _l, _v = plain.attention(q.view(6, nq, hd), [k], [v], *rows_of(n, 6), scale)
+    at, seq = (x.int().cuda() for x in rows_of(n, 6))
+    out = torch.full((6, nq * hd), 9.0, dtype=BF16, device="cuda")
+    ops.paged_attention_int4(q.cuda(), nq * hd, out, *pages, table, seq, at, nq, nkv, hd, page, scale)
+    assert group_errors(out.view(6, nq, hd).double().cpu(), want) <= HALF_STEP + 2.0 ** -10
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("call", [decode, portion])
+def test_the_smallest_scales_and_queries(ops, call):
+    """Scores below any number: every token weighs the same, and masked ones nothing."""
+    n, nq, nkv, hd, page, g = 190, 4, 2, 64, 16, torch.Generator().manual_seed(2)
+    pages, table, (k, v) = cache_of(torch.randn(n, nkv, hd, generator=g), positive(g, n, nkv, hd), page)
+    q = (torch.randn(6, nq * hd, generator=g) * 1e-36).to(BF16)
+    rows = rows_of(n, 6) if call is portion else (torch.tensor([n - 1] * 6), torch.zeros(6, dtype=torch.int32))
+    want, _l, _v = plain.attention(q.view(6, nq, hd), [k], [v], *rows, 1e-38)
+    assert group_errors(call(ops, q, pages, table, n, nq, nkv, hd, page, 1e-38), want) <= HALF_STEP + 2.0 ** -10
     ops.check_kernel_status()
