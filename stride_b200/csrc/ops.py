@@ -2237,7 +2237,8 @@ def decode_int4_scratch_floats(tokens: int, nq: int, nkv: int, hd: int, max_cont
 def paged_attention_decode_int4(q, q_stride: int, out, k_pages, v_pages, block_table, seq_of_token, positions, scratch, nq: int, nkv: int, hd: int,
                                 page_size: int, scale: float, window: int, max_context: int, softcap: float = 0.0, sinks=None, slopes=None) -> None:
     """``paged_attention_decode`` over pages held in 4 bits: one query per row, bfloat16, head sizes 64 and 128. ``max_context`` exceeds every
-    position; ``scratch``: float32, zero when it is first used, at least ``decode_int4_scratch_floats`` elements, for one stream at a time."""
+    position; ``scratch``: float32, zero when it is first used, at least ``decode_int4_scratch_floats`` elements, for one stream at a time. ``scale``
+    is positive."""
     device, qp, op, k, v, pages, table, width, requests = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size,
                                                                                window, softcap, torch.bfloat16)
     if not scale > 0:
@@ -2274,7 +2275,7 @@ def paged_attention_prefill_int4(q, q_stride: int, out, k_pages, v_pages, block_
     ``prefill_int4_scratch_ints`` elements, for one stream at a time. The keys and values that the portions see are expanded once, to pages
     of 64 in 16-bit floating point, scaled by a power of two for each page and key head (a rounding of 2^-11 of an entry at most, or of
     2^-40 of the page's largest), and attended to from there. A weight whose product with its page's largest value lies below 2^-32 of the
-    largest such product of the row counts in the denominator alone."""
+    largest such product of the row counts in the denominator alone. ``scale`` is positive."""
     device, qp, op, k, v, pages, rows, width, requests = _int4_attention_args(q, q_stride, out, k_pages, v_pages, block_table, nq, nkv, hd, page_size,
                                                                               window, softcap, torch.bfloat16)
     if not fast_attention_supported(q.dtype, nq, nkv, hd):
